@@ -642,6 +642,31 @@ int mggan_copy_small(const void* descs, int n, mggan_stream_t stream);
 int mggan_crop_patches(const unsigned char* atlas, const long long* img_off, const int* img_hw, const int* centers,
                        int n, int margin, float* out, mggan_stream_t stream);
 
+/* ---- transformer block: the layers that are matrix products (mggan/hip/blocks.py; no counterpart in the reference, whose
+ * nn.Linear stacks are utils.py:134-149) -------------------------------------------------------------------------------
+ * dtype: 0 f32, 1 bf16 -- of every operand and output; sums and activations in f32, one rounding at the end.  act: 0 none,
+ * 1 LeakyReLU(slope), 2 sigmoid, 4 SiLU, 5 GELU (exact).  x (rows, K) with row stride ldx (elements), any alignment; weights (N, K)
+ * contiguous; everything else contiguous and 16-byte aligned.  `ws`: mggan_block_layer_workspace bytes, 256-byte aligned, free
+ * again when the call's work on `stream` is done.  Limits: rows <= 2^21, K, N <= 2^20. */
+size_t mggan_block_layer_workspace(int rows, int K, int N, int gated, int backward, int dtype);
+/* y = act(x W^T + bias) + residual; bias, residual or NULL.  z (or NULL): the activation's input, which the backward pass reads. */
+int mggan_block_linear_fwd(const void* x, long ldx, const void* w, const void* bias, const void* residual, void* y, void* z,
+                           int rows, int K, int N, int act, float slope, int dtype, void* ws, size_t ws_bytes,
+                           mggan_stream_t stream);
+/* dZ = dy act'(z) (z may be NULL for act 0): dx (rows, K) = dZ W, dw (N, K) = dZ^T x, db (N) = column sums; each NULL if not
+ * wanted.  Written, not accumulated; fixed order of summation. */
+int mggan_block_linear_bwd(const void* dy, const void* z, const void* x, long ldx, const void* w, void* dx, void* dw, void* db,
+                           int rows, int K, int N, int act, float slope, int dtype, void* ws, size_t ws_bytes,
+                           mggan_stream_t stream);
+/* y = act(x Wg^T + bg) * (x Wu^T + bu); z_gate, z_up (both or neither): the two linear results for the backward pass. */
+int mggan_block_gated_fwd(const void* x, long ldx, const void* w_gate, const void* w_up, const void* b_gate, const void* b_up,
+                          void* y, void* z_gate, void* z_up, int rows, int K, int N, int act, float slope, int dtype,
+                          void* ws, size_t ws_bytes, mggan_stream_t stream);
+/* dx (rows, K); dw (2 N, K): the gate weight's gradient, then the up weight's; db (2 N) likewise. */
+int mggan_block_gated_bwd(const void* dy, const void* z_gate, const void* z_up, const void* x, long ldx, const void* w_gate,
+                          const void* w_up, void* dx, void* dw, void* db, int rows, int K, int N, int act, float slope,
+                          int dtype, void* ws, size_t ws_bytes, mggan_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
