@@ -667,6 +667,24 @@ int mggan_block_gated_bwd(const void* dy, const void* z_gate, const void* z_up, 
                           const void* w_up, void* dx, void* dw, void* db, int rows, int K, int N, int act, float slope,
                           int dtype, void* ws, size_t ws_bytes, mggan_stream_t stream);
 
+/* ---- transformer block: attention over the rows of scenes (mggan/hip/blocks.py: attention) ---------------------------
+ * out_i = sum_j P_ij v_j, P_i = softmax over the visible keys j of cap tanh(scale q_i.k_j / cap) - slopes[h] |xy_i - kv_xy_j|.
+ * `args`: a host structure
+ *   { const void *q, *k, *v, *dout; void *out, *dq, *dk, *dv; float* dslopes; const int *scenes, *kv_scenes, *prefix;
+ *     const float *xy, *kv_xy, *slopes; float* lse; int* spans; void* ws;
+ *     long ws_bytes, q_row, q_head, k_row, k_head, v_row, v_head; int N, M, H, Hkv, D, S, causal, axes, dtype; float scale, cap; }
+ * q (N, H, D), k, v (M, Hkv, D) with the given row and head strides in elements (multiples of 16 bytes, width contiguous); out,
+ * dout, dq (N, H, D), dk, dv (M, Hkv, D) contiguous; dtype 0 f32, 1 bf16; D a multiple of 8 up to 128; scenes, kv_scenes (S, 2) rows
+ * [start, end) (clamped to the operands); prefix (S) or NULL; axes 0, 1 or 2 (then xy (N, axes), kv_xy (M, axes), slopes (H)); cap 0:
+ * none; lse (H, N): written if not NULL, the backward pass reads it.  spans: mggan_block_attention_span_ints(N) int32, 16-byte
+ * aligned, written by the forward call and read by the backward call.  Rows without keys: zeros. */
+size_t mggan_block_attention_span_ints(int rows);
+int mggan_block_attention_fwd(const void* args, mggan_stream_t stream);
+/* dq, dk, dv, and dslopes (H) if not NULL, written in a fixed order of summation; out, lse, spans as the forward call left them.
+ * ws: mggan_block_attention_bwd_workspace bytes. */
+size_t mggan_block_attention_bwd_workspace(int rows, int heads);
+int mggan_block_attention_bwd(const void* args, mggan_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

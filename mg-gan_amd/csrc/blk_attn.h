@@ -1,0 +1,237 @@
+// Shared pieces of the attention kernels (blk_attn.hip: forward, blk_attn_bwd.hip: backward).
+//
+//   out_i = sum_j P_ij v_j,   P_i = softmax over the keys j that row i sees of   cap tanh(scale q_i.k_j / cap) - slope_h |xy_i - kv_xy_j|
+//
+// Which keys a row sees is one interval [lo_i, hi_i): those of its scene, cut off behind the row's own place (causal) or behind the
+// prefix.  blk_spans_kernel writes the intervals, every kernel compares indices with them: documents, prefixes and padding are one test.
+//
+// All products run transposed on the matrix cores.  The side that owns the result (queries, or keys in the dK / dV kernel) lies in
+// registers as the second operand, one row per lane; the other side streams through LDS in tiles of BK rows.  S^T = K Q^T leaves
+// lane 16 g + i with row i's scores of keys 32 p + 8 g + {0..7} (the rows of K are read in that order: a product may number its
+// result rows as it likes) -- which is how the next product wants its second operand: P never leaves the registers.
+#pragma once
+#include "blk.h"
+
+struct BlkAttnArgs {  // mirrored by mggan/hip/blocks.py
+  const void *q, *k, *v, *dout;
+  void *out, *dq, *dk, *dv;
+  float* dslopes;
+  const int *scenes, *kv_scenes, *prefix;
+  const float *xy, *kv_xy, *slopes;
+  float* lse;   // (H, N): log2 of the softmax denominators, -inf for a row that sees nothing
+  int* spans;   // mggan_block_attention_span_ints(N): lo, hi, and {min lo, max hi, max lo, min hi} of every 32 rows
+  void* ws;
+  long ws_bytes;
+  long q_row, q_head, k_row, k_head, v_row, v_head;  // strides in elements
+  int N, M, H, Hkv, D, S, causal, axes, dtype;
+  float scale, cap;
+};
+
+namespace {
+
+__device__ __attribute__((aligned(16))) const unsigned blk_attn_zeros[4] = {0, 0, 0, 0};
+
+constexpr float LOG2E = 1.44269504f;
+
+template <class T, int DP>
+struct Geo {
+  static constexpr int CH = Mf<T>::CH;
+  static constexpr int NCH = DP / CH;          // 16-byte chunks of a row
+  static constexpr int SK = NCH / 4;           // steps of a product over the width
+  static constexpr int BK = 128 / sizeof(T);   // streamed rows of a tile: 64 bf16, 32 f32
+  static constexpr int F = BK / 16;            // their 16-row fragments
+  static constexpr int DF = DP / 16;           // 16-column fragments of the width
+  static constexpr int TILE = BK * NCH;        // chunks of a tile
+  // the streamed row that fragment f's row i is, and the row of a lane's r-th value (r, g -> i = 4 g + r)
+  static __device__ __forceinline__ int row_of(int f, int i) {
+    return sizeof(T) == 2 ? 32 * (f >> 1) + 8 * (i >> 2) + 4 * (f & 1) + (i & 3) : 16 * f + i;
+  }
+  static __device__ __forceinline__ int row4(int f, int g) { return sizeof(T) == 2 ? 32 * (f >> 1) + 8 * g + 4 * (f & 1) : 16 * f + 4 * g; }
+  // place of a chunk in its row: eight lanes that read the same chunk of eight rows meet eight different bank groups
+  static __device__ __forceinline__ int swz(int r) {
+    return NCH % 8 == 0 ? (r & 7) ^ ((r >> 1) & 4) : ((r >> 1) & 3) ^ ((r >> 2) & 2);
+  }
+};
+
+// Rows [first, first + BK) of a (rows, heads, D) operand into LDS; rows outside [lo, hi) and columns from D on as zeros.
+template <class T, int DP>
+__device__ __forceinline__ void copy_tile(const T* base, long row_stride, int first, int lo, int hi, int nd, u32x4* lds) {
+  using G = Geo<T, DP>;
+  const int wave = mg_wave();
+#pragma unroll
+  for (int i = 0; i < G::TILE / 256; ++i) {
+    const int slot = i * 256 + (int)threadIdx.x, row = slot / G::NCH, c = (slot % G::NCH) ^ G::swz(row), at = first + row;
+    const bool in = at >= lo && at < hi && c < nd;
+    const char* src = (const char*)(base + (long)at * row_stride) + c * 16;
+    lds_copy16(in ? src : (const char*)blk_attn_zeros, lds + i * 256 + wave * 64);
+  }
+}
+// 4 bytes of each of 64 rows: element `at` of row `first + lane` of rows of `stride` (rows clamped to [0, n)).
+__device__ __forceinline__ void copy_meta(const void* base, long stride, long at, int first, int n, void* lds) {
+  const int r = first + mg_lane(), row = r < 0 ? 0 : r < n ? r : n - 1;
+  __builtin_amdgcn_global_load_lds((MG_GLB const void*)((const char*)base + 4 * (row * stride + at)), (MG_LDS void*)lds, 4, 0, 0);
+}
+
+// The chunk of an owner row that a lane holds as second operand; zeros outside.
+template <class T>
+__device__ __forceinline__ u32x4 owner_chunk(const T* row, int c, int nd) {
+  if (c < nd) return *(const u32x4*)((const char*)row + c * 16);
+  return u32x4{0, 0, 0, 0};
+}
+
+// First operand over the width: fragment f's rows, chunk 4 s + g.
+template <class T, int DP>
+__device__ __forceinline__ u32x4 row_frag(const u32x4* tile, int f, int s, int lane) {
+  using G = Geo<T, DP>;
+  const int row = G::row_of(f, lane & 15);
+  return tile[row * G::NCH + ((4 * s + (lane >> 4)) ^ G::swz(row))];
+}
+
+// D fragments of scores: sum over the width of streamed rows x owner rows.
+template <class T, int DP, int QF>
+__device__ __forceinline__ void scores(const u32x4* tile, const u32x4 (&own)[QF][Geo<T, DP>::SK], f32x4 (&out)[QF][Geo<T, DP>::F], int lane) {
+  using G = Geo<T, DP>;
+#pragma unroll
+  for (int f = 0; f < G::F; ++f) {
+#pragma unroll
+    for (int j = 0; j < QF; ++j) out[j][f] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int s = 0; s < G::SK; ++s) {
+      const u32x4 a = row_frag<T, DP>(tile, f, s, lane);
+#pragma unroll
+      for (int j = 0; j < QF; ++j) out[j][f] = Mf<T>::step(a, own[j][s], out[j][f]);
+    }
+  }
+}
+
+// acc[d][owner row] += sum over streamed rows of tile[row][d] * coef[row][owner row].  The tile is read transposed: bf16 through the
+// transposing LDS read (4 rows x 16 columns a go), f32 an element a lane.  Result fragment fd's row i is column 32 (fd / 2) + 8 (i / 4)
+// + 4 (fd % 2) + i % 4, so a lane ends up with eight neighbouring columns of its owner row in every pair of fragments.
+template <class T, int DP, int QF>
+__device__ __forceinline__ void accumulate(const u32x4* tile, const f32x4 (&coef)[QF][Geo<T, DP>::F], f32x4 (&acc)[QF][Geo<T, DP>::DF], int lane) {
+  using G = Geo<T, DP>;
+  const int i16 = lane & 15, g = lane >> 4;
+  if constexpr (sizeof(T) == 2) {
+#pragma unroll
+    for (int p = 0; p < G::F / 2; ++p) {
+      bf16x8 b[QF];
+#pragma unroll
+      for (int j = 0; j < QF; ++j)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) b[j][r] = (bf16)coef[j][2 * p][r], b[j][4 + r] = (bf16)coef[j][2 * p + 1][r];
+      const int r0 = 32 * p + 8 * g + (i16 >> 2), r1 = r0 + 4;
+      const char* t0 = (const char*)(tile + r0 * G::NCH);
+      const char* t1 = (const char*)(tile + r1 * G::NCH);
+      const int s0 = G::swz(r0), s1 = G::swz(r1);
+#pragma unroll
+      for (int fd = 0; fd < G::DF; ++fd) {
+        const int c = 4 * (fd >> 1) + (i16 & 3), half = 8 * (fd & 1);
+        const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((MG_LDS s16x4*)(t0 + (c ^ s0) * 16 + half));
+        const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((MG_LDS s16x4*)(t1 + (c ^ s1) * 16 + half));
+        const bf16x8 a = __builtin_bit_cast(bf16x8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+        for (int j = 0; j < QF; ++j) acc[j][fd] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b[j], acc[j][fd], 0, 0, 0);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int f = 0; f < G::F; ++f)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int row = 16 * f + 4 * g + r, sw = G::swz(row);
+        const float* t = (const float*)(tile + row * G::NCH);
+#pragma unroll
+        for (int fd = 0; fd < G::DF; ++fd) {
+          const int c = 8 * (fd >> 1) + 2 * (i16 >> 2) + (fd & 1);
+          const float a = t[(c ^ sw) * 4 + (i16 & 3)];
+#pragma unroll
+          for (int j = 0; j < QF; ++j) acc[j][fd] = __builtin_amdgcn_mfma_f32_16x16x4f32(a, coef[j][f][r], acc[j][fd], 0, 0, 0);
+        }
+      }
+  }
+}
+
+// Whether any value of the tile is infinite or not a number (a masked place's zero coefficient would turn it into one).
+template <class T, int DP>
+__device__ __forceinline__ bool tile_not_finite(const u32x4* tile, int lane) {
+  using G = Geo<T, DP>;
+  bool bad = false;
+  for (int i = lane; i < G::TILE; i += 64) {
+    const u32x4 v = tile[i];
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      if (sizeof(T) == 2)
+        bad |= (v[w] & 0x7f80u) == 0x7f80u || (v[w] & 0x7f800000u) == 0x7f800000u;
+      else
+        bad |= (v[w] & 0x7f800000u) == 0x7f800000u;
+    }
+  }
+  return __ballot(bad) != 0;
+}
+// accumulate() row by row over the places that `sees` only: the way of tiles that are partly masked AND hold such a value.
+template <class T, int DP, int QF, class See>
+__device__ __forceinline__ void accumulate_seen(const u32x4* tile, const f32x4 (&coef)[QF][Geo<T, DP>::F],
+                                                          f32x4 (&acc)[QF][Geo<T, DP>::DF], int lane, See sees) {
+  using G = Geo<T, DP>;
+  const int i16 = lane & 15, g = lane >> 4;
+  for (int row = 0; row < G::BK; ++row) {
+    int f, gg, r = row & 3;
+    if (sizeof(T) == 2)
+      f = 2 * (row >> 5) + ((row >> 2) & 1), gg = (row >> 3) & 3;
+    else
+      f = row >> 4, gg = (row >> 2) & 3;
+    const T* t = (const T*)(tile + row * G::NCH);
+    const int sw = G::swz(row);
+#pragma unroll
+    for (int j = 0; j < QF; ++j) {
+      float c = 0.f;
+#pragma unroll
+      for (int a = 0; a < G::F; ++a)
+#pragma unroll
+        for (int b = 0; b < 4; ++b) c = a == f && b == r ? coef[j][a][b] : c;
+      c = __shfl(c, i16 + 16 * gg, 64);
+      if (!sees(j, row)) continue;
+#pragma unroll
+      for (int fd = 0; fd < G::DF; ++fd)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int d = 32 * (fd >> 1) + 8 * g + 4 * (fd & 1) + e;
+          acc[j][fd][e] = fmaf(c, (float)t[((d / G::CH) ^ sw) * G::CH + d % G::CH], acc[j][fd][e]);
+        }
+    }
+  }
+}
+
+// tanh.  f32 operands: near zero by its series (to x^11: 2^-26 of the value at 0.35), so that a score keeps its relative precision
+// through the cap; bf16 operands carry 2^-9 themselves, there the quotient does everywhere.
+template <class T>
+__device__ __forceinline__ float blk_tanh(float x) {
+  const float big = fmaf(-2.0f, mg_rcp(__builtin_amdgcn_exp2f(x * (2.f * LOG2E)) + 1.0f), 1.0f);
+  if constexpr (sizeof(T) == 2) return big;
+  const float y = x * x;
+  const float s = fmaf(y, fmaf(y, fmaf(y, fmaf(y, fmaf(y, -0.0088632355f, 0.0218694885f), -0.0539682540f), 0.1333333333f), -0.3333333333f), 1.f) * x;
+  return fabsf(x) < 0.35f ? s : big;
+}
+
+__device__ __forceinline__ float blk_dist(int axes, float ax, float ay, float bx, float by) {
+  const float dx = ax - bx;
+  if (axes == 1) return fabsf(dx);
+  const float dy = ay - by;
+  return __builtin_amdgcn_sqrtf(fmaf(dx, dx, dy * dy));
+}
+
+// Eight neighbouring columns of an owner row, scaled.
+template <class T>
+__device__ __forceinline__ void store_pair(T* p, const f32x4& a, const f32x4& b, float scale) {
+  if constexpr (sizeof(T) == 2) {
+    bf16x8 x;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) x[r] = (bf16)(a[r] * scale), x[4 + r] = (bf16)(b[r] * scale);
+    *(bf16x8*)p = x;
+  } else {
+    *(f32x4*)p = a * scale;
+    *(f32x4*)(p + 4) = b * scale;
+  }
+}
+
+}  // namespace

@@ -1,5 +1,6 @@
 """Operators of a transformer block over the rows of scenes, f32 or bf16, with their backward passes:
 
+    attention(q, k, v, scenes, ...)                   softmax(cap tanh(scale q k / cap) - slope |xy - kv_xy|) v within each scene
     linear_residual(x, weight, bias, residual, act)   act(x W^T + b) + residual
     gated_linear(x, w_gate, w_up, b_gate, b_up, act)  act(x Wg^T + bg) * (x Wu^T + bu)
 
@@ -7,11 +8,14 @@ All operands of a call have one type and live on one device; sums, activations a
 rounded once.  Work goes to torch's current stream, outputs and workspaces come from torch's allocator (so a call can be captured
 into a HIP graph), gradients are returned through autograd and are the same bits in every run.  Arguments that do not fit raise
 ValueError, a failing launch raises HipError; there is no CPU path."""
+import ctypes
+import math
+
 import torch
 from torch.autograd import Function
 from torch.autograd.function import once_differentiable
 
-from .functions import ACT_LEAKY, ACT_NONE, ACT_SIGMOID, _p, _s
+from .functions import ACT_LEAKY, ACT_NONE, ACT_SIGMOID, BoundedCache, _p, _s
 from .lib import lib
 
 ACT_SILU, ACT_GELU = 4, 5
@@ -186,3 +190,163 @@ def gated_linear(x, w_gate, w_up, b_gate=None, b_up=None, act=ACT_SILU, slope=0.
         else:
             y = _gated_fwd(x, w_gate, w_up, b_gate, b_up, act, slope, False)[0]
     return y.reshape(*lead, N)
+
+
+# ---- attention ---------------------------------------------------------------------------------------------------------------
+
+class _AttnArgs(ctypes.Structure):  # mirrors csrc/blk_attn.h: BlkAttnArgs
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("q", "k", "v", "dout", "out", "dq", "dk", "dv", "dslopes", "scenes", "kv_scenes", "prefix",
+                                                "xy", "kv_xy", "slopes", "lse", "spans", "ws")]
+                + [(n, ctypes.c_long) for n in ("ws_bytes", "q_row", "q_head", "k_row", "k_head", "v_row", "v_head")]
+                + [(n, ctypes.c_int) for n in ("N", "M", "H", "Hkv", "D", "S", "causal", "axes", "dtype")]
+                + [("scale", ctypes.c_float), ("cap", ctypes.c_float)])
+
+
+_TABLES = BoundedCache(64)
+
+
+def _table(name, rows, device, limit, width):
+    """int32 device tensor of a scene list (width 2) or of per-scene numbers (width 1): checked and kept by its contents when it is a
+    host list, taken as it is when it is a device tensor."""
+    if isinstance(rows, torch.Tensor) and rows.is_cuda:
+        _check(rows.dtype == torch.int32 and rows.device == device and rows.dim() == width and (width == 1 or rows.shape[1] == 2),
+               "attention: {} has to be an int32 tensor of (scenes{}) on {}", name, ", 2" if width == 2 else "", device)
+        return rows.contiguous()
+    try:
+        key = tuple((int(a), int(b)) for a, b in rows) if width == 2 else tuple(int(a) for a in rows)
+    except (TypeError, ValueError):
+        raise ValueError("attention: {} has to be a list or an int32 device tensor".format(name)) from None
+    if width == 2:
+        for a, b in key:
+            _check(0 <= a <= b <= limit, "attention: {} names rows [{}, {}) of {}", name, a, b, limit)
+    else:
+        _check(all(abs(a) < 2 ** 31 for a in key), "attention: {} out of range", name)
+    hit = _TABLES.get((key, device))
+    if hit is None:
+        hit = torch.tensor(key, dtype=torch.int32).reshape((-1, 2) if width == 2 else (-1,)).to(device)
+        _TABLES.put((key, device), hit)
+    return hit
+
+
+def _heads(t):
+    """An operand whose rows and heads start at multiples of 16 bytes and whose width is contiguous (a copy where they do not)."""
+    ch = 16 // t.element_size()
+    ok = t.stride(2) == 1 and t.data_ptr() % 16 == 0 and all(t.shape[i] == 1 or (t.stride(i) % ch == 0 and t.stride(i) >= 0) for i in (0, 1))
+    if not ok:
+        t = t.contiguous()
+        t = t.clone() if t.data_ptr() % 16 else t
+    return t, tuple(t.stride(i) if t.shape[i] > 1 else 0 for i in (0, 1))
+
+
+def _attn_args(q, k, v, scenes, kv_scenes, prefix, xy, kv_xy, slopes, causal, scale, cap):
+    a = _AttnArgs()
+    (q, (a.q_row, a.q_head)), (k, (a.k_row, a.k_head)), (v, (a.v_row, a.v_head)) = _heads(q), _heads(k), _heads(v)
+    a.q, a.k, a.v = _p(q), _p(k), _p(v)
+    a.scenes, a.kv_scenes, a.prefix, a.xy, a.kv_xy, a.slopes = _p(scenes), _p(kv_scenes), _p(prefix), _p(xy), _p(kv_xy), _p(slopes)
+    (a.N, a.H, a.D), a.M, a.Hkv = q.shape, k.shape[0], k.shape[1]
+    a.S, a.causal, a.axes, a.dtype = scenes.shape[0], int(causal), 0 if xy is None else xy.shape[1], _DTYPES[q.dtype]
+    a.scale, a.cap = scale, cap
+    return a, (q, k, v)
+
+
+def _attn_fwd(a, q, keep):
+    out = torch.empty(a.N, a.H, a.D, dtype=q.dtype, device=q.device)
+    lse = torch.empty(a.H, a.N, dtype=torch.float32, device=q.device) if keep else None
+    spans = torch.empty(lib.mggan_block_attention_span_ints(a.N), dtype=torch.int32, device=q.device)
+    a.out, a.lse, a.spans = _p(out), _p(lse), _p(spans)
+    lib.mggan_block_attention_fwd(ctypes.addressof(a), _s())
+    return out, lse, spans
+
+
+class AttentionFn(Function):
+    @staticmethod
+    def forward(ctx, q, k, v, slopes, rest):
+        scenes, kv_scenes, prefix, xy, kv_xy, causal, scale, cap = rest
+        ctx.rest = rest
+        if q.shape[0] == 0 or k.shape[0] == 0:
+            ctx.save_for_backward(q, k, v, slopes)
+            ctx.empty = True
+            return torch.zeros(q.shape, dtype=q.dtype, device=q.device)
+        ctx.empty = False
+        a, (q, k, v) = _attn_args(q, k, v, scenes, kv_scenes, prefix, xy, kv_xy, slopes, causal, scale, cap)
+        out, lse, spans = _attn_fwd(a, q, True)
+        ctx.save_for_backward(q, k, v, slopes, out, lse, spans)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        scenes, kv_scenes, prefix, xy, kv_xy, causal, scale, cap = ctx.rest
+        if ctx.empty:
+            return tuple(None if t is None else torch.zeros_like(t) for t in ctx.saved_tensors) + (None,)
+        q, k, v, slopes, out, lse, spans = ctx.saved_tensors
+        a, _ = _attn_args(q, k, v, scenes, kv_scenes, prefix, xy, kv_xy, slopes, causal, scale, cap)
+        dout = _aligned(dout)
+        dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        dk, dv = (torch.empty(k.shape, dtype=q.dtype, device=q.device) for _ in range(2))
+        dslopes = torch.empty_like(slopes) if slopes is not None and ctx.needs_input_grad[3] else None
+        a.ws_bytes = lib.mggan_block_attention_bwd_workspace(a.N, a.H)
+        ws = torch.empty(a.ws_bytes // 4, dtype=torch.float32, device=q.device)
+        a.dout, a.out, a.lse, a.spans, a.ws = _p(dout), _p(out), _p(lse), _p(spans), _p(ws)
+        a.dq, a.dk, a.dv, a.dslopes = _p(dq), _p(dk), _p(dv), _p(dslopes)
+        lib.mggan_block_attention_bwd(ctypes.addressof(a), _s())
+        return dq, dk, dv, dslopes, None
+
+
+def attention(q, k, v, scenes, kv_scenes=None, *, causal=False, prefix=None, scale=None, cap=0.0, xy=None, kv_xy=None, slopes=None):
+    """Attention of every row of a scene over the keys of the same scene: q (N, H, D), k and v (M, Hkv, D) -> (N, H, D); H a multiple
+    of Hkv (head h reads key head h // (H // Hkv)), D a multiple of 8 up to 128.
+
+        out_i = sum_j P_ij v_j,    P_i = softmax over the visible j of   s_ij - slopes[h] |xy_i - kv_xy_j|,    s = cap tanh(scale q k / cap)
+
+    scenes, kv_scenes: rows [start, end) of q and of k / v that belong to each scene, as a list of pairs (the framework's
+    seq_start_end) or as an int32 device tensor (scenes, 2), which is read when the kernel runs (and clamped to the operands' rows);
+    kv_scenes defaults to scenes.  In any order; scenes may share keys; of a row that several scenes name the last one counts.  Rows of
+    no scene and rows that see no key give zeros.  What lies outside a row's visible keys is never mixed in, infinities and NaN included.
+    causal: row i of a scene of Lq rows and Lk keys sees keys j <= i + Lk - Lq, and in any case those before prefix[scene] (list or int32
+    device tensor).  One new row over a long cache is Lq = 1.  scale: > 0, D ** -0.5 by default; cap: 0 for none.
+    xy (N, axes) and kv_xy (M, axes; by default xy), f32 with one or two axes, and slopes (H), f32: the bias by distance.  Gradients go to q,
+    k, v and slopes, not to positions."""
+    name = "attention"
+    _same(name, q, k=k, v=v)
+    _check(q.dim() == 3 and k.dim() == 3 and k.shape == v.shape and q.shape[2] == k.shape[2], "{}: q {}, k {}, v {}", name, tuple(q.shape),
+           tuple(k.shape), tuple(v.shape))
+    (N, H, D), (M, Hkv, _) = q.shape, k.shape
+    _check(0 < H <= 1024 and Hkv > 0 and H % Hkv == 0, "{}: {} heads over {} key heads", name, H, Hkv)
+    _check(D % 8 == 0 and 0 < D <= 128, "{}: a width of {} (a multiple of 8 up to 128)", name, D)
+    _check(N <= 1 << 24 and M <= 1 << 30, "{}: {} rows, {} keys", name, N, M)
+    scale = D ** -0.5 if scale is None else float(scale)
+    cap = 0.0 if cap is None else float(cap)
+    _check(scale > 0 and math.isfinite(scale), "{}: scale {} (it has to be positive)", name, scale)
+    _check(cap >= 0 and math.isfinite(cap), "{}: cap {}", name, cap)
+    _check(prefix is None or causal, "{}: a prefix without causal", name)
+    _check((xy is None) == (slopes is None) and (xy is not None or kv_xy is None), "{}: positions and slopes come together", name)
+    if xy is not None:
+        kv_xy = xy if kv_xy is None else kv_xy
+        for n, t, rows in (("xy", xy, N), ("kv_xy", kv_xy, M)):
+            _check(t.dtype == torch.float32 and t.dim() == 2 and t.shape[0] == rows and t.shape[1] in (1, 2) and t.shape[1] == xy.shape[1],
+                   "{}: {} {} {} for {} rows and one or two axes, f32", name, n, t.dtype, tuple(t.shape), rows)
+            _check(t.device == q.device, "{}: {} is on {}", name, n, t.device)
+            _check(not (t.requires_grad and torch.is_grad_enabled()), "{}: {} requires a gradient, positions have none: detach it", name, n)
+        _check(slopes.dtype == torch.float32 and tuple(slopes.shape) == (H,) and slopes.device == q.device, "{}: slopes {} {} on {}", name,
+               slopes.dtype, tuple(slopes.shape), slopes.device)
+    _on_gpu(name, q)
+    with torch.cuda.device(q.device):
+        table = _table("scenes", scenes, q.device, N, 2)
+        kv_table = table if kv_scenes is None else _table("kv_scenes", kv_scenes, q.device, M, 2)
+        if kv_scenes is None:
+            _check(M >= N, "{}: {} rows over {} keys need kv_scenes", name, N, M)
+        _check(table.shape == kv_table.shape, "{}: {} scenes of rows, {} of keys", name, table.shape[0], kv_table.shape[0])
+        if prefix is not None:
+            prefix = _table("prefix", prefix, q.device, 0, 1)
+            _check(prefix.shape[0] == table.shape[0], "{}: {} prefixes for {} scenes", name, prefix.shape[0], table.shape[0])
+        if xy is not None:
+            same = kv_xy is xy
+            xy, slopes = xy.detach().contiguous(), slopes.contiguous()
+            kv_xy = xy if same else kv_xy.detach().contiguous()
+        if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, slopes)):
+            return AttentionFn.apply(q, k, v, slopes, (table, kv_table, prefix, xy, kv_xy, causal, scale, cap))
+        if N == 0 or M == 0:
+            return torch.zeros(q.shape, dtype=q.dtype, device=q.device)
+        a, ops = _attn_args(q, k, v, table, kv_table, prefix, xy, kv_xy, slopes, causal, scale, cap)
+        return _attn_fwd(a, ops[0], False)[0]
