@@ -649,21 +649,22 @@ int mggan_crop_patches(const unsigned char* atlas, const long long* img_off, con
  * contiguous; everything else contiguous and 16-byte aligned.  `ws`: mggan_block_layer_workspace bytes, 256-byte aligned, free
  * again when the call's work on `stream` is done.  Limits: rows <= 2^21, K, N <= 2^20. */
 size_t mggan_block_layer_workspace(int rows, int K, int N, int gated, int backward, int dtype);
-/* y = act(x W^T + bias) + residual; bias, residual or NULL.  z (or NULL): the activation's input, which the backward pass reads. */
-int mggan_block_linear_fwd(const void* x, long ldx, const void* w, const void* bias, const void* residual, void* y, void* z,
+/* y = act(x W^T + bias) + residual; bias, residual or NULL.  z (or NULL): the activation's input in f32,
+ * which the backward pass reads. */
+int mggan_block_linear_fwd(const void* x, long ldx, const void* w, const void* bias, const void* residual, void* y, float* z,
                            int rows, int K, int N, int act, float slope, int dtype, void* ws, size_t ws_bytes,
                            mggan_stream_t stream);
 /* dZ = dy act'(z) (z may be NULL for act 0): dx (rows, K) = dZ W, dw (N, K) = dZ^T x, db (N) = column sums; each NULL if not
  * wanted.  Written, not accumulated; fixed order of summation. */
-int mggan_block_linear_bwd(const void* dy, const void* z, const void* x, long ldx, const void* w, void* dx, void* dw, void* db,
+int mggan_block_linear_bwd(const void* dy, const float* z, const void* x, long ldx, const void* w, void* dx, void* dw, void* db,
                            int rows, int K, int N, int act, float slope, int dtype, void* ws, size_t ws_bytes,
                            mggan_stream_t stream);
-/* y = act(x Wg^T + bg) * (x Wu^T + bu); z_gate, z_up (both or neither): the two linear results for the backward pass. */
+/* y = act(x Wg^T + bg) * (x Wu^T + bu); z_gate, z_up (both or neither): the two linear results in f32 for the backward pass. */
 int mggan_block_gated_fwd(const void* x, long ldx, const void* w_gate, const void* w_up, const void* b_gate, const void* b_up,
-                          void* y, void* z_gate, void* z_up, int rows, int K, int N, int act, float slope, int dtype,
+                          void* y, float* z_gate, float* z_up, int rows, int K, int N, int act, float slope, int dtype,
                           void* ws, size_t ws_bytes, mggan_stream_t stream);
 /* dx (rows, K); dw (2 N, K): the gate weight's gradient, then the up weight's; db (2 N) likewise. */
-int mggan_block_gated_bwd(const void* dy, const void* z_gate, const void* z_up, const void* x, long ldx, const void* w_gate,
+int mggan_block_gated_bwd(const void* dy, const float* z_gate, const float* z_up, const void* x, long ldx, const void* w_gate,
                           const void* w_up, void* dx, void* dw, void* db, int rows, int K, int N, int act, float slope,
                           int dtype, void* ws, size_t ws_bytes, mggan_stream_t stream);
 
@@ -671,16 +672,20 @@ int mggan_block_gated_bwd(const void* dy, const void* z_gate, const void* z_up, 
  * out_i = sum_j P_ij v_j, P_i = softmax over the visible keys j of cap tanh(scale q_i.k_j / cap) - slopes[h] |xy_i - kv_xy_j|.
  * `args`: a host structure
  *   { const void *q, *k, *v, *dout; void *out, *dq, *dk, *dv; float* dslopes; const int *scenes, *kv_scenes, *prefix;
- *     const float *xy, *kv_xy, *slopes; float* lse; int* spans; void* ws;
+ *     const float *xy, *kv_xy, *slopes; float *lse, *out32; int* spans; void* ws;
  *     long ws_bytes, q_row, q_head, k_row, k_head, v_row, v_head; int N, M, H, Hkv, D, S, causal, axes, dtype; float scale, cap; }
  * q (N, H, D), k, v (M, Hkv, D) with the given row and head strides in elements (multiples of 16 bytes, width contiguous); out,
  * dout, dq (N, H, D), dk, dv (M, Hkv, D) contiguous; dtype 0 f32, 1 bf16; D a multiple of 8 up to 128; scenes, kv_scenes (S, 2) rows
  * [start, end) (clamped to the operands); prefix (S) or NULL; axes 0, 1 or 2 (then xy (N, axes), kv_xy (M, axes), slopes (H)); cap 0:
- * none; lse (H, N): written if not NULL, the backward pass reads it.  spans: mggan_block_attention_span_ints(N) int32, 16-byte
+ * none; lse (2, H, N) and, with bf16, out32 (the output before its rounding): written if not NULL, the backward pass reads them (out32
+ * = out with f32).  spans: mggan_block_attention_span_ints(N) int32, 16-byte
  * aligned, written by the forward call and read by the backward call.  Rows without keys: zeros. */
 size_t mggan_block_attention_span_ints(int rows);
+/* Without lse (nothing kept for a backward pass) single rows over long caches are split over their keys: ws as large as this says
+ * (0: none needed). */
+size_t mggan_block_attention_fwd_workspace(int rows, int keys, int heads, int kv_heads, int width, int scenes);
 int mggan_block_attention_fwd(const void* args, mggan_stream_t stream);
-/* dq, dk, dv, and dslopes (H) if not NULL, written in a fixed order of summation; out, lse, spans as the forward call left them.
+/* dq, dk, dv, and dslopes (H) if not NULL, written in a fixed order of summation; out32, lse, spans as the forward call left them.
  * ws: mggan_block_attention_bwd_workspace bytes. */
 size_t mggan_block_attention_bwd_workspace(int rows, int heads);
 int mggan_block_attention_bwd(const void* args, mggan_stream_t stream);

@@ -18,7 +18,9 @@ struct BlkAttnArgs {  // mirrored by mggan/hip/blocks.py
   float* dslopes;
   const int *scenes, *kv_scenes, *prefix;
   const float *xy, *kv_xy, *slopes;
-  float* lse;   // (H, N): log2 of the softmax denominators, -inf for a row that sees nothing
+  float* lse;    // (2, H, N): the row's largest score (as the exponent takes it) and one over its sum of exp(score - largest)
+  float* out32;  // the output before it is rounded (f32: the output): what sum(dO O) is formed of -- from the rounded one every row's
+                 // gradient would carry a common error, which the sums over rows (the slopes' gradient) do not average away
   int* spans;   // mggan_block_attention_span_ints(N): lo, hi, and {min lo, max hi, max lo, min hi} of every 32 rows
   void* ws;
   long ws_bytes;
@@ -33,12 +35,24 @@ __device__ __attribute__((aligned(16))) const unsigned blk_attn_zeros[4] = {0, 0
 
 constexpr float LOG2E = 1.44269504f;
 
-template <class T, int DP>
+// Scores are exponentiated as exp2((s - max) log2e) where their last bits matter (f32; scores that got a bias or a cap, whose gradients
+// are f32): log2e rounded into the scores first would stretch all of them by a common 2^-25, which shows in the slopes' gradient.  Plain
+// bf16 scores, whose gradients are rounded at 2^-9, take the fused form exp2(s c - max c), an operation less.
+template <class T, bool EXTRA>
+struct Soft {
+  static constexpr bool NATURAL = EXTRA || sizeof(T) == 4;
+  static __device__ __forceinline__ float weight(float s, float top, float c2) {
+    return NATURAL ? __builtin_amdgcn_exp2f((s - top) * LOG2E) : __builtin_amdgcn_exp2f(fmaf(s, c2, -top));
+  }
+};
+
+template <class T_, int DP_, int BK_ = 128 / (int)sizeof(T_)>
 struct Geo {
-  static constexpr int CH = Mf<T>::CH;
+  using T = T_;
+  static constexpr int DP = DP_, CH = Mf<T>::CH;
   static constexpr int NCH = DP / CH;          // 16-byte chunks of a row
   static constexpr int SK = NCH / 4;           // steps of a product over the width
-  static constexpr int BK = 128 / sizeof(T);   // streamed rows of a tile: 64 bf16, 32 f32
+  static constexpr int BK = BK_;               // streamed rows of a tile: 64 bf16, 32 f32
   static constexpr int F = BK / 16;            // their 16-row fragments
   static constexpr int DF = DP / 16;           // 16-column fragments of the width
   static constexpr int TILE = BK * NCH;        // chunks of a tile
@@ -54,16 +68,16 @@ struct Geo {
 };
 
 // Rows [first, first + BK) of a (rows, heads, D) operand into LDS; rows outside [lo, hi) and columns from D on as zeros.
-template <class T, int DP>
-__device__ __forceinline__ void copy_tile(const T* base, long row_stride, int first, int lo, int hi, int nd, u32x4* lds) {
-  using G = Geo<T, DP>;
-  const int wave = mg_wave();
+// The workgroup's (threads = 256) or one wave's (64) work.
+template <class G, int threads = 256>
+__device__ __forceinline__ void copy_tile(const typename G::T* base, long row_stride, int first, int lo, int hi, int nd, u32x4* lds) {
+  const int wave = threads == 64 ? 0 : mg_wave();
 #pragma unroll
-  for (int i = 0; i < G::TILE / 256; ++i) {
-    const int slot = i * 256 + (int)threadIdx.x, row = slot / G::NCH, c = (slot % G::NCH) ^ G::swz(row), at = first + row;
+  for (int i = 0; i < G::TILE / threads; ++i) {
+    const int slot = i * threads + (threads == 64 ? mg_lane() : (int)threadIdx.x), row = slot / G::NCH, c = (slot % G::NCH) ^ G::swz(row), at = first + row;
     const bool in = at >= lo && at < hi && c < nd;
     const char* src = (const char*)(base + (long)at * row_stride) + c * 16;
-    lds_copy16(in ? src : (const char*)blk_attn_zeros, lds + i * 256 + wave * 64);
+    lds_copy16(in ? src : (const char*)blk_attn_zeros, lds + i * threads + wave * 64);
   }
 }
 // 4 bytes of each of 64 rows: element `at` of row `first + lane` of rows of `stride` (rows clamped to [0, n)).
@@ -80,26 +94,24 @@ __device__ __forceinline__ u32x4 owner_chunk(const T* row, int c, int nd) {
 }
 
 // First operand over the width: fragment f's rows, chunk 4 s + g.
-template <class T, int DP>
+template <class G>
 __device__ __forceinline__ u32x4 row_frag(const u32x4* tile, int f, int s, int lane) {
-  using G = Geo<T, DP>;
   const int row = G::row_of(f, lane & 15);
   return tile[row * G::NCH + ((4 * s + (lane >> 4)) ^ G::swz(row))];
 }
 
 // D fragments of scores: sum over the width of streamed rows x owner rows.
-template <class T, int DP, int QF>
-__device__ __forceinline__ void scores(const u32x4* tile, const u32x4 (&own)[QF][Geo<T, DP>::SK], f32x4 (&out)[QF][Geo<T, DP>::F], int lane) {
-  using G = Geo<T, DP>;
+template <class G, int QF>
+__device__ __forceinline__ void scores(const u32x4* tile, const u32x4 (&own)[QF][G::SK], f32x4 (&out)[QF][G::F], int lane) {
 #pragma unroll
   for (int f = 0; f < G::F; ++f) {
 #pragma unroll
     for (int j = 0; j < QF; ++j) out[j][f] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int s = 0; s < G::SK; ++s) {
-      const u32x4 a = row_frag<T, DP>(tile, f, s, lane);
+      const u32x4 a = row_frag<G>(tile, f, s, lane);
 #pragma unroll
-      for (int j = 0; j < QF; ++j) out[j][f] = Mf<T>::step(a, own[j][s], out[j][f]);
+      for (int j = 0; j < QF; ++j) out[j][f] = Mf<typename G::T>::step(a, own[j][s], out[j][f]);
     }
   }
 }
@@ -107,9 +119,9 @@ __device__ __forceinline__ void scores(const u32x4* tile, const u32x4 (&own)[QF]
 // acc[d][owner row] += sum over streamed rows of tile[row][d] * coef[row][owner row].  The tile is read transposed: bf16 through the
 // transposing LDS read (4 rows x 16 columns a go), f32 an element a lane.  Result fragment fd's row i is column 32 (fd / 2) + 8 (i / 4)
 // + 4 (fd % 2) + i % 4, so a lane ends up with eight neighbouring columns of its owner row in every pair of fragments.
-template <class T, int DP, int QF>
-__device__ __forceinline__ void accumulate(const u32x4* tile, const f32x4 (&coef)[QF][Geo<T, DP>::F], f32x4 (&acc)[QF][Geo<T, DP>::DF], int lane) {
-  using G = Geo<T, DP>;
+template <class G, int QF>
+__device__ __forceinline__ void accumulate(const u32x4* tile, const f32x4 (&coef)[QF][G::F], f32x4 (&acc)[QF][G::DF], int lane) {
+  using T = typename G::T;
   const int i16 = lane & 15, g = lane >> 4;
   if constexpr (sizeof(T) == 2) {
 #pragma unroll
@@ -152,15 +164,14 @@ __device__ __forceinline__ void accumulate(const u32x4* tile, const f32x4 (&coef
 }
 
 // Whether any value of the tile is infinite or not a number (a masked place's zero coefficient would turn it into one).
-template <class T, int DP>
+template <class G>
 __device__ __forceinline__ bool tile_not_finite(const u32x4* tile, int lane) {
-  using G = Geo<T, DP>;
   bool bad = false;
   for (int i = lane; i < G::TILE; i += 64) {
     const u32x4 v = tile[i];
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
-      if (sizeof(T) == 2)
+      if (sizeof(typename G::T) == 2)
         bad |= (v[w] & 0x7f80u) == 0x7f80u || (v[w] & 0x7f800000u) == 0x7f800000u;
       else
         bad |= (v[w] & 0x7f800000u) == 0x7f800000u;
@@ -169,10 +180,9 @@ __device__ __forceinline__ bool tile_not_finite(const u32x4* tile, int lane) {
   return __ballot(bad) != 0;
 }
 // accumulate() row by row over the places that `sees` only: the way of tiles that are partly masked AND hold such a value.
-template <class T, int DP, int QF, class See>
-__device__ __forceinline__ void accumulate_seen(const u32x4* tile, const f32x4 (&coef)[QF][Geo<T, DP>::F],
-                                                          f32x4 (&acc)[QF][Geo<T, DP>::DF], int lane, See sees) {
-  using G = Geo<T, DP>;
+template <class G, int QF, class See>
+__device__ __forceinline__ void accumulate_seen(const u32x4* tile, const f32x4 (&coef)[QF][G::F], f32x4 (&acc)[QF][G::DF], int lane, See sees) {
+  using T = typename G::T;
   const int i16 = lane & 15, g = lane >> 4;
   for (int row = 0; row < G::BK; ++row) {
     int f, gg, r = row & 3;

@@ -5,9 +5,21 @@
 
 namespace {
 
+// The interval of keys that row r of scene s sees (s < 0: of none).  What the tables say is clamped to the operands' rows.
+__device__ __forceinline__ int2 blk_span(const BlkAttnArgs& p, int s, int r) {
+  if (s < 0) return make_int2(0, 0);
+  const int q0 = max(p.scenes[2 * s], 0), q1 = min(p.scenes[2 * s + 1], p.N);
+  const int k0 = min(max(p.kv_scenes[2 * s], 0), p.M), k1 = min(max(p.kv_scenes[2 * s + 1], k0), p.M);
+  int n = k1 - k0;
+  if (p.causal) {
+    const int pre = p.prefix ? p.prefix[s] : 0;
+    n = max(0, min(n, max(pre, r - q0 + 1 + n - (q1 - q0))));
+  }
+  return n > 0 ? make_int2(k0, k0 + n) : make_int2(0, 0);
+}
+
 // The interval of keys that each of 64 rows sees, and what every 32 rows have in common.  All scenes are looked through (in any
-// order; the last one that names a row counts), so that nothing is asked of a list in device memory; what it says is clamped to the
-// operands' rows.
+// order; the last one that names a row counts), so that nothing is asked of a list in device memory.
 __global__ __launch_bounds__(256) void blk_spans_kernel(BlkAttnArgs p, int np) {
   __shared__ int scene[64];
   const int r0 = blockIdx.x * 64, tid = threadIdx.x;
@@ -20,17 +32,8 @@ __global__ __launch_bounds__(256) void blk_spans_kernel(BlkAttnArgs p, int np) {
   __syncthreads();
   if (tid >= 64) return;
   const int s = scene[tid];
-  int lo = 0, hi = 0;
-  if (s >= 0) {
-    const int q0 = max(p.scenes[2 * s], 0), q1 = min(p.scenes[2 * s + 1], p.N);
-    const int k0 = min(max(p.kv_scenes[2 * s], 0), p.M), k1 = min(max(p.kv_scenes[2 * s + 1], k0), p.M);
-    int n = k1 - k0;
-    if (p.causal) {
-      const int pre = p.prefix ? p.prefix[s] : 0;
-      n = max(0, min(n, max(pre, r0 + tid - q0 + 1 + n - (q1 - q0))));
-    }
-    if (n > 0) lo = k0, hi = k0 + n;
-  }
+  const int2 span = blk_span(p, s, r0 + tid);
+  const int lo = span.x, hi = span.y;
   p.spans[r0 + tid] = lo;
   p.spans[np + r0 + tid] = hi;
   const bool some = hi > lo;
@@ -97,8 +100,8 @@ __global__ __launch_bounds__(256) void blk_attn_fwd_kernel(BlkAttnArgs p, int np
   const T* kb = (const T*)p.k + hk * p.k_head;
   const T* vb = (const T*)p.v + hk * p.v_head;
   auto fetch = [&](int k0, int buf) {
-    copy_tile<T, DP>(kb, p.k_row, k0, glo, ghi, nd, lk[buf]);
-    copy_tile<T, DP>(vb, p.v_row, k0, glo, ghi, nd, lv[buf]);
+    copy_tile<G>(kb, p.k_row, k0, glo, ghi, nd, lk[buf]);
+    copy_tile<G>(vb, p.v_row, k0, glo, ghi, nd, lv[buf]);
     if (EXTRA && wave < p.axes) copy_meta(p.kv_xy, p.axes, wave, k0, p.M, lx[buf][wave]);
   };
 
@@ -111,7 +114,8 @@ __global__ __launch_bounds__(256) void blk_attn_fwd_kernel(BlkAttnArgs p, int np
 #pragma unroll
     for (int d = 0; d < G::DF; ++d) acc[j][d] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
-  const float c2 = p.scale * LOG2E, slope2 = EXTRA && p.axes ? p.slopes[h] * LOG2E : 0.f, icap = EXTRA && p.cap > 0.f ? p.scale / p.cap : 0.f;
+  using W = Soft<T, EXTRA>;
+  const float c2 = p.scale * LOG2E, slope = EXTRA && p.axes ? p.slopes[h] : 0.f, icap = EXTRA && p.cap > 0.f ? p.scale / p.cap : 0.f;
 
   if (glo < ghi) fetch(glo, 0);
   int buf = 0;
@@ -120,7 +124,7 @@ __global__ __launch_bounds__(256) void blk_attn_fwd_kernel(BlkAttnArgs p, int np
     if (k0 + G::BK < ghi) fetch(k0 + G::BK, buf ^ 1);
     if (k0 >= whi || k0 + G::BK <= wlo) continue;  // (the wave's: nothing of this tile is seen)
     f32x4 s[QF][G::F];
-    scores<T, DP, QF>(lk[buf], q, s, lane);
+    scores<G, QF>(lk[buf], q, s, lane);
     const bool part = k0 < flo || k0 + G::BK > fhi;
     if (EXTRA) {
 #pragma unroll
@@ -132,14 +136,19 @@ __global__ __launch_bounds__(256) void blk_attn_fwd_kernel(BlkAttnArgs p, int np
 #pragma unroll
           for (int j = 0; j < QF; ++j) {
             float x = s[j][f][r];
-            x = p.cap > 0.f ? p.cap * LOG2E * blk_tanh<T>(x * icap) : x * c2;
-            if (p.axes) x = fmaf(-slope2, blk_dist(p.axes, qx[j], qy[j], bx, by), x);
+            x = p.cap > 0.f ? p.cap * blk_tanh<T>(x * icap) : x * p.scale;
+            if (p.axes) x = fmaf(-slope, blk_dist(p.axes, qx[j], qy[j], bx, by), x);
             s[j][f][r] = x;
           }
         }
       }
     }
-    const float cs = EXTRA ? 1.f : c2;
+    if (W::NATURAL && !EXTRA) {
+#pragma unroll
+      for (int j = 0; j < QF; ++j)
+#pragma unroll
+        for (int f = 0; f < G::F; ++f) s[j][f] *= p.scale;
+    }
     if (part) {
 #pragma unroll
       for (int f = 0; f < G::F; ++f)
@@ -155,9 +164,9 @@ __global__ __launch_bounds__(256) void blk_attn_fwd_kernel(BlkAttnArgs p, int np
       float t = -INFINITY;
 #pragma unroll
       for (int f = 0; f < G::F; ++f) t = fmaxf(t, fmaxf(fmaxf(s[j][f][0], s[j][f][1]), fmaxf(s[j][f][2], s[j][f][3])));
-      t = quarters_max(t) * cs;
+      t = quarters_max(t) * (W::NATURAL ? 1.f : c2);
       if (__ballot(t > m[j])) {
-        const float mn = fmaxf(m[j], t), al = __builtin_amdgcn_exp2f(mn == -INFINITY ? 0.f : m[j] - mn);
+        const float mn = fmaxf(m[j], t), al = __builtin_amdgcn_exp2f(mn == -INFINITY ? 0.f : (m[j] - mn) * (W::NATURAL ? LOG2E : 1.f));
         m[j] = mn;
         l[j] *= al;
 #pragma unroll
@@ -169,16 +178,16 @@ __global__ __launch_bounds__(256) void blk_attn_fwd_kernel(BlkAttnArgs p, int np
       for (int f = 0; f < G::F; ++f)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const float e = __builtin_amdgcn_exp2f(fmaf(s[j][f][r], cs, -mm));
+          const float e = W::weight(s[j][f][r], mm, c2);
           s[j][f][r] = e;
           sum += e;
         }
       l[j] += sum;
     }
-    if (part && tile_not_finite<T, DP>(lv[buf], lane))
-      accumulate_seen<T, DP, QF>(lv[buf], s, acc, lane, [&](int j, int row) { return k0 + row >= lo[j] && k0 + row < hi[j]; });
+    if (part && tile_not_finite<G>(lv[buf], lane))
+      accumulate_seen<G, QF>(lv[buf], s, acc, lane, [&](int j, int row) { return k0 + row >= lo[j] && k0 + row < hi[j]; });
     else
-      accumulate<T, DP, QF>(lv[buf], s, acc, lane);
+      accumulate<G, QF>(lv[buf], s, acc, lane);
   }
 
 #pragma unroll
@@ -186,18 +195,200 @@ __global__ __launch_bounds__(256) void blk_attn_fwd_kernel(BlkAttnArgs p, int np
     const int r = w0 + 16 * j + i16;
     const float sum = quarters_sum(l[j]), inv = hi[j] > lo[j] ? 1.f / sum : 0.f;
     if (r >= p.N) continue;
-    if (g == 0 && p.lse) p.lse[(long)h * p.N + r] = m[j] + __log2f(sum);
-    T* out = (T*)p.out + ((long)r * p.H + h) * p.D;
+    if (g == 0 && p.lse) {
+      p.lse[(long)h * p.N + r] = m[j];
+      p.lse[(long)(p.H + h) * p.N + r] = inv;
+    }
+    const long at = ((long)r * p.H + h) * p.D;
 #pragma unroll
     for (int d = 0; d < G::DF; d += 2)
-      if (16 * d + 8 * g < p.D) store_pair<T>(out + 16 * d + 8 * g, acc[j][d], acc[j][d + 1], inv);
+      if (16 * d + 8 * g < p.D) {
+        store_pair<T>((T*)p.out + at + 16 * d + 8 * g, acc[j][d], acc[j][d + 1], inv);
+        if (sizeof(T) == 2 && p.out32) store_pair<float>(p.out32 + at + 16 * d + 8 * g, acc[j][d], acc[j][d + 1], inv);
+      }
   }
+}
+
+// Single rows over long caches.  A workgroup takes one row, the heads of one key head (up to 16: the columns of the matrix
+// instruction) and one of `splits` shares of the row's keys; its four waves take the share's tiles in turn, each with LDS of its own and
+// no barrier between them: what counts is bytes in flight (two tiles of keys and values a wave, 64 KB a CU at width 128).  Shares leave
+// maximum, sum and unnormalised output, which blk_attn_join_kernel puts together in their order.
+template <class T, int DP, bool EXTRA>
+__global__ __launch_bounds__(256) void blk_attn_row_kernel(BlkAttnArgs p, int splits, int hgroups, float* part) {
+  using G = Geo<T, DP, 64 / (int)sizeof(T)>;
+  using W = Soft<T, EXTRA>;
+  constexpr int LOADS = 2 * G::TILE / 64;  // copies of a tile of keys and one of values
+  __shared__ u32x4 tiles[4][2][2][G::TILE];
+  __shared__ int scene;
+  const int lane = mg_lane(), wave = mg_wave(), i16 = lane & 15, g = lane >> 4, nd = p.D / G::CH;
+  int id = blockIdx.x;
+  const int sp = id % splits;
+  id /= splits;
+  const int hg = id % hgroups;
+  id /= hgroups;
+  const int hk = id % p.Hkv, r = id / p.Hkv, group = p.H / p.Hkv;
+  const int head = hk * group + hg * 16 + i16;
+  const bool mine = hg * 16 + i16 < group;
+
+  if (threadIdx.x == 0) scene = -1;
+  __syncthreads();
+  for (int s = threadIdx.x; s < p.S; s += 256)
+    if (p.scenes[2 * s] <= r && r < p.scenes[2 * s + 1]) atomicMax(&scene, s);
+  __syncthreads();
+  const int2 span = blk_span(p, scene, r);
+  const int n = span.y - span.x, per = ((n + splits - 1) / splits + G::BK - 1) / G::BK * G::BK;
+  const int lo = min(span.x + sp * per, span.y), hi = min(lo + per, span.y);
+
+  u32x4 q[1][G::SK];
+#pragma unroll
+  for (int s = 0; s < G::SK; ++s)
+    q[0][s] = mine ? owner_chunk((const T*)p.q + r * p.q_row + head * p.q_head, 4 * s + g, nd) : u32x4{0, 0, 0, 0};
+  const float qx = EXTRA && p.axes ? p.xy[(long)r * p.axes] : 0.f, qy = EXTRA && p.axes > 1 ? p.xy[(long)r * p.axes + 1] : 0.f;
+  const float slope = EXTRA && p.axes && mine ? p.slopes[head] : 0.f, icap = EXTRA && p.cap > 0.f ? p.scale / p.cap : 0.f, c2 = p.scale * LOG2E;
+
+  f32x4 acc[1][G::DF];
+#pragma unroll
+  for (int d = 0; d < G::DF; ++d) acc[0][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+  float m = -INFINITY, l = 0.f;
+  auto fetch = [&](int k0, int buf) {
+    copy_tile<G, 64>((const T*)p.k + hk * p.k_head, p.k_row, k0, lo, hi, nd, tiles[wave][buf][0]);
+    copy_tile<G, 64>((const T*)p.v + hk * p.v_head, p.v_row, k0, lo, hi, nd, tiles[wave][buf][1]);
+  };
+  int buf = 0;
+  const int first = lo + wave * G::BK;
+  if (first < hi) fetch(first, 0);
+  for (int k0 = first; k0 < hi; k0 += 4 * G::BK, buf ^= 1) {
+    if (k0 + 4 * G::BK < hi) {
+      fetch(k0 + 4 * G::BK, buf ^ 1);
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LOADS) : "memory");  // (copies end in their order: this tile's have)
+    } else {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    }
+    f32x4 s[1][G::F];
+    scores<G, 1>(tiles[wave][buf][0], q, s, lane);
+    float t = -INFINITY;
+#pragma unroll
+    for (int f = 0; f < G::F; ++f)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int key = k0 + G::row4(f, g) + e;
+        float x = s[0][f][e];
+        if (EXTRA) {
+          x = p.cap > 0.f ? p.cap * blk_tanh<T>(x * icap) : x * p.scale;
+          if (p.axes) {
+            const long at = (long)min(key, p.M - 1) * p.axes;
+            x = fmaf(-slope, blk_dist(p.axes, qx, qy, p.kv_xy[at], p.axes > 1 ? p.kv_xy[at + 1] : 0.f), x);
+          }
+        } else if (W::NATURAL) {
+          x *= p.scale;
+        }
+        x = key < hi ? x : -INFINITY;
+        s[0][f][e] = x;
+        t = fmaxf(t, x);
+      }
+    t = quarters_max(t) * (W::NATURAL ? 1.f : c2);
+    if (__ballot(t > m)) {
+      const float mn = fmaxf(m, t), al = __builtin_amdgcn_exp2f(mn == -INFINITY ? 0.f : (m - mn) * (W::NATURAL ? LOG2E : 1.f));
+      m = mn;
+      l *= al;
+#pragma unroll
+      for (int d = 0; d < G::DF; ++d) acc[0][d] *= al;
+    }
+    const float mm = m == -INFINITY ? 0.f : m;
+#pragma unroll
+    for (int f = 0; f < G::F; ++f)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        s[0][f][e] = W::weight(s[0][f][e], mm, c2);
+        l += s[0][f][e];
+      }
+    accumulate<G, 1>(tiles[wave][buf][1], s, acc, lane);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (this tile is read before the next copy goes into it)
+  }
+  l = quarters_sum(l);
+
+  // the four waves' results, joined by wave 0 .. 3 in turn order
+  __syncthreads();
+  float* sm = (float*)&tiles[0][0][0][0];  // [wave][16 heads][m, l], then [wave][DP][16 heads]
+  if (g == 0) sm[wave * 32 + i16] = m, sm[wave * 32 + 16 + i16] = l;
+  float* so = sm + 128 + wave * DP * 16;
+#pragma unroll
+  for (int d = 0; d < G::DF; ++d)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) so[(32 * (d >> 1) + 8 * g + 4 * (d & 1) + e) * 16 + i16] = acc[0][d][e];
+  __syncthreads();
+  const int heads = min(16, group - hg * 16);
+  for (int i = threadIdx.x; i < heads * p.D; i += 256) {
+    const int d = i % p.D, hh = i / p.D;
+    float mt = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) mt = fmaxf(mt, sm[w * 32 + hh]);
+    float lt = 0.f, o = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float mw = sm[w * 32 + hh], f = __builtin_amdgcn_exp2f(mt == -INFINITY ? 0.f : (mw - mt) * (W::NATURAL ? LOG2E : 1.f));
+      lt = fmaf(f, sm[w * 32 + 16 + hh], lt);
+      o = fmaf(f, sm[128 + (w * DP + d) * 16 + hh], o);
+    }
+    const int h = hk * group + hg * 16 + hh;
+    if (splits > 1) {
+      float* out = part + (((long)r * p.H + h) * splits + sp) * (p.D + 4);
+      out[d] = o;
+      if (d == 0) out[p.D] = mt, out[p.D + 1] = lt, out[p.D + 2] = n > 0 ? 1.f : 0.f;
+    } else {
+      const float inv = n > 0 ? 1.f / lt : 0.f;
+      ((T*)p.out)[((long)r * p.H + h) * p.D + d] = (T)(o * inv);
+    }
+  }
+}
+
+template <class T, bool NATURAL>
+__global__ __launch_bounds__(128) void blk_attn_join_kernel(BlkAttnArgs p, int splits, const float* part) {
+  const int d = threadIdx.x;
+  const float* in = part + (long)blockIdx.x * splits * (p.D + 4);
+  float mt = -INFINITY;
+  for (int s = 0; s < splits; ++s) mt = fmaxf(mt, in[(long)s * (p.D + 4) + p.D]);
+  float lt = 0.f, o = 0.f;
+  for (int s = 0; s < splits; ++s) {
+    const float* x = in + (long)s * (p.D + 4);
+    const float f = __builtin_amdgcn_exp2f(mt == -INFINITY ? 0.f : (x[p.D] - mt) * (NATURAL ? LOG2E : 1.f));
+    lt = fmaf(f, x[p.D + 1], lt);
+    if (d < p.D) o = fmaf(f, x[d], o);
+  }
+  const float inv = in[p.D + 2] != 0.f ? 1.f / lt : 0.f;
+  if (d < p.D) ((T*)p.out)[(long)blockIdx.x * p.D + d] = (T)(o * inv);
+}
+
+// Single rows over long caches (no gradient kept): how many shares of the keys; 0 where the tile kernel runs instead.
+int row_splits(const BlkAttnArgs& p) {
+  if (p.lse || p.S == 0 || p.N > 2L * p.S || p.M / p.S < 64) return 0;
+  const long blocks = (long)p.N * p.Hkv * cdiv(p.H / p.Hkv, 16);
+  long n = cdiv(1024, blocks);
+  if (n > p.M / p.S / 128) n = p.M / p.S / 128;
+  return n < 1 ? 1 : n > 64 ? 64 : (int)n;
 }
 
 template <class T, int DP>
 void launch_fwd(const BlkAttnArgs& p, hipStream_t st) {
-  const int np = cdiv(p.N, 128) * 128;
   const bool extra = p.cap > 0.f || p.axes > 0;
+  const int splits = row_splits(p);
+  if (splits) {
+    const int hgroups = cdiv(p.H / p.Hkv, 16);
+    const dim3 grid((unsigned)((long)p.N * p.Hkv * hgroups * splits));
+    if (extra)
+      MG_LAUNCH((blk_attn_row_kernel<T, DP, true>), grid, dim3(256), 0, st, p, splits, hgroups, (float*)p.ws);
+    else
+      MG_LAUNCH((blk_attn_row_kernel<T, DP, false>), grid, dim3(256), 0, st, p, splits, hgroups, (float*)p.ws);
+    if (splits > 1) {
+      if (extra || sizeof(T) == 4)
+        MG_LAUNCH((blk_attn_join_kernel<T, true>), dim3(p.N * p.H), dim3(128), 0, st, p, splits, (const float*)p.ws);
+      else
+        MG_LAUNCH((blk_attn_join_kernel<T, false>), dim3(p.N * p.H), dim3(128), 0, st, p, splits, (const float*)p.ws);
+    }
+    return;
+  }
+  const int np = cdiv(p.N, 128) * 128;
+  MG_LAUNCH(blk_spans_kernel, dim3(np / 64), dim3(256), 0, st, p, np);
   const bool wide = (long)cdiv(p.N, 128) * p.H >= 256;  // enough workgroups of 128 rows to fill the chip
   const dim3 grid(cdiv(p.N, wide ? 128 : 64) * p.H);
   if (wide) {
@@ -222,6 +413,11 @@ void launch_fwd_width(const BlkAttnArgs& p, hipStream_t st) {
     launch_fwd<T, 96>(p, st);
   else
     launch_fwd<T, 128>(p, st);
+}
+
+size_t fwd_workspace(const BlkAttnArgs& p) {
+  const int splits = row_splits(p);
+  return splits > 1 ? (size_t)p.N * p.H * splits * (p.D + 4) * 4 : 0;
 }
 
 }  // namespace
@@ -250,13 +446,19 @@ size_t mggan_block_attention_span_ints(int rows) {
   return 2 * np + np / 8;
 }
 
+size_t mggan_block_attention_fwd_workspace(int rows, int keys, int heads, int kv_heads, int width, int scenes) {
+  BlkAttnArgs p = {};
+  p.N = rows, p.M = keys, p.H = heads, p.Hkv = kv_heads, p.D = width, p.S = scenes;
+  return rows > 0 && heads > 0 && kv_heads > 0 && width > 0 && scenes > 0 ? fwd_workspace(p) : 0;
+}
+
 int mggan_block_attention_fwd(const void* args, hipStream_t stream) {
   const BlkAttnArgs* a = (const BlkAttnArgs*)args;
   const int rc = blk_attn_check(a, "block_attention_fwd");
   if (rc != MGGAN_OK) return rc;
   MG_CHECK_ARG(a->out && (size_t)a->out % 16 == 0 && (size_t)a->spans % 16 == 0, "block_attention_fwd: output or spans null or unaligned");
-  const int np = cdiv(a->N, 128) * 128;
-  MG_LAUNCH(blk_spans_kernel, dim3(np / 64), dim3(256), 0, stream, *a, np);
+  const size_t need = fwd_workspace(*a);
+  MG_CHECK_ARG(!need || (a->ws && (size_t)a->ws_bytes >= need), "block_attention_fwd: workspace of %zu bytes (got %ld)", need, a->ws_bytes);
   if (a->dtype == BLK_BF16)
     launch_fwd_width<bf16>(*a, stream);
   else

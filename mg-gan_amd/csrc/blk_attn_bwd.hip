@@ -1,6 +1,6 @@
 // Attention over the rows of scenes, backward.  Two kernels and no atomics: one owns queries (dQ, the rows' sum(dO O), the slopes'
 // gradient), one owns keys (dK, dV, summed over the heads that share them); both form the scores again from the operands and the kept
-// softmax denominators.  With P and D = sum(dO O):
+// softmax statistics.  With P and D = sum(dO O):
 //   dV = P^T dO      dL = P (dO V^T - D)      dslope = -sum dL |xy - kv_xy|      dS = dL (1 - tanh^2)      dQ = scale dS K      dK = scale dS^T Q
 // P and dS are rounded to the operands' type where they enter a product, as every operand is.
 #include <limits.h>
@@ -11,22 +11,22 @@ int blk_attn_check(const BlkAttnArgs* a, const char* name);
 
 namespace {
 
-// One score and what its gradient needs: x = log2 of the unnormalised weight, fac = d(capped score)/d(score).
+// One score and what its gradient needs: fac = d(capped score)/d(score).
 template <class T>
-__device__ __forceinline__ void extra_score(float& x, float& fac, float& dist, const BlkAttnArgs& p, float icap, float c2, float slope2, float ax,
-                                            float ay, float bx, float by) {
+__device__ __forceinline__ void extra_score(float& x, float& fac, float& dist, const BlkAttnArgs& p, float icap, float slope, float ax, float ay,
+                                            float bx, float by) {
   fac = 1.f;
   if (p.cap > 0.f) {
     const float t = blk_tanh<T>(x * icap);
     fac = fmaf(-t, t, 1.f);
-    x = p.cap * LOG2E * t;
+    x = p.cap * t;
   } else {
-    x *= c2;
+    x *= p.scale;
   }
   dist = 0.f;
   if (p.axes) {
     dist = blk_dist(p.axes, ax, ay, bx, by);
-    x = fmaf(-slope2, dist, x);
+    x = fmaf(-slope, dist, x);
   }
 }
 
@@ -49,7 +49,7 @@ __global__ __launch_bounds__(256) void blk_attn_dq_kernel(BlkAttnArgs p, int np,
     ghi = max(ghi, s.y);
   }
   int lo[QF], hi[QF], wlo = INT_MAX, whi = 0, flo = 0, fhi = INT_MAX;
-  float qx[QF], qy[QF], lse[QF], dsum[QF];
+  float qx[QF], qy[QF], top[QF], inv[QF], dsum[QF];
   u32x4 q[QF][G::SK], dO[QF][G::SK];
 #pragma unroll
   for (int j = 0; j < QF; ++j) {
@@ -66,19 +66,20 @@ __global__ __launch_bounds__(256) void blk_attn_dq_kernel(BlkAttnArgs p, int np,
     for (int s = 0; s < G::SK; ++s) {
       q[j][s] = owner_chunk(row, 4 * s + g, nd);
       dO[j][s] = owner_chunk((const T*)p.dout + at, 4 * s + g, nd);
-      const u32x4 o = owner_chunk((const T*)p.out + at, 4 * s + g, nd);
-      if constexpr (sizeof(T) == 2) {
-        const bf16x8 a = __builtin_bit_cast(bf16x8, o), b = __builtin_bit_cast(bf16x8, dO[j][s]);
+      const float* o = p.out32 + at + (4 * s + g) * G::CH;
+      if (4 * s + g < nd) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) d = fmaf((float)a[e], (float)b[e], d);
-      } else {
-        const f32x4 a = __builtin_bit_cast(f32x4, o), b = __builtin_bit_cast(f32x4, dO[j][s]);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) d = fmaf(a[e], b[e], d);
+        for (int e = 0; e < G::CH; ++e) {
+          if constexpr (sizeof(T) == 2)
+            d = fmaf(o[e], (float)__builtin_bit_cast(bf16x8, dO[j][s])[e], d);
+          else
+            d = fmaf(o[e], __builtin_bit_cast(f32x4, dO[j][s])[e], d);
+        }
       }
     }
     dsum[j] = quarters_sum(d);
-    lse[j] = p.lse[(long)h * p.N + rc];
+    top[j] = p.lse[(long)h * p.N + rc];
+    inv[j] = p.lse[(long)(p.H + h) * p.N + rc];
     if (r < p.N && g == 0) delta[(long)h * p.N + r] = dsum[j];
     if (EXTRA && p.axes) {
       qx[j] = p.xy[(long)rc * p.axes];
@@ -98,8 +99,8 @@ __global__ __launch_bounds__(256) void blk_attn_dq_kernel(BlkAttnArgs p, int np,
   const T* kb = (const T*)p.k + hk * p.k_head;
   const T* vb = (const T*)p.v + hk * p.v_head;
   auto fetch = [&](int k0, int buf) {
-    copy_tile<T, DP>(kb, p.k_row, k0, glo, ghi, nd, lk[buf]);
-    copy_tile<T, DP>(vb, p.v_row, k0, glo, ghi, nd, lv[buf]);
+    copy_tile<G>(kb, p.k_row, k0, glo, ghi, nd, lk[buf]);
+    copy_tile<G>(vb, p.v_row, k0, glo, ghi, nd, lv[buf]);
     if (EXTRA && wave < p.axes) copy_meta(p.kv_xy, p.axes, wave, k0, p.M, lx[buf][wave]);
   };
 
@@ -108,8 +109,11 @@ __global__ __launch_bounds__(256) void blk_attn_dq_kernel(BlkAttnArgs p, int np,
   for (int j = 0; j < QF; ++j)
 #pragma unroll
     for (int d = 0; d < G::DF; ++d) acc[j][d] = f32x4{0.f, 0.f, 0.f, 0.f};
-  float slope_sum = 0.f;
-  const float c2 = p.scale * LOG2E, slope2 = EXTRA && p.axes ? p.slopes[h] * LOG2E : 0.f, icap = EXTRA && p.cap > 0.f ? p.scale / p.cap : 0.f;
+  // the slopes' gradient is f32 and a sum over all pairs, so it takes the rows' sum(P dO V^T) from the same P: -sum (P dP dist) + sum(P dP)
+  // sum(P dist) row by row, with nothing in it that was rounded to the operands' type
+  float sa[QF] = {}, sb[QF] = {}, sc[QF] = {};
+  using W = Soft<T, EXTRA>;
+  const float c2 = p.scale * LOG2E, slope = EXTRA && p.axes ? p.slopes[h] : 0.f, icap = EXTRA && p.cap > 0.f ? p.scale / p.cap : 0.f;
 
   if (glo < ghi) fetch(glo, 0);
   int buf = 0;
@@ -118,10 +122,10 @@ __global__ __launch_bounds__(256) void blk_attn_dq_kernel(BlkAttnArgs p, int np,
     if (k0 + G::BK < ghi) fetch(k0 + G::BK, buf ^ 1);
     if (k0 >= whi || k0 + G::BK <= wlo) continue;
     f32x4 s[QF][G::F], dp[QF][G::F];
-    scores<T, DP, QF>(lk[buf], q, s, lane);
-    scores<T, DP, QF>(lv[buf], dO, dp, lane);
+    scores<G, QF>(lk[buf], q, s, lane);
+    scores<G, QF>(lv[buf], dO, dp, lane);
     const bool part = k0 < flo || k0 + G::BK > fhi;
-    float tile_sum = 0.f;
+    float ta[QF] = {}, tb[QF] = {}, tc[QF] = {};
 #pragma unroll
     for (int f = 0; f < G::F; ++f) {
       const int kr = G::row4(f, g);
@@ -132,32 +136,41 @@ __global__ __launch_bounds__(256) void blk_attn_dq_kernel(BlkAttnArgs p, int np,
         for (int j = 0; j < QF; ++j) {
           float x = s[j][f][r], fac = 1.f, dist = 0.f, w, dl;
           if (EXTRA) {
-            extra_score<T>(x, fac, dist, p, icap, c2, slope2, qx[j], qy[j], bx, by);
-            w = __builtin_amdgcn_exp2f(x - lse[j]);
-          } else {
-            w = __builtin_amdgcn_exp2f(fmaf(x, c2, -lse[j]));
+            extra_score<T>(x, fac, dist, p, icap, slope, qx[j], qy[j], bx, by);
+          } else if (W::NATURAL) {
+            x *= p.scale;
           }
+          w = W::weight(x, top[j], c2) * inv[j];
           dl = w * (dp[j][f][r] - dsum[j]);
+          if (EXTRA) dl *= fac;
+          float wd = w * dp[j][f][r];
           if (part) {
             const int key = k0 + kr + r;
             const bool seen = key >= lo[j] && key < hi[j];
             dl = seen ? dl : 0.f;
-            dist = seen ? dist : 0.f;
-            fac = seen ? fac : 0.f;
+            if (EXTRA) {
+              w = seen ? w : 0.f;
+              wd = seen ? wd : 0.f;
+              dist = seen ? dist : 0.f;
+            }
           }
-          if (EXTRA) {
-            tile_sum = fmaf(dl, dist, tile_sum);
-            dl *= fac;
+          if (EXTRA && p.dslopes) {
+            ta[j] = fmaf(wd, dist, ta[j]);
+            tb[j] = fmaf(w, dist, tb[j]);
+            tc[j] += wd;
           }
           s[j][f][r] = dl;
         }
       }
     }
-    slope_sum += tile_sum;
-    if (part && tile_not_finite<T, DP>(lk[buf], lane))
-      accumulate_seen<T, DP, QF>(lk[buf], s, acc, lane, [&](int j, int row) { return k0 + row >= lo[j] && k0 + row < hi[j]; });
+    if (EXTRA && p.dslopes) {
+#pragma unroll
+      for (int j = 0; j < QF; ++j) sa[j] += ta[j], sb[j] += tb[j], sc[j] += tc[j];
+    }
+    if (part && tile_not_finite<G>(lk[buf], lane))
+      accumulate_seen<G, QF>(lk[buf], s, acc, lane, [&](int j, int row) { return k0 + row >= lo[j] && k0 + row < hi[j]; });
     else
-      accumulate<T, DP, QF>(lk[buf], s, acc, lane);
+      accumulate<G, QF>(lk[buf], s, acc, lane);
   }
 
 #pragma unroll
@@ -170,6 +183,12 @@ __global__ __launch_bounds__(256) void blk_attn_dq_kernel(BlkAttnArgs p, int np,
       if (16 * d + 8 * g < p.D) store_pair<T>(out + 16 * d + 8 * g, acc[j][d], acc[j][d + 1], p.scale);
   }
   if (EXTRA && p.dslopes) {
+    float slope_sum = 0.f;
+#pragma unroll
+    for (int j = 0; j < QF; ++j) {
+      const float a = quarters_sum(sa[j]), b = quarters_sum(sb[j]), c = quarters_sum(sc[j]);
+      if (g == 0 && w0 + 16 * j + i16 < p.N) slope_sum += fmaf(-c, b, a);
+    }
     __syncthreads();
     const float w = wave_sum(slope_sum);
     if (lane == 0) lx[0][0][wave] = w;
@@ -193,7 +212,7 @@ template <class T, int DP, int QF, bool EXTRA>
 __global__ __launch_bounds__(256) void blk_attn_dkv_kernel(BlkAttnArgs p, int np, const float* delta) {
   using G = Geo<T, DP>;
   __shared__ u32x4 lq[2][G::TILE], lo_[2][G::TILE];
-  __shared__ __attribute__((aligned(16))) float lm[2][6][64];  // of each streamed row: lse, sum(dO O), lo, hi, x, y
+  __shared__ __attribute__((aligned(16))) float lm[2][7][64];  // of each streamed row: largest score, sum(dO O), lo, hi, x, y, 1 / sum
   __shared__ int range[2];
   const int lane = mg_lane(), wave = mg_wave(), i16 = lane & 15, g = lane >> 4;
   const int hk = blockIdx.x % p.Hkv, kt = blockIdx.x / p.Hkv, group = p.H / p.Hkv;
@@ -236,15 +255,17 @@ __global__ __launch_bounds__(256) void blk_attn_dkv_kernel(BlkAttnArgs p, int np
   for (int j = 0; j < QF; ++j)
 #pragma unroll
     for (int d = 0; d < G::DF; ++d) dk[j][d] = dv[j][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+  using W = Soft<T, EXTRA>;
   const float c2 = p.scale * LOG2E, icap = EXTRA && p.cap > 0.f ? p.scale / p.cap : 0.f;
 
   // (head, tile) pairs in one sequence, so that the copies of the next head's first tile are under way too
   const int nt = qb > qa ? (qb - qa + G::BK - 1) / G::BK : 0, total = nt * group;
   auto fetch = [&](int t, int buf) {
     const int h = hk * group + t / nt, q0 = qa + t % nt * G::BK;
-    copy_tile<T, DP>((const T*)p.q + h * p.q_head, p.q_row, q0, 0, p.N, nd, lq[buf]);
-    copy_tile<T, DP>((const T*)p.dout + (long)h * p.D, (long)p.H * p.D, q0, 0, p.N, nd, lo_[buf]);
+    copy_tile<G>((const T*)p.q + h * p.q_head, p.q_row, q0, 0, p.N, nd, lq[buf]);
+    copy_tile<G>((const T*)p.dout + (long)h * p.D, (long)p.H * p.D, q0, 0, p.N, nd, lo_[buf]);
     if (wave == 0) copy_meta(p.lse + (long)h * p.N, 1, 0, q0, p.N, lm[buf][0]);
+    if (wave == 3) copy_meta(p.lse + (long)(p.H + h) * p.N, 1, 0, q0, p.N, lm[buf][6]);
     if (wave == 1) copy_meta(delta + (long)h * p.N, 1, 0, q0, p.N, lm[buf][1]);
     if (wave == 2) copy_meta(p.spans, 1, 0, q0, np, lm[buf][2]);
     if (wave == 3) copy_meta(p.spans + np, 1, 0, q0, np, lm[buf][3]);
@@ -263,14 +284,14 @@ __global__ __launch_bounds__(256) void blk_attn_dkv_kernel(BlkAttnArgs p, int np
     }
     if (slo >= w0 + 16 * QF || shi <= w0) continue;
     const bool part = w0 < flo || w0 + 16 * QF > fhi;
-    const float slope2 = EXTRA && p.axes ? p.slopes[h] * LOG2E : 0.f;
+    const float slope = EXTRA && p.axes ? p.slopes[h] : 0.f;
     f32x4 s[QF][G::F], dp[QF][G::F];
-    scores<T, DP, QF>(lq[buf], k, s, lane);
-    scores<T, DP, QF>(lo_[buf], v, dp, lane);
+    scores<G, QF>(lq[buf], k, s, lane);
+    scores<G, QF>(lo_[buf], v, dp, lane);
 #pragma unroll
     for (int f = 0; f < G::F; ++f) {
       const int qr = G::row4(f, g);
-      const f32x4 lse = *(const f32x4*)&lm[buf][0][qr], dsum = *(const f32x4*)&lm[buf][1][qr];
+      const f32x4 top = *(const f32x4*)&lm[buf][0][qr], dsum = *(const f32x4*)&lm[buf][1][qr], inv = *(const f32x4*)&lm[buf][6][qr];
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const float ax = EXTRA && p.axes ? lm[buf][4][qr + r] : 0.f, ay = EXTRA && p.axes > 1 ? lm[buf][5][qr + r] : 0.f;
@@ -278,11 +299,11 @@ __global__ __launch_bounds__(256) void blk_attn_dkv_kernel(BlkAttnArgs p, int np
         for (int j = 0; j < QF; ++j) {
           float x = s[j][f][r], fac = 1.f, dist, w, dl;
           if (EXTRA) {
-            extra_score<T>(x, fac, dist, p, icap, c2, slope2, ax, ay, kx[j], ky[j]);
-            w = __builtin_amdgcn_exp2f(x - lse[r]);
-          } else {
-            w = __builtin_amdgcn_exp2f(fmaf(x, c2, -lse[r]));
+            extra_score<T>(x, fac, dist, p, icap, slope, ax, ay, kx[j], ky[j]);
+          } else if (W::NATURAL) {
+            x *= p.scale;
           }
+          w = W::weight(x, top[r], c2) * inv[r];
           dl = w * (dp[j][f][r] - dsum[r]);
           if (EXTRA) dl *= fac;
           if (part) {
@@ -300,12 +321,12 @@ __global__ __launch_bounds__(256) void blk_attn_dkv_kernel(BlkAttnArgs p, int np
       const int key = w0 + 16 * j + i16;
       return key >= __float_as_int(lm[buf][2][row]) && key < __float_as_int(lm[buf][3][row]);
     };
-    if (part && (tile_not_finite<T, DP>(lo_[buf], lane) || tile_not_finite<T, DP>(lq[buf], lane))) {
-      accumulate_seen<T, DP, QF>(lo_[buf], s, dv, lane, sees);
-      accumulate_seen<T, DP, QF>(lq[buf], dp, dk, lane, sees);
+    if (part && (tile_not_finite<G>(lo_[buf], lane) || tile_not_finite<G>(lq[buf], lane))) {
+      accumulate_seen<G, QF>(lo_[buf], s, dv, lane, sees);
+      accumulate_seen<G, QF>(lq[buf], dp, dk, lane, sees);
     } else {
-      accumulate<T, DP, QF>(lo_[buf], s, dv, lane);
-      accumulate<T, DP, QF>(lq[buf], dp, dk, lane);
+      accumulate<G, QF>(lo_[buf], s, dv, lane);
+      accumulate<G, QF>(lq[buf], dp, dk, lane);
     }
   }
 #pragma unroll
@@ -362,8 +383,8 @@ int mggan_block_attention_bwd(const void* args, hipStream_t stream) {
   const BlkAttnArgs* a = (const BlkAttnArgs*)args;
   const int rc = blk_attn_check(a, "block_attention_bwd");
   if (rc != MGGAN_OK) return rc;
-  MG_CHECK_ARG(a->out && a->lse && a->dout && a->dq && a->dk && a->dv, "block_attention_bwd: null operand");
-  MG_CHECK_ARG(((size_t)a->out | (size_t)a->dout | (size_t)a->dq | (size_t)a->dk | (size_t)a->dv | (size_t)a->spans) % 16 == 0,
+  MG_CHECK_ARG(a->out32 && a->lse && a->dout && a->dq && a->dk && a->dv, "block_attention_bwd: null operand");
+  MG_CHECK_ARG(((size_t)a->out32 | (size_t)a->dout | (size_t)a->dq | (size_t)a->dk | (size_t)a->dv | (size_t)a->spans) % 16 == 0,
                "block_attention_bwd: operands have to be 16-byte aligned");
   const size_t need = mggan_block_attention_bwd_workspace(a->N, a->H);
   MG_CHECK_ARG(a->ws && (size_t)a->ws_bytes >= need, "block_attention_bwd: workspace of %zu bytes (got %ld)", need, a->ws_bytes);

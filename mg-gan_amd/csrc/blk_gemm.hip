@@ -21,8 +21,8 @@ struct GemmP {
   int tiles_m, tiles_n, kt_split;
   void* C;
   long ldc;
-  void* Z;   // inputs of the activation, kept for the backward pass (or null)
-  void* Z2;
+  float* Z;  // inputs of the activation, kept for the backward pass (or null) in f32: rounded to bf16 they would put a second
+  float* Z2; // half step next to dZ's own into every gradient
   const void* bias;
   const void* bias2;
   const void* res;  // (M, N) contiguous
@@ -89,8 +89,8 @@ __device__ __forceinline__ void epilogue8(const GemmP& p, int m, int n, float (&
 #pragma unroll
     for (int i = 0; i < 8; ++i) u[i] += t[i];
   }
-  if (p.Z) store8<T>((T*)p.Z + at, vec, left, v);
-  if (EPI == EPI_GATED && p.Z2) store8<T>((T*)p.Z2 + at, vec, left, u);
+  if (p.Z) store8<float>(p.Z + at, vec, left, v);
+  if (EPI == EPI_GATED && p.Z2) store8<float>(p.Z2 + at, vec, left, u);
   if (p.act != ACT_NONE) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = blk_act(v[i], p.act, p.slope);
@@ -284,8 +284,8 @@ __global__ __launch_bounds__(256) void blk_transpose_kernel(const T* in, long ld
 // type once: it is an operand of both products, and half a step is what every operand has.
 struct DzP {
   const void* dY;
-  const void* Z;
-  const void* Z2;
+  const float* Z;
+  const float* Z2;
   void* dZ;
   void* dZt;
   float* sums;  // (tiles of rows, N or 2 N)
@@ -308,11 +308,11 @@ __global__ __launch_bounds__(256) void blk_dz_kernel(DzP p) {
       const long at = (long)m * p.N + n;
       const float dy = (float)((const T*)p.dY)[at];
       if (GATED) {
-        const float z = (float)((const T*)p.Z)[at], u = (float)((const T*)p.Z2)[at];
+        const float z = p.Z[at], u = p.Z2[at];
         a = dy * u * blk_act_grad(z, p.act, p.slope);
         b = dy * blk_act(z, p.act, p.slope);
       } else {
-        a = p.Z ? dy * blk_act_grad((float)((const T*)p.Z)[at], p.act, p.slope) : dy;
+        a = p.Z ? dy * blk_act_grad(p.Z[at], p.act, p.slope) : dy;
       }
     }
     s0 += a;
@@ -434,7 +434,8 @@ void transpose(const void* in, long ldi, void* out, long ldo, int rows, int cols
 struct LayerP {
   const void *x, *w, *w2, *b, *b2, *res, *dy;
   long ldx;
-  void *y, *z, *z2, *dx, *dw, *db;
+  float *z, *z2;
+  void *y, *dx, *dw, *db;
   int M, K, N, act;
   float slope;
 };
@@ -545,7 +546,7 @@ size_t mggan_block_layer_workspace(int rows, int K, int N, int gated, int backwa
   return need;
 }
 
-int mggan_block_linear_fwd(const void* x, long ldx, const void* w, const void* bias, const void* residual, void* y, void* z, int rows, int K,
+int mggan_block_linear_fwd(const void* x, long ldx, const void* w, const void* bias, const void* residual, void* y, float* z, int rows, int K,
                            int N, int act, float slope, int dtype, void* ws, size_t ws_bytes, hipStream_t stream) {
   LayerP l = {};
   l.x = x, l.ldx = ldx, l.w = w, l.b = bias, l.res = residual, l.y = y, l.z = z, l.M = rows, l.K = K, l.N = N, l.act = act, l.slope = slope;
@@ -555,10 +556,10 @@ int mggan_block_linear_fwd(const void* x, long ldx, const void* w, const void* b
   return layer(l, false, false, dtype, ws, nullptr, stream);
 }
 
-int mggan_block_linear_bwd(const void* dy, const void* z, const void* x, long ldx, const void* w, void* dx, void* dw, void* db, int rows, int K,
+int mggan_block_linear_bwd(const void* dy, const float* z, const void* x, long ldx, const void* w, void* dx, void* dw, void* db, int rows, int K,
                            int N, int act, float slope, int dtype, void* ws, size_t ws_bytes, hipStream_t stream) {
   LayerP l = {};
-  l.dy = dy, l.z = (void*)z, l.x = x, l.ldx = ldx, l.w = w, l.dx = dx, l.dw = dw, l.db = db, l.M = rows, l.K = K, l.N = N, l.act = act,
+  l.dy = dy, l.z = (float*)z, l.x = x, l.ldx = ldx, l.w = w, l.dx = dx, l.dw = dw, l.db = db, l.M = rows, l.K = K, l.N = N, l.act = act,
   l.slope = slope;
   const int rc = check("block_linear_bwd", l, dtype, ws, ws_bytes, false, true);
   if (rc != MGGAN_OK) return rc;
@@ -566,8 +567,8 @@ int mggan_block_linear_bwd(const void* dy, const void* z, const void* x, long ld
   return layer(l, false, true, dtype, ws, nullptr, stream);
 }
 
-int mggan_block_gated_fwd(const void* x, long ldx, const void* w_gate, const void* w_up, const void* b_gate, const void* b_up, void* y, void* z_gate,
-                          void* z_up, int rows, int K, int N, int act, float slope, int dtype, void* ws, size_t ws_bytes, hipStream_t stream) {
+int mggan_block_gated_fwd(const void* x, long ldx, const void* w_gate, const void* w_up, const void* b_gate, const void* b_up, void* y, float* z_gate,
+                          float* z_up, int rows, int K, int N, int act, float slope, int dtype, void* ws, size_t ws_bytes, hipStream_t stream) {
   LayerP l = {};
   l.x = x, l.ldx = ldx, l.w = w_gate, l.w2 = w_up, l.b = b_gate, l.b2 = b_up, l.y = y, l.z = z_gate, l.z2 = z_up, l.M = rows, l.K = K, l.N = N;
   l.act = act, l.slope = slope;
@@ -577,11 +578,11 @@ int mggan_block_gated_fwd(const void* x, long ldx, const void* w_gate, const voi
   return layer(l, true, false, dtype, ws, nullptr, stream);
 }
 
-int mggan_block_gated_bwd(const void* dy, const void* z_gate, const void* z_up, const void* x, long ldx, const void* w_gate, const void* w_up,
+int mggan_block_gated_bwd(const void* dy, const float* z_gate, const float* z_up, const void* x, long ldx, const void* w_gate, const void* w_up,
                           void* dx, void* dw, void* db, int rows, int K, int N, int act, float slope, int dtype, void* ws, size_t ws_bytes,
                           hipStream_t stream) {
   LayerP l = {};
-  l.dy = dy, l.z = (void*)z_gate, l.z2 = (void*)z_up, l.x = x, l.ldx = ldx, l.w = w_gate, l.w2 = w_up, l.dx = dx, l.dw = dw, l.db = db;
+  l.dy = dy, l.z = (float*)z_gate, l.z2 = (float*)z_up, l.x = x, l.ldx = ldx, l.w = w_gate, l.w2 = w_up, l.dx = dx, l.dw = dw, l.db = db;
   l.M = rows, l.K = K, l.N = N, l.act = act, l.slope = slope;
   const int rc = check("block_gated_bwd", l, dtype, ws, ws_bytes, true, true);
   if (rc != MGGAN_OK) return rc;

@@ -81,7 +81,7 @@ def _linear_fwd(x, weight, bias, residual, act, slope, keep):
     (x, ldx), weight, bias, residual = _rows(x), weight.contiguous(), _aligned(bias), _aligned(residual)
     (M, K), N = x.shape, weight.shape[0]
     y = torch.empty(M, N, dtype=x.dtype, device=x.device)
-    z = torch.empty_like(y) if keep and act != ACT_NONE else None
+    z = torch.empty(M, N, dtype=torch.float32, device=x.device) if keep and act != ACT_NONE else None
     if M:
         ws, n = _workspace(x, M, K, N, 0, 0)
         lib.mggan_block_linear_fwd(_p(x), ldx, _p(weight), _p(bias), _p(residual), _p(y), _p(z), M, K, N, act, float(slope),
@@ -137,7 +137,7 @@ def _gated_fwd(x, w_gate, w_up, b_gate, b_up, act, slope, keep):
     (x, ldx), w_gate, w_up, b_gate, b_up = _rows(x), w_gate.contiguous(), w_up.contiguous(), _aligned(b_gate), _aligned(b_up)
     (M, K), N = x.shape, w_gate.shape[0]
     y = torch.empty(M, N, dtype=x.dtype, device=x.device)
-    z, u = (torch.empty_like(y), torch.empty_like(y)) if keep else (None, None)
+    z, u = (torch.empty(M, N, dtype=torch.float32, device=x.device) for _ in range(2)) if keep else (None, None)
     if M:
         ws, n = _workspace(x, M, K, N, 1, 0)
         lib.mggan_block_gated_fwd(_p(x), ldx, _p(w_gate), _p(w_up), _p(b_gate), _p(b_up), _p(y), _p(z), _p(u), M, K, N, act, float(slope),
@@ -196,7 +196,7 @@ def gated_linear(x, w_gate, w_up, b_gate=None, b_up=None, act=ACT_SILU, slope=0.
 
 class _AttnArgs(ctypes.Structure):  # mirrors csrc/blk_attn.h: BlkAttnArgs
     _fields_ = ([(n, ctypes.c_void_p) for n in ("q", "k", "v", "dout", "out", "dq", "dk", "dv", "dslopes", "scenes", "kv_scenes", "prefix",
-                                                "xy", "kv_xy", "slopes", "lse", "spans", "ws")]
+                                                "xy", "kv_xy", "slopes", "lse", "out32", "spans", "ws")]
                 + [(n, ctypes.c_long) for n in ("ws_bytes", "q_row", "q_head", "k_row", "k_head", "v_row", "v_head")]
                 + [(n, ctypes.c_int) for n in ("N", "M", "H", "Hkv", "D", "S", "causal", "axes", "dtype")]
                 + [("scale", ctypes.c_float), ("cap", ctypes.c_float)])
@@ -251,11 +251,17 @@ def _attn_args(q, k, v, scenes, kv_scenes, prefix, xy, kv_xy, slopes, causal, sc
 
 def _attn_fwd(a, q, keep):
     out = torch.empty(a.N, a.H, a.D, dtype=q.dtype, device=q.device)
-    lse = torch.empty(a.H, a.N, dtype=torch.float32, device=q.device) if keep else None
+    lse = torch.empty(2, a.H, a.N, dtype=torch.float32, device=q.device) if keep else None
+    out32 = None if not keep else out if q.dtype == torch.float32 else torch.empty(out.shape, dtype=torch.float32, device=q.device)
     spans = torch.empty(lib.mggan_block_attention_span_ints(a.N), dtype=torch.int32, device=q.device)
-    a.out, a.lse, a.spans = _p(out), _p(lse), _p(spans)
+    ws = None
+    if not keep:
+        a.ws_bytes = lib.mggan_block_attention_fwd_workspace(a.N, a.M, a.H, a.Hkv, a.D, a.S)
+        ws = torch.empty(a.ws_bytes // 4, dtype=torch.float32, device=q.device) if a.ws_bytes else None
+        a.ws = _p(ws)
+    a.out, a.lse, a.out32, a.spans = _p(out), _p(lse), _p(out32), _p(spans)
     lib.mggan_block_attention_fwd(ctypes.addressof(a), _s())
-    return out, lse, spans
+    return out, lse, out32, spans
 
 
 class AttentionFn(Function):
@@ -269,8 +275,8 @@ class AttentionFn(Function):
             return torch.zeros(q.shape, dtype=q.dtype, device=q.device)
         ctx.empty = False
         a, (q, k, v) = _attn_args(q, k, v, scenes, kv_scenes, prefix, xy, kv_xy, slopes, causal, scale, cap)
-        out, lse, spans = _attn_fwd(a, q, True)
-        ctx.save_for_backward(q, k, v, slopes, out, lse, spans)
+        out, lse, out32, spans = _attn_fwd(a, q, True)
+        ctx.save_for_backward(q, k, v, slopes, out32, lse, spans)
         return out
 
     @staticmethod
@@ -279,7 +285,7 @@ class AttentionFn(Function):
         scenes, kv_scenes, prefix, xy, kv_xy, causal, scale, cap = ctx.rest
         if ctx.empty:
             return tuple(None if t is None else torch.zeros_like(t) for t in ctx.saved_tensors) + (None,)
-        q, k, v, slopes, out, lse, spans = ctx.saved_tensors
+        q, k, v, slopes, out32, lse, spans = ctx.saved_tensors
         a, _ = _attn_args(q, k, v, scenes, kv_scenes, prefix, xy, kv_xy, slopes, causal, scale, cap)
         dout = _aligned(dout)
         dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
@@ -287,7 +293,7 @@ class AttentionFn(Function):
         dslopes = torch.empty_like(slopes) if slopes is not None and ctx.needs_input_grad[3] else None
         a.ws_bytes = lib.mggan_block_attention_bwd_workspace(a.N, a.H)
         ws = torch.empty(a.ws_bytes // 4, dtype=torch.float32, device=q.device)
-        a.dout, a.out, a.lse, a.spans, a.ws = _p(dout), _p(out), _p(lse), _p(spans), _p(ws)
+        a.dout, a.out32, a.lse, a.spans, a.ws = _p(dout), _p(out32), _p(lse), _p(spans), _p(ws)
         a.dq, a.dk, a.dv, a.dslopes = _p(dq), _p(dk), _p(dv), _p(dslopes)
         lib.mggan_block_attention_bwd(ctypes.addressof(a), _s())
         return dq, dk, dv, dslopes, None
