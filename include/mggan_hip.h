@@ -644,29 +644,20 @@ int mggan_crop_patches(const unsigned char* atlas, const long long* img_off, con
 
 /* ---- transformer block: the layers that are matrix products (mggan/hip/blocks.py; no counterpart in the reference, whose
  * nn.Linear stacks are utils.py:134-149) -------------------------------------------------------------------------------
- * dtype: 0 f32, 1 bf16 -- of every operand and output; sums and activations in f32, one rounding at the end.  act: 0 none,
- * 1 LeakyReLU(slope), 2 sigmoid, 4 SiLU, 5 GELU (exact).  x (rows, K) with row stride ldx (elements), any alignment; weights (N, K)
- * contiguous; everything else contiguous and 16-byte aligned.  `ws`: mggan_block_layer_workspace bytes, 256-byte aligned, free
- * again when the call's work on `stream` is done.  Limits: rows <= 2^21, K, N <= 2^20. */
-size_t mggan_block_layer_workspace(int rows, int K, int N, int gated, int backward, int dtype);
-/* y = act(x W^T + bias) + residual; bias, residual or NULL.  z (or NULL): the activation's input in f32,
- * which the backward pass reads. */
-int mggan_block_linear_fwd(const void* x, long ldx, const void* w, const void* bias, const void* residual, void* y, float* z,
-                           int rows, int K, int N, int act, float slope, int dtype, void* ws, size_t ws_bytes,
-                           mggan_stream_t stream);
-/* dZ = dy act'(z) (z may be NULL for act 0): dx (rows, K) = dZ W, dw (N, K) = dZ^T x, db (N) = column sums; each NULL if not
- * wanted.  Written, not accumulated; fixed order of summation. */
-int mggan_block_linear_bwd(const void* dy, const float* z, const void* x, long ldx, const void* w, void* dx, void* dw, void* db,
-                           int rows, int K, int N, int act, float slope, int dtype, void* ws, size_t ws_bytes,
-                           mggan_stream_t stream);
-/* y = act(x Wg^T + bg) * (x Wu^T + bu); z_gate, z_up (both or neither): the two linear results in f32 for the backward pass. */
-int mggan_block_gated_fwd(const void* x, long ldx, const void* w_gate, const void* w_up, const void* b_gate, const void* b_up,
-                          void* y, float* z_gate, float* z_up, int rows, int K, int N, int act, float slope, int dtype,
-                          void* ws, size_t ws_bytes, mggan_stream_t stream);
-/* dx (rows, K); dw (2 N, K): the gate weight's gradient, then the up weight's; db (2 N) likewise. */
-int mggan_block_gated_bwd(const void* dy, const float* z_gate, const float* z_up, const void* x, long ldx, const void* w_gate,
-                          const void* w_up, void* dx, void* dw, void* db, int rows, int K, int N, int act, float slope,
-                          int dtype, void* ws, size_t ws_bytes, mggan_stream_t stream);
+ * y = act(x w^T + b) + res, or with w2 y = act(x w^T + b) * (x w2^T + b2).  `args`: a host structure
+ *   { const void *x, *w, *w2, *b, *b2, *res, *dy; float *z, *z2; void *y, *dx, *dw, *db, *ws; long ws_bytes, ldx;
+ *     int M, K, N, act, dtype; float slope; }
+ * dtype: 0 f32, 1 bf16 -- of every operand and output but z; sums and activations in f32, one rounding at the end.  act: 0 none,
+ * 1 LeakyReLU(slope), 2 sigmoid, 4 SiLU, 5 GELU (exact).  x (M, K) with row stride ldx (elements), w, w2 (N, K), b, b2 (N), res, dy, y,
+ * z, z2 (M, N) contiguous; b, b2, res NULL for none; 16-byte aligned (with K no multiple of 16 bytes: x, w, w2 in any place).  z, z2: the
+ * activation's input and the up result in f32, written by the forward call if not NULL, read by the backward call (act 0 without w2:
+ * NULL).  Backward: dx (M, K), dw (N, K), db (N), each NULL if not wanted; with w2 dw is (off + N, K), off = N rounded up to 128 bytes of
+ * elements: the gate weight's gradient in rows [0, N), the up weight's from off on; db (2 N).  Written, not accumulated; fixed order of
+ * summation.  ws: mggan_block_layer_workspace bytes, 256-byte aligned, free again when the call's work on `stream` is done.  Limits:
+ * M <= 2^21, K, N <= 2^20. */
+size_t mggan_block_layer_workspace(int rows, int K, int N, int gated, int backward, int act, int dtype);
+int mggan_block_layer_fwd(const void* args, mggan_stream_t stream);
+int mggan_block_layer_bwd(const void* args, mggan_stream_t stream);
 
 /* ---- transformer block: attention over the rows of scenes (mggan/hip/blocks.py: attention) ---------------------------
  * out_i = sum_j P_ij v_j, P_i = softmax over the visible keys j of cap tanh(scale q_i.k_j / cap) - slopes[h] |xy_i - kv_xy_j|.

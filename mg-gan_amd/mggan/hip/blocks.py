@@ -8,8 +8,9 @@ All operands of a call have one type and live on one device; sums, activations a
 rounded once.  Work goes to torch's current stream, outputs and workspaces come from torch's allocator (so a call can be captured
 into a HIP graph), gradients are returned through autograd and are the same bits in every run.  Arguments that do not fit raise
 ValueError, a failing launch raises HipError; there is no CPU path."""
-import ctypes
+import functools
 import math
+import struct
 
 import torch
 from torch.autograd import Function
@@ -21,186 +22,206 @@ from .lib import lib
 ACT_SILU, ACT_GELU = 4, 5
 _ACTS = (ACT_NONE, ACT_LEAKY, ACT_SIGMOID, ACT_SILU, ACT_GELU)
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1}
+_F32 = torch.float32
+
+# The calls' arguments as the C structures of csrc/blk_gemm.hip and csrc/blk_attn.h lay them out, packed in one go (a small call is
+# bound by the host: filling a ctypes structure field by field took 6 us of a 36 us forward call).
+_LAYER = struct.Struct("=14Q2q5if")
+_ATTN = struct.Struct("=19Q7q9i2f4x")
 
 
-def _check(ok, text, *args):
-    if not ok:
-        raise ValueError(text.format(*args))
+@functools.lru_cache(maxsize=1024)
+def _layer_workspace(M, K, N, gated, backward, act, dtype):
+    return lib.mggan_block_layer_workspace(M, K, N, gated, backward, act, dtype)
 
 
-def _same(name, x, **others):
-    """Every operand has x's type and device, and a device this process can launch on."""
-    _check(isinstance(x, torch.Tensor) and x.dtype in _DTYPES, "{}: f32 or bf16 tensors, got {}", name, getattr(x, "dtype", type(x)))
-    for n, t in others.items():
-        if t is not None:
-            _check(isinstance(t, torch.Tensor) and t.dtype == x.dtype, "{}: {} is {}, the first operand is {}", name, n,
-                   getattr(t, "dtype", type(t)), x.dtype)
-            _check(t.device == x.device, "{}: {} is on {}, the first operand on {}", name, n, t.device, x.device)
+@functools.lru_cache(maxsize=1024)
+def _attn_sizes(N, M, H, Hkv, D, S):
+    """(int32 of the row intervals, bytes for splitting the keys of single rows, bytes of the backward pass)"""
+    return (lib.mggan_block_attention_span_ints(N), lib.mggan_block_attention_fwd_workspace(N, M, H, Hkv, D, S),
+            lib.mggan_block_attention_bwd_workspace(N, H))
 
 
-def _on_gpu(name, x):
-    _check(x.is_cuda, "{}: the operands are on {}; there is no CPU path", name, x.device)
+def _bytes(n, like):
+    return torch.empty(n, dtype=torch.uint8, device=like.device) if n else None
+
+
+def _same(name, x, *others):
+    """Every operand has x's type and device."""
+    if x.dtype not in _DTYPES:
+        raise ValueError("{}: f32 or bf16 tensors, got {}".format(name, x.dtype))
+    for t in others:
+        if t is not None and (t.dtype != x.dtype or t.device != x.device):
+            raise ValueError("{}: one operand is {} on {}, the first one {} on {}".format(name, t.dtype, t.device, x.dtype, x.device))
+
+
+def _on_current(name, x):
+    """Whether x lives on the current device (the call is repeated under its own otherwise)."""
+    if not x.is_cuda:
+        raise ValueError("{}: the operands are on {}; there is no CPU path".format(name, x.device))
+    return x.get_device() == torch.cuda.current_device()
 
 
 def _aligned(t):
     """Contiguous and 16-byte aligned (a copy where it is not)."""
     if t is None:
         return None
-    t = t.contiguous()
+    if not t.is_contiguous():
+        t = t.contiguous()
     return t.clone() if t.data_ptr() % 16 else t
 
 
-def _rows(x):
-    """(rows, K) view of x with unit inner stride, and its row stride."""
-    x = x.reshape(-1, x.shape[-1])
-    if x.stride(1) != 1 or (x.shape[0] > 1 and x.stride(0) < x.shape[1]):
-        x = x.contiguous()
-    return x, (x.stride(0) if x.shape[0] > 1 else x.shape[1])
+def _needs_grad(*tensors):
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
-def _workspace(x, rows, K, N, gated, backward):
-    n = lib.mggan_block_layer_workspace(rows, K, N, gated, backward, _DTYPES[x.dtype])
-    return torch.empty(n, dtype=torch.uint8, device=x.device), n
+# ---- layers ------------------------------------------------------------------------------------------------------------------
+
+def _rows(x, K):
+    """x as (rows, K) with unit inner stride, rows that start at multiples of 16 bytes (unless K does not), and its row stride."""
+    if x.dim() != 2:
+        x = x.reshape(-1, K)
+    M, ch = x.shape[0], 16 // x.element_size()
+    ld = x.stride(0) if M > 1 else K
+    if (x.stride(1) != 1 and K > 1) or ld < K:
+        x, ld = x.contiguous(), K
+    if K % ch == 0:
+        if ld % ch:
+            x, ld = x.contiguous(), K
+        if x.data_ptr() % 16:
+            x, ld = x.clone(memory_format=torch.contiguous_format), K
+    return x, ld
 
 
-def _check_layer(name, x, weight, act, bias, residual=None):
-    _check(x.dim() >= 1 and weight.dim() == 2 and x.shape[-1] == weight.shape[1], "{}: rows of {} and a weight of {}", name,
-           tuple(x.shape), tuple(weight.shape))
-    _check(weight.shape[0] > 0 and weight.shape[1] > 0, "{}: an empty weight {}", name, tuple(weight.shape))
-    _check(x.numel() // weight.shape[1] <= 1 << 21 and max(weight.shape) <= 1 << 20, "{}: sizes {} x {} over 2^21 rows, 2^20 columns", name,
-           tuple(x.shape), tuple(weight.shape))
-    _check(act in _ACTS, "{}: unknown activation {}", name, act)
-    _check(bias is None or tuple(bias.shape) == (weight.shape[0],), "{}: a bias of {} for {} outputs", name,
-           None if bias is None else tuple(bias.shape), weight.shape[0])
-    _check(residual is None or tuple(residual.shape) == tuple(x.shape[:-1]) + (weight.shape[0],),
-           "{}: a residual of {} for outputs of {} (it is not broadcast)", name, None if residual is None else tuple(residual.shape),
-           tuple(x.shape[:-1]) + (weight.shape[0],))
+def _check_layer(name, x, weight, bias, act):
+    if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1] or not weight.numel():
+        raise ValueError("{}: rows of {} and a weight of {}".format(name, tuple(x.shape), tuple(weight.shape)))
+    N, K = weight.shape
+    if x.numel() > K << 21 or N > 1 << 20 or K > 1 << 20:
+        raise ValueError("{}: sizes {} x {} over 2^21 rows, 2^20 columns".format(name, tuple(x.shape), tuple(weight.shape)))
+    if act not in _ACTS:
+        raise ValueError("{}: unknown activation {}".format(name, act))
+    if bias is not None and (bias.dim() != 1 or bias.shape[0] != N):
+        raise ValueError("{}: a bias of {} for {} outputs".format(name, tuple(bias.shape), N))
 
 
-def _linear_fwd(x, weight, bias, residual, act, slope, keep):
-    (x, ldx), weight, bias, residual = _rows(x), weight.contiguous(), _aligned(bias), _aligned(residual)
-    (M, K), N = x.shape, weight.shape[0]
-    y = torch.empty(M, N, dtype=x.dtype, device=x.device)
-    z = torch.empty(M, N, dtype=torch.float32, device=x.device) if keep and act != ACT_NONE else None
+def _layer_fwd(x, w, w2, b, b2, res, act, slope, keep):
+    """-> y, kept inputs of the activation, operands as the kernels read them"""
+    N, K = w.shape
+    (x, ldx), w, b = _rows(x, K), _aligned(w), _aligned(b)
+    gated = w2 is not None
+    if gated:
+        w2, b2 = _aligned(w2), _aligned(b2)
+    M, dev, code = x.shape[0], x.device, _DTYPES[x.dtype]
+    y = torch.empty(M, N, dtype=x.dtype, device=dev)
+    z = torch.empty((1 + gated, M, N), dtype=_F32, device=dev) if keep and (gated or act != ACT_NONE) else None
     if M:
-        ws, n = _workspace(x, M, K, N, 0, 0)
-        lib.mggan_block_linear_fwd(_p(x), ldx, _p(weight), _p(bias), _p(residual), _p(y), _p(z), M, K, N, act, float(slope),
-                                   _DTYPES[x.dtype], _p(ws), n, _s())
-    return y, z, x, weight
+        res = _aligned(res)
+        n = _layer_workspace(M, K, N, gated, 0, act, code)
+        ws = _bytes(n, x)
+        pz = _p(z)
+        # (z2 lies M N f32 behind z: 16-byte aligned as the workspace of a call has to be only where M N is a multiple of four)
+        z2 = None
+        if gated and z is not None:
+            z2 = pz + 4 * M * N
+            if z2 % 16:
+                z = torch.empty((2, M * N + (-M * N) % 4), dtype=_F32, device=dev)
+                pz = _p(z)
+                z2 = pz + 4 * z.stride(0)
+        lib.mggan_block_layer_fwd(_LAYER.pack(_p(x), _p(w), _p(w2), _p(b), _p(b2), _p(res), 0, pz, z2 or 0, _p(y), 0, 0, 0, _p(ws), n, ldx,
+                                              M, K, N, act, code, slope), _s())
+    return y, z, x, w, w2
 
 
-class LinearResidualFn(Function):
+def _layer_bwd(ctx, dy):
+    x, w, w2 = ctx.saved_tensors
+    gated, need = w2 is not None, ctx.needs_input_grad
+    (x, ldx), (N, K) = _rows(x, w.shape[1]), w.shape
+    M, dev, dt = x.shape[0], x.device, x.dtype
+    code = _DTYPES[dt]
+    off = -(-N // (128 // x.element_size())) * (128 // x.element_size()) if gated else 0  # where the up weight's gradient starts
+    make = torch.empty if M else torch.zeros
+    dx = make(M, K, dtype=dt, device=dev) if need[0] else None
+    dw = make(off + N, K, dtype=dt, device=dev) if need[1] or need[2] else None
+    db = make((1 + gated) * N, dtype=dt, device=dev) if need[3] or need[4] else None
+    if M and (dx is not None or dw is not None or db is not None):
+        g, z = _aligned(dy), ctx.z
+        n = _layer_workspace(M, K, N, gated, 1, ctx.act, code)
+        ws = _bytes(n, x)
+        lib.mggan_block_layer_bwd(_LAYER.pack(_p(x), _p(w), _p(w2), 0, 0, 0, _p(g), _p(z), _p(z) + 4 * z.stride(0) if gated else 0, 0, _p(dx),
+                                              _p(dw), _p(db), _p(ws), n, ldx, M, K, N, ctx.act, code, ctx.slope), _s())
+    if not gated:
+        return dx, dw, None, db, None, (dy if need[5] else None), None, None
+    return (dx, dw[:N] if need[1] else None, dw[off:] if need[2] else None, db[:N] if need[3] else None, db[N:] if need[4] else None, None, None,
+            None)
+
+
+_layer_bwd_once = once_differentiable(_layer_bwd)
+
+
+class LayerFn(Function):
+    """Both layers: a linear one has no second weight and may have a residual."""
+
     @staticmethod
-    def forward(ctx, x, weight, bias, residual, act, slope):
-        y, z, x, weight = _linear_fwd(x, weight, bias, residual, act, slope, True)
+    def forward(ctx, x, w, w2, b, b2, res, act, slope):
+        y, ctx.z, x, w, w2 = _layer_fwd(x, w, w2, b, b2, res, act, slope, True)
         ctx.act, ctx.slope = act, slope
-        ctx.save_for_backward(x, weight, z)
+        ctx.save_for_backward(x, w, w2)
         return y
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy):
-        x, weight, z = ctx.saved_tensors
-        x, ldx = _rows(x)
-        (M, K), N = x.shape, weight.shape[0]
-        need = ctx.needs_input_grad
-        like = dict(dtype=x.dtype, device=x.device)
-        make = torch.empty if M else torch.zeros
-        dx = make(M, K, **like) if need[0] else None
-        dw = make(N, K, **like) if need[1] else None
-        db = make(N, **like) if need[2] else None
-        if M and any(need[:3]):
-            g = _aligned(dy)
-            ws, n = _workspace(x, M, K, N, 0, 1)
-            lib.mggan_block_linear_bwd(_p(g), _p(z), _p(x), ldx, _p(weight), _p(dx), _p(dw), _p(db), M, K, N, ctx.act, float(ctx.slope),
-                                       _DTYPES[x.dtype], _p(ws), n, _s())
-        return dx, dw, db, (dy if need[3] else None), None, None
+        return _layer_bwd_once(ctx, dy) if torch.is_grad_enabled() else _layer_bwd(ctx, dy)
 
 
 def linear_residual(x, weight, bias=None, residual=None, act=ACT_NONE, slope=0.0):
-    """act(x W^T + bias) + residual: x (..., K), weight (N, K), bias (N) or None, residual (..., N) or None -> (..., N).
+    """act(x W^T + b) + residual: x (..., K), weight (N, K), bias (N) or None, residual (..., N) or None -> (..., N).
     act: ACT_NONE, ACT_LEAKY (with `slope`; 0 is ReLU), ACT_SIGMOID, ACT_SILU or ACT_GELU.  x may be a view with any row stride."""
-    _same("linear_residual", x, weight=weight, bias=bias, residual=residual)
-    _check_layer("linear_residual", x, weight, act, bias, residual)
-    _on_gpu("linear_residual", x)
-    lead, N = x.shape[:-1], weight.shape[0]
-    x, r = x.reshape(-1, x.shape[-1]), None if residual is None else residual.reshape(-1, N)
-    with torch.cuda.device(x.device):
-        if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, r)):
-            y = LinearResidualFn.apply(x, weight, bias, r, act, slope)
-        else:
-            y = _linear_fwd(x, weight, bias, r, act, slope, False)[0]
-    return y.reshape(*lead, N)
-
-
-def _gated_fwd(x, w_gate, w_up, b_gate, b_up, act, slope, keep):
-    (x, ldx), w_gate, w_up, b_gate, b_up = _rows(x), w_gate.contiguous(), w_up.contiguous(), _aligned(b_gate), _aligned(b_up)
-    (M, K), N = x.shape, w_gate.shape[0]
-    y = torch.empty(M, N, dtype=x.dtype, device=x.device)
-    z, u = (torch.empty(M, N, dtype=torch.float32, device=x.device) for _ in range(2)) if keep else (None, None)
-    if M:
-        ws, n = _workspace(x, M, K, N, 1, 0)
-        lib.mggan_block_gated_fwd(_p(x), ldx, _p(w_gate), _p(w_up), _p(b_gate), _p(b_up), _p(y), _p(z), _p(u), M, K, N, act, float(slope),
-                                  _DTYPES[x.dtype], _p(ws), n, _s())
-    return y, z, u, x, w_gate, w_up
-
-
-class GatedLinearFn(Function):
-    @staticmethod
-    def forward(ctx, x, w_gate, w_up, b_gate, b_up, act, slope):
-        y, z, u, x, w_gate, w_up = _gated_fwd(x, w_gate, w_up, b_gate, b_up, act, slope, True)
-        ctx.act, ctx.slope = act, slope
-        ctx.save_for_backward(x, w_gate, w_up, z, u)
-        return y
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        x, w_gate, w_up, z, u = ctx.saved_tensors
-        x, ldx = _rows(x)
-        (M, K), N = x.shape, w_gate.shape[0]
-        need = ctx.needs_input_grad
-        like = dict(dtype=x.dtype, device=x.device)
-        make = torch.empty if M else torch.zeros
-        dx = make(M, K, **like) if need[0] else None
-        dw = make(2 * N, K, **like) if need[1] or need[2] else None
-        db = make(2 * N, **like) if need[3] or need[4] else None
-        if M:
-            g = _aligned(dy)
-            ws, n = _workspace(x, M, K, N, 1, 1)
-            lib.mggan_block_gated_bwd(_p(g), _p(z), _p(u), _p(x), ldx, _p(w_gate), _p(w_up), _p(dx), _p(dw), _p(db), M, K, N, ctx.act,
-                                      float(ctx.slope), _DTYPES[x.dtype], _p(ws), n, _s())
-        return (dx, dw[:N] if need[1] else None, dw[N:] if need[2] else None, db[:N] if need[3] else None, db[N:] if need[4] else None,
-                None, None)
+    _same("linear_residual", x, weight, bias, residual)
+    _check_layer("linear_residual", x, weight, bias, act)
+    N, two = weight.shape[0], x.dim() == 2
+    if residual is not None and residual.shape != x.shape[:-1] + (N,):
+        raise ValueError("linear_residual: a residual of {} for outputs of {} (it is not broadcast)".format(
+            tuple(residual.shape), tuple(x.shape[:-1]) + (N,)))
+    if not _on_current("linear_residual", x):
+        with torch.cuda.device(x.device):
+            return linear_residual(x, weight, bias, residual, act, slope)
+    lead = x.shape[:-1]
+    if not two:
+        x, residual = x.reshape(-1, x.shape[-1]), None if residual is None else residual.reshape(-1, N)
+    if _needs_grad(x, weight, bias, residual):
+        y = LayerFn.apply(x, weight, None, bias, None, residual, act, float(slope))
+    else:
+        y = _layer_fwd(x, weight, None, bias, None, residual, act, slope, False)[0]
+    return y if two else y.reshape(*lead, N)
 
 
 def gated_linear(x, w_gate, w_up, b_gate=None, b_up=None, act=ACT_SILU, slope=0.0):
     """act(x Wg^T + bg) * (x Wu^T + bu): x (..., K), w_gate and w_up (N, K), biases (N) or None -> (..., N); activations as in
     linear_residual."""
-    _same("gated_linear", x, w_gate=w_gate, w_up=w_up, b_gate=b_gate, b_up=b_up)
-    _check_layer("gated_linear", x, w_gate, act, b_gate)
-    _check_layer("gated_linear", x, w_up, act, b_up)
-    _check(w_gate.shape == w_up.shape, "gated_linear: weights of {} and {}", tuple(w_gate.shape), tuple(w_up.shape))
-    _on_gpu("gated_linear", x)
-    lead, N = x.shape[:-1], w_gate.shape[0]
-    x = x.reshape(-1, x.shape[-1])
-    with torch.cuda.device(x.device):
-        if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, w_gate, w_up, b_gate, b_up)):
-            y = GatedLinearFn.apply(x, w_gate, w_up, b_gate, b_up, act, slope)
-        else:
-            y = _gated_fwd(x, w_gate, w_up, b_gate, b_up, act, slope, False)[0]
-    return y.reshape(*lead, N)
+    _same("gated_linear", x, w_gate, w_up, b_gate, b_up)
+    _check_layer("gated_linear", x, w_gate, b_gate, act)
+    _check_layer("gated_linear", x, w_up, b_up, act)
+    if w_gate.shape != w_up.shape:
+        raise ValueError("gated_linear: weights of {} and {}".format(tuple(w_gate.shape), tuple(w_up.shape)))
+    if not _on_current("gated_linear", x):
+        with torch.cuda.device(x.device):
+            return gated_linear(x, w_gate, w_up, b_gate, b_up, act, slope)
+    lead, two = x.shape[:-1], x.dim() == 2
+    if not two:
+        x = x.reshape(-1, x.shape[-1])
+    if _needs_grad(x, w_gate, w_up, b_gate, b_up):
+        y = LayerFn.apply(x, w_gate, w_up, b_gate, b_up, None, act, float(slope))
+    else:
+        y = _layer_fwd(x, w_gate, w_up, b_gate, b_up, None, act, slope, False)[0]
+    return y if two else y.reshape(*lead, w_gate.shape[0])
 
 
 # ---- attention ---------------------------------------------------------------------------------------------------------------
-
-class _AttnArgs(ctypes.Structure):  # mirrors csrc/blk_attn.h: BlkAttnArgs
-    _fields_ = ([(n, ctypes.c_void_p) for n in ("q", "k", "v", "dout", "out", "dq", "dk", "dv", "dslopes", "scenes", "kv_scenes", "prefix",
-                                                "xy", "kv_xy", "slopes", "lse", "out32", "spans", "ws")]
-                + [(n, ctypes.c_long) for n in ("ws_bytes", "q_row", "q_head", "k_row", "k_head", "v_row", "v_head")]
-                + [(n, ctypes.c_int) for n in ("N", "M", "H", "Hkv", "D", "S", "causal", "axes", "dtype")]
-                + [("scale", ctypes.c_float), ("cap", ctypes.c_float)])
-
 
 _TABLES = BoundedCache(64)
 
@@ -209,18 +230,18 @@ def _table(name, rows, device, limit, width):
     """int32 device tensor of a scene list (width 2) or of per-scene numbers (width 1): checked and kept by its contents when it is a
     host list, taken as it is when it is a device tensor."""
     if isinstance(rows, torch.Tensor) and rows.is_cuda:
-        _check(rows.dtype == torch.int32 and rows.device == device and rows.dim() == width and (width == 1 or rows.shape[1] == 2),
-               "attention: {} has to be an int32 tensor of (scenes{}) on {}", name, ", 2" if width == 2 else "", device)
-        return rows.contiguous()
+        if rows.dtype != torch.int32 or rows.device != device or rows.dim() != width or (width == 2 and rows.shape[1] != 2):
+            raise ValueError("attention: {} has to be an int32 tensor of (scenes{}) on {}".format(name, ", 2" if width == 2 else "", device))
+        return rows if rows.is_contiguous() else rows.contiguous()
     try:
         key = tuple((int(a), int(b)) for a, b in rows) if width == 2 else tuple(int(a) for a in rows)
     except (TypeError, ValueError):
         raise ValueError("attention: {} has to be a list or an int32 device tensor".format(name)) from None
-    if width == 2:
-        for a, b in key:
-            _check(0 <= a <= b <= limit, "attention: {} names rows [{}, {}) of {}", name, a, b, limit)
-    else:
-        _check(all(abs(a) < 2 ** 31 for a in key), "attention: {} out of range", name)
+    for k in key:
+        if width == 2 and not 0 <= k[0] <= k[1] <= limit:
+            raise ValueError("attention: {} names rows [{}, {}) of {}".format(name, k[0], k[1], limit))
+        if width == 1 and abs(k) >= 1 << 31:
+            raise ValueError("attention: {} out of range".format(name))
     hit = _TABLES.get((key, device))
     if hit is None:
         hit = torch.tensor(key, dtype=torch.int32).reshape((-1, 2) if width == 2 else (-1,)).to(device)
@@ -229,74 +250,82 @@ def _table(name, rows, device, limit, width):
 
 
 def _heads(t):
-    """An operand whose rows and heads start at multiples of 16 bytes and whose width is contiguous (a copy where they do not)."""
+    """An operand whose rows and heads start at multiples of 16 bytes and whose width is contiguous (a copy where they do not), and its
+    two strides."""
+    rows, heads, width = t.stride()
+    n, h, _ = t.shape
     ch = 16 // t.element_size()
-    ok = t.stride(2) == 1 and t.data_ptr() % 16 == 0 and all(t.shape[i] == 1 or (t.stride(i) % ch == 0 and t.stride(i) >= 0) for i in (0, 1))
-    if not ok:
+    if width != 1 or t.data_ptr() % 16 or (n > 1 and (rows % ch or rows < 0)) or (h > 1 and (heads % ch or heads < 0)):
         t = t.contiguous()
         t = t.clone() if t.data_ptr() % 16 else t
-    return t, tuple(t.stride(i) if t.shape[i] > 1 else 0 for i in (0, 1))
+        rows, heads, _ = t.stride()
+    return t, (rows if n > 1 else 0), (heads if h > 1 else 0)
 
 
-def _attn_args(q, k, v, scenes, kv_scenes, prefix, xy, kv_xy, slopes, causal, scale, cap):
-    a = _AttnArgs()
-    (q, (a.q_row, a.q_head)), (k, (a.k_row, a.k_head)), (v, (a.v_row, a.v_head)) = _heads(q), _heads(k), _heads(v)
-    a.q, a.k, a.v = _p(q), _p(k), _p(v)
-    a.scenes, a.kv_scenes, a.prefix, a.xy, a.kv_xy, a.slopes = _p(scenes), _p(kv_scenes), _p(prefix), _p(xy), _p(kv_xy), _p(slopes)
-    (a.N, a.H, a.D), a.M, a.Hkv = q.shape, k.shape[0], k.shape[1]
-    a.S, a.causal, a.axes, a.dtype = scenes.shape[0], int(causal), 0 if xy is None else xy.shape[1], _DTYPES[q.dtype]
-    a.scale, a.cap = scale, cap
-    return a, (q, k, v)
+def _attn_fwd(q, k, v, slopes, rest, keep):
+    """-> out, the output in f32, row statistics, the operands as the kernels read them"""
+    scenes, kv_scenes, prefix, xy, kv_xy, causal, scale, cap = rest
+    (q, q_row, q_head), (k, k_row, k_head), (v, v_row, v_head) = _heads(q), _heads(k), _heads(v)
+    (N, H, D), (M, Hkv, _), S, dev = q.shape, k.shape, scenes.shape[0], q.device
+    ints, n, _ = _attn_sizes(N, M, H, Hkv, D, S)
+    out = torch.empty((N, H, D), dtype=q.dtype, device=dev)
+    at = 2 * H * N + (-2 * H * N) % 4 if keep else 0  # the row intervals lie behind the softmax statistics
+    stats = torch.empty(at + ints, dtype=_F32, device=dev)
+    out32 = ws = None
+    if keep:
+        out32, n = out if q.dtype == _F32 else torch.empty((N, H, D), dtype=_F32, device=dev), 0
+    else:
+        ws = _bytes(n, q)
+    ps = _p(stats)
+    lib.mggan_block_attention_fwd(_ATTN.pack(
+        _p(q), _p(k), _p(v), 0, _p(out), 0, 0, 0, 0, _p(scenes), _p(kv_scenes), _p(prefix), _p(xy), _p(kv_xy), _p(slopes), ps if keep else 0,
+        _p(out32), ps + 4 * at, _p(ws), n, q_row, q_head, k_row, k_head, v_row, v_head, N, M, H, Hkv, D, S, causal,
+        0 if xy is None else xy.shape[1], _DTYPES[q.dtype], scale, cap), _s())
+    return out, out32, stats, q, k, v
 
 
-def _attn_fwd(a, q, keep):
-    out = torch.empty(a.N, a.H, a.D, dtype=q.dtype, device=q.device)
-    lse = torch.empty(2, a.H, a.N, dtype=torch.float32, device=q.device) if keep else None
-    out32 = None if not keep else out if q.dtype == torch.float32 else torch.empty(out.shape, dtype=torch.float32, device=q.device)
-    spans = torch.empty(lib.mggan_block_attention_span_ints(a.N), dtype=torch.int32, device=q.device)
-    ws = None
-    if not keep:
-        a.ws_bytes = lib.mggan_block_attention_fwd_workspace(a.N, a.M, a.H, a.Hkv, a.D, a.S)
-        ws = torch.empty(a.ws_bytes // 4, dtype=torch.float32, device=q.device) if a.ws_bytes else None
-        a.ws = _p(ws)
-    a.out, a.lse, a.out32, a.spans = _p(out), _p(lse), _p(out32), _p(spans)
-    lib.mggan_block_attention_fwd(ctypes.addressof(a), _s())
-    return out, lse, out32, spans
+def _attn_bwd(ctx, dout):
+    q, k, v, slopes, out = ctx.saved_tensors
+    if ctx.stats is None:
+        return tuple(None if t is None else torch.zeros_like(t) for t in (q, k, v, slopes)) + (None,)
+    scenes, kv_scenes, prefix, xy, kv_xy, causal, scale, cap = ctx.rest
+    (q, q_row, q_head), (k, k_row, k_head), (v, v_row, v_head) = _heads(q), _heads(k), _heads(v)
+    (N, H, D), (M, Hkv, _), S, dev, dt = q.shape, k.shape, scenes.shape[0], q.device, q.dtype
+    dout = _aligned(dout)
+    dq = torch.empty((N, H, D), dtype=dt, device=dev)
+    dk = torch.empty((M, Hkv, D), dtype=dt, device=dev)
+    dv = torch.empty((M, Hkv, D), dtype=dt, device=dev)
+    dslopes = torch.empty(H, dtype=_F32, device=dev) if slopes is not None and ctx.needs_input_grad[3] else None
+    n = _attn_sizes(N, M, H, Hkv, D, S)[2]
+    ws = _bytes(n, q)
+    ps = _p(ctx.stats)
+    at = 2 * H * N + (-2 * H * N) % 4
+    lib.mggan_block_attention_bwd(_ATTN.pack(
+        _p(q), _p(k), _p(v), _p(dout), 0, _p(dq), _p(dk), _p(dv), _p(dslopes), _p(scenes), _p(kv_scenes), _p(prefix), _p(xy), _p(kv_xy),
+        _p(slopes), ps, _p(out if ctx.out32 is None else ctx.out32), ps + 4 * at, _p(ws), n, q_row, q_head, k_row, k_head, v_row, v_head, N, M, H,
+        Hkv, D, S, causal, 0 if xy is None else xy.shape[1], _DTYPES[dt], scale, cap), _s())
+    return dq, dk, dv, dslopes, None
+
+
+_attn_bwd_once = once_differentiable(_attn_bwd)
 
 
 class AttentionFn(Function):
     @staticmethod
     def forward(ctx, q, k, v, slopes, rest):
-        scenes, kv_scenes, prefix, xy, kv_xy, causal, scale, cap = rest
-        ctx.rest = rest
+        ctx.rest, ctx.stats, ctx.out32, out = rest, None, None, None
         if q.shape[0] == 0 or k.shape[0] == 0:
-            ctx.save_for_backward(q, k, v, slopes)
-            ctx.empty = True
+            ctx.save_for_backward(q, k, v, slopes, None)
             return torch.zeros(q.shape, dtype=q.dtype, device=q.device)
-        ctx.empty = False
-        a, (q, k, v) = _attn_args(q, k, v, scenes, kv_scenes, prefix, xy, kv_xy, slopes, causal, scale, cap)
-        out, lse, out32, spans = _attn_fwd(a, q, True)
-        ctx.save_for_backward(q, k, v, slopes, out32, lse, spans)
+        out, out32, ctx.stats, q, k, v = _attn_fwd(q, k, v, slopes, rest, True)
+        if out32 is not out:
+            ctx.out32 = out32
+        ctx.save_for_backward(q, k, v, slopes, out if out32 is out else None)
         return out
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dout):
-        scenes, kv_scenes, prefix, xy, kv_xy, causal, scale, cap = ctx.rest
-        if ctx.empty:
-            return tuple(None if t is None else torch.zeros_like(t) for t in ctx.saved_tensors) + (None,)
-        q, k, v, slopes, out32, lse, spans = ctx.saved_tensors
-        a, _ = _attn_args(q, k, v, scenes, kv_scenes, prefix, xy, kv_xy, slopes, causal, scale, cap)
-        dout = _aligned(dout)
-        dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        dk, dv = (torch.empty(k.shape, dtype=q.dtype, device=q.device) for _ in range(2))
-        dslopes = torch.empty_like(slopes) if slopes is not None and ctx.needs_input_grad[3] else None
-        a.ws_bytes = lib.mggan_block_attention_bwd_workspace(a.N, a.H)
-        ws = torch.empty(a.ws_bytes // 4, dtype=torch.float32, device=q.device)
-        a.dout, a.out32, a.lse, a.spans, a.ws = _p(dout), _p(out32), _p(lse), _p(spans), _p(ws)
-        a.dq, a.dk, a.dv, a.dslopes = _p(dq), _p(dk), _p(dv), _p(dslopes)
-        lib.mggan_block_attention_bwd(ctypes.addressof(a), _s())
-        return dq, dk, dv, dslopes, None
+        return _attn_bwd_once(ctx, dout) if torch.is_grad_enabled() else _attn_bwd(ctx, dout)
 
 
 def attention(q, k, v, scenes, kv_scenes=None, *, causal=False, prefix=None, scale=None, cap=0.0, xy=None, kv_xy=None, slopes=None):
@@ -313,46 +342,53 @@ def attention(q, k, v, scenes, kv_scenes=None, *, causal=False, prefix=None, sca
     device tensor).  One new row over a long cache is Lq = 1.  scale: > 0, D ** -0.5 by default; cap: 0 for none.
     xy (N, axes) and kv_xy (M, axes; by default xy), f32 with one or two axes, and slopes (H), f32: the bias by distance.  Gradients go to q,
     k, v and slopes, not to positions."""
-    name = "attention"
-    _same(name, q, k=k, v=v)
-    _check(q.dim() == 3 and k.dim() == 3 and k.shape == v.shape and q.shape[2] == k.shape[2], "{}: q {}, k {}, v {}", name, tuple(q.shape),
-           tuple(k.shape), tuple(v.shape))
+    _same("attention", q, k, v)
+    if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape or q.shape[2] != k.shape[2]:
+        raise ValueError("attention: q {}, k {}, v {}".format(tuple(q.shape), tuple(k.shape), tuple(v.shape)))
     (N, H, D), (M, Hkv, _) = q.shape, k.shape
-    _check(0 < H <= 1024 and Hkv > 0 and H % Hkv == 0, "{}: {} heads over {} key heads", name, H, Hkv)
-    _check(D % 8 == 0 and 0 < D <= 128, "{}: a width of {} (a multiple of 8 up to 128)", name, D)
-    _check(N <= 1 << 24 and M <= 1 << 30, "{}: {} rows, {} keys", name, N, M)
+    if not 0 < H <= 1024 or not Hkv or H % Hkv:
+        raise ValueError("attention: {} heads over {} key heads".format(H, Hkv))
+    if D % 8 or not 0 < D <= 128:
+        raise ValueError("attention: a width of {} (a multiple of 8 up to 128)".format(D))
+    if N > 1 << 24 or M > 1 << 30:
+        raise ValueError("attention: {} rows, {} keys (at most 2^24, 2^30)".format(N, M))
     scale = D ** -0.5 if scale is None else float(scale)
     cap = 0.0 if cap is None else float(cap)
-    _check(scale > 0 and math.isfinite(scale), "{}: scale {} (it has to be positive)", name, scale)
-    _check(cap >= 0 and math.isfinite(cap), "{}: cap {}", name, cap)
-    _check(prefix is None or causal, "{}: a prefix without causal", name)
-    _check((xy is None) == (slopes is None) and (xy is not None or kv_xy is None), "{}: positions and slopes come together", name)
+    if not 0 < scale < math.inf or not 0 <= cap < math.inf:
+        raise ValueError("attention: scale {} (has to be positive), cap {} (0 or positive)".format(scale, cap))
+    if prefix is not None and not causal:
+        raise ValueError("attention: a prefix without causal")
+    if (xy is None) != (slopes is None) or (xy is None and kv_xy is not None):
+        raise ValueError("attention: positions and slopes come together")
+    if kv_scenes is None and M < N:
+        raise ValueError("attention: {} rows over {} keys need kv_scenes".format(N, M))
     if xy is not None:
         kv_xy = xy if kv_xy is None else kv_xy
-        for n, t, rows in (("xy", xy, N), ("kv_xy", kv_xy, M)):
-            _check(t.dtype == torch.float32 and t.dim() == 2 and t.shape[0] == rows and t.shape[1] in (1, 2) and t.shape[1] == xy.shape[1],
-                   "{}: {} {} {} for {} rows and one or two axes, f32", name, n, t.dtype, tuple(t.shape), rows)
-            _check(t.device == q.device, "{}: {} is on {}", name, n, t.device)
-            _check(not (t.requires_grad and torch.is_grad_enabled()), "{}: {} requires a gradient, positions have none: detach it", name, n)
-        _check(slopes.dtype == torch.float32 and tuple(slopes.shape) == (H,) and slopes.device == q.device, "{}: slopes {} {} on {}", name,
-               slopes.dtype, tuple(slopes.shape), slopes.device)
-    _on_gpu(name, q)
-    with torch.cuda.device(q.device):
-        table = _table("scenes", scenes, q.device, N, 2)
-        kv_table = table if kv_scenes is None else _table("kv_scenes", kv_scenes, q.device, M, 2)
-        if kv_scenes is None:
-            _check(M >= N, "{}: {} rows over {} keys need kv_scenes", name, N, M)
-        _check(table.shape == kv_table.shape, "{}: {} scenes of rows, {} of keys", name, table.shape[0], kv_table.shape[0])
-        if prefix is not None:
-            prefix = _table("prefix", prefix, q.device, 0, 1)
-            _check(prefix.shape[0] == table.shape[0], "{}: {} prefixes for {} scenes", name, prefix.shape[0], table.shape[0])
-        if xy is not None:
-            same = kv_xy is xy
-            xy, slopes = xy.detach().contiguous(), slopes.contiguous()
-            kv_xy = xy if same else kv_xy.detach().contiguous()
-        if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, slopes)):
-            return AttentionFn.apply(q, k, v, slopes, (table, kv_table, prefix, xy, kv_xy, causal, scale, cap))
-        if N == 0 or M == 0:
-            return torch.zeros(q.shape, dtype=q.dtype, device=q.device)
-        a, ops = _attn_args(q, k, v, table, kv_table, prefix, xy, kv_xy, slopes, causal, scale, cap)
-        return _attn_fwd(a, ops[0], False)[0]
+        for t, rows in ((xy, N), (kv_xy, M)):
+            if t.dtype != _F32 or t.dim() != 2 or t.shape[0] != rows or t.shape[1] not in (1, 2) or t.shape[1] != xy.shape[1] or t.device != q.device:
+                raise ValueError("attention: positions {} {} on {} for {} rows: f32, one or two axes".format(t.dtype, tuple(t.shape), t.device, rows))
+            if t.requires_grad and torch.is_grad_enabled():
+                raise ValueError("attention: positions have no gradient: detach them")
+        if slopes.dtype != _F32 or slopes.dim() != 1 or slopes.shape[0] != H or slopes.device != q.device:
+            raise ValueError("attention: slopes {} {} on {} for {} heads".format(slopes.dtype, tuple(slopes.shape), slopes.device, H))
+    if not _on_current("attention", q):
+        with torch.cuda.device(q.device):
+            return attention(q, k, v, scenes, kv_scenes, causal=causal, prefix=prefix, scale=scale, cap=cap, xy=xy, kv_xy=kv_xy, slopes=slopes)
+    table = _table("scenes", scenes, q.device, N, 2)
+    kv_table = table if kv_scenes is None else _table("kv_scenes", kv_scenes, q.device, M, 2)
+    if table.shape[0] != kv_table.shape[0]:
+        raise ValueError("attention: {} scenes of rows, {} of keys".format(table.shape[0], kv_table.shape[0]))
+    if prefix is not None:
+        prefix = _table("prefix", prefix, q.device, 0, 1)
+        if prefix.shape[0] != table.shape[0]:
+            raise ValueError("attention: {} prefixes for {} scenes".format(prefix.shape[0], table.shape[0]))
+    if xy is not None:
+        same = kv_xy is xy
+        xy, slopes = xy.contiguous(), slopes.contiguous()
+        kv_xy = xy if same else kv_xy.contiguous()
+    rest = (table, kv_table, prefix, xy, kv_xy, bool(causal), scale, cap)
+    if _needs_grad(q, k, v, slopes):
+        return AttentionFn.apply(q, k, v, slopes, rest)
+    if N == 0 or M == 0:
+        return torch.zeros(q.shape, dtype=q.dtype, device=q.device)
+    return _attn_fwd(q, k, v, slopes, rest, False)[0]
