@@ -651,7 +651,7 @@ int mggan_crop_patches(const unsigned char* atlas, const long long* img_off, con
  * 1 LeakyReLU(slope), 2 sigmoid, 4 SiLU, 5 GELU (exact).  x (M, K) with row stride ldx (elements), w, w2 (N, K), b, b2 (N), res, dy, y,
  * z, z2 (M, N) contiguous; b, b2, res NULL for none; 16-byte aligned (with K no multiple of 16 bytes: x, w, w2 in any place).  z, z2: the
  * activation's input and the up result in f32, written by the forward call if not NULL, read by the backward call (act 0 without w2:
- * NULL).  Backward: dx (M, K), dw (N, K), db (N), each NULL if not wanted; with w2 dw is (off + N, K), off = N rounded up to 128 bytes of
+ * NULL).  Backward: dx (M, K), dw (N, K), db (N), each NULL if not wanted; with w2 dw is (off + N, K), off = N rounded up to 64 bytes of
  * elements: the gate weight's gradient in rows [0, N), the up weight's from off on; db (2 N).  Written, not accumulated; fixed order of
  * summation.  ws: mggan_block_layer_workspace bytes, 256-byte aligned, free again when the call's work on `stream` is done.  Limits:
  * M <= 2^21, K, N <= 2^20. */

@@ -35,15 +35,58 @@ __device__ __attribute__((aligned(16))) const unsigned blk_attn_zeros[4] = {0, 0
 
 constexpr float LOG2E = 1.44269504f;
 
-// Scores are exponentiated as exp2((s - max) log2e) where their last bits matter (f32; scores that got a bias or a cap, whose gradients
-// are f32): log2e rounded into the scores first would stretch all of them by a common 2^-25, which shows in the slopes' gradient.  Plain
-// bf16 scores, whose gradients are rounded at 2^-9, take the fused form exp2(s c - max c), an operation less.
-template <class T, bool EXTRA>
+// tanh.  f32 operands: near zero by its series (to x^11: 2^-26 of the value at 0.35), so that a score keeps its relative precision
+// through the cap; bf16 operands carry 2^-9 themselves, there the quotient does everywhere.
+template <class T>
+__device__ __forceinline__ float blk_tanh(float x) {
+  const float big = fmaf(-2.0f, mg_rcp(__builtin_amdgcn_exp2f(x * (2.f * LOG2E)) + 1.0f), 1.0f);
+  if constexpr (sizeof(T) == 2) return big;
+  const float y = x * x;
+  const float s = fmaf(y, fmaf(y, fmaf(y, fmaf(y, fmaf(y, -0.0088632355f, 0.0218694885f), -0.0539682540f), 0.1333333333f), -0.3333333333f), 1.f) * x;
+  return fabsf(x) < 0.35f ? s : big;
+}
+
+// What is done to a score q.k, by the kernels' template argument X: bit 0 a cap, bits 1-2 the axes of the distance.
+// Scores are exponentiated as exp2((s - max) log2e) where their last bits matter (f32; scores with a distance, whose slopes' gradient is
+// f32): log2e rounded into the scores first would stretch all of them by a common 2^-25, which shows in the slopes' gradient.  The others
+// (bf16, gradients rounded at 2^-9) are kept times log2e and take exp2(s - max), an operation less.
+template <class T, int X>
 struct Soft {
-  static constexpr bool NATURAL = EXTRA || sizeof(T) == 4;
-  static __device__ __forceinline__ float weight(float s, float top, float c2) {
-    return NATURAL ? __builtin_amdgcn_exp2f((s - top) * LOG2E) : __builtin_amdgcn_exp2f(fmaf(s, c2, -top));
+  static constexpr bool CAP = X & 1, NATURAL = (X >> 1) || sizeof(T) == 4;
+  static constexpr int AXES = X >> 1;
+  float c, k, cap, slope;  // c: a plain score's factor
+  __device__ __forceinline__ Soft(const BlkAttnArgs& p, float slope_) {
+    c = p.scale * (NATURAL ? 1.f : LOG2E);
+    cap = p.cap * (NATURAL ? 1.f : LOG2E);
+    k = CAP ? p.scale / p.cap : 0.f;
+    slope = slope_;
   }
+  // the score as it is exponentiated; fac = d(capped)/d(score), dist: what the slope multiplies
+  __device__ __forceinline__ float score(float x, float ax, float ay, float bx, float by, float& fac, float& dist) const {
+    fac = 1.f, dist = 0.f;
+    if constexpr (CAP) {
+      const float t = blk_tanh<T>(x * k);
+      fac = fmaf(-t, t, 1.f);
+      x = cap * t;
+    } else {
+      x *= c;
+    }
+    if constexpr (AXES == 1) dist = fabsf(ax - bx);
+    if constexpr (AXES == 2) {
+      const float dx = ax - bx, dy = ay - by;
+      dist = __builtin_amdgcn_sqrtf(fmaf(dx, dx, dy * dy));
+    }
+    if constexpr (AXES) x = fmaf(-slope, dist, x);
+    return x;
+  }
+  // whether scores are left as the product gives them and weight() multiplies (one operation for both)
+  static constexpr bool RAW = X == 0 && !NATURAL;
+  __device__ __forceinline__ float weight(float s, float top) const {
+    if (RAW) return __builtin_amdgcn_exp2f(fmaf(s, c, -top));
+    return __builtin_amdgcn_exp2f(NATURAL ? (s - top) * LOG2E : s - top);
+  }
+  // exp(a - b) of two maxima
+  static __device__ __forceinline__ float ratio(float a, float b) { return __builtin_amdgcn_exp2f(NATURAL ? (a - b) * LOG2E : a - b); }
 };
 
 template <class T_, int DP_, int BK_ = 128 / (int)sizeof(T_)>
@@ -61,9 +104,54 @@ struct Geo {
     return sizeof(T) == 2 ? 32 * (f >> 1) + 8 * (i >> 2) + 4 * (f & 1) + (i & 3) : 16 * f + i;
   }
   static __device__ __forceinline__ int row4(int f, int g) { return sizeof(T) == 2 ? 32 * (f >> 1) + 8 * g + 4 * (f & 1) : 16 * f + 4 * g; }
-  // place of a chunk in its row: eight lanes that read the same chunk of eight rows meet eight different bank groups
+  // Place of a chunk in its row.  Row reads take one chunk of 16 rows ({0-3, 8-11, ..} (+4) with bf16, 0-15 with f32): any eight lanes meet
+  // eight bank groups.  The transposing reads of bf16 take two chunks of rows 8 g + {0..3}: eight bank groups again.  Neither depends on which
+  // fragment it is, so a lane's addresses are a few bases plus constants (Lane).
   static __device__ __forceinline__ int swz(int r) {
-    return NCH % 8 == 0 ? (r & 7) ^ ((r >> 1) & 4) : ((r >> 1) & 3) ^ ((r >> 2) & 2);
+    if (sizeof(T) == 4) return (r & 7) ^ ((r >> 1) & 4);
+    return NCH % 8 == 0 ? (r & 3) << 1 | ((r >> 3) & 1) : (r & 2) | ((r >> 3) & 1);
+  }
+};
+
+// Byte offsets of a lane's reads in a tile.
+template <class G>
+struct Lane {
+  static constexpr int ROW = G::NCH * 16;
+  static constexpr bool WIDE = G::NCH % 8 == 0;
+  int row[2];  // of a row's chunk 4 s + g, by s & 1
+  int col[8];  // of the transposed reads: bf16 by column fragment, f32 by r + 4 (column fragment & 1)
+  __device__ __forceinline__ void init(int lane) {
+    const int i16 = lane & 15, g = lane >> 4, r = G::row_of(0, i16);
+#pragma unroll
+    for (int k = 0; k < 2; ++k) row[k] = r * ROW + (WIDE ? ((4 * k + g) ^ G::swz(r)) & 7 : g ^ G::swz(r)) * 16;
+    if (sizeof(typename G::T) == 2) {
+      const int k = 8 * g + (i16 >> 2);
+#pragma unroll
+      for (int f = 0; f < 4; ++f)
+        col[f] = k * ROW + 8 * (i16 & 1) + (WIDE ? ((2 * f + ((i16 & 3) >> 1)) ^ G::swz(k)) & 7 : ((2 * (f & 1) + ((i16 & 3) >> 1)) ^ G::swz(k)) & 3) * 16;
+    } else {
+#pragma unroll
+      for (int f = 0; f < 8; ++f) {
+        const int k = 4 * g + (f & 3);
+        col[f] = k * ROW + 4 * (i16 & 3) + (((4 * (f >> 2) + (i16 >> 2)) ^ G::swz(k)) & 7) * 16;
+      }
+    }
+  }
+  // fragment f's rows, chunk 4 s + g: first operand of a product over the width
+  __device__ __forceinline__ u32x4 rows(const char* tile, int f, int s) const {
+    const int at = sizeof(typename G::T) == 2 ? (32 * (f >> 1) + 4 * (f & 1)) * ROW : 16 * f * ROW;
+    return *(const u32x4*)(tile + row[WIDE ? s & 1 : 0] + at + (WIDE ? (s >> 1) * 128 : s * 64));
+  }
+  // bf16: columns 16 fd + i of rows 32 p + 8 g + {0..7}, transposed: first operand of a product over the tile's rows
+  __device__ __forceinline__ bf16x8 cols(const char* tile, int p, int fd) const {
+    const char* a = tile + col[WIDE ? fd & 3 : fd & 1] + 32 * p * ROW + (WIDE ? (fd >> 2) * 128 : (fd >> 1) * 64);
+    const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((MG_LDS s16x4*)a);
+    const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((MG_LDS s16x4*)(a + 4 * ROW));
+    return __builtin_bit_cast(bf16x8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+  }
+  // f32: column 16 fd + i of row 16 f + 4 g + r
+  __device__ __forceinline__ float col1(const char* tile, int f, int r, int fd) const {
+    return *(const float*)(tile + col[r + 4 * (fd & 1)] + 16 * f * ROW + (fd >> 1) * 128);
   }
 };
 
@@ -93,37 +181,27 @@ __device__ __forceinline__ u32x4 owner_chunk(const T* row, int c, int nd) {
   return u32x4{0, 0, 0, 0};
 }
 
-// First operand over the width: fragment f's rows, chunk 4 s + g.
-template <class G>
-__device__ __forceinline__ u32x4 row_frag(const u32x4* tile, int f, int s, int lane) {
-  const int row = G::row_of(f, lane & 15);
-  return tile[row * G::NCH + ((4 * s + (lane >> 4)) ^ G::swz(row))];
-}
-
 // D fragments of scores: sum over the width of streamed rows x owner rows.
 template <class G, int QF>
-__device__ __forceinline__ void scores(const u32x4* tile, const u32x4 (&own)[QF][G::SK], f32x4 (&out)[QF][G::F], int lane) {
+__device__ __forceinline__ void scores(const void* tile, const u32x4 (&own)[QF][G::SK], f32x4 (&out)[QF][G::F], const Lane<G>& at) {
 #pragma unroll
   for (int f = 0; f < G::F; ++f) {
 #pragma unroll
     for (int j = 0; j < QF; ++j) out[j][f] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int s = 0; s < G::SK; ++s) {
-      const u32x4 a = row_frag<G>(tile, f, s, lane);
+      const u32x4 a = at.rows((const char*)tile, f, s);
 #pragma unroll
       for (int j = 0; j < QF; ++j) out[j][f] = Mf<typename G::T>::step(a, own[j][s], out[j][f]);
     }
   }
 }
 
-// acc[d][owner row] += sum over streamed rows of tile[row][d] * coef[row][owner row].  The tile is read transposed: bf16 through the
-// transposing LDS read (4 rows x 16 columns a go), f32 an element a lane.  Result fragment fd's row i is column 32 (fd / 2) + 8 (i / 4)
-// + 4 (fd % 2) + i % 4, so a lane ends up with eight neighbouring columns of its owner row in every pair of fragments.
+// acc[d][owner row] += sum over streamed rows of tile[row][d] * coef[row][owner row], the tile read transposed.  Column fragment fd's row
+// i is column 16 fd + i: a lane ends up with columns 16 fd + 4 g + {0..3} of its owner row.
 template <class G, int QF>
-__device__ __forceinline__ void accumulate(const u32x4* tile, const f32x4 (&coef)[QF][G::F], f32x4 (&acc)[QF][G::DF], int lane) {
-  using T = typename G::T;
-  const int i16 = lane & 15, g = lane >> 4;
-  if constexpr (sizeof(T) == 2) {
+__device__ __forceinline__ void accumulate(const void* tile, const f32x4 (&coef)[QF][G::F], f32x4 (&acc)[QF][G::DF], const Lane<G>& at) {
+  if constexpr (sizeof(typename G::T) == 2) {
 #pragma unroll
     for (int p = 0; p < G::F / 2; ++p) {
       bf16x8 b[QF];
@@ -131,16 +209,9 @@ __device__ __forceinline__ void accumulate(const u32x4* tile, const f32x4 (&coef
       for (int j = 0; j < QF; ++j)
 #pragma unroll
         for (int r = 0; r < 4; ++r) b[j][r] = (bf16)coef[j][2 * p][r], b[j][4 + r] = (bf16)coef[j][2 * p + 1][r];
-      const int r0 = 32 * p + 8 * g + (i16 >> 2), r1 = r0 + 4;
-      const char* t0 = (const char*)(tile + r0 * G::NCH);
-      const char* t1 = (const char*)(tile + r1 * G::NCH);
-      const int s0 = G::swz(r0), s1 = G::swz(r1);
 #pragma unroll
       for (int fd = 0; fd < G::DF; ++fd) {
-        const int c = 4 * (fd >> 1) + (i16 & 3), half = 8 * (fd & 1);
-        const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((MG_LDS s16x4*)(t0 + (c ^ s0) * 16 + half));
-        const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((MG_LDS s16x4*)(t1 + (c ^ s1) * 16 + half));
-        const bf16x8 a = __builtin_bit_cast(bf16x8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+        const bf16x8 a = at.cols((const char*)tile, p, fd);
 #pragma unroll
         for (int j = 0; j < QF; ++j) acc[j][fd] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b[j], acc[j][fd], 0, 0, 0);
       }
@@ -149,17 +220,13 @@ __device__ __forceinline__ void accumulate(const u32x4* tile, const f32x4 (&coef
 #pragma unroll
     for (int f = 0; f < G::F; ++f)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int row = 16 * f + 4 * g + r, sw = G::swz(row);
-        const float* t = (const float*)(tile + row * G::NCH);
+      for (int r = 0; r < 4; ++r)
 #pragma unroll
         for (int fd = 0; fd < G::DF; ++fd) {
-          const int c = 8 * (fd >> 1) + 2 * (i16 >> 2) + (fd & 1);
-          const float a = t[(c ^ sw) * 4 + (i16 & 3)];
+          const float a = at.col1((const char*)tile, f, r, fd);
 #pragma unroll
           for (int j = 0; j < QF; ++j) acc[j][fd] = __builtin_amdgcn_mfma_f32_16x16x4f32(a, coef[j][f][r], acc[j][fd], 0, 0, 0);
         }
-      }
   }
 }
 
@@ -205,42 +272,23 @@ __device__ __forceinline__ void accumulate_seen(const u32x4* tile, const f32x4 (
       for (int fd = 0; fd < G::DF; ++fd)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const int d = 32 * (fd >> 1) + 8 * g + 4 * (fd & 1) + e;
+          const int d = 16 * fd + 4 * g + e;
           acc[j][fd][e] = fmaf(c, (float)t[((d / G::CH) ^ sw) * G::CH + d % G::CH], acc[j][fd][e]);
         }
     }
   }
 }
 
-// tanh.  f32 operands: near zero by its series (to x^11: 2^-26 of the value at 0.35), so that a score keeps its relative precision
-// through the cap; bf16 operands carry 2^-9 themselves, there the quotient does everywhere.
+// Four neighbouring columns of an owner row, scaled.
 template <class T>
-__device__ __forceinline__ float blk_tanh(float x) {
-  const float big = fmaf(-2.0f, mg_rcp(__builtin_amdgcn_exp2f(x * (2.f * LOG2E)) + 1.0f), 1.0f);
-  if constexpr (sizeof(T) == 2) return big;
-  const float y = x * x;
-  const float s = fmaf(y, fmaf(y, fmaf(y, fmaf(y, fmaf(y, -0.0088632355f, 0.0218694885f), -0.0539682540f), 0.1333333333f), -0.3333333333f), 1.f) * x;
-  return fabsf(x) < 0.35f ? s : big;
-}
-
-__device__ __forceinline__ float blk_dist(int axes, float ax, float ay, float bx, float by) {
-  const float dx = ax - bx;
-  if (axes == 1) return fabsf(dx);
-  const float dy = ay - by;
-  return __builtin_amdgcn_sqrtf(fmaf(dx, dx, dy * dy));
-}
-
-// Eight neighbouring columns of an owner row, scaled.
-template <class T>
-__device__ __forceinline__ void store_pair(T* p, const f32x4& a, const f32x4& b, float scale) {
+__device__ __forceinline__ void store4(T* p, const f32x4& a, float scale) {
   if constexpr (sizeof(T) == 2) {
-    bf16x8 x;
+    bf16x4 x;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) x[r] = (bf16)(a[r] * scale), x[4 + r] = (bf16)(b[r] * scale);
-    *(bf16x8*)p = x;
+    for (int r = 0; r < 4; ++r) x[r] = (bf16)(a[r] * scale);
+    *(bf16x4*)p = x;
   } else {
     *(f32x4*)p = a * scale;
-    *(f32x4*)(p + 4) = b * scale;
   }
 }
 

@@ -49,11 +49,13 @@ __global__ __launch_bounds__(256) void blk_spans_kernel(BlkAttnArgs p, int np) {
 }
 
 // A workgroup: 64 QF query rows of one head, four waves of 16 QF rows each; keys and values in tiles of BK rows, two buffers.
-template <class T, int DP, int QF, bool EXTRA>
-__global__ __launch_bounds__(256) void blk_attn_fwd_kernel(BlkAttnArgs p, int np) {
+template <class T, int DP, int QF, int X>
+__global__ __launch_bounds__(256, 2) void blk_attn_fwd_kernel(BlkAttnArgs p, int np) {
   using G = Geo<T, DP>;
+  using W = Soft<T, X>;
+  constexpr int AXES = W::AXES;
   __shared__ u32x4 lk[2][G::TILE], lv[2][G::TILE];
-  __shared__ float lx[2][2][64];
+  __shared__ __attribute__((aligned(16))) float lx[2][2][64];
   const int lane = mg_lane(), wave = mg_wave(), i16 = lane & 15, g = lane >> 4;
   const int h = blockIdx.x % p.H, hk = h / (p.H / p.Hkv);
   const int qt = gridDim.x / p.H - 1 - (int)(blockIdx.x / p.H);  // the rows at the end first: behind a causal mask they see the most
@@ -82,10 +84,8 @@ __global__ __launch_bounds__(256) void blk_attn_fwd_kernel(BlkAttnArgs p, int np
     const T* row = (const T*)p.q + rc * p.q_row + h * p.q_head;
 #pragma unroll
     for (int s = 0; s < G::SK; ++s) q[j][s] = owner_chunk(row, 4 * s + g, nd);
-    if (EXTRA && p.axes) {
-      qx[j] = p.xy[(long)rc * p.axes];
-      qy[j] = p.axes > 1 ? p.xy[(long)rc * p.axes + 1] : 0.f;
-    }
+    qx[j] = AXES ? p.xy[(long)rc * AXES] : 0.f;
+    qy[j] = AXES > 1 ? p.xy[(long)rc * AXES + 1] : 0.f;
   }
 #pragma unroll
   for (int o = 1; o < 16; o <<= 1) {
@@ -102,7 +102,7 @@ __global__ __launch_bounds__(256) void blk_attn_fwd_kernel(BlkAttnArgs p, int np
   auto fetch = [&](int k0, int buf) {
     copy_tile<G>(kb, p.k_row, k0, glo, ghi, nd, lk[buf]);
     copy_tile<G>(vb, p.v_row, k0, glo, ghi, nd, lv[buf]);
-    if (EXTRA && wave < p.axes) copy_meta(p.kv_xy, p.axes, wave, k0, p.M, lx[buf][wave]);
+    if (wave < AXES) copy_meta(p.kv_xy, AXES, wave, k0, p.M, lx[buf][wave]);
   };
 
   f32x4 acc[QF][G::DF];
@@ -114,8 +114,9 @@ __global__ __launch_bounds__(256) void blk_attn_fwd_kernel(BlkAttnArgs p, int np
 #pragma unroll
     for (int d = 0; d < G::DF; ++d) acc[j][d] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
-  using W = Soft<T, EXTRA>;
-  const float c2 = p.scale * LOG2E, slope = EXTRA && p.axes ? p.slopes[h] : 0.f, icap = EXTRA && p.cap > 0.f ? p.scale / p.cap : 0.f;
+  const W soft(p, AXES ? p.slopes[h] : 0.f);
+  Lane<G> at;
+  at.init(lane);
 
   if (glo < ghi) fetch(glo, 0);
   int buf = 0;
@@ -124,30 +125,23 @@ __global__ __launch_bounds__(256) void blk_attn_fwd_kernel(BlkAttnArgs p, int np
     if (k0 + G::BK < ghi) fetch(k0 + G::BK, buf ^ 1);
     if (k0 >= whi || k0 + G::BK <= wlo) continue;  // (the wave's: nothing of this tile is seen)
     f32x4 s[QF][G::F];
-    scores<G, QF>(lk[buf], q, s, lane);
+    scores<G, QF>(lk[buf], q, s, at);
     const bool part = k0 < flo || k0 + G::BK > fhi;
-    if (EXTRA) {
+    if (!W::RAW) {
 #pragma unroll
       for (int f = 0; f < G::F; ++f) {
         const int kr = G::row4(f, g);
+        f32x4 bx = {}, by = {};
+        if (AXES) bx = *(const f32x4*)&lx[buf][0][kr];
+        if (AXES > 1) by = *(const f32x4*)&lx[buf][1][kr];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const float bx = p.axes ? lx[buf][0][kr + r] : 0.f, by = p.axes > 1 ? lx[buf][1][kr + r] : 0.f;
+        for (int r = 0; r < 4; ++r)
 #pragma unroll
           for (int j = 0; j < QF; ++j) {
-            float x = s[j][f][r];
-            x = p.cap > 0.f ? p.cap * blk_tanh<T>(x * icap) : x * p.scale;
-            if (p.axes) x = fmaf(-slope, blk_dist(p.axes, qx[j], qy[j], bx, by), x);
-            s[j][f][r] = x;
+            float fac, dist;
+            s[j][f][r] = soft.score(s[j][f][r], qx[j], qy[j], bx[r], by[r], fac, dist);
           }
-        }
       }
-    }
-    if (W::NATURAL && !EXTRA) {
-#pragma unroll
-      for (int j = 0; j < QF; ++j)
-#pragma unroll
-        for (int f = 0; f < G::F; ++f) s[j][f] *= p.scale;
     }
     if (part) {
 #pragma unroll
@@ -164,9 +158,9 @@ __global__ __launch_bounds__(256) void blk_attn_fwd_kernel(BlkAttnArgs p, int np
       float t = -INFINITY;
 #pragma unroll
       for (int f = 0; f < G::F; ++f) t = fmaxf(t, fmaxf(fmaxf(s[j][f][0], s[j][f][1]), fmaxf(s[j][f][2], s[j][f][3])));
-      t = quarters_max(t) * (W::NATURAL ? 1.f : c2);
+      t = quarters_max(t) * (W::RAW ? soft.c : 1.f);
       if (__ballot(t > m[j])) {
-        const float mn = fmaxf(m[j], t), al = __builtin_amdgcn_exp2f(mn == -INFINITY ? 0.f : (m[j] - mn) * (W::NATURAL ? LOG2E : 1.f));
+        const float mn = fmaxf(m[j], t), al = mn == -INFINITY ? 1.f : W::ratio(m[j], mn);
         m[j] = mn;
         l[j] *= al;
 #pragma unroll
@@ -178,7 +172,7 @@ __global__ __launch_bounds__(256) void blk_attn_fwd_kernel(BlkAttnArgs p, int np
       for (int f = 0; f < G::F; ++f)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const float e = W::weight(s[j][f][r], mm, c2);
+          const float e = soft.weight(s[j][f][r], mm);
           s[j][f][r] = e;
           sum += e;
         }
@@ -187,7 +181,7 @@ __global__ __launch_bounds__(256) void blk_attn_fwd_kernel(BlkAttnArgs p, int np
     if (part && tile_not_finite<G>(lv[buf], lane))
       accumulate_seen<G, QF>(lv[buf], s, acc, lane, [&](int j, int row) { return k0 + row >= lo[j] && k0 + row < hi[j]; });
     else
-      accumulate<G, QF>(lv[buf], s, acc, lane);
+      accumulate<G, QF>(lv[buf], s, acc, at);
   }
 
 #pragma unroll
@@ -199,12 +193,12 @@ __global__ __launch_bounds__(256) void blk_attn_fwd_kernel(BlkAttnArgs p, int np
       p.lse[(long)h * p.N + r] = m[j];
       p.lse[(long)(p.H + h) * p.N + r] = inv;
     }
-    const long at = ((long)r * p.H + h) * p.D;
+    const long o = ((long)r * p.H + h) * p.D;
 #pragma unroll
-    for (int d = 0; d < G::DF; d += 2)
-      if (16 * d + 8 * g < p.D) {
-        store_pair<T>((T*)p.out + at + 16 * d + 8 * g, acc[j][d], acc[j][d + 1], inv);
-        if (sizeof(T) == 2 && p.out32) store_pair<float>(p.out32 + at + 16 * d + 8 * g, acc[j][d], acc[j][d + 1], inv);
+    for (int d = 0; d < G::DF; ++d)
+      if (16 * d + 4 * g < p.D) {
+        store4<T>((T*)p.out + o + 16 * d + 4 * g, acc[j][d], inv);
+        if (sizeof(T) == 2 && p.out32) store4<float>(p.out32 + o + 16 * d + 4 * g, acc[j][d], inv);
       }
   }
 }
@@ -213,10 +207,11 @@ __global__ __launch_bounds__(256) void blk_attn_fwd_kernel(BlkAttnArgs p, int np
 // instruction) and one of `splits` shares of the row's keys; its four waves take the share's tiles in turn, each with LDS of its own and
 // no barrier between them: what counts is bytes in flight (two tiles of keys and values a wave, 64 KB a CU at width 128).  Shares leave
 // maximum, sum and unnormalised output, which blk_attn_join_kernel puts together in their order.
-template <class T, int DP, bool EXTRA>
+template <class T, int DP, int X>
 __global__ __launch_bounds__(256) void blk_attn_row_kernel(BlkAttnArgs p, int splits, int hgroups, float* part) {
   using G = Geo<T, DP, 64 / (int)sizeof(T)>;
-  using W = Soft<T, EXTRA>;
+  using W = Soft<T, X>;
+  constexpr int AXES = W::AXES;
   constexpr int LOADS = 2 * G::TILE / 64;  // copies of a tile of keys and one of values
   __shared__ u32x4 tiles[4][2][2][G::TILE];
   __shared__ int scene;
@@ -243,9 +238,10 @@ __global__ __launch_bounds__(256) void blk_attn_row_kernel(BlkAttnArgs p, int sp
 #pragma unroll
   for (int s = 0; s < G::SK; ++s)
     q[0][s] = mine ? owner_chunk((const T*)p.q + r * p.q_row + head * p.q_head, 4 * s + g, nd) : u32x4{0, 0, 0, 0};
-  const float qx = EXTRA && p.axes ? p.xy[(long)r * p.axes] : 0.f, qy = EXTRA && p.axes > 1 ? p.xy[(long)r * p.axes + 1] : 0.f;
-  const float slope = EXTRA && p.axes && mine ? p.slopes[head] : 0.f, icap = EXTRA && p.cap > 0.f ? p.scale / p.cap : 0.f, c2 = p.scale * LOG2E;
-
+  const float qx = AXES ? p.xy[(long)r * AXES] : 0.f, qy = AXES > 1 ? p.xy[(long)r * AXES + 1] : 0.f;
+  const W soft(p, AXES && mine ? p.slopes[head] : 0.f);
+  Lane<G> at;
+  at.init(lane);
   f32x4 acc[1][G::DF];
 #pragma unroll
   for (int d = 0; d < G::DF; ++d) acc[0][d] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -265,7 +261,7 @@ __global__ __launch_bounds__(256) void blk_attn_row_kernel(BlkAttnArgs p, int sp
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     }
     f32x4 s[1][G::F];
-    scores<G, 1>(tiles[wave][buf][0], q, s, lane);
+    scores<G, 1>(tiles[wave][buf][0], q, s, at);
     float t = -INFINITY;
 #pragma unroll
     for (int f = 0; f < G::F; ++f)
@@ -273,22 +269,18 @@ __global__ __launch_bounds__(256) void blk_attn_row_kernel(BlkAttnArgs p, int sp
       for (int e = 0; e < 4; ++e) {
         const int key = k0 + G::row4(f, g) + e;
         float x = s[0][f][e];
-        if (EXTRA) {
-          x = p.cap > 0.f ? p.cap * blk_tanh<T>(x * icap) : x * p.scale;
-          if (p.axes) {
-            const long at = (long)min(key, p.M - 1) * p.axes;
-            x = fmaf(-slope, blk_dist(p.axes, qx, qy, p.kv_xy[at], p.axes > 1 ? p.kv_xy[at + 1] : 0.f), x);
-          }
-        } else if (W::NATURAL) {
-          x *= p.scale;
+        if (!W::RAW) {
+          const long k = (long)min(key, p.M - 1) * AXES;
+          float fac, dist;
+          x = soft.score(x, qx, qy, AXES ? p.kv_xy[k] : 0.f, AXES > 1 ? p.kv_xy[k + 1] : 0.f, fac, dist);
         }
         x = key < hi ? x : -INFINITY;
         s[0][f][e] = x;
         t = fmaxf(t, x);
       }
-    t = quarters_max(t) * (W::NATURAL ? 1.f : c2);
+    t = quarters_max(t) * (W::RAW ? soft.c : 1.f);
     if (__ballot(t > m)) {
-      const float mn = fmaxf(m, t), al = __builtin_amdgcn_exp2f(mn == -INFINITY ? 0.f : (m - mn) * (W::NATURAL ? LOG2E : 1.f));
+      const float mn = fmaxf(m, t), al = mn == -INFINITY ? 1.f : W::ratio(m, mn);
       m = mn;
       l *= al;
 #pragma unroll
@@ -299,10 +291,10 @@ __global__ __launch_bounds__(256) void blk_attn_row_kernel(BlkAttnArgs p, int sp
     for (int f = 0; f < G::F; ++f)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        s[0][f][e] = W::weight(s[0][f][e], mm, c2);
+        s[0][f][e] = soft.weight(s[0][f][e], mm);
         l += s[0][f][e];
       }
-    accumulate<G, 1>(tiles[wave][buf][1], s, acc, lane);
+    accumulate<G, 1>(tiles[wave][buf][1], s, acc, at);
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (this tile is read before the next copy goes into it)
   }
   l = quarters_sum(l);
@@ -315,7 +307,7 @@ __global__ __launch_bounds__(256) void blk_attn_row_kernel(BlkAttnArgs p, int sp
 #pragma unroll
   for (int d = 0; d < G::DF; ++d)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) so[(32 * (d >> 1) + 8 * g + 4 * (d & 1) + e) * 16 + i16] = acc[0][d][e];
+    for (int e = 0; e < 4; ++e) so[(16 * d + 4 * g + e) * 16 + i16] = acc[0][d][e];
   __syncthreads();
   const int heads = min(16, group - hg * 16);
   for (int i = threadIdx.x; i < heads * p.D; i += 256) {
@@ -326,7 +318,7 @@ __global__ __launch_bounds__(256) void blk_attn_row_kernel(BlkAttnArgs p, int sp
     float lt = 0.f, o = 0.f;
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
-      const float mw = sm[w * 32 + hh], f = __builtin_amdgcn_exp2f(mt == -INFINITY ? 0.f : (mw - mt) * (W::NATURAL ? LOG2E : 1.f));
+      const float f = mt == -INFINITY ? 1.f : W::ratio(sm[w * 32 + hh], mt);
       lt = fmaf(f, sm[w * 32 + 16 + hh], lt);
       o = fmaf(f, sm[128 + (w * DP + d) * 16 + hh], o);
     }
@@ -351,7 +343,7 @@ __global__ __launch_bounds__(128) void blk_attn_join_kernel(BlkAttnArgs p, int s
   float lt = 0.f, o = 0.f;
   for (int s = 0; s < splits; ++s) {
     const float* x = in + (long)s * (p.D + 4);
-    const float f = __builtin_amdgcn_exp2f(mt == -INFINITY ? 0.f : (x[p.D] - mt) * (NATURAL ? LOG2E : 1.f));
+    const float f = mt == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((x[p.D] - mt) * (NATURAL ? LOG2E : 1.f));
     lt = fmaf(f, x[p.D + 1], lt);
     if (d < p.D) o = fmaf(f, x[d], o);
   }
@@ -368,39 +360,33 @@ int row_splits(const BlkAttnArgs& p) {
   return n < 1 ? 1 : n > 64 ? 64 : (int)n;
 }
 
-template <class T, int DP>
-void launch_fwd(const BlkAttnArgs& p, hipStream_t st) {
-  const bool extra = p.cap > 0.f || p.axes > 0;
+template <class T, int DP, int X>
+void launch_fwd_x(const BlkAttnArgs& p, hipStream_t st) {
   const int splits = row_splits(p);
   if (splits) {
     const int hgroups = cdiv(p.H / p.Hkv, 16);
     const dim3 grid((unsigned)((long)p.N * p.Hkv * hgroups * splits));
-    if (extra)
-      MG_LAUNCH((blk_attn_row_kernel<T, DP, true>), grid, dim3(256), 0, st, p, splits, hgroups, (float*)p.ws);
-    else
-      MG_LAUNCH((blk_attn_row_kernel<T, DP, false>), grid, dim3(256), 0, st, p, splits, hgroups, (float*)p.ws);
-    if (splits > 1) {
-      if (extra || sizeof(T) == 4)
-        MG_LAUNCH((blk_attn_join_kernel<T, true>), dim3(p.N * p.H), dim3(128), 0, st, p, splits, (const float*)p.ws);
-      else
-        MG_LAUNCH((blk_attn_join_kernel<T, false>), dim3(p.N * p.H), dim3(128), 0, st, p, splits, (const float*)p.ws);
-    }
+    MG_LAUNCH((blk_attn_row_kernel<T, DP, X>), grid, dim3(256), 0, st, p, splits, hgroups, (float*)p.ws);
+    if (splits > 1)
+      MG_LAUNCH((blk_attn_join_kernel<T, Soft<T, X>::NATURAL>), dim3(p.N * p.H), dim3(128), 0, st, p, splits, (const float*)p.ws);
     return;
   }
   const int np = cdiv(p.N, 128) * 128;
   MG_LAUNCH(blk_spans_kernel, dim3(np / 64), dim3(256), 0, st, p, np);
-  const bool wide = (long)cdiv(p.N, 128) * p.H >= 256;  // enough workgroups of 128 rows to fill the chip
-  const dim3 grid(cdiv(p.N, wide ? 128 : 64) * p.H);
-  if (wide) {
-    if (extra)
-      MG_LAUNCH((blk_attn_fwd_kernel<T, DP, 2, true>), grid, dim3(256), 0, st, p, np);
-    else
-      MG_LAUNCH((blk_attn_fwd_kernel<T, DP, 2, false>), grid, dim3(256), 0, st, p, np);
-  } else {
-    if (extra)
-      MG_LAUNCH((blk_attn_fwd_kernel<T, DP, 1, true>), grid, dim3(256), 0, st, p, np);
-    else
-      MG_LAUNCH((blk_attn_fwd_kernel<T, DP, 1, false>), grid, dim3(256), 0, st, p, np);
+  if ((long)cdiv(p.N, 128) * p.H >= 256)  // enough workgroups of 128 rows to fill the chip
+    MG_LAUNCH((blk_attn_fwd_kernel<T, DP, 2, X>), dim3(cdiv(p.N, 128) * p.H), dim3(256), 0, st, p, np);
+  else
+    MG_LAUNCH((blk_attn_fwd_kernel<T, DP, 1, X>), dim3(cdiv(p.N, 64) * p.H), dim3(256), 0, st, p, np);
+}
+template <class T, int DP>
+void launch_fwd(const BlkAttnArgs& p, hipStream_t st) {
+  switch ((p.cap > 0.f ? 1 : 0) + 2 * p.axes) {
+    case 0: return launch_fwd_x<T, DP, 0>(p, st);
+    case 1: return launch_fwd_x<T, DP, 1>(p, st);
+    case 2: return launch_fwd_x<T, DP, 2>(p, st);
+    case 3: return launch_fwd_x<T, DP, 3>(p, st);
+    case 4: return launch_fwd_x<T, DP, 4>(p, st);
+    default: return launch_fwd_x<T, DP, 5>(p, st);
   }
 }
 template <class T>

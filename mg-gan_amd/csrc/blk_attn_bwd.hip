@@ -11,30 +11,13 @@ int blk_attn_check(const BlkAttnArgs* a, const char* name);
 
 namespace {
 
-// One score and what its gradient needs: fac = d(capped score)/d(score).
-template <class T>
-__device__ __forceinline__ void extra_score(float& x, float& fac, float& dist, const BlkAttnArgs& p, float icap, float slope, float ax, float ay,
-                                            float bx, float by) {
-  fac = 1.f;
-  if (p.cap > 0.f) {
-    const float t = blk_tanh<T>(x * icap);
-    fac = fmaf(-t, t, 1.f);
-    x = p.cap * t;
-  } else {
-    x *= p.scale;
-  }
-  dist = 0.f;
-  if (p.axes) {
-    dist = blk_dist(p.axes, ax, ay, bx, by);
-    x = fmaf(-slope, dist, x);
-  }
-}
-
-template <class T, int DP, int QF, bool EXTRA>
-__global__ __launch_bounds__(256) void blk_attn_dq_kernel(BlkAttnArgs p, int np, float* delta, float* slope_part) {
+template <class T, int DP, int QF, int X>
+__global__ __launch_bounds__(256, 2) void blk_attn_dq_kernel(BlkAttnArgs p, int np, float* delta, float* slope_part) {
   using G = Geo<T, DP>;
+  using W = Soft<T, X>;
+  constexpr int AXES = W::AXES;
   __shared__ u32x4 lk[2][G::TILE], lv[2][G::TILE];
-  __shared__ float lx[2][2][64];
+  __shared__ __attribute__((aligned(16))) float lx[2][2][64];
   const int lane = mg_lane(), wave = mg_wave(), i16 = lane & 15, g = lane >> 4;
   const int h = blockIdx.x % p.H, hk = h / (p.H / p.Hkv);
   const int nqt = gridDim.x / p.H, qt = nqt - 1 - (int)(blockIdx.x / p.H);
@@ -81,10 +64,8 @@ __global__ __launch_bounds__(256) void blk_attn_dq_kernel(BlkAttnArgs p, int np,
     top[j] = p.lse[(long)h * p.N + rc];
     inv[j] = p.lse[(long)(p.H + h) * p.N + rc];
     if (r < p.N && g == 0) delta[(long)h * p.N + r] = dsum[j];
-    if (EXTRA && p.axes) {
-      qx[j] = p.xy[(long)rc * p.axes];
-      qy[j] = p.axes > 1 ? p.xy[(long)rc * p.axes + 1] : 0.f;
-    }
+    qx[j] = AXES ? p.xy[(long)rc * AXES] : 0.f;
+    qy[j] = AXES > 1 ? p.xy[(long)rc * AXES + 1] : 0.f;
   }
 #pragma unroll
   for (int o = 1; o < 16; o <<= 1) {
@@ -101,7 +82,7 @@ __global__ __launch_bounds__(256) void blk_attn_dq_kernel(BlkAttnArgs p, int np,
   auto fetch = [&](int k0, int buf) {
     copy_tile<G>(kb, p.k_row, k0, glo, ghi, nd, lk[buf]);
     copy_tile<G>(vb, p.v_row, k0, glo, ghi, nd, lv[buf]);
-    if (EXTRA && wave < p.axes) copy_meta(p.kv_xy, p.axes, wave, k0, p.M, lx[buf][wave]);
+    if (wave < AXES) copy_meta(p.kv_xy, AXES, wave, k0, p.M, lx[buf][wave]);
   };
 
   f32x4 acc[QF][G::DF];
@@ -112,8 +93,9 @@ __global__ __launch_bounds__(256) void blk_attn_dq_kernel(BlkAttnArgs p, int np,
   // the slopes' gradient is f32 and a sum over all pairs, so it takes the rows' sum(P dO V^T) from the same P: -sum (P dP dist) + sum(P dP)
   // sum(P dist) row by row, with nothing in it that was rounded to the operands' type
   float sa[QF] = {}, sb[QF] = {}, sc[QF] = {};
-  using W = Soft<T, EXTRA>;
-  const float c2 = p.scale * LOG2E, slope = EXTRA && p.axes ? p.slopes[h] : 0.f, icap = EXTRA && p.cap > 0.f ? p.scale / p.cap : 0.f;
+  const W soft(p, AXES ? p.slopes[h] : 0.f);
+  Lane<G> at;
+  at.init(lane);
 
   if (glo < ghi) fetch(glo, 0);
   int buf = 0;
@@ -122,55 +104,51 @@ __global__ __launch_bounds__(256) void blk_attn_dq_kernel(BlkAttnArgs p, int np,
     if (k0 + G::BK < ghi) fetch(k0 + G::BK, buf ^ 1);
     if (k0 >= whi || k0 + G::BK <= wlo) continue;
     f32x4 s[QF][G::F], dp[QF][G::F];
-    scores<G, QF>(lk[buf], q, s, lane);
-    scores<G, QF>(lv[buf], dO, dp, lane);
+    scores<G, QF>(lk[buf], q, s, at);
+    scores<G, QF>(lv[buf], dO, dp, at);
     const bool part = k0 < flo || k0 + G::BK > fhi;
     float ta[QF] = {}, tb[QF] = {}, tc[QF] = {};
 #pragma unroll
     for (int f = 0; f < G::F; ++f) {
       const int kr = G::row4(f, g);
+      f32x4 bx = {}, by = {};
+      if (AXES) bx = *(const f32x4*)&lx[buf][0][kr];
+      if (AXES > 1) by = *(const f32x4*)&lx[buf][1][kr];
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const float bx = EXTRA && p.axes ? lx[buf][0][kr + r] : 0.f, by = EXTRA && p.axes > 1 ? lx[buf][1][kr + r] : 0.f;
+      for (int r = 0; r < 4; ++r)
 #pragma unroll
         for (int j = 0; j < QF; ++j) {
-          float x = s[j][f][r], fac = 1.f, dist = 0.f, w, dl;
-          if (EXTRA) {
-            extra_score<T>(x, fac, dist, p, icap, slope, qx[j], qy[j], bx, by);
-          } else if (W::NATURAL) {
-            x *= p.scale;
-          }
-          w = W::weight(x, top[j], c2) * inv[j];
-          dl = w * (dp[j][f][r] - dsum[j]);
-          if (EXTRA) dl *= fac;
+          float x = s[j][f][r], fac = 1.f, dist = 0.f;
+          if (!W::RAW) x = soft.score(x, qx[j], qy[j], bx[r], by[r], fac, dist);
+          float w = soft.weight(x, top[j]) * inv[j], dl = w * (dp[j][f][r] - dsum[j]);
+          if (W::CAP) dl *= fac;
           float wd = w * dp[j][f][r];
           if (part) {
             const int key = k0 + kr + r;
             const bool seen = key >= lo[j] && key < hi[j];
             dl = seen ? dl : 0.f;
-            if (EXTRA) {
+            if (AXES) {
               w = seen ? w : 0.f;
               wd = seen ? wd : 0.f;
               dist = seen ? dist : 0.f;
             }
           }
-          if (EXTRA && p.dslopes) {
+          if (AXES) {
             ta[j] = fmaf(wd, dist, ta[j]);
             tb[j] = fmaf(w, dist, tb[j]);
             tc[j] += wd;
           }
           s[j][f][r] = dl;
         }
-      }
     }
-    if (EXTRA && p.dslopes) {
+    if (AXES) {
 #pragma unroll
       for (int j = 0; j < QF; ++j) sa[j] += ta[j], sb[j] += tb[j], sc[j] += tc[j];
     }
     if (part && tile_not_finite<G>(lk[buf], lane))
       accumulate_seen<G, QF>(lk[buf], s, acc, lane, [&](int j, int row) { return k0 + row >= lo[j] && k0 + row < hi[j]; });
     else
-      accumulate<G, QF>(lk[buf], s, acc, lane);
+      accumulate<G, QF>(lk[buf], s, acc, at);
   }
 
 #pragma unroll
@@ -179,10 +157,10 @@ __global__ __launch_bounds__(256) void blk_attn_dq_kernel(BlkAttnArgs p, int np,
     if (r >= p.N) continue;
     T* out = (T*)p.dq + ((long)r * p.H + h) * p.D;
 #pragma unroll
-    for (int d = 0; d < G::DF; d += 2)
-      if (16 * d + 8 * g < p.D) store_pair<T>(out + 16 * d + 8 * g, acc[j][d], acc[j][d + 1], p.scale);
+    for (int d = 0; d < G::DF; ++d)
+      if (16 * d + 4 * g < p.D) store4<T>(out + 16 * d + 4 * g, acc[j][d], p.scale);
   }
-  if (EXTRA && p.dslopes) {
+  if (AXES && p.dslopes) {
     float slope_sum = 0.f;
 #pragma unroll
     for (int j = 0; j < QF; ++j) {
@@ -208,9 +186,11 @@ __global__ __launch_bounds__(64) void blk_slopes_kernel(const float* part, int n
 }
 
 // A workgroup: 64 QF keys of one key head; the queries of every head that shares it, in tiles of BK rows.
-template <class T, int DP, int QF, bool EXTRA>
-__global__ __launch_bounds__(256) void blk_attn_dkv_kernel(BlkAttnArgs p, int np, const float* delta) {
+template <class T, int DP, int QF, int X>
+__global__ __launch_bounds__(256, 2) void blk_attn_dkv_kernel(BlkAttnArgs p, int np, const float* delta) {
   using G = Geo<T, DP>;
+  using W = Soft<T, X>;
+  constexpr int AXES = W::AXES;
   __shared__ u32x4 lq[2][G::TILE], lo_[2][G::TILE];
   __shared__ __attribute__((aligned(16))) float lm[2][7][64];  // of each streamed row: largest score, sum(dO O), lo, hi, x, y, 1 / sum
   __shared__ int range[2];
@@ -245,18 +225,16 @@ __global__ __launch_bounds__(256) void blk_attn_dkv_kernel(BlkAttnArgs p, int np
       k[j][s] = owner_chunk(kr, 4 * s + g, nd);
       v[j][s] = owner_chunk(vr, 4 * s + g, nd);
     }
-    if (EXTRA && p.axes) {
-      kx[j] = p.kv_xy[(long)rc * p.axes];
-      ky[j] = p.axes > 1 ? p.kv_xy[(long)rc * p.axes + 1] : 0.f;
-    }
+    kx[j] = AXES ? p.kv_xy[(long)rc * AXES] : 0.f;
+    ky[j] = AXES > 1 ? p.kv_xy[(long)rc * AXES + 1] : 0.f;
   }
   f32x4 dk[QF][G::DF], dv[QF][G::DF];
 #pragma unroll
   for (int j = 0; j < QF; ++j)
 #pragma unroll
     for (int d = 0; d < G::DF; ++d) dk[j][d] = dv[j][d] = f32x4{0.f, 0.f, 0.f, 0.f};
-  using W = Soft<T, EXTRA>;
-  const float c2 = p.scale * LOG2E, icap = EXTRA && p.cap > 0.f ? p.scale / p.cap : 0.f;
+  Lane<G> at;
+  at.init(lane);
 
   // (head, tile) pairs in one sequence, so that the copies of the next head's first tile are under way too
   const int nt = qb > qa ? (qb - qa + G::BK - 1) / G::BK : 0, total = nt * group;
@@ -269,7 +247,7 @@ __global__ __launch_bounds__(256) void blk_attn_dkv_kernel(BlkAttnArgs p, int np
     if (wave == 1) copy_meta(delta + (long)h * p.N, 1, 0, q0, p.N, lm[buf][1]);
     if (wave == 2) copy_meta(p.spans, 1, 0, q0, np, lm[buf][2]);
     if (wave == 3) copy_meta(p.spans + np, 1, 0, q0, np, lm[buf][3]);
-    if (EXTRA && wave < p.axes) copy_meta(p.xy, p.axes, wave, q0, p.N, lm[buf][4 + wave]);
+    if (wave < AXES) copy_meta(p.xy, AXES, wave, q0, p.N, lm[buf][4 + wave]);
   };
   if (total > 0) fetch(0, 0);
   for (int t = 0; t < total; ++t) {
@@ -284,37 +262,39 @@ __global__ __launch_bounds__(256) void blk_attn_dkv_kernel(BlkAttnArgs p, int np
     }
     if (slo >= w0 + 16 * QF || shi <= w0) continue;
     const bool part = w0 < flo || w0 + 16 * QF > fhi;
-    const float slope = EXTRA && p.axes ? p.slopes[h] : 0.f;
+    const W soft(p, AXES ? p.slopes[h] : 0.f);
     f32x4 s[QF][G::F], dp[QF][G::F];
-    scores<G, QF>(lq[buf], k, s, lane);
-    scores<G, QF>(lo_[buf], v, dp, lane);
+    scores<G, QF>(lq[buf], k, s, at);
+    scores<G, QF>(lo_[buf], v, dp, at);
 #pragma unroll
     for (int f = 0; f < G::F; ++f) {
       const int qr = G::row4(f, g);
       const f32x4 top = *(const f32x4*)&lm[buf][0][qr], dsum = *(const f32x4*)&lm[buf][1][qr], inv = *(const f32x4*)&lm[buf][6][qr];
+      f32x4 ax = {}, ay = {};
+      if (AXES) ax = *(const f32x4*)&lm[buf][4][qr];
+      if (AXES > 1) ay = *(const f32x4*)&lm[buf][5][qr];
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const float ax = EXTRA && p.axes ? lm[buf][4][qr + r] : 0.f, ay = EXTRA && p.axes > 1 ? lm[buf][5][qr + r] : 0.f;
+      for (int r = 0; r < 4; ++r)
 #pragma unroll
         for (int j = 0; j < QF; ++j) {
-          float x = s[j][f][r], fac = 1.f, dist, w, dl;
-          if (EXTRA) {
-            extra_score<T>(x, fac, dist, p, icap, slope, ax, ay, kx[j], ky[j]);
-          } else if (W::NATURAL) {
-            x *= p.scale;
-          }
-          w = W::weight(x, top[r], c2) * inv[r];
-          dl = w * (dp[j][f][r] - dsum[r]);
-          if (EXTRA) dl *= fac;
-          if (part) {
-            const int key = w0 + 16 * j + i16;
-            const bool seen = key >= __float_as_int(lm[buf][2][qr + r]) && key < __float_as_int(lm[buf][3][qr + r]);
-            w = seen ? w : 0.f;
-            dl = seen ? dl : 0.f;
-          }
+          float x = s[j][f][r], fac = 1.f, dist;
+          if (!W::RAW) x = soft.score(x, ax[r], ay[r], kx[j], ky[j], fac, dist);
+          float w = soft.weight(x, top[r]) * inv[r], dl = w * (dp[j][f][r] - dsum[r]);
+          if (W::CAP) dl *= fac;
           s[j][f][r] = w;
           dp[j][f][r] = dl;
         }
+      if (part) {
+        const f32x4 from = *(const f32x4*)&lm[buf][2][qr], to = *(const f32x4*)&lm[buf][3][qr];
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int j = 0; j < QF; ++j) {
+            const int key = w0 + 16 * j + i16;
+            const bool seen = key >= __float_as_int(from[r]) && key < __float_as_int(to[r]);
+            s[j][f][r] = seen ? s[j][f][r] : 0.f;
+            dp[j][f][r] = seen ? dp[j][f][r] : 0.f;
+          }
       }
     }
     auto sees = [&](int j, int row) {
@@ -325,39 +305,44 @@ __global__ __launch_bounds__(256) void blk_attn_dkv_kernel(BlkAttnArgs p, int np
       accumulate_seen<G, QF>(lo_[buf], s, dv, lane, sees);
       accumulate_seen<G, QF>(lq[buf], dp, dk, lane, sees);
     } else {
-      accumulate<G, QF>(lo_[buf], s, dv, lane);
-      accumulate<G, QF>(lq[buf], dp, dk, lane);
+      accumulate<G, QF>(lo_[buf], s, dv, at);
+      accumulate<G, QF>(lq[buf], dp, dk, at);
     }
   }
 #pragma unroll
   for (int j = 0; j < QF; ++j) {
     const int r = w0 + 16 * j + i16;
     if (r >= p.M) continue;
-    const long at = ((long)r * p.Hkv + hk) * p.D;
+    const long o = ((long)r * p.Hkv + hk) * p.D;
 #pragma unroll
-    for (int d = 0; d < G::DF; d += 2)
-      if (16 * d + 8 * g < p.D) {
-        store_pair<T>((T*)p.dk + at + 16 * d + 8 * g, dk[j][d], dk[j][d + 1], p.scale);
-        store_pair<T>((T*)p.dv + at + 16 * d + 8 * g, dv[j][d], dv[j][d + 1], 1.f);
+    for (int d = 0; d < G::DF; ++d)
+      if (16 * d + 4 * g < p.D) {
+        store4<T>((T*)p.dk + o + 16 * d + 4 * g, dk[j][d], p.scale);
+        store4<T>((T*)p.dv + o + 16 * d + 4 * g, dv[j][d], 1.f);
       }
   }
 }
 
-template <class T, int DP, int QF, bool EXTRA>
-void launch_bwd_tile(const BlkAttnArgs& p, hipStream_t st) {
+template <class T, int DP, int X>
+void launch_bwd_x(const BlkAttnArgs& p, hipStream_t st) {
+  constexpr int QF = 1;
   const int np = cdiv(p.N, 128) * 128, nqt = cdiv(p.N, 64 * QF);
   float* delta = (float*)p.ws;
   float* part = delta + (size_t)p.H * p.N;
-  MG_LAUNCH((blk_attn_dq_kernel<T, DP, QF, EXTRA>), dim3(nqt * p.H), dim3(256), 0, st, p, np, delta, part);
-  if (EXTRA && p.dslopes) MG_LAUNCH(blk_slopes_kernel, dim3(p.H), dim3(64), 0, st, (const float*)part, nqt, p.dslopes);
-  MG_LAUNCH((blk_attn_dkv_kernel<T, DP, QF, EXTRA>), dim3(cdiv(p.M, 64 * QF) * p.Hkv), dim3(256), 0, st, p, np, (const float*)delta);
+  MG_LAUNCH((blk_attn_dq_kernel<T, DP, QF, X>), dim3(nqt * p.H), dim3(256), 0, st, p, np, delta, part);
+  if (X > 1 && p.dslopes) MG_LAUNCH(blk_slopes_kernel, dim3(p.H), dim3(64), 0, st, (const float*)part, nqt, p.dslopes);
+  MG_LAUNCH((blk_attn_dkv_kernel<T, DP, QF, X>), dim3(cdiv(p.M, 64 * QF) * p.Hkv), dim3(256), 0, st, p, np, (const float*)delta);
 }
 template <class T, int DP>
 void launch_bwd(const BlkAttnArgs& p, hipStream_t st) {
-  if (p.cap > 0.f || p.axes > 0)
-    launch_bwd_tile<T, DP, 1, true>(p, st);
-  else
-    launch_bwd_tile<T, DP, 1, false>(p, st);
+  switch ((p.cap > 0.f ? 1 : 0) + 2 * p.axes) {
+    case 0: return launch_bwd_x<T, DP, 0>(p, st);
+    case 1: return launch_bwd_x<T, DP, 1>(p, st);
+    case 2: return launch_bwd_x<T, DP, 2>(p, st);
+    case 3: return launch_bwd_x<T, DP, 3>(p, st);
+    case 4: return launch_bwd_x<T, DP, 4>(p, st);
+    default: return launch_bwd_x<T, DP, 5>(p, st);
+  }
 }
 template <class T>
 void launch_bwd_width(const BlkAttnArgs& p, hipStream_t st) {

@@ -42,6 +42,9 @@ struct GemmP {
   float* part;  // split reduction: (splits, M, N or 2 N)
 };
 
+#ifndef BLK_W256
+#define BLK_W256 4
+#endif
 enum { EPI_LINEAR = 0, EPI_GATED = 1 };
 
 template <class T, int W>
@@ -120,23 +123,22 @@ __device__ __forceinline__ void epilogue(const GemmP& p, int m, int n, float (&v
   store_n<T, W>((T*)p.C + (long)m * p.ldc + n, vec, left, v);
 }
 
-// One operand of a tile in LDS: R outputs by 128 bytes of k, filled by NT threads.  The copies land lane by lane, so the swizzle that
+// One operand of a tile in LDS: R outputs by 64 bytes of k, filled by NT threads.  The copies land lane by lane, so the swizzle that
 // keeps a wave's reads off each other's banks is in which chunk a lane fetches.
-//   rows:    [R][8 chunks], chunk c of row r at c ^ s(r): a wave reads one chunk of 16 rows, rows 0-15 or {0-3, 8-11, 16-19, 24-27} (+4);
+//   rows:    [R][4 chunks], chunk c of row r at c ^ s(r): a wave reads one chunk of 16 rows, rows 0-15 or {0-3, 8-11, 16-19, 24-27} (+4);
 //            any eight lanes of either set fall on eight bank groups.
-//   columns: [128 / sizeof(T) values of k][R / CH chunks]: bf16 is read by the transposing LDS read (16 lanes take 4 k x 16 columns: four
+//   columns: [64 / sizeof(T) values of k][R / CH chunks]: bf16 is read by the transposing LDS read (16 lanes take 4 k x 16 columns: four
 //            rows of two chunks each, on eight bank groups), f32 element by element (4 k x 16 columns: two passes, the least for 256 bytes).
 template <class T, int R, int NT, bool COLS>
 struct Side {
-  static constexpr int CH = Mf<T>::CH, L = R * 8 / NT, NC = COLS ? R / CH : 8;
+  static constexpr int CH = Mf<T>::CH, KS = 4 * CH, L = R * 4 / NT, NC = COLS ? R / CH : 4, SIZE = R * 4;
   const char* src[L];
   int c;         // the chunk this lane copies
   long step;     // bytes from one k step to the next
   int k_row;     // columns: the k of this lane's first copy
-  bool in, all;  // columns: the chunk lies inside the operand, the wave's all do
 
   static __device__ __forceinline__ int swz(int r) {
-    if (!COLS) return (r & 7) ^ ((r >> 1) & 4);
+    if (!COLS) return ((r >> 1) & 3) ^ ((r >> 2) & 2);
     return sizeof(T) == 2 ? (r & 3) << 1 : r & 4;
   }
   // base(row) -> first byte of an operand row; o0: the tile's first output, cols: columns that may be read, k0: first k
@@ -144,43 +146,36 @@ struct Side {
   __device__ __forceinline__ void init(Base base, long ld, int o0, int cols, long k0) {
     const int tid = threadIdx.x;
     if constexpr (!COLS) {
-      c = (tid & 7) ^ swz(tid >> 3);  // (a lane's rows differ by multiples of 16)
-      step = 128;
+      c = (tid & 3) ^ swz(tid >> 2);  // (a lane's rows differ by multiples of 16)
+      step = 64;
 #pragma unroll
-      for (int i = 0; i < L; ++i) src[i] = base((i * NT + tid) >> 3, true) + k0 * sizeof(T) + c * 16;
+      for (int i = 0; i < L; ++i) src[i] = base((i * NT + tid) >> 2, true) + k0 * sizeof(T) + c * 16;
     } else {
       k_row = tid / NC;  // (a lane's k differ by NT / NC: multiples of 8)
-      c = (tid % NC) ^ swz(k_row);
-      in = o0 + c * CH < cols;
-      all = __all(in);
-      step = ld * (128 / sizeof(T)) * sizeof(T);
+      c = min((tid % NC) ^ swz(k_row), (cols - o0) / CH - 1);  // (outputs past the end are not stored: any column will do for them)
+      step = ld * KS * sizeof(T);
 #pragma unroll
       for (int i = 0; i < L; ++i) src[i] = base(0, false) + ((k0 + k_row + i * (NT / NC)) * ld + o0) * sizeof(T) + c * 16;
     }
   }
-  // the copies of one k step into d; `left`: k from this step's first to the end
+  // the copies of one k step into d; WHOLE: it lies inside k, else `left` values of k do and zeros stand for the rest
+  template <bool WHOLE>
   __device__ __forceinline__ void fetch(u32x4* d, int left, const char* zeros) {
     d += mg_wave() * 64;
-    if (!COLS ? left >= 128 / (int)sizeof(T) : left >= 128 / (int)sizeof(T) && all) {
 #pragma unroll
-      for (int i = 0; i < L; ++i) lds_copy16(src[i], d + i * NT);
-    } else {  // what lies past the end of k, or of the columns, comes from a page of zeros
-#pragma unroll
-      for (int i = 0; i < L; ++i) {
-        const bool ok = COLS ? in && k_row + i * (NT / NC) < left : c * CH < left;
-        lds_copy16(ok ? src[i] : zeros, d + i * NT);
-      }
+    for (int i = 0; i < L; ++i) {
+      const bool ok = WHOLE || (COLS ? k_row + i * (NT / NC) < left : c * CH < left);
+      lds_copy16(ok ? src[i] : zeros, d + i * NT);
+      src[i] += step;
     }
-#pragma unroll
-    for (int i = 0; i < L; ++i) src[i] += step;
   }
-  // fragment of 16 outputs for the s-th half of the step: rows given by `row` (this lane's), columns by their first
-  static __device__ __forceinline__ u32x4 frag(const u32x4* t, int row, int first, int s, int lane) {
+  // fragment of 16 outputs: rows given by `row` (this lane's), columns by their first
+  static __device__ __forceinline__ u32x4 frag(const u32x4* t, int row, int first, int lane) {
     const int i16 = lane & 15, g = lane >> 4;
     if constexpr (!COLS) {
-      return t[row * 8 + ((4 * s + g) ^ swz(row))];
+      return t[row * 4 + (g ^ swz(row))];
     } else if constexpr (sizeof(T) == 2) {
-      const int k = 32 * s + 8 * g + (i16 >> 2), sw = swz(k), ch = (first >> 3) + ((i16 & 3) >> 1);
+      const int k = 8 * g + (i16 >> 2), sw = swz(k), ch = (first >> 3) + ((i16 & 3) >> 1);
       const char* a = (const char*)(t + k * NC + (ch ^ sw)) + 8 * (i16 & 1);
       const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((MG_LDS s16x4*)a);
       const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((MG_LDS s16x4*)(a + 4 * NC * 16));  // (k + 4: the same swizzle)
@@ -189,7 +184,7 @@ struct Side {
       u32x4 v;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const int k = 16 * s + 4 * g + e, col = first + i16;
+        const int k = 4 * g + e, col = first + i16;
         v[e] = ((const unsigned*)(t + k * NC + ((col >> 2) ^ swz(k))))[col & 3];
       }
       return v;
@@ -197,14 +192,24 @@ struct Side {
   }
 };
 
-// A tile of BM x BN outputs, WM x WN waves; k in steps of 128 bytes, two LDS buffers: the copies of step t+1 are under way while step t
-// is multiplied.
+// Waits until at most n of this wave's copies are under way (they end in their order), then for the other waves.
+template <int n>
+__device__ __forceinline__ void wait_copies() {
+  asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(n) : "memory");
+}
+
+// A tile of BM x BN outputs, WM x WN waves; k in steps of 64 bytes through a ring of four LDS buffers.  In step t the copies of step
+// t+3 start, the fragments of step t+1 are read into registers and those of step t are multiplied: the matrix cores wait neither for
+// memory (two steps of slack) nor for LDS (one step).
 template <class T, int BM, int BN, int WM, int WN, int EPI, bool SPLIT, bool CA, bool CB>
 __global__ __launch_bounds__(WM* WN * 64) void blk_gemm_kernel(GemmP p) {
-  constexpr int NT = WM * WN * 64, CH = Mf<T>::CH, KS = 8 * CH;
+  constexpr int NT = WM * WN * 64, CH = Mf<T>::CH, KS = 4 * CH;
   constexpr int TM = BM / WM, TN = BN / WN, FM = TM / 16, FN = TN / 16;
   constexpr int NB = EPI == EPI_GATED ? BN / 2 : BN;  // output columns of the tile
-  __shared__ u32x4 lds[2][(BM + BN) * 8];
+  using SA = Side<T, BM, NT, CA>;
+  using SB = Side<T, BN, NT, CB>;
+  constexpr int BUF = SA::SIZE + SB::SIZE, LOADS = SA::L + SB::L;
+  __shared__ u32x4 lds[4 * BUF];
 
   int t = blockIdx.x;
   {  // neighbouring tiles to the same XCD (blocks are dealt round the eight of them), in columns of eight row tiles
@@ -215,10 +220,10 @@ __global__ __launch_bounds__(WM* WN * 64) void blk_gemm_kernel(GemmP p) {
   const int m0 = (8 * grp + rem % gm) * BM, n0 = (rem / gm) * NB;
   const int lane = mg_lane(), wave = mg_wave(), i16 = lane & 15, g = lane >> 4;
   const int steps = (p.K + KS - 1) / KS;
-  const int kt0 = SPLIT ? blockIdx.y * p.kt_split : 0, kt1 = SPLIT ? min(kt0 + p.kt_split, steps) : steps;
+  const int kt0 = SPLIT ? blockIdx.y * p.kt_split : 0, n = (SPLIT ? min(kt0 + p.kt_split, steps) : steps) - kt0;
 
-  Side<T, BM, NT, CA> sa;
-  Side<T, BN, NT, CB> sb;
+  SA sa;
+  SB sb;
   sa.init([&](int row, bool rows) { return (const char*)p.A + (rows ? (long)min(m0 + row, p.M - 1) * p.lda * sizeof(T) : 0); }, p.lda, m0,
           p.ca, (long)kt0 * KS);
   auto base_b = [&](bool second) {
@@ -229,14 +234,23 @@ __global__ __launch_bounds__(WM* WN * 64) void blk_gemm_kernel(GemmP p) {
   };
   const bool second = CB && p.seg && kt0 >= p.seg;
   sb.init(base_b(second), p.ldb, n0, p.cb, (long)(second ? kt0 - p.seg : kt0) * KS);
-  auto fetch = [&](int kt, int buf) {
+  auto fetch = [&](int t) {
+    const int kt = kt0 + t;
     int kb = kt;
     if (CB && p.seg && kt >= p.seg) {
       kb -= p.seg;
-      if (kb == 0 && kt != kt0) sb.init(base_b(true), p.ldb, n0, p.cb, 0);
+      if (kb == 0 && t) sb.init(base_b(true), p.ldb, n0, p.cb, 0);
     }
-    sa.fetch(&lds[buf][0], p.K - kt * KS, (const char*)blk_zeros);
-    sb.fetch(&lds[buf][BM * 8], (CB ? p.kb : p.K) - kb * KS, (const char*)blk_zeros);
+    u32x4* d = lds + (t & 3) * BUF;
+    const int la = p.K - kt * KS, lb = (CB ? p.kb : p.K) - kb * KS;
+    if (la >= KS)
+      sa.template fetch<true>(d, la, (const char*)blk_zeros);
+    else
+      sa.template fetch<false>(d, la, (const char*)blk_zeros);
+    if (lb >= KS)
+      sb.template fetch<true>(d + SA::SIZE, lb, (const char*)blk_zeros);
+    else
+      sb.template fetch<false>(d + SA::SIZE, lb, (const char*)blk_zeros);
   };
 
   f32x4 acc[FN][FM];
@@ -255,25 +269,76 @@ __global__ __launch_bounds__(WM* WN * 64) void blk_gemm_kernel(GemmP p) {
     rb[f] = (EPI == EPI_GATED ? (f / (FN / 2)) * NB + wn * (TN / 2) : wn * TN);
     rb[f] += CB ? 16 * q : 32 * (q >> 1) + 8 * (i16 >> 2) + 4 * (q & 1) + (i16 & 3);
   }
+  struct Frags {
+    u32x4 a[FM], b[FN];
+  };
+  auto read = [&](int t, Frags& f) {
+    const u32x4* la = lds + (t & 3) * BUF;
+    const u32x4* lb = la + SA::SIZE;
+#pragma unroll
+    for (int i = 0; i < FN; ++i) f.b[i] = SB::frag(lb, rb[i], rb[i], lane);
+#pragma unroll
+    for (int j = 0; j < FM; ++j) f.a[j] = SA::frag(la, wm * TM + 16 * j + i16, wm * TM + 16 * j, lane);
+  };
+  auto multiply = [&](const Frags& f) {
+#pragma unroll
+    for (int i = 0; i < FN; ++i)
+#pragma unroll
+      for (int j = 0; j < FM; ++j) acc[i][j] = Mf<T>::step(f.b[i], f.a[j], acc[i][j]);
+  };
+  // a step whose copies and multiplications are all there: straight code, in which the reads of the next fragments and the copies are
+  // dealt out among the multiplications
+  auto steady = [&](int t, const Frags& now, Frags& next) {
+    wait_copies<LOADS>();
+    read(t + 1, next);
+    u32x4* d = lds + ((t + 3) & 3) * BUF;
+    sa.template fetch<true>(d, 0, nullptr);
+    sb.template fetch<true>(d + SA::SIZE, 0, nullptr);
+    multiply(now);
+    constexpr int READS = (CA ? (sizeof(T) == 2 ? 2 : 4) : 1) * FM + (CB ? (sizeof(T) == 2 ? 2 : 4) : 1) * FN;
+    constexpr int MM = FM * FN * (sizeof(T) == 2 ? 1 : 4), EACH = MM / (READS + LOADS) > 0 ? MM / (READS + LOADS) : 1;
+#pragma unroll
+    for (int i = 0; i < READS; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);     // an LDS read
+      __builtin_amdgcn_sched_group_barrier(0x008, EACH, 0);  // multiplications
+    }
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);  // a copy
+      __builtin_amdgcn_sched_group_barrier(0x008, EACH, 0);
+    }
+  };
+  auto any = [&](int t, const Frags& now, Frags& next) {
+    if (t + 2 < n)
+      wait_copies<LOADS>();
+    else
+      wait_copies<0>();
+    if (t + 3 < n) fetch(t + 3);
+    read(t + 1 < n ? t + 1 : t, next);  // (after the last step: read again, not used)
+    multiply(now);
+  };
 
-  if (kt0 < kt1) fetch(kt0, 0);
-  for (int kt = kt0; kt < kt1; ++kt) {
-    const int buf = (kt - kt0) & 1;
-    __syncthreads();  // (waits for this step's copies; everyone is done reading the other buffer)
-    if (kt + 1 < kt1) fetch(kt + 1, buf ^ 1);
-    const u32x4* la = &lds[buf][0];
-    const u32x4* lb = &lds[buf][BM * 8];
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      u32x4 fa[FM], fb[FN];
-#pragma unroll
-      for (int j = 0; j < FM; ++j) fa[j] = sa.frag(la, wm * TM + 16 * j + i16, wm * TM + 16 * j, s, lane);
-#pragma unroll
-      for (int i = 0; i < FN; ++i) fb[i] = sb.frag(lb, rb[i], rb[i], s, lane);
-#pragma unroll
-      for (int i = 0; i < FN; ++i)
-#pragma unroll
-        for (int j = 0; j < FM; ++j) acc[i][j] = Mf<T>::step(fb[i], fa[j], acc[i][j]);
+  if (n > 0) {
+    Frags f0, f1;
+    fetch(0);
+    if (n > 1) fetch(1);
+    if (n > 2) fetch(2);
+    if (n > 2)
+      wait_copies<2 * LOADS>();
+    else
+      wait_copies<0>();
+    read(0, f0);
+    int t = 0;
+    if (!(CB && p.seg)) {
+      const int whole = min(p.K / KS - kt0, n);  // (steps that lie inside k)
+      for (; t + 4 < whole; t += 2) {
+        steady(t, f0, f1);
+        steady(t + 1, f1, f0);
+      }
+    }
+    for (; t < n; t += 2) {
+      any(t, f0, f1);
+      if (t + 1 < n) any(t + 1, f1, f0);
     }
   }
 
@@ -285,7 +350,7 @@ __global__ __launch_bounds__(WM* WN * 64) void blk_gemm_kernel(GemmP p) {
     if (m >= p.M) continue;
 #pragma unroll
     for (int f = 0; f < FO; f += P) {
-      const int n = n0 + wn * (FO * 16) + 16 * f + W * g;
+      const int n = n0 + wn * (FO * 16) + 16 * f + W * g;  // (the lane's first output)
       float v[W], u[W];
 #pragma unroll
       for (int e = 0; e < W; ++e) {
@@ -442,7 +507,7 @@ struct Plan {
 };
 Plan plan_of(int M, int N, long K, int ch, bool gated) {
   const int half = gated ? 2 : 1;
-  const long steps = (K + 8 * ch - 1) / (8 * ch);
+  const long steps = (K + 4 * ch - 1) / (4 * ch);
   Plan best = {};
   double least = 1e30;
   const int tiles[3] = {256, 128, 64};
@@ -450,7 +515,7 @@ Plan plan_of(int M, int N, long K, int ch, bool gated) {
     const int b = tiles[i];
     const long nt = (long)cdiv(M, b) * cdiv(N, b / half);
     // cycles of one step of one tile on a CU, per workgroup with the CU to itself; a CU holds `res` of them
-    const double flops = 2. * b * b * 8 * ch, rate = ch == 4 ? (b == 256 ? 230. : b == 128 ? 220. : 200.) : (b == 256 ? 2600. : b == 128 ? 1900. : 1000.);
+    const double flops = 2. * b * b * 4 * ch, rate = ch == 4 ? (b == 256 ? 230. : b == 128 ? 220. : 200.) : (b == 256 ? 2600. : b == 128 ? 1900. : 1000.);
     const int res = b == 256 ? 1 : b == 128 ? 2 : 4;
     for (int splits = 1; splits <= 64 && splits <= steps; splits *= 2) {
       if (splits > 1 && nt * splits > 2048) break;
@@ -491,7 +556,7 @@ int gemm(GemmP p, void* ws, hipStream_t st) {
   const Plan q = plan_of(p.M, p.N, p.K, Mf<T>::CH, EPI == EPI_GATED);
   p.part = (float*)ws;
   switch (q.tile) {
-    case 256: return gemm_tile<T, 256, 2, 4, EPI, CA, CB>(p, q, st);
+    case 256: return gemm_tile<T, 256, 2, BLK_W256, EPI, CA, CB>(p, q, st);
     case 128: return gemm_tile<T, 128, 2, 2, EPI, CA, CB>(p, q, st);
     default: return gemm_tile<T, 64, 4, 1, EPI, CA, CB>(p, q, st);
   }
@@ -554,7 +619,7 @@ template <class T, bool GATED>
 int layer_bwd(const BlkLayerArgs& l, Arena ws, size_t* need, hipStream_t st) {
   constexpr int CH = Mf<T>::CH, two = GATED ? 2 : 1;
   const long tiles = cdiv(l.M, DZ_ROWS);
-  const long off = up(l.N, GATED ? 8 * CH : CH), ldz = two * off;  // (gated: dU starts with a step of dX's product)
+  const long off = up(l.N, GATED ? 4 * CH : CH), ldz = two * off;  // (gated: dU starts with a step of dX's product)
   const bool plain = !GATED && l.act == ACT_NONE && off == l.N;    // dZ is dY
   const Padded<T, GATED> o(l, ws, !need, l.dw != nullptr, l.dx != nullptr, st);
   void* dz = plain ? nullptr : ws.take((size_t)l.M * ldz * sizeof(T));
@@ -578,7 +643,7 @@ int layer_bwd(const BlkLayerArgs& l, Arena ws, size_t* need, hipStream_t st) {
   p.act = ACT_NONE;
   p.A = plain ? l.dy : dz, p.lda = ldz, p.ldc = l.K, p.N = l.K;
   if (l.dx) {
-    p.B = o.w, p.B2 = o.w2, p.ldb = o.Kp, p.cb = o.Kp, p.kb = l.N, p.seg = GATED ? (int)(off / (8 * CH)) : 0;
+    p.B = o.w, p.B2 = o.w2, p.ldb = o.Kp, p.cb = o.Kp, p.kb = l.N, p.seg = GATED ? (int)(off / (4 * CH)) : 0;
     p.M = l.M, p.K = (int)ldz, p.C = l.dx;
     const int rc = gemm<T, EPI_LINEAR, false, true>(p, part, st);
     if (rc != MGGAN_OK) return rc;

@@ -143,7 +143,7 @@ def _layer_bwd(ctx, dy):
     (x, ldx), (N, K) = _rows(x, w.shape[1]), w.shape
     M, dev, dt = x.shape[0], x.device, x.dtype
     code = _DTYPES[dt]
-    off = -(-N // (128 // x.element_size())) * (128 // x.element_size()) if gated else 0  # where the up weight's gradient starts
+    off = -(-N // (64 // x.element_size())) * (64 // x.element_size()) if gated else 0  # where the up weight's gradient starts
     make = torch.empty if M else torch.zeros
     dx = make(M, K, dtype=dt, device=dev) if need[0] else None
     dw = make(off + N, K, dtype=dt, device=dev) if need[1] or need[2] else None
