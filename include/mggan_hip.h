@@ -677,8 +677,8 @@ size_t mggan_block_attention_span_ints(int rows);
 size_t mggan_block_attention_fwd_workspace(int rows, int keys, int heads, int kv_heads, int width, int scenes);
 int mggan_block_attention_fwd(const void* args, mggan_stream_t stream);
 /* dq, dk, dv, and dslopes (H) if not NULL, written in a fixed order of summation; out32, lse, spans as the forward call left them.
- * ws: mggan_block_attention_bwd_workspace bytes. */
-size_t mggan_block_attention_bwd_workspace(int rows, int heads);
+ * ws: mggan_block_attention_bwd_workspace bytes, 256-byte aligned. */
+size_t mggan_block_attention_bwd_workspace(int rows, int keys, int heads, int kv_heads, int width);
 int mggan_block_attention_bwd(const void* args, mggan_stream_t stream);
 
 #ifdef __cplusplus

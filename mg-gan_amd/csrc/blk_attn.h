@@ -18,7 +18,7 @@ struct BlkAttnArgs {  // mirrored by mggan/hip/blocks.py
   float* dslopes;
   const int *scenes, *kv_scenes, *prefix;
   const float *xy, *kv_xy, *slopes;
-  float* lse;    // (2, H, N): the row's largest score (as the exponent takes it) and one over its sum of exp(score - largest)
+  float* lse;    // (2, H, N): what the exponents of a row's weights were taken less (about its largest), and one over the weights' sum
   float* out32;  // the output before it is rounded (f32: the output): what sum(dO O) is formed of -- from the rounded one every row's
                  // gradient would carry a common error, which the sums over rows (the slopes' gradient) do not average away
   int* spans;   // mggan_block_attention_span_ints(N): lo, hi, and {min lo, max hi, max lo, min hi} of every 32 rows
@@ -47,9 +47,11 @@ __device__ __forceinline__ float blk_tanh(float x) {
 }
 
 // What is done to a score q.k, by the kernels' template argument X: bit 0 a cap, bits 1-2 the axes of the distance.
-// Scores are exponentiated as exp2((s - max) log2e) where their last bits matter (f32; scores with a distance, whose slopes' gradient is
-// f32): log2e rounded into the scores first would stretch all of them by a common 2^-25, which shows in the slopes' gradient.  The others
-// (bf16, gradients rounded at 2^-9) are kept times log2e and take exp2(s - max), an operation less.
+// Weights are exp2(s E - top), one fused operation, with top = max s E.  E = log2e over scores in their own units where the last bits
+// matter (f32; scores with a distance, whose slopes' gradient is f32): scale log2e and slope log2e rounded into one factor first would
+// stretch all scores by a common 2^-25, which shows in the slopes' gradient (log2e itself is 2^-26 off, top's rounding divides out).
+// bf16, with gradients rounded at 2^-9: plain scores are left as the product gives them and E = scale log2e, capped ones are multiplied
+// by log2e with the cap and E = 1.
 template <class T, int X>
 struct Soft {
   static constexpr bool CAP = X & 1, NATURAL = (X >> 1) || sizeof(T) == 4;
@@ -79,14 +81,11 @@ struct Soft {
     if constexpr (AXES) x = fmaf(-slope, dist, x);
     return x;
   }
-  // whether scores are left as the product gives them and weight() multiplies (one operation for both)
-  static constexpr bool RAW = X == 0 && !NATURAL;
+  static constexpr bool RAW = X == 0 && !NATURAL;  // score() is not called
+  __device__ __forceinline__ float top(float s) const { return RAW ? s * c : NATURAL ? s * LOG2E : s; }
   __device__ __forceinline__ float weight(float s, float top) const {
-    if (RAW) return __builtin_amdgcn_exp2f(fmaf(s, c, -top));
-    return __builtin_amdgcn_exp2f(NATURAL ? (s - top) * LOG2E : s - top);
+    return __builtin_amdgcn_exp2f(RAW ? fmaf(s, c, -top) : NATURAL ? fmaf(s, LOG2E, -top) : s - top);
   }
-  // exp(a - b) of two maxima
-  static __device__ __forceinline__ float ratio(float a, float b) { return __builtin_amdgcn_exp2f(NATURAL ? (a - b) * LOG2E : a - b); }
 };
 
 template <class T_, int DP_, int BK_ = 128 / (int)sizeof(T_)>
@@ -159,6 +158,7 @@ struct Lane {
 // The workgroup's (threads = 256) or one wave's (64) work.
 template <class G, int threads = 256>
 __device__ __forceinline__ void copy_tile(const typename G::T* base, long row_stride, int first, int lo, int hi, int nd, u32x4* lds) {
+  static_assert(G::TILE % threads == 0, "a tile is copied in whole passes");
   const int wave = threads == 64 ? 0 : mg_wave();
 #pragma unroll
   for (int i = 0; i < G::TILE / threads; ++i) {
@@ -181,19 +181,26 @@ __device__ __forceinline__ u32x4 owner_chunk(const T* row, int c, int nd) {
   return u32x4{0, 0, 0, 0};
 }
 
-// D fragments of scores: sum over the width of streamed rows x owner rows.
+// D fragments of scores: sum over the width of streamed rows x owner rows.  The reads of a fragment's rows are issued before the
+// multiplications of the one before (and no earlier: left to itself the compiler reads everything ahead and runs out of registers).
 template <class G, int QF>
 __device__ __forceinline__ void scores(const void* tile, const u32x4 (&own)[QF][G::SK], f32x4 (&out)[QF][G::F], const Lane<G>& at) {
+  u32x4 a[2][G::SK];
+#pragma unroll
+  for (int s = 0; s < G::SK; ++s) a[0][s] = at.rows((const char*)tile, 0, s);
 #pragma unroll
   for (int f = 0; f < G::F; ++f) {
+    if (f + 1 < G::F) {
+#pragma unroll
+      for (int s = 0; s < G::SK; ++s) a[(f + 1) & 1][s] = at.rows((const char*)tile, f + 1, s);
+    }
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int j = 0; j < QF; ++j) out[j][f] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int s = 0; s < G::SK; ++s) {
-      const u32x4 a = at.rows((const char*)tile, f, s);
+    for (int s = 0; s < G::SK; ++s)
 #pragma unroll
-      for (int j = 0; j < QF; ++j) out[j][f] = Mf<typename G::T>::step(a, own[j][s], out[j][f]);
-    }
+      for (int j = 0; j < QF; ++j) out[j][f] = Mf<typename G::T>::step(a[f & 1][s], own[j][s], out[j][f]);
   }
 }
 
@@ -202,18 +209,28 @@ __device__ __forceinline__ void scores(const void* tile, const u32x4 (&own)[QF][
 template <class G, int QF>
 __device__ __forceinline__ void accumulate(const void* tile, const f32x4 (&coef)[QF][G::F], f32x4 (&acc)[QF][G::DF], const Lane<G>& at) {
   if constexpr (sizeof(typename G::T) == 2) {
+    constexpr int C = G::DF % 4 == 0 ? 4 : 2;  // column fragments read together
 #pragma unroll
     for (int p = 0; p < G::F / 2; ++p) {
-      bf16x8 b[QF];
+      bf16x8 a[2][C], b[QF];
+#pragma unroll
+      for (int c = 0; c < C; ++c) a[0][c] = at.cols((const char*)tile, p, c);
 #pragma unroll
       for (int j = 0; j < QF; ++j)
 #pragma unroll
         for (int r = 0; r < 4; ++r) b[j][r] = (bf16)coef[j][2 * p][r], b[j][4 + r] = (bf16)coef[j][2 * p + 1][r];
 #pragma unroll
-      for (int fd = 0; fd < G::DF; ++fd) {
-        const bf16x8 a = at.cols((const char*)tile, p, fd);
+      for (int k = 0; k < G::DF / C; ++k) {
+        if (k + 1 < G::DF / C) {
 #pragma unroll
-        for (int j = 0; j < QF; ++j) acc[j][fd] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b[j], acc[j][fd], 0, 0, 0);
+          for (int c = 0; c < C; ++c) a[(k + 1) & 1][c] = at.cols((const char*)tile, p, (k + 1) * C + c);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+          for (int j = 0; j < QF; ++j)
+            acc[j][k * C + c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[k & 1][c], b[j], acc[j][k * C + c], 0, 0, 0);
       }
     }
   } else {
@@ -246,37 +263,94 @@ __device__ __forceinline__ bool tile_not_finite(const u32x4* tile, int lane) {
   }
   return __ballot(bad) != 0;
 }
-// accumulate() row by row over the places that `sees` only: the way of tiles that are partly masked AND hold such a value.
+// accumulate() for a tile that is partly masked AND holds such values: they are taken as zeros, and where a row sees one (a second product,
+// of where they are with what `sees`) the sum becomes the infinity or the NaN that it would have been.  It is in a second copy of the
+// kernels' loops (SAFE) that a workgroup runs, from the start, only if its first run came upon such a tile: beside the plain way in one
+// loop it would cost every run 40 to 100 registers.
 template <class G, int QF, class See>
-__device__ __forceinline__ void accumulate_seen(const u32x4* tile, const f32x4 (&coef)[QF][G::F], f32x4 (&acc)[QF][G::DF], int lane, See sees) {
-  using T = typename G::T;
-  const int i16 = lane & 15, g = lane >> 4;
-  for (int row = 0; row < G::BK; ++row) {
-    int f, gg, r = row & 3;
-    if (sizeof(T) == 2)
-      f = 2 * (row >> 5) + ((row >> 2) & 1), gg = (row >> 3) & 3;
-    else
-      f = row >> 4, gg = (row >> 2) & 3;
-    const T* t = (const T*)(tile + row * G::NCH);
-    const int sw = G::swz(row);
+__device__ __forceinline__ void accumulate_seen(const void* tile, const f32x4 (&coef)[QF][G::F], f32x4 (&acc)[QF][G::DF], const Lane<G>& at, int lane,
+                                                See sees) {
+  constexpr bool HALF = sizeof(typename G::T) == 2;
+  const int g = lane >> 4;
 #pragma unroll
-    for (int j = 0; j < QF; ++j) {
-      float c = 0.f;
+  for (int fd = 0; fd < G::DF; ++fd) {
+    f32x4 up[QF] = {}, down[QF] = {};
 #pragma unroll
-      for (int a = 0; a < G::F; ++a)
+    for (int p = 0; p < (HALF ? G::F / 2 : G::F * 4); ++p) {
+      if constexpr (HALF) {
+        const bf16x8 a = at.cols((const char*)tile, p, fd);
+        bf16x8 clean, hi, lo, b, one;
 #pragma unroll
-        for (int b = 0; b < 4; ++b) c = a == f && b == r ? coef[j][a][b] : c;
-      c = __shfl(c, i16 + 16 * gg, 64);
-      if (!sees(j, row)) continue;
-#pragma unroll
-      for (int fd = 0; fd < G::DF; ++fd)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int d = 16 * fd + 4 * g + e;
-          acc[j][fd][e] = fmaf(c, (float)t[((d / G::CH) ^ sw) * G::CH + d % G::CH], acc[j][fd][e]);
+        for (int e = 0; e < 8; ++e) {
+          const float x = (float)a[e];
+          const bool odd = !(fabsf(x) < INFINITY);
+          clean[e] = odd ? (bf16)0.f : a[e];
+          hi[e] = (bf16)(odd && !(x < 0.f) ? 1.f : 0.f);
+          lo[e] = (bf16)(odd && !(x > 0.f) ? 1.f : 0.f);
         }
+#pragma unroll
+        for (int j = 0; j < QF; ++j) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            b[e] = (bf16)coef[j][2 * p + (e >> 2)][e & 3];
+            one[e] = (bf16)(sees(j, 32 * p + 8 * g + e) ? 1.f : 0.f);
+          }
+          acc[j][fd] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(clean, b, acc[j][fd], 0, 0, 0);
+          up[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hi, one, up[j], 0, 0, 0);
+          down[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(lo, one, down[j], 0, 0, 0);
+        }
+      } else {
+        const float x = at.col1((const char*)tile, p >> 2, p & 3, fd);
+        const bool odd = !(fabsf(x) < INFINITY);
+#pragma unroll
+        for (int j = 0; j < QF; ++j) {
+          const float one = sees(j, 16 * (p >> 2) + 4 * g + (p & 3)) ? 1.f : 0.f;
+          acc[j][fd] = __builtin_amdgcn_mfma_f32_16x16x4f32(odd ? 0.f : x, coef[j][p >> 2][p & 3], acc[j][fd], 0, 0, 0);
+          up[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(odd && !(x < 0.f) ? 1.f : 0.f, one, up[j], 0, 0, 0);
+          down[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(odd && !(x > 0.f) ? 1.f : 0.f, one, down[j], 0, 0, 0);
+        }
+      }
     }
+#pragma unroll
+    for (int j = 0; j < QF; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (up[j][e] > 0.f) acc[j][fd][e] += INFINITY;
+        if (down[j][e] > 0.f) acc[j][fd][e] -= INFINITY;
+      }
+    __builtin_amdgcn_sched_barrier(0);
   }
+}
+
+// What 32 n rows from row r0 on see between them: the first and the end of it.
+template <int n>
+__device__ __forceinline__ int2 group_span(const BlkAttnArgs& p, int np, int r0) {
+  int lo = 0x7fffffff, hi = 0;
+#pragma unroll
+  for (int i = 0; i < n; ++i) {
+    const int4 s = *(const int4*)(p.spans + 2 * np + 4 * ((r0 >> 5) + i));
+    lo = min(lo, s.x);
+    hi = max(hi, s.y);
+  }
+  return make_int2(lo, hi);
+}
+// From the 16 lanes' own: the first and the end of what any row of the wave sees, and of what all do.
+__device__ __forceinline__ void wave_span(int& wlo, int& whi, int& flo, int& fhi) {
+#pragma unroll
+  for (int o = 1; o < 16; o <<= 1) {
+    wlo = min(wlo, __shfl_xor(wlo, o, 64));
+    whi = max(whi, __shfl_xor(whi, o, 64));
+    flo = max(flo, __shfl_xor(flo, o, 64));
+    fhi = min(fhi, __shfl_xor(fhi, o, 64));
+  }
+  wlo = __builtin_amdgcn_readfirstlane(wlo), whi = __builtin_amdgcn_readfirstlane(whi);
+  flo = __builtin_amdgcn_readfirstlane(flo), fhi = __builtin_amdgcn_readfirstlane(fhi);
+}
+
+// A value that the compiler knows nothing of: what is computed from it is not kept from an earlier computation.
+__device__ __forceinline__ int afresh(int x) {
+  asm volatile("" : "+v"(x));
+  return __builtin_amdgcn_readfirstlane(x);
 }
 
 // Four neighbouring columns of an owner row, scaled.

@@ -48,28 +48,13 @@ __global__ __launch_bounds__(256) void blk_spans_kernel(BlkAttnArgs p, int np) {
   if ((tid & 31) == 0) *(int4*)(p.spans + 2 * np + 4 * ((r0 + tid) >> 5)) = make_int4(v[0], v[1], v[2], v[3]);
 }
 
-// A workgroup: 64 QF query rows of one head, four waves of 16 QF rows each; keys and values in tiles of BK rows, two buffers.
-template <class T, int DP, int QF, int X>
-__global__ __launch_bounds__(256, 2) void blk_attn_fwd_kernel(BlkAttnArgs p, int np) {
+// 64 QF query rows of one head: four waves of 16 QF rows each (this one's start at w0); keys and values in tiles of BK rows, two buffers.
+template <class T, int DP, int QF, int X, bool SAFE>
+__device__ __forceinline__ void attn_fwd_rows(const BlkAttnArgs& p, int np, int h, int glo, int ghi, int w0, u32x4* lk, u32x4* lv, float* lx, int* odd) {
   using G = Geo<T, DP>;
   using W = Soft<T, X>;
   constexpr int AXES = W::AXES;
-  __shared__ u32x4 lk[2][G::TILE], lv[2][G::TILE];
-  __shared__ __attribute__((aligned(16))) float lx[2][2][64];
-  const int lane = mg_lane(), wave = mg_wave(), i16 = lane & 15, g = lane >> 4;
-  const int h = blockIdx.x % p.H, hk = h / (p.H / p.Hkv);
-  const int qt = gridDim.x / p.H - 1 - (int)(blockIdx.x / p.H);  // the rows at the end first: behind a causal mask they see the most
-  const int r0 = qt * 64 * QF, w0 = r0 + wave * 16 * QF;
-  const int nd = p.D / G::CH;
-
-  // what the workgroup's rows and this wave's rows see
-  int glo = INT_MAX, ghi = 0;
-#pragma unroll
-  for (int i = 0; i < 2 * QF; ++i) {
-    const int4 s = *(const int4*)(p.spans + 2 * np + 4 * ((r0 >> 5) + i));
-    glo = min(glo, s.x);
-    ghi = max(ghi, s.y);
-  }
+  const int lane = mg_lane(), wave = mg_wave(), i16 = lane & 15, g = lane >> 4, hk = h / (p.H / p.Hkv), nd = p.D / G::CH;
   int lo[QF], hi[QF], wlo = INT_MAX, whi = 0, flo = 0, fhi = INT_MAX;
   float qx[QF], qy[QF];
   u32x4 q[QF][G::SK];
@@ -87,22 +72,14 @@ __global__ __launch_bounds__(256, 2) void blk_attn_fwd_kernel(BlkAttnArgs p, int
     qx[j] = AXES ? p.xy[(long)rc * AXES] : 0.f;
     qy[j] = AXES > 1 ? p.xy[(long)rc * AXES + 1] : 0.f;
   }
-#pragma unroll
-  for (int o = 1; o < 16; o <<= 1) {
-    wlo = min(wlo, __shfl_xor(wlo, o, 64));
-    whi = max(whi, __shfl_xor(whi, o, 64));
-    flo = max(flo, __shfl_xor(flo, o, 64));
-    fhi = min(fhi, __shfl_xor(fhi, o, 64));
-  }
-  wlo = __builtin_amdgcn_readfirstlane(wlo), whi = __builtin_amdgcn_readfirstlane(whi);
-  flo = __builtin_amdgcn_readfirstlane(flo), fhi = __builtin_amdgcn_readfirstlane(fhi);
+  wave_span(wlo, whi, flo, fhi);
 
   const T* kb = (const T*)p.k + hk * p.k_head;
   const T* vb = (const T*)p.v + hk * p.v_head;
   auto fetch = [&](int k0, int buf) {
-    copy_tile<G>(kb, p.k_row, k0, glo, ghi, nd, lk[buf]);
-    copy_tile<G>(vb, p.v_row, k0, glo, ghi, nd, lv[buf]);
-    if (wave < AXES) copy_meta(p.kv_xy, AXES, wave, k0, p.M, lx[buf][wave]);
+    copy_tile<G>(kb, p.k_row, k0, glo, ghi, nd, lk + buf * G::TILE);
+    copy_tile<G>(vb, p.v_row, k0, glo, ghi, nd, lv + buf * G::TILE);
+    if (wave < AXES) copy_meta(p.kv_xy, AXES, wave, k0, p.M, lx + (2 * buf + wave) * 64);
   };
 
   f32x4 acc[QF][G::DF];
@@ -124,16 +101,17 @@ __global__ __launch_bounds__(256, 2) void blk_attn_fwd_kernel(BlkAttnArgs p, int
     __syncthreads();
     if (k0 + G::BK < ghi) fetch(k0 + G::BK, buf ^ 1);
     if (k0 >= whi || k0 + G::BK <= wlo) continue;  // (the wave's: nothing of this tile is seen)
+    const u32x4* tv = lv + buf * G::TILE;
     f32x4 s[QF][G::F];
-    scores<G, QF>(lk[buf], q, s, at);
+    scores<G, QF>(lk + buf * G::TILE, q, s, at);
     const bool part = k0 < flo || k0 + G::BK > fhi;
     if (!W::RAW) {
 #pragma unroll
       for (int f = 0; f < G::F; ++f) {
         const int kr = G::row4(f, g);
         f32x4 bx = {}, by = {};
-        if (AXES) bx = *(const f32x4*)&lx[buf][0][kr];
-        if (AXES > 1) by = *(const f32x4*)&lx[buf][1][kr];
+        if (AXES) bx = *(const f32x4*)(lx + 2 * buf * 64 + kr);
+        if (AXES > 1) by = *(const f32x4*)(lx + (2 * buf + 1) * 64 + kr);
 #pragma unroll
         for (int r = 0; r < 4; ++r)
 #pragma unroll
@@ -144,6 +122,7 @@ __global__ __launch_bounds__(256, 2) void blk_attn_fwd_kernel(BlkAttnArgs p, int
       }
     }
     if (part) {
+      if (!SAFE && tile_not_finite<G>(tv, lane)) *odd = 1;
 #pragma unroll
       for (int f = 0; f < G::F; ++f)
 #pragma unroll
@@ -158,9 +137,9 @@ __global__ __launch_bounds__(256, 2) void blk_attn_fwd_kernel(BlkAttnArgs p, int
       float t = -INFINITY;
 #pragma unroll
       for (int f = 0; f < G::F; ++f) t = fmaxf(t, fmaxf(fmaxf(s[j][f][0], s[j][f][1]), fmaxf(s[j][f][2], s[j][f][3])));
-      t = quarters_max(t) * (W::RAW ? soft.c : 1.f);
-      if (__ballot(t > m[j])) {
-        const float mn = fmaxf(m[j], t), al = mn == -INFINITY ? 1.f : W::ratio(m[j], mn);
+      t = soft.top(quarters_max(t));
+      if (__ballot(t > m[j] + 8.f)) {  // (weights up to 2^8 are as good: most tiles leave the sums as they are)
+        const float mn = fmaxf(m[j], t), al = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[j] - mn);
         m[j] = mn;
         l[j] *= al;
 #pragma unroll
@@ -178,10 +157,14 @@ __global__ __launch_bounds__(256, 2) void blk_attn_fwd_kernel(BlkAttnArgs p, int
         }
       l[j] += sum;
     }
-    if (part && tile_not_finite<G>(lv[buf], lane))
-      accumulate_seen<G, QF>(lv[buf], s, acc, lane, [&](int j, int row) { return k0 + row >= lo[j] && k0 + row < hi[j]; });
+    if (SAFE && part && tile_not_finite<G>(tv, lane))
+      accumulate_seen<G, QF>(tv, s, acc, at, lane, [&](int j, int row) { return k0 + row >= lo[j] && k0 + row < hi[j]; });
     else
-      accumulate<G, QF>(lv[buf], s, acc, at);
+      accumulate<G, QF>(tv, s, acc, at);
+  }
+  if (!SAFE) {
+    __syncthreads();
+    if (*odd) return;
   }
 
 #pragma unroll
@@ -200,6 +183,26 @@ __global__ __launch_bounds__(256, 2) void blk_attn_fwd_kernel(BlkAttnArgs p, int
         store4<T>((T*)p.out + o + 16 * d + 4 * g, acc[j][d], inv);
         if (sizeof(T) == 2 && p.out32) store4<float>(p.out32 + o + 16 * d + 4 * g, acc[j][d], inv);
       }
+  }
+}
+
+template <class T, int DP, int QF, int X>
+__global__ __launch_bounds__(256, 2) void blk_attn_fwd_kernel(BlkAttnArgs p, int np) {
+  using G = Geo<T, DP>;
+  __shared__ u32x4 lk[2 * G::TILE], lv[2 * G::TILE];
+  __shared__ __attribute__((aligned(16))) float lx[2 * 2 * 64];
+  __shared__ int odd;
+  const int h = blockIdx.x % p.H;
+  const int qt = gridDim.x / p.H - 1 - (int)(blockIdx.x / p.H);  // the rows at the end first: behind a causal mask they see the most
+  const int r0 = qt * 64 * QF, w0 = r0 + mg_wave() * 16 * QF;
+  if (threadIdx.x == 0) odd = 0;
+  __syncthreads();
+  const int2 keys = group_span<2 * QF>(p, np, r0);  // (what the workgroup's rows see)
+  attn_fwd_rows<T, DP, QF, X, false>(p, np, h, keys.x, keys.y, w0, lk, lv, lx, &odd);
+  if (!odd) return;
+  for (int j = 0; j < QF; ++j) {
+    __syncthreads();
+    attn_fwd_rows<T, DP, 1, X, true>(p, np, h, keys.x, keys.y, afresh(w0 + 16 * j), lk, lv, lx, &odd);
   }
 }
 
@@ -278,9 +281,9 @@ __global__ __launch_bounds__(256) void blk_attn_row_kernel(BlkAttnArgs p, int sp
         s[0][f][e] = x;
         t = fmaxf(t, x);
       }
-    t = quarters_max(t) * (W::RAW ? soft.c : 1.f);
-    if (__ballot(t > m)) {
-      const float mn = fmaxf(m, t), al = mn == -INFINITY ? 1.f : W::ratio(m, mn);
+    t = soft.top(quarters_max(t));
+    if (__ballot(t > m + 8.f)) {
+      const float mn = fmaxf(m, t), al = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
       m = mn;
       l *= al;
 #pragma unroll
@@ -318,7 +321,7 @@ __global__ __launch_bounds__(256) void blk_attn_row_kernel(BlkAttnArgs p, int sp
     float lt = 0.f, o = 0.f;
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
-      const float f = mt == -INFINITY ? 1.f : W::ratio(sm[w * 32 + hh], mt);
+      const float f = mt == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(sm[w * 32 + hh] - mt);
       lt = fmaf(f, sm[w * 32 + 16 + hh], lt);
       o = fmaf(f, sm[128 + (w * DP + d) * 16 + hh], o);
     }
@@ -334,7 +337,7 @@ __global__ __launch_bounds__(256) void blk_attn_row_kernel(BlkAttnArgs p, int sp
   }
 }
 
-template <class T, bool NATURAL>
+template <class T>
 __global__ __launch_bounds__(128) void blk_attn_join_kernel(BlkAttnArgs p, int splits, const float* part) {
   const int d = threadIdx.x;
   const float* in = part + (long)blockIdx.x * splits * (p.D + 4);
@@ -343,7 +346,7 @@ __global__ __launch_bounds__(128) void blk_attn_join_kernel(BlkAttnArgs p, int s
   float lt = 0.f, o = 0.f;
   for (int s = 0; s < splits; ++s) {
     const float* x = in + (long)s * (p.D + 4);
-    const float f = mt == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((x[p.D] - mt) * (NATURAL ? LOG2E : 1.f));
+    const float f = mt == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(x[p.D] - mt);
     lt = fmaf(f, x[p.D + 1], lt);
     if (d < p.D) o = fmaf(f, x[d], o);
   }
@@ -368,7 +371,7 @@ void launch_fwd_x(const BlkAttnArgs& p, hipStream_t st) {
     const dim3 grid((unsigned)((long)p.N * p.Hkv * hgroups * splits));
     MG_LAUNCH((blk_attn_row_kernel<T, DP, X>), grid, dim3(256), 0, st, p, splits, hgroups, (float*)p.ws);
     if (splits > 1)
-      MG_LAUNCH((blk_attn_join_kernel<T, Soft<T, X>::NATURAL>), dim3(p.N * p.H), dim3(128), 0, st, p, splits, (const float*)p.ws);
+      MG_LAUNCH((blk_attn_join_kernel<T>), dim3(p.N * p.H), dim3(128), 0, st, p, splits, (const float*)p.ws);
     return;
   }
   const int np = cdiv(p.N, 128) * 128;

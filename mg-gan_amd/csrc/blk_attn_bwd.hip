@@ -11,26 +11,18 @@ int blk_attn_check(const BlkAttnArgs* a, const char* name);
 
 namespace {
 
-template <class T, int DP, int QF, int X>
-__global__ __launch_bounds__(256, 2) void blk_attn_dq_kernel(BlkAttnArgs p, int np, float* delta, float* slope_part) {
-  using G = Geo<T, DP>;
+// Tiles of 32 rows: the scores' gradients need registers next to the scores.  (bf16 of width 32 and 96: 64, whole passes of 256 copies.)
+template <class T, int DP>
+using BwdGeo = Geo<T, DP, sizeof(T) == 2 && DP % 64 ? 64 : 32>;
+
+// dQ of 64 QF rows of one head (this wave's start at w0), and the sum that the rows' slopes' gradient is.
+template <class T, int DP, int QF, int X, bool SAFE>
+__device__ __forceinline__ float attn_dq_rows(const BlkAttnArgs& p, int np, float* delta, int h, int glo, int ghi, int w0, u32x4* lk, u32x4* lv,
+                                              float* lx, int* odd) {
+  using G = BwdGeo<T, DP>;
   using W = Soft<T, X>;
   constexpr int AXES = W::AXES;
-  __shared__ u32x4 lk[2][G::TILE], lv[2][G::TILE];
-  __shared__ __attribute__((aligned(16))) float lx[2][2][64];
-  const int lane = mg_lane(), wave = mg_wave(), i16 = lane & 15, g = lane >> 4;
-  const int h = blockIdx.x % p.H, hk = h / (p.H / p.Hkv);
-  const int nqt = gridDim.x / p.H, qt = nqt - 1 - (int)(blockIdx.x / p.H);
-  const int r0 = qt * 64 * QF, w0 = r0 + wave * 16 * QF;
-  const int nd = p.D / G::CH;
-
-  int glo = INT_MAX, ghi = 0;
-#pragma unroll
-  for (int i = 0; i < 2 * QF; ++i) {
-    const int4 s = *(const int4*)(p.spans + 2 * np + 4 * ((r0 >> 5) + i));
-    glo = min(glo, s.x);
-    ghi = max(ghi, s.y);
-  }
+  const int lane = mg_lane(), wave = mg_wave(), i16 = lane & 15, g = lane >> 4, hk = h / (p.H / p.Hkv), nd = p.D / G::CH;
   int lo[QF], hi[QF], wlo = INT_MAX, whi = 0, flo = 0, fhi = INT_MAX;
   float qx[QF], qy[QF], top[QF], inv[QF], dsum[QF];
   u32x4 q[QF][G::SK], dO[QF][G::SK];
@@ -67,22 +59,14 @@ __global__ __launch_bounds__(256, 2) void blk_attn_dq_kernel(BlkAttnArgs p, int 
     qx[j] = AXES ? p.xy[(long)rc * AXES] : 0.f;
     qy[j] = AXES > 1 ? p.xy[(long)rc * AXES + 1] : 0.f;
   }
-#pragma unroll
-  for (int o = 1; o < 16; o <<= 1) {
-    wlo = min(wlo, __shfl_xor(wlo, o, 64));
-    whi = max(whi, __shfl_xor(whi, o, 64));
-    flo = max(flo, __shfl_xor(flo, o, 64));
-    fhi = min(fhi, __shfl_xor(fhi, o, 64));
-  }
-  wlo = __builtin_amdgcn_readfirstlane(wlo), whi = __builtin_amdgcn_readfirstlane(whi);
-  flo = __builtin_amdgcn_readfirstlane(flo), fhi = __builtin_amdgcn_readfirstlane(fhi);
+  wave_span(wlo, whi, flo, fhi);
 
   const T* kb = (const T*)p.k + hk * p.k_head;
   const T* vb = (const T*)p.v + hk * p.v_head;
   auto fetch = [&](int k0, int buf) {
-    copy_tile<G>(kb, p.k_row, k0, glo, ghi, nd, lk[buf]);
-    copy_tile<G>(vb, p.v_row, k0, glo, ghi, nd, lv[buf]);
-    if (wave < AXES) copy_meta(p.kv_xy, AXES, wave, k0, p.M, lx[buf][wave]);
+    copy_tile<G>(kb, p.k_row, k0, glo, ghi, nd, lk + buf * G::TILE);
+    copy_tile<G>(vb, p.v_row, k0, glo, ghi, nd, lv + buf * G::TILE);
+    if (wave < AXES) copy_meta(p.kv_xy, AXES, wave, k0, p.M, lx + (2 * buf + wave) * 64);
   };
 
   f32x4 acc[QF][G::DF];
@@ -104,25 +88,26 @@ __global__ __launch_bounds__(256, 2) void blk_attn_dq_kernel(BlkAttnArgs p, int 
     if (k0 + G::BK < ghi) fetch(k0 + G::BK, buf ^ 1);
     if (k0 >= whi || k0 + G::BK <= wlo) continue;
     f32x4 s[QF][G::F], dp[QF][G::F];
-    scores<G, QF>(lk[buf], q, s, at);
-    scores<G, QF>(lv[buf], dO, dp, at);
+    scores<G, QF>(lk + buf * G::TILE, q, s, at);
+    scores<G, QF>(lv + buf * G::TILE, dO, dp, at);
+    const u32x4* tk = lk + buf * G::TILE;
     const bool part = k0 < flo || k0 + G::BK > fhi;
+    if (!SAFE && part && tile_not_finite<G>(tk, lane)) *odd = 1;
     float ta[QF] = {}, tb[QF] = {}, tc[QF] = {};
 #pragma unroll
     for (int f = 0; f < G::F; ++f) {
       const int kr = G::row4(f, g);
       f32x4 bx = {}, by = {};
-      if (AXES) bx = *(const f32x4*)&lx[buf][0][kr];
-      if (AXES > 1) by = *(const f32x4*)&lx[buf][1][kr];
+      if (AXES) bx = *(const f32x4*)(lx + 2 * buf * 64 + kr);
+      if (AXES > 1) by = *(const f32x4*)(lx + (2 * buf + 1) * 64 + kr);
 #pragma unroll
       for (int r = 0; r < 4; ++r)
 #pragma unroll
         for (int j = 0; j < QF; ++j) {
           float x = s[j][f][r], fac = 1.f, dist = 0.f;
           if (!W::RAW) x = soft.score(x, qx[j], qy[j], bx[r], by[r], fac, dist);
-          float w = soft.weight(x, top[j]) * inv[j], dl = w * (dp[j][f][r] - dsum[j]);
+          float w = soft.weight(x, top[j]) * inv[j], wd = w * dp[j][f][r], dl = fmaf(-w, dsum[j], wd);
           if (W::CAP) dl *= fac;
-          float wd = w * dp[j][f][r];
           if (part) {
             const int key = k0 + kr + r;
             const bool seen = key >= lo[j] && key < hi[j];
@@ -145,10 +130,14 @@ __global__ __launch_bounds__(256, 2) void blk_attn_dq_kernel(BlkAttnArgs p, int 
 #pragma unroll
       for (int j = 0; j < QF; ++j) sa[j] += ta[j], sb[j] += tb[j], sc[j] += tc[j];
     }
-    if (part && tile_not_finite<G>(lk[buf], lane))
-      accumulate_seen<G, QF>(lk[buf], s, acc, lane, [&](int j, int row) { return k0 + row >= lo[j] && k0 + row < hi[j]; });
+    if (SAFE && part && tile_not_finite<G>(tk, lane))
+      accumulate_seen<G, QF>(tk, s, acc, at, lane, [&](int j, int row) { return k0 + row >= lo[j] && k0 + row < hi[j]; });
     else
-      accumulate<G, QF>(lk[buf], s, acc, at);
+      accumulate<G, QF>(tk, s, acc, at);
+  }
+  if (!SAFE) {
+    __syncthreads();
+    if (*odd) return 0.f;
   }
 
 #pragma unroll
@@ -160,18 +149,40 @@ __global__ __launch_bounds__(256, 2) void blk_attn_dq_kernel(BlkAttnArgs p, int 
     for (int d = 0; d < G::DF; ++d)
       if (16 * d + 4 * g < p.D) store4<T>(out + 16 * d + 4 * g, acc[j][d], p.scale);
   }
-  if (AXES && p.dslopes) {
-    float slope_sum = 0.f;
+  float slope_sum = 0.f;
 #pragma unroll
+  for (int j = 0; j < QF; ++j) {
+    const float a = quarters_sum(sa[j]), b = quarters_sum(sb[j]), c = quarters_sum(sc[j]);
+    if (g == 0 && w0 + 16 * j + i16 < p.N) slope_sum += fmaf(-c, b, a);
+  }
+  return slope_sum;
+}
+
+template <class T, int DP, int QF, int X>
+__global__ __launch_bounds__(256, 2) void blk_attn_dq_kernel(BlkAttnArgs p, int np, float* delta, float* slope_part) {
+  using G = BwdGeo<T, DP>;
+  __shared__ u32x4 lk[2 * G::TILE], lv[2 * G::TILE];
+  __shared__ __attribute__((aligned(16))) float lx[2 * 2 * 64];
+  __shared__ int odd;
+  const int wave = mg_wave(), h = blockIdx.x % p.H, nqt = gridDim.x / p.H, qt = nqt - 1 - (int)(blockIdx.x / p.H);
+  const int r0 = qt * 64 * QF, w0 = r0 + wave * 16 * QF;
+  if (threadIdx.x == 0) odd = 0;
+  __syncthreads();
+  const int2 keys = group_span<2 * QF>(p, np, r0);
+  float sum = attn_dq_rows<T, DP, QF, X, false>(p, np, delta, h, keys.x, keys.y, w0, lk, lv, lx, &odd);
+  if (odd) {
+    sum = 0.f;
     for (int j = 0; j < QF; ++j) {
-      const float a = quarters_sum(sa[j]), b = quarters_sum(sb[j]), c = quarters_sum(sc[j]);
-      if (g == 0 && w0 + 16 * j + i16 < p.N) slope_sum += fmaf(-c, b, a);
+      __syncthreads();
+      sum += attn_dq_rows<T, DP, 1, X, true>(p, np, delta, h, keys.x, keys.y, afresh(w0 + 16 * j), lk, lv, lx, &odd);
     }
+  }
+  if (X > 1 && p.dslopes) {
     __syncthreads();
-    const float w = wave_sum(slope_sum);
-    if (lane == 0) lx[0][0][wave] = w;
+    sum = wave_sum(sum);
+    if (mg_lane() == 0) lx[wave] = sum;
     __syncthreads();
-    if (threadIdx.x == 0) slope_part[(long)h * nqt + qt] = (lx[0][0][0] + lx[0][0][1]) + (lx[0][0][2] + lx[0][0][3]);
+    if (threadIdx.x == 0) slope_part[(long)h * nqt + qt] = (lx[0] + lx[1]) + (lx[2] + lx[3]);
   }
 }
 
@@ -185,34 +196,15 @@ __global__ __launch_bounds__(64) void blk_slopes_kernel(const float* part, int n
   if (lane == 0) out[blockIdx.x] = (float)-s;
 }
 
-// A workgroup: 64 QF keys of one key head; the queries of every head that shares it, in tiles of BK rows.
-template <class T, int DP, int QF, int X>
-__global__ __launch_bounds__(256, 2) void blk_attn_dkv_kernel(BlkAttnArgs p, int np, const float* delta) {
-  using G = Geo<T, DP>;
+// dK and dV of 64 QF keys of one key head (this wave's start at w0) from the queries [qa, qb) of `heads` heads from h0 on, in tiles of BK
+// rows; `part`: of one head alone, left in f32 for blk_attn_sum_kernel.
+template <class T, int DP, int QF, int X, bool SAFE>
+__device__ __forceinline__ void attn_dkv_rows(const BlkAttnArgs& p, int np, const float* delta, float* part, int h0, int heads, int qa, int qb, int w0,
+                                              u32x4* lq, u32x4* lo_, float* lm, int* odd) {
+  using G = BwdGeo<T, DP>;
   using W = Soft<T, X>;
   constexpr int AXES = W::AXES;
-  __shared__ u32x4 lq[2][G::TILE], lo_[2][G::TILE];
-  __shared__ __attribute__((aligned(16))) float lm[2][7][64];  // of each streamed row: largest score, sum(dO O), lo, hi, x, y, 1 / sum
-  __shared__ int range[2];
-  const int lane = mg_lane(), wave = mg_wave(), i16 = lane & 15, g = lane >> 4;
-  const int hk = blockIdx.x % p.Hkv, kt = blockIdx.x / p.Hkv, group = p.H / p.Hkv;
-  const int b0 = kt * 64 * QF, w0 = b0 + wave * 16 * QF;
-  const int nd = p.D / G::CH;
-
-  // the rows that see any of the workgroup's keys lie between the first and the last 32 that do
-  if (threadIdx.x == 0) range[0] = INT_MAX, range[1] = -1;
-  __syncthreads();
-  for (int u = threadIdx.x; u < np / 32; u += 256) {
-    const int4 s = *(const int4*)(p.spans + 2 * np + 4 * u);
-    if (s.x < b0 + 64 * QF && s.y > b0) {
-      atomicMin(&range[0], u);
-      atomicMax(&range[1], u);
-    }
-  }
-  __syncthreads();
-  const int first = range[0], last = range[1];
-  const int qa = last < 0 ? 0 : first * 32 / G::BK * G::BK, qb = (last + 1) * 32;
-
+  const int lane = mg_lane(), wave = mg_wave(), i16 = lane & 15, g = lane >> 4, hk = h0 / (p.H / p.Hkv), nd = p.D / G::CH;
   float kx[QF], ky[QF];
   u32x4 k[QF][G::SK], v[QF][G::SK];
 #pragma unroll
@@ -236,22 +228,23 @@ __global__ __launch_bounds__(256, 2) void blk_attn_dkv_kernel(BlkAttnArgs p, int
   Lane<G> at;
   at.init(lane);
 
+  auto meta = [&](int buf, int i) { return lm + (7 * buf + i) * 64; };
   // (head, tile) pairs in one sequence, so that the copies of the next head's first tile are under way too
-  const int nt = qb > qa ? (qb - qa + G::BK - 1) / G::BK : 0, total = nt * group;
+  const int nt = qb > qa ? (qb - qa + G::BK - 1) / G::BK : 0, total = nt * heads;
   auto fetch = [&](int t, int buf) {
-    const int h = hk * group + t / nt, q0 = qa + t % nt * G::BK;
-    copy_tile<G>((const T*)p.q + h * p.q_head, p.q_row, q0, 0, p.N, nd, lq[buf]);
-    copy_tile<G>((const T*)p.dout + (long)h * p.D, (long)p.H * p.D, q0, 0, p.N, nd, lo_[buf]);
-    if (wave == 0) copy_meta(p.lse + (long)h * p.N, 1, 0, q0, p.N, lm[buf][0]);
-    if (wave == 3) copy_meta(p.lse + (long)(p.H + h) * p.N, 1, 0, q0, p.N, lm[buf][6]);
-    if (wave == 1) copy_meta(delta + (long)h * p.N, 1, 0, q0, p.N, lm[buf][1]);
-    if (wave == 2) copy_meta(p.spans, 1, 0, q0, np, lm[buf][2]);
-    if (wave == 3) copy_meta(p.spans + np, 1, 0, q0, np, lm[buf][3]);
-    if (wave < AXES) copy_meta(p.xy, AXES, wave, q0, p.N, lm[buf][4 + wave]);
+    const int h = h0 + t / nt, q0 = qa + t % nt * G::BK;
+    copy_tile<G>((const T*)p.q + h * p.q_head, p.q_row, q0, 0, p.N, nd, lq + buf * G::TILE);
+    copy_tile<G>((const T*)p.dout + (long)h * p.D, (long)p.H * p.D, q0, 0, p.N, nd, lo_ + buf * G::TILE);
+    if (wave == 0) copy_meta(p.lse + (long)h * p.N, 1, 0, q0, p.N, meta(buf, 0));
+    if (wave == 3) copy_meta(p.lse + (long)(p.H + h) * p.N, 1, 0, q0, p.N, meta(buf, 6));
+    if (wave == 1) copy_meta(delta + (long)h * p.N, 1, 0, q0, p.N, meta(buf, 1));
+    if (wave == 2) copy_meta(p.spans, 1, 0, q0, np, meta(buf, 2));
+    if (wave == 3) copy_meta(p.spans + np, 1, 0, q0, np, meta(buf, 3));
+    if (wave < AXES) copy_meta(p.xy, AXES, wave, q0, p.N, meta(buf, 4 + wave));
   };
   if (total > 0) fetch(0, 0);
   for (int t = 0; t < total; ++t) {
-    const int buf = t & 1, q0 = qa + t % nt * G::BK, h = hk * group + t / nt;
+    const int buf = t & 1, q0 = qa + t % nt * G::BK, h = h0 + t / nt;
     __syncthreads();
     if (t + 1 < total) fetch(t + 1, buf ^ 1);
     int slo = INT_MAX, shi = 0, flo = 0, fhi = INT_MAX;
@@ -261,18 +254,19 @@ __global__ __launch_bounds__(256, 2) void blk_attn_dkv_kernel(BlkAttnArgs p, int
       slo = min(slo, u.x), shi = max(shi, u.y), flo = max(flo, u.z), fhi = min(fhi, u.w);
     }
     if (slo >= w0 + 16 * QF || shi <= w0) continue;
-    const bool part = w0 < flo || w0 + 16 * QF > fhi;
+    const bool cut = w0 < flo || w0 + 16 * QF > fhi;
     const W soft(p, AXES ? p.slopes[h] : 0.f);
     f32x4 s[QF][G::F], dp[QF][G::F];
-    scores<G, QF>(lq[buf], k, s, at);
-    scores<G, QF>(lo_[buf], v, dp, at);
+    const u32x4 *tq = lq + buf * G::TILE, *to = lo_ + buf * G::TILE;
+    scores<G, QF>(tq, k, s, at);
+    scores<G, QF>(to, v, dp, at);
 #pragma unroll
     for (int f = 0; f < G::F; ++f) {
       const int qr = G::row4(f, g);
-      const f32x4 top = *(const f32x4*)&lm[buf][0][qr], dsum = *(const f32x4*)&lm[buf][1][qr], inv = *(const f32x4*)&lm[buf][6][qr];
+      const f32x4 top = *(const f32x4*)(meta(buf, 0) + qr), dsum = *(const f32x4*)(meta(buf, 1) + qr), inv = *(const f32x4*)(meta(buf, 6) + qr);
       f32x4 ax = {}, ay = {};
-      if (AXES) ax = *(const f32x4*)&lm[buf][4][qr];
-      if (AXES > 1) ay = *(const f32x4*)&lm[buf][5][qr];
+      if (AXES) ax = *(const f32x4*)(meta(buf, 4) + qr);
+      if (AXES > 1) ay = *(const f32x4*)(meta(buf, 5) + qr);
 #pragma unroll
       for (int r = 0; r < 4; ++r)
 #pragma unroll
@@ -284,8 +278,8 @@ __global__ __launch_bounds__(256, 2) void blk_attn_dkv_kernel(BlkAttnArgs p, int
           s[j][f][r] = w;
           dp[j][f][r] = dl;
         }
-      if (part) {
-        const f32x4 from = *(const f32x4*)&lm[buf][2][qr], to = *(const f32x4*)&lm[buf][3][qr];
+      if (cut) {
+        const f32x4 from = *(const f32x4*)(meta(buf, 2) + qr), to = *(const f32x4*)(meta(buf, 3) + qr);
 #pragma unroll
         for (int r = 0; r < 4; ++r)
 #pragma unroll
@@ -299,39 +293,120 @@ __global__ __launch_bounds__(256, 2) void blk_attn_dkv_kernel(BlkAttnArgs p, int
     }
     auto sees = [&](int j, int row) {
       const int key = w0 + 16 * j + i16;
-      return key >= __float_as_int(lm[buf][2][row]) && key < __float_as_int(lm[buf][3][row]);
+      return key >= __float_as_int(meta(buf, 2)[row]) && key < __float_as_int(meta(buf, 3)[row]);
     };
-    if (part && (tile_not_finite<G>(lo_[buf], lane) || tile_not_finite<G>(lq[buf], lane))) {
-      accumulate_seen<G, QF>(lo_[buf], s, dv, lane, sees);
-      accumulate_seen<G, QF>(lq[buf], dp, dk, lane, sees);
+    const bool bad = cut && (tile_not_finite<G>(to, lane) || tile_not_finite<G>(tq, lane));
+    if (!SAFE && bad) *odd = 1;
+    if (SAFE && bad) {
+      accumulate_seen<G, QF>(to, s, dv, at, lane, sees);
+      accumulate_seen<G, QF>(tq, dp, dk, at, lane, sees);
     } else {
-      accumulate<G, QF>(lo_[buf], s, dv, at);
-      accumulate<G, QF>(lq[buf], dp, dk, at);
+      accumulate<G, QF>(to, s, dv, at);
+      accumulate<G, QF>(tq, dp, dk, at);
     }
+  }
+  if (!SAFE) {
+    __syncthreads();
+    if (*odd) return;
   }
 #pragma unroll
   for (int j = 0; j < QF; ++j) {
     const int r = w0 + 16 * j + i16;
     if (r >= p.M) continue;
-    const long o = ((long)r * p.Hkv + hk) * p.D;
+    const long o = ((long)r * p.Hkv + hk) * p.D, po = ((long)h0 * p.M + r) * p.D;
 #pragma unroll
     for (int d = 0; d < G::DF; ++d)
       if (16 * d + 4 * g < p.D) {
+        if (part) {
+          store4<float>(part + po + 16 * d + 4 * g, dk[j][d], p.scale);
+          store4<float>(part + (long)p.H * p.M * p.D + po + 16 * d + 4 * g, dv[j][d], 1.f);
+          continue;
+        }
         store4<T>((T*)p.dk + o + 16 * d + 4 * g, dk[j][d], p.scale);
         store4<T>((T*)p.dv + o + 16 * d + 4 * g, dv[j][d], 1.f);
       }
   }
 }
 
+template <class T, int DP, int QF, int X>
+__global__ __launch_bounds__(256, 2) void blk_attn_dkv_kernel(BlkAttnArgs p, int np, const float* delta, float* part) {
+  using G = BwdGeo<T, DP>;
+  __shared__ u32x4 lq[2 * G::TILE], lo_[2 * G::TILE];
+  __shared__ __attribute__((aligned(16))) float lm[2 * 7 * 64];  // of each streamed row: top, sum(dO O), lo, hi, x, y, 1 / sum
+  __shared__ int range[2], odd;
+  const int group = p.H / p.Hkv, nh = part ? p.H : p.Hkv, h0 = part ? blockIdx.x % nh : blockIdx.x % nh * group, heads = part ? 1 : group;
+  const int b0 = blockIdx.x / nh * 64 * QF, w0 = b0 + mg_wave() * 16 * QF;
+
+  // the rows that see any of the workgroup's keys lie between the first and the last 32 that do
+  if (threadIdx.x == 0) range[0] = INT_MAX, range[1] = -1, odd = 0;
+  __syncthreads();
+  for (int u = threadIdx.x; u < np / 32; u += 256) {
+    const int4 s = *(const int4*)(p.spans + 2 * np + 4 * u);
+    if (s.x < b0 + 64 * QF && s.y > b0) {
+      atomicMin(&range[0], u);
+      atomicMax(&range[1], u);
+    }
+  }
+  __syncthreads();
+  const int first = range[0], last = range[1], qa = last < 0 ? 0 : first * 32 / G::BK * G::BK, qb = (last + 1) * 32;
+  attn_dkv_rows<T, DP, QF, X, false>(p, np, delta, part, h0, heads, qa, qb, w0, lq, lo_, lm, &odd);
+  if (!odd) return;
+  for (int j = 0; j < QF; ++j) {
+    __syncthreads();
+    attn_dkv_rows<T, DP, 1, X, true>(p, np, delta, part, h0, heads, qa, qb, afresh(w0 + 16 * j), lq, lo_, lm, &odd);
+  }
+}
+
+// dK and dV (blockIdx.y) of a key head: the sums over the heads that share it, in their order; four columns a thread.
+template <class T>
+__global__ __launch_bounds__(256) void blk_attn_sum_kernel(BlkAttnArgs p, const float* part) {
+  const long per = (long)p.M * p.D, id = ((long)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (id >= per * p.Hkv) return;
+  const int group = p.H / p.Hkv;
+  const long hk = id / per, at = id - hk * per, r = at / p.D, d = at - r * p.D;
+  const float* in = part + (blockIdx.y * (long)p.H + hk * group) * per + at;
+  f32x4 s = {};
+  for (int g = 0; g < group; ++g) s += *(const f32x4*)(in + g * per);
+  store4<T>((T*)(blockIdx.y ? p.dv : p.dk) + (r * p.Hkv + hk) * p.D + d, s, 1.f);
+}
+
+// The workspace: sum(dO O), the slopes' partial sums, and -- where the heads of a key head are taken apart -- dK and dV of every head.
+// They are where a key head's keys alone are too few workgroups: the first keys behind a causal mask are seen by all rows of all those
+// heads, and one workgroup's walk over them would be the whole time.
+struct Parts {
+  size_t slopes, heads, bytes;
+};
+Parts parts_of(int N, int M, int H, int Hkv, int D) {
+  Parts w;
+  auto up = [](size_t n) { return (n + 255) / 256 * 256; };
+  w.slopes = up((size_t)H * N * 4);
+  w.heads = w.slopes + up((size_t)H * cdiv(N, 64) * 4);
+  w.bytes = w.heads;
+  if (H > Hkv && (long)cdiv(M, 64) * Hkv < 2048) w.bytes += (size_t)2 * H * M * D * 4;
+  return w;
+}
+
+template <class T, int DP, int QF, int QK, int X>
+void launch_bwd_tile(const BlkAttnArgs& p, hipStream_t st) {
+  const int np = cdiv(p.N, 128) * 128, nqt = cdiv(p.N, 64 * QF);
+  const Parts w = parts_of(p.N, p.M, p.H, p.Hkv, p.D);
+  float* delta = (float*)p.ws;
+  float* slopes = (float*)((char*)p.ws + w.slopes);
+  float* heads = w.bytes > w.heads ? (float*)((char*)p.ws + w.heads) : nullptr;
+  MG_LAUNCH((blk_attn_dq_kernel<T, DP, QF, X>), dim3(nqt * p.H), dim3(256), 0, st, p, np, delta, slopes);
+  if (X > 1 && p.dslopes) MG_LAUNCH(blk_slopes_kernel, dim3(p.H), dim3(64), 0, st, (const float*)slopes, nqt, p.dslopes);
+  MG_LAUNCH((blk_attn_dkv_kernel<T, DP, QK, X>), dim3(cdiv(p.M, 64 * QK) * (heads ? p.H : p.Hkv)), dim3(256), 0, st, p, np, (const float*)delta, heads);
+  if (heads) MG_LAUNCH((blk_attn_sum_kernel<T>), dim3(cdiv((long)p.M * p.Hkv * p.D, 1024), 2), dim3(256), 0, st, p, (const float*)heads);
+}
 template <class T, int DP, int X>
 void launch_bwd_x(const BlkAttnArgs& p, hipStream_t st) {
-  constexpr int QF = 1;
-  const int np = cdiv(p.N, 128) * 128, nqt = cdiv(p.N, 64 * QF);
-  float* delta = (float*)p.ws;
-  float* part = delta + (size_t)p.H * p.N;
-  MG_LAUNCH((blk_attn_dq_kernel<T, DP, QF, X>), dim3(nqt * p.H), dim3(256), 0, st, p, np, delta, part);
-  if (X > 1 && p.dslopes) MG_LAUNCH(blk_slopes_kernel, dim3(p.H), dim3(64), 0, st, (const float*)part, nqt, p.dslopes);
-  MG_LAUNCH((blk_attn_dkv_kernel<T, DP, QF, X>), dim3(cdiv(p.M, 64 * QF) * p.Hkv), dim3(256), 0, st, p, np, (const float*)delta);
+  // 128 rows a workgroup halve the LDS reads a score; f32 fragments are twice as large and do not fit at the larger widths, nor do the
+  // two results of the keys' side
+  constexpr int QF = sizeof(T) == 2 || DP <= 64 ? 2 : 1, QK = DP <= 64 ? 2 : 1;
+  if ((long)cdiv(p.N, 128) * p.H >= 256)
+    launch_bwd_tile<T, DP, QF, QK, X>(p, st);
+  else
+    launch_bwd_tile<T, DP, 1, 1, X>(p, st);
 }
 template <class T, int DP>
 void launch_bwd(const BlkAttnArgs& p, hipStream_t st) {
@@ -360,8 +435,8 @@ void launch_bwd_width(const BlkAttnArgs& p, hipStream_t st) {
 
 extern "C" {
 
-size_t mggan_block_attention_bwd_workspace(int rows, int heads) {
-  return rows > 0 && heads > 0 ? ((size_t)heads * rows + (size_t)heads * cdiv(rows, 64)) * 4 : 0;
+size_t mggan_block_attention_bwd_workspace(int rows, int keys, int heads, int kv_heads, int width) {
+  return rows > 0 && keys > 0 && heads > 0 && kv_heads > 0 && width > 0 ? parts_of(rows, keys, heads, kv_heads, width).bytes : 0;
 }
 
 int mggan_block_attention_bwd(const void* args, hipStream_t stream) {
@@ -371,8 +446,9 @@ int mggan_block_attention_bwd(const void* args, hipStream_t stream) {
   MG_CHECK_ARG(a->out32 && a->lse && a->dout && a->dq && a->dk && a->dv, "block_attention_bwd: null operand");
   MG_CHECK_ARG(((size_t)a->out32 | (size_t)a->dout | (size_t)a->dq | (size_t)a->dk | (size_t)a->dv | (size_t)a->spans) % 16 == 0,
                "block_attention_bwd: operands have to be 16-byte aligned");
-  const size_t need = mggan_block_attention_bwd_workspace(a->N, a->H);
-  MG_CHECK_ARG(a->ws && (size_t)a->ws_bytes >= need, "block_attention_bwd: workspace of %zu bytes (got %ld)", need, a->ws_bytes);
+  const size_t need = parts_of(a->N, a->M, a->H, a->Hkv, a->D).bytes;
+  MG_CHECK_ARG(a->ws && (size_t)a->ws_bytes >= need && (size_t)a->ws % 256 == 0, "block_attention_bwd: workspace of %zu bytes, 256-byte aligned (got %ld)", need,
+               a->ws_bytes);
   if (a->dtype == BLK_BF16)
     launch_bwd_width<bf16>(*a, stream);
   else

@@ -39,7 +39,7 @@ def _layer_workspace(M, K, N, gated, backward, act, dtype):
 def _attn_sizes(N, M, H, Hkv, D, S):
     """(int32 of the row intervals, bytes for splitting the keys of single rows, bytes of the backward pass)"""
     return (lib.mggan_block_attention_span_ints(N), lib.mggan_block_attention_fwd_workspace(N, M, H, Hkv, D, S),
-            lib.mggan_block_attention_bwd_workspace(N, H))
+            lib.mggan_block_attention_bwd_workspace(N, M, H, Hkv, D))
 
 
 def _bytes(n, like):
