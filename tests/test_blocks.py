@@ -1,0 +1,131 @@
+"""CPU: what the transformer-block operators (mggan/hip/blocks.py) refuse, and that their C structures match."""
+import os
+import re
+
+import pytest
+import torch
+
+from mggan.hip import HipError, blocks as B, lib as L
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+
+def x(*shape, dtype=torch.float32):
+    return torch.zeros(*shape, dtype=dtype)
+
+
+@pytest.mark.parametrize("args,kw", [
+    ((x(3, 4), x(5, 3)), {}),                                              # widths differ
+    ((x(3, 4), x(5, 4, 1)), {}),
+    ((x(3, 4), x(0, 4)), {}),
+    ((x(3, 0), x(5, 0)), {}),
+    ((x(3, 4), x(5, 4), x(4)), {}),                                        # bias
+    ((x(3, 4), x(5, 4), x(1, 5)), {}),
+    ((x(3, 4), x(5, 4), None, x(5)), {}),                                  # a residual is not broadcast
+    ((x(3, 4), x(5, 4), None, x(1, 5)), {}),
+    ((x(3, 4), x(5, 4, dtype=torch.bfloat16)), {}),                        # types
+    ((x(3, 4, dtype=torch.float16), x(5, 4, dtype=torch.float16)), {}),
+    ((x(3, 4, dtype=torch.float64), x(5, 4, dtype=torch.float64)), {}),
+    ((x(3, 4), x(5, 4)), {"act": 3}),
+    ((x(3, 4), x(5, 4)), {"act": "gelu"}),
+    ((x(3, 4), x(5, 4)), {}),                                              # (all fits, but for the device)
+])
+def test_linear_refuses(args, kw):
+    with pytest.raises(ValueError, match="linear_residual"):
+        B.linear_residual(*args, **kw)
+
+
+@pytest.mark.parametrize("args,kw", [
+    ((x(3, 4), x(5, 4), x(6, 4)), {}),
+    ((x(3, 4), x(5, 4), x(5, 3)), {}),
+    ((x(3, 4), x(5, 4), x(5, 4), x(4)), {}),
+    ((x(3, 4), x(5, 4), x(5, 4), None, x(6)), {}),
+    ((x(3, 4), x(5, 4), x(5, 4, dtype=torch.bfloat16)), {}),
+    ((x(3, 4), x(5, 4), x(5, 4)), {"act": 17}),
+    ((x(3, 4), x(5, 4), x(5, 4)), {}),
+])
+def test_gated_refuses(args, kw):
+    with pytest.raises(ValueError, match="gated_linear"):
+        B.gated_linear(*args, **kw)
+
+
+QKV = (x(6, 4, 16), x(6, 2, 16), x(6, 2, 16))
+S = [(0, 6)]
+
+
+@pytest.mark.parametrize("args,kw", [
+    ((x(6, 4), x(6, 4), x(6, 4), S), {}),
+    ((x(6, 4, 16), x(6, 3, 16), x(6, 3, 16), S), {}),                      # heads
+    ((x(6, 4, 16), x(6, 2, 16), x(6, 4, 16), S), {}),
+    ((x(6, 4, 12), x(6, 2, 12), x(6, 2, 12), S), {}),                      # widths
+    ((x(6, 4, 136), x(6, 2, 136), x(6, 2, 136), S), {}),
+    ((x(6, 4, 16), x(6, 2, 8), x(6, 2, 8), S), {}),
+    ((x(6, 4, 16), x(5, 2, 16), x(5, 2, 16), S), {}),                      # fewer keys without kv_scenes
+    ((x(6, 4, 16, dtype=torch.bfloat16), x(6, 2, 16), x(6, 2, 16), S), {}),
+    (QKV + (S,), {"scale": 0.0}),
+    (QKV + (S,), {"scale": -1.0}),
+    (QKV + (S,), {"scale": float("nan")}),
+    (QKV + (S,), {"cap": -1.0}),
+    (QKV + (S,), {"cap": float("inf")}),
+    (QKV + (S,), {"prefix": [1]}),                                         # without causal
+    (QKV + (S,), {"xy": x(6, 2)}),                                         # positions without slopes
+    (QKV + (S,), {"slopes": x(4)}),
+    (QKV + (S,), {"kv_xy": x(6, 2)}),
+    (QKV + (S,), {"xy": x(6, 3), "slopes": x(4)}),
+    (QKV + (S,), {"xy": x(5, 2), "slopes": x(4)}),
+    (QKV + (S,), {"xy": x(6, 2), "kv_xy": x(6, 1), "slopes": x(4)}),
+    (QKV + (S,), {"xy": x(6, 2, dtype=torch.float64), "slopes": x(4)}),
+    (QKV + (S,), {"xy": x(6, 2), "slopes": x(3)}),
+    (QKV + (S,), {"xy": x(6, 2).requires_grad_(), "slopes": x(4)}),
+    (QKV + (S,), {}),
+])
+def test_attention_refuses(args, kw):
+    with pytest.raises(ValueError, match="attention"):
+        B.attention(*args, **kw)
+
+
+@pytest.mark.parametrize("rows,width", [([(0, 7)], 2), ([(-1, 3)], 2), ([(4, 3)], 2), ([(0, 1, 2)], 2), (["ab"], 2), (5, 2), ([1 << 31], 1),
+                                        ([(0, 1)], 1)])
+def test_tables_refuse(rows, width):
+    with pytest.raises(ValueError, match="attention"):
+        B._table("scenes", rows, torch.device("cpu"), 6, width)
+
+
+def test_c_structures_and_the_packed_arguments_agree():
+    """Field by field: the order and types of the C structures are those of the packing formats."""
+    sizes = {"long": "q", "int": "i", "float": "f"}
+    for path, name, fmt in (("blk_gemm.hip", "BlkLayerArgs", B._LAYER), ("blk_attn.h", "BlkAttnArgs", B._ATTN)):
+        src = open(os.path.join(ROOT, "mg-gan_amd", "csrc", path)).read()
+        body = re.search(r"struct %s \{(.*?)\n\};" % name, src, re.S).group(1)
+        body = re.sub(r"//[^\n]*", "", body)
+        got = ""
+        for decl in filter(None, (" ".join(d.split()) for d in body.split(";"))):
+            kind, names = re.match(r"(?:const )?(\w+) ?(.*)", decl).groups()
+            for field in names.split(","):
+                got += "Q" if "*" in field else sizes[kind]
+        want = "".join(c * int(n or 1) for n, c in re.findall(r"(\d*)([Qqif])", fmt.format))
+        assert got == want, (name, got, want)
+
+
+def test_c_entries_refuse_before_anything_runs():
+    lib = L
+    ok = dict(x=256, w=512, w2=0, b=0, b2=0, res=0, dy=0, z=0, z2=0, y=768, dx=0, dw=0, db=0, ws=0, ws_bytes=0, ldx=64, M=4, K=64, N=64, act=0,
+              dtype=0, slope=0.0)
+    for change in (dict(dtype=2), dict(M=0), dict(N=(1 << 20) + 1), dict(x=0), dict(act=3), dict(act=9), dict(ldx=63), dict(ldx=66), dict(x=260),
+                   dict(y=772), dict(y=0), dict(M=4, K=8192, N=64, ldx=8192), dict(w2=1024, z=2048)):
+        with pytest.raises(HipError):
+            lib.mggan_block_layer_fwd(B._LAYER.pack(*{**ok, **change}.values()), 0)
+    with pytest.raises(HipError):
+        lib.mggan_block_layer_bwd(B._LAYER.pack(*ok.values()), 0)
+    attn = dict(q=256, k=256, v=256, dout=0, out=256, dq=0, dk=0, dv=0, dslopes=0, scenes=256, kv_scenes=256, prefix=0, xy=0, kv_xy=0, slopes=0, lse=0,
+                out32=0, spans=256, ws=0, ws_bytes=0, q_row=64, q_head=16, k_row=32, k_head=16, v_row=32, v_head=16, N=8, M=8, H=4, Hkv=2, D=16, S=1,
+                causal=0, axes=0, dtype=0, scale=1.0, cap=0.0)
+    for change in (dict(dtype=5), dict(N=0), dict(M=0), dict(H=3), dict(D=12), dict(D=136), dict(axes=3), dict(axes=1), dict(scale=0.0), dict(cap=-1.0),
+                   dict(q=0), dict(k=264), dict(q_row=66), dict(spans=0), dict(spans=260), dict(out=0), dict(scenes=0), dict(S=-1),
+                   dict(N=1, M=4096, S=1)):
+        with pytest.raises(HipError):
+            lib.mggan_block_attention_fwd(B._ATTN.pack(*{**attn, **change}.values()), 0)
+    with pytest.raises(HipError):
+        lib.mggan_block_attention_bwd(B._ATTN.pack(*attn.values()), 0)
+    with pytest.raises(HipError):
+        lib.mggan_block_attention_fwd(0, 0)

@@ -292,3 +292,321 @@ def test_attention(case, dtype):
         assert not alone[blind].any() and not got["out"][blind].any() and not got["dq"][blind].any()
         unseen = ~see.any(0)
         assert not got["dk"][unseen].any() and not got["dv"][unseen].any()
+
+
+BAD = [float("nan"), float("inf"), float("-inf")]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("width,cap,axes", [(32, 0.0, 2), (64, 20.0, 0), (128, 0.0, 1)])
+def test_attention_values_that_are_not_finite_stay_in_their_scene(width, cap, axes, dtype):
+    """Scene 1 of three holds NaN and infinities in every operand, and rows no scene names do: the others' results are what they were."""
+    gen = torch.Generator().manual_seed(width)
+    scenes, N = [(0, 21), (21, 60), (60, 147)], 150
+    clean = {n: rnd(gen, N, h, width, dtype=dtype) for n, h in (("q", 4), ("k", 2), ("v", 2), ("dout", 4))}
+    xy = (torch.rand(N, axes, generator=gen) * 9).cuda() if axes else None
+    slopes = torch.rand(4, generator=gen).cuda() if axes else None
+    ok = torch.ones(N, dtype=torch.bool)
+    ok[21:60] = ok[147:] = False
+    runs = []
+    for poisoned in (False, True):
+        t = {n: x.clone() for n, x in clean.items()}
+        if poisoned:
+            for i, x in enumerate(t.values()):
+                x[147:] = BAD[0]
+                x[40, :, i] = BAD[i % 3]
+                x[25, 0, 5 + i:] = BAD[(i + 1) % 3]
+        p = xy.clone() if axes else None
+        if axes and poisoned:
+            p[30] = BAD[1]
+            p[148:] = BAD[0]
+        opt = dict(causal=width == 64, prefix=[3, 9, 50] if width == 64 else None, cap=cap, xy=p, kv_xy=p, slopes=slopes.clone() if axes else None)
+        r = run_attention(t["q"], t["k"], t["v"], t["dout"], scenes, scenes, opt)
+        with torch.no_grad():
+            r["alone"] = B().attention(t["q"], t["k"], t["v"], scenes, **opt)
+        runs.append(r)
+    for name in ("out", "alone", "dq", "dk", "dv"):
+        got, want = runs[1][name][ok.cuda()], runs[0][name][ok.cuda()]
+        assert torch.isfinite(got).all(), name
+        # the sums are the same ones, through another product: off by their rounding at most
+        torch.testing.assert_close(got.double(), want.double(), rtol=4 * U[dtype], atol=64 * F * float(want.abs().max()))
+        assert not torch.isfinite(runs[1][name][21:60]).all(), name
+    assert not torch.isfinite(runs[1]["out"][40]).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_attention_values_that_are_not_finite_behind_the_causal_mask(dtype):
+    """A key that a row does not see yet may be anything; rows that see it get what the definition gives, column by column."""
+    gen = torch.Generator().manual_seed(5)
+    N, at = 100, 70
+    q, k, v = (rnd(gen, N, 2, 64, dtype=dtype) for _ in range(3))
+    with torch.no_grad():
+        want = B().attention(q, k, v, [(0, N)], causal=True)
+        v[at, 0, 3], v[at, 0, 4], v[at + 5, 0, 4], v[at, 0, 5] = BAD[0], BAD[1], BAD[2], BAD[2]
+        got = B().attention(q, k, v, [(0, N)], causal=True)
+    seen = torch.zeros(N, 2, 64, dtype=torch.bool, device="cuda")
+    seen[at:, 0, 3:6] = True
+    torch.testing.assert_close(got[~seen].double(), want[~seen].double(), rtol=4 * U[dtype], atol=1e-5)
+    assert got[at:, 0, 3].isnan().all()
+    assert (got[at:at + 5, 0, 4] == float("inf")).all() and got[at + 5:, 0, 4].isnan().all()
+    assert (got[at:, 0, 5] == float("-inf")).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_attention_reads_views_of_packed_and_unaligned_operands(dtype):
+    gen = torch.Generator().manual_seed(8)
+    N, H, D, scenes = 90, 4, 40, [(0, 33), (33, 90)]
+    packed = rnd(gen, N, 3, H, D, dtype=dtype)
+    odd = rnd(gen, N * H * D + 1, dtype=dtype)[1:].view(N, H, D)
+    dout = rnd(gen, N, D, H, dtype=dtype).transpose(1, 2)
+    B_ = B()
+    views = [(packed[:, 0], packed[:, 1], packed[:, 2]), (odd, packed[:, 1], packed[:, 2].transpose(0, 1).contiguous().transpose(0, 1)),
+             (packed.transpose(2, 3).contiguous().transpose(2, 3)[:, 0], odd, odd)]
+    for q, k, v in views:
+        plain = [x.detach().clone(memory_format=torch.contiguous_format).requires_grad_() for x in (q, k, v)]
+        leaves = [x.detach().requires_grad_() for x in (q, k, v)]
+        a, b = B_.attention(*leaves, scenes), B_.attention(*plain, scenes)
+        assert torch.equal(a, b)
+        for x, y in zip(torch.autograd.grad(a, leaves, dout), torch.autograd.grad(b, plain, dout.contiguous())):
+            assert torch.equal(x, y)
+
+
+def test_attention_scene_tables():
+    """Device tables in any order, with rows that several scenes name, padding entries and rows behind the operands."""
+    gen = torch.Generator().manual_seed(9)
+    N, B_ = 70, B()
+    q, k, v = (rnd(gen, N, 2, 32, dtype=torch.float32) for _ in range(3))
+    table = lambda rows: torch.tensor(rows, dtype=torch.int32, device="cuda")
+    with torch.no_grad():
+        want = B_.attention(q, k, v, [(0, 30), (30, 64)])
+        assert torch.equal(B_.attention(q, k, v, table([[30, 64], [0, 30], [0, 0], [70, 70]])), want)
+        assert torch.equal(B_.attention(q, k, v, table([[0, 64], [30, 64], [0, 30]])), want)  # the last one that names a row
+        far = B_.attention(q, k, v, table([[0, 30], [30, 64], [64, 5000]]), table([[0, 30], [30, 64], [-7, 100000]]))
+        assert torch.equal(far[:64], want[:64])
+        assert torch.equal(far[64:], B_.attention(q, k, v, [(64, 70)], [(0, 70)])[64:])
+        assert not B_.attention(q, k, v, table([[0, 0]])).any()
+        assert not B_.attention(q, k, v, torch.zeros(0, 2, dtype=torch.int32, device="cuda")).any()
+        assert B_.attention(q[:0], k, v, [(0, 0)]).shape == (0, 2, 32)
+        assert not B_.attention(q, k[:0], v[:0], [(0, 70)], [(0, 0)]).any()
+    # scenes that share keys: the gradients of the keys add up
+    qq, kk, vv = (x[:40].clone().requires_grad_() for x in (q, k, v))
+    shared = B_.attention(qq, kk, vv, [(0, 10), (10, 40)], [(0, 40), (0, 40)])
+    one = B_.attention(qq, kk, vv, [(0, 40)])
+    assert torch.equal(shared, one)
+    for a, b in zip(torch.autograd.grad(shared, [qq, kk, vv], q[:40]), torch.autograd.grad(one, [qq, kk, vv], q[:40])):
+        assert torch.equal(a, b)
+
+
+def test_layers_read_views_and_empty_batches():
+    gen = torch.Generator().manual_seed(10)
+    B_ = B()
+    for dtype in TYPES:
+        wide = rnd(gen, 50, 100, dtype=dtype)
+        w, up = rnd(gen, 24, 40, dtype=dtype), rnd(gen, 24, 40, dtype=dtype)
+        bias = rnd(gen, 25, dtype=dtype)[1:]
+        res = rnd(gen, 24, 50, dtype=dtype).t()
+        for x in (wide[:, 8:48], wide[:, 3:43], wide[::2, 16:56], rnd(gen, 40, 50, dtype=dtype).t(), wide[:, :40].reshape(5, 10, 40)):
+            plain, leaf = x.contiguous().clone().requires_grad_(), x.detach().requires_grad_()
+            r = res[:x.shape[0]] if x.dim() == 2 else res.reshape(5, 10, 24)
+            for f in (lambda t: B_.linear_residual(t, w, bias, r, act=B_.ACT_GELU), lambda t: B_.gated_linear(t, w, up, bias, None)):
+                a, b = f(leaf), f(plain)
+                assert torch.equal(a, b)
+                assert torch.equal(torch.autograd.grad(a, leaf, torch.ones_like(a))[0], torch.autograd.grad(b, plain, torch.ones_like(b))[0])
+        none = torch.zeros(0, 40, dtype=dtype, device="cuda", requires_grad=True)
+        w_ = w.clone().requires_grad_()
+        for y in (B_.linear_residual(none, w_, act=B_.ACT_SILU), B_.gated_linear(none, w_, up)):
+            assert y.shape == (0, 24)
+            dx, dw = torch.autograd.grad(y, [none, w_], y)
+            assert dx.shape == (0, 40) and not dw.any()
+        t = wide[:, :40].clone().requires_grad_()  # only some gradients wanted; a gradient that is broadcast
+        y = B_.gated_linear(t, w, up)
+        assert torch.equal(torch.autograd.grad(y.sum(), t)[0], torch.autograd.grad(B_.gated_linear(t, w, up), t, torch.ones_like(y))[0])
+
+
+def block(x, p, table, heads, xy, slopes):
+    """Attention and feed-forward of one block, as a user composes them."""
+    B_ = B()
+    N, C = x.shape
+    qkv = B_.linear_residual(x, p["qkv"], p["qkv_b"]).view(N, 3, heads, C // heads)
+    mixed = B_.attention(qkv[:, 0], qkv[:, 1], qkv[:, 2], table, causal=xy is None, cap=25.0, xy=xy, slopes=slopes)
+    x = B_.linear_residual(mixed.reshape(N, C), p["out"], p["out_b"], x)
+    return B_.linear_residual(B_.gated_linear(x, p["gate"], p["up"], act=B_.ACT_GELU), p["down"], None, x)
+
+
+def block64(x, p, scenes, heads, xy, slopes):
+    N, C = x.shape
+    qkv = (x @ p["qkv"].t() + p["qkv_b"]).view(N, 3, heads, C // heads)
+    see = visible(N, N, scenes, scenes, xy is None, None)
+    q, k, v = (qkv[:, i].transpose(0, 1) for i in range(3))
+    s = 25.0 * torch.tanh(q @ k.transpose(1, 2) * (C // heads) ** -0.5 / 25.0)
+    if xy is not None:
+        s = s - slopes[:, None, None] * (xy[:, None] - xy[None]).square().sum(-1).add(1e-300).sqrt()
+    mixed = (torch.softmax(s.masked_fill(~see, -torch.inf), -1) @ v).transpose(0, 1).reshape(N, C)
+    x = mixed @ p["out"].t() + p["out_b"] + x
+    h = torch.nn.functional.gelu(x @ p["gate"].t()) * (x @ p["up"].t())
+    return h @ p["down"].t() + x
+
+
+def block_inputs(dtype, spatial, seed=3):
+    gen = torch.Generator().manual_seed(seed)
+    C, heads, hidden, lengths = 96, 3, 200, [20, 1, 33, 7, 64, 50]
+    scenes, N = lengths_to_scenes(lengths), sum(lengths)
+    sizes = {"qkv": (3 * C, C), "qkv_b": (3 * C,), "out": (C, C), "out_b": (C,), "gate": (hidden, C), "up": (hidden, C), "down": (C, hidden)}
+    p = {n: rnd(gen, *s, dtype=dtype, std=s[-1] ** -0.5 if len(s) > 1 else 0.1) for n, s in sizes.items()}
+    x, dy = rnd(gen, N, C, dtype=dtype), rnd(gen, N, C, dtype=dtype)
+    xy = (torch.rand(N, 2, generator=gen) * 10).cuda() if spatial else None
+    slopes = (torch.rand(heads, generator=gen) * 0.3).cuda() if spatial else None
+    return x, dy, p, scenes, heads, xy, slopes
+
+
+@pytest.mark.parametrize("spatial", [False, True])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_block_of_all_three(dtype, spatial):
+    """A block's output and every gradient against the same in 64 bits, by 2-norm.  Ten roundings to the operands' type lie in a row on the
+    longest way (projections, scores' weights, outputs, their gradients), each at most u of its value; errors of products of independent
+    terms add in squares, and a residual stream keeps what passes by them: 12 u; in f32 sums of up to 200 terms and 16-step functions
+    count as 40 u."""
+    x, dy, p, scenes, heads, xy, slopes = block_inputs(dtype, spatial)
+    leaves = [x] + list(p.values()) + ([slopes] if spatial else [])
+    for t in leaves:
+        t.requires_grad_()
+    y = block(x, p, scenes, heads, xy, slopes)
+    got = torch.autograd.grad(y, leaves, dy)
+    up = lambda t: t.detach().double().requires_grad_()
+    x64, p64, s64 = up(x), {n: up(t) for n, t in p.items()}, up(slopes) if spatial else None
+    y64 = block64(x64, p64, scenes, heads, None if xy is None else xy.double(), s64)
+    want = torch.autograd.grad(y64, [x64] + list(p64.values()) + ([s64] if spatial else []), dy.double())
+    for name, a, b in [("y", y, y64)] + list(zip(["x"] + list(p) + ["slopes"], got, want)):
+        rel = float((a.detach().double() - b.detach()).norm() / b.detach().norm())
+        assert rel <= (12 if dtype == torch.bfloat16 else 40) * U[dtype], (name, rel)
+
+
+def test_gradients_against_differences():
+    """Directional derivatives of the f32 block from values of the same kernels: central differences of step h have an error of h^2 times
+    the third derivative and of 2^-24 |y| sqrt(terms) / h; h = 2^-6 leaves both below 2e-3 of the derivative here."""
+    x, dy, p, scenes, heads, xy, slopes = block_inputs(torch.float32, True, seed=12)
+    leaves = {"x": x, **p, "slopes": slopes}
+    for t in leaves.values():
+        t.requires_grad_()
+    grads = dict(zip(leaves, torch.autograd.grad(block(x, p, scenes, heads, xy, slopes), list(leaves.values()), dy)))
+    gen, h = torch.Generator().manual_seed(2), 2.0 ** -6
+    for name, t in leaves.items():
+        d = torch.randn(t.shape, generator=gen).cuda()
+        d = (d / d.norm() * 0.5 + grads[name] / grads[name].norm() * 0.5).detach()
+        value = []
+        for sign in (1, -1):
+            moved = {n: (u + sign * h * d if n == name else u).detach() for n, u in leaves.items()}
+            with torch.no_grad():
+                y = block(moved["x"], {n: moved[n] for n in p}, scenes, heads, xy, moved["slopes"])
+            value.append(float((y.double() * dy.double()).sum()))
+        numeric, formula = (value[0] - value[1]) / (2 * h), float((grads[name].double() * d.double()).sum())
+        assert abs(numeric - formula) <= 5e-3 * abs(formula) + 5e-3, (name, numeric, formula)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_runs_streams_and_graphs_give_the_same_bits(dtype):
+    x, dy, p, scenes, heads, xy, slopes = block_inputs(dtype, True, seed=4)
+    table = torch.tensor(scenes, dtype=torch.int32, device="cuda")
+    leaves = [x] + list(p.values()) + [slopes]
+    for t in leaves:
+        t.requires_grad_()
+
+    def step():
+        y = block(x, p, table, heads, xy, slopes)
+        return (y,) + torch.autograd.grad(y, leaves, dy)
+
+    first = [t.detach().clone() for t in step()]
+    for t, u in zip(first, step()):
+        assert torch.equal(t, u)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        on_side = [step() for _ in range(2)]  # (two calls in flight on one stream, the first one's results alive)
+    # two captured graphs of the same leaves, replayed in turn, with eager work between
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    for r in on_side:
+        for t, u in zip(first, r):
+            assert torch.equal(t, u)
+    del on_side, r, u, t
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            outs = step()
+        graphs.append((g, [t.detach() for t in outs]))
+        del outs
+    for i in range(4):
+        for g, outs in graphs:
+            for t in outs:
+                t.zero_()
+            g.replay()
+            torch.cuda.synchronize()
+            for t, u in zip(first, outs):
+                assert torch.equal(t, u), i
+        eager = step()
+        assert torch.equal(eager[0], first[0])
+        del eager
+    # new values in place: a replay reads them, and the scene table in device memory too
+    with torch.no_grad():
+        x.mul_(0.5)
+        table.copy_(torch.tensor([[0, 20], [20, 54], [54, 54], [54, 61], [61, 125], [125, 175]], dtype=torch.int32))
+    want = [t.detach() for t in step()]
+    for g, outs in graphs:
+        g.replay()
+        torch.cuda.synchronize()
+        for t, u in zip(want, outs):
+            assert torch.equal(t, u)
+
+
+def test_serving_step_in_a_graph():
+    """One new row per sequence over a growing cache: the graph reads the lengths when it runs."""
+    gen = torch.Generator().manual_seed(6)
+    S, room, H, Hkv, D = 5, 300, 8, 2, 64
+    q = rnd(gen, S, H, D, dtype=torch.bfloat16)
+    k, v = (rnd(gen, S * room, Hkv, D, dtype=torch.bfloat16) for _ in range(2))
+    lens = [1, 17, 64, 200, 299]
+    rows = torch.tensor([[s, s + 1] for s in range(S)], dtype=torch.int32, device="cuda")
+    kv = torch.tensor([[s * room, s * room + n] for s, n in enumerate(lens)], dtype=torch.int32, device="cuda")
+    B_ = B()
+    with torch.no_grad():
+        B_.attention(q, k, v, rows, kv)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = B_.attention(q, k, v, rows, kv)
+        for step in range(3):
+            g.replay()
+            assert torch.equal(out, B_.attention(q, k, v, rows, kv))
+            see = visible(S, S * room, [(s, s + 1) for s in range(S)], kv.tolist(), False, None)
+            want = reference(q, k, v, see, q, D ** -0.5, 0.0, None, None, None)["out"]
+            close(out, *want, "out")
+            kv[:, 1] += torch.tensor([1, 1, 1, 1, 0 if step else 1], dtype=torch.int32, device="cuda")
+            q.copy_(rnd(gen, S, H, D, dtype=torch.bfloat16))
+            torch.cuda.synchronize()
+
+
+def test_caches_beyond_32_bit_offsets():
+    """Keys whose byte offsets pass 2^32 (2.2e9 elements of bf16): rows at both ends of the cache."""
+    M, D = 17_200_000, 128
+    k = torch.zeros(M, 1, D, dtype=torch.bfloat16, device="cuda")
+    gen = torch.Generator().manual_seed(1)
+    tail = rnd(gen, 700, 1, D, dtype=torch.bfloat16)
+    k[-700:] = tail
+    q = rnd(gen, 200, 2, D, dtype=torch.bfloat16)
+    B_ = B()
+    with torch.no_grad():
+        a = B_.attention(q, k, k, [(0, 200)], [(M - 700, M)], causal=True)
+        assert torch.equal(a, B_.attention(q, tail, tail, [(0, 200)], [(0, 700)], causal=True))
+        a = B_.attention(q[:1], k, k, [(0, 1)], [(M - 700, M)])
+        b = B_.attention(q[:1], tail, tail, [(0, 1)], [(0, 700)])
+        torch.testing.assert_close(a.double(), b.double(), rtol=4 * U[torch.bfloat16], atol=1e-4)
+
+
+def test_a_second_derivative_is_refused():
+    gen = torch.Generator().manual_seed(1)
+    x, w = rnd(gen, 4, 8, dtype=torch.float32).requires_grad_(), rnd(gen, 8, 8, dtype=torch.float32)
+    for y in (B().linear_residual(x, w, act=B().ACT_SILU), B().attention(x.view(4, 1, 8), x.view(4, 1, 8), x.view(4, 1, 8), [(0, 4)])):
+        g, = torch.autograd.grad(y.sum(), x, create_graph=True)
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(g.sum(), x)
