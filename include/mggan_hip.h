@@ -668,7 +668,7 @@ int mggan_block_layer_bwd(const void* args, mggan_stream_t stream);
  * q (N, H, D), k, v (M, Hkv, D) with the given row and head strides in elements (multiples of 16 bytes, width contiguous); out,
  * dout, dq (N, H, D), dk, dv (M, Hkv, D) contiguous; dtype 0 f32, 1 bf16; D a multiple of 8 up to 128; scenes, kv_scenes (S, 2) rows
  * [start, end) (clamped to the operands); prefix (S) or NULL; axes 0, 1 or 2 (then xy (N, axes), kv_xy (M, axes), slopes (H)); cap 0:
- * none; lse (2, H, N) and, with bf16, out32 (the output before its rounding): written if not NULL, the backward pass reads them (out32
+ * none; lse (3, H, N) and, with bf16, out32 (the output before its rounding): written if not NULL, the backward pass reads them (out32
  * = out with f32).  spans: mggan_block_attention_span_ints(N) int32, 16-byte
  * aligned, written by the forward call and read by the backward call.  Rows without keys: zeros. */
 size_t mggan_block_attention_span_ints(int rows);

@@ -18,7 +18,8 @@ struct BlkAttnArgs {  // mirrored by mggan/hip/blocks.py
   float* dslopes;
   const int *scenes, *kv_scenes, *prefix;
   const float *xy, *kv_xy, *slopes;
-  float* lse;    // (2, H, N): what the exponents of a row's weights were taken less (about its largest), and one over the weights' sum
+  float* lse;    // (3, H, N): what the exponents of a row's weights were taken less (about the largest), one over the weights' sum, and both in
+                 // one (the exponent less this is the log2 of the softmax: exact to 2^-21 or so, which is enough where bf16 follows)
   float* out32;  // the output before it is rounded (f32: the output): what sum(dO O) is formed of -- from the rounded one every row's
                  // gradient would carry a common error, which the sums over rows (the slopes' gradient) do not average away
   int* spans;   // mggan_block_attention_span_ints(N): lo, hi, and {min lo, max hi, max lo, min hi} of every 32 rows
@@ -35,13 +36,13 @@ __device__ __attribute__((aligned(16))) const unsigned blk_attn_zeros[4] = {0, 0
 
 constexpr float LOG2E = 1.44269504f;
 
-// tanh.  f32 operands: near zero by its series (to x^11: 2^-26 of the value at 0.35), so that a score keeps its relative precision
-// through the cap; bf16 operands carry 2^-9 themselves, there the quotient does everywhere.
+// tanh(x) from z = 2 log2e x.  f32 operands: near zero by its series (to x^11: 2^-26 of the value at 0.35), so that a score keeps its
+// relative precision through the cap; bf16 operands carry 2^-9 themselves, there the quotient does everywhere.
 template <class T>
-__device__ __forceinline__ float blk_tanh(float x) {
-  const float big = fmaf(-2.0f, mg_rcp(__builtin_amdgcn_exp2f(x * (2.f * LOG2E)) + 1.0f), 1.0f);
+__device__ __forceinline__ float blk_tanh(float z) {
+  const float big = fmaf(-2.0f, mg_rcp(__builtin_amdgcn_exp2f(z) + 1.0f), 1.0f);
   if constexpr (sizeof(T) == 2) return big;
-  const float y = x * x;
+  const float x = z * (0.5f / LOG2E), y = x * x;
   const float s = fmaf(y, fmaf(y, fmaf(y, fmaf(y, fmaf(y, -0.0088632355f, 0.0218694885f), -0.0539682540f), 0.1333333333f), -0.3333333333f), 1.f) * x;
   return fabsf(x) < 0.35f ? s : big;
 }
@@ -50,28 +51,30 @@ __device__ __forceinline__ float blk_tanh(float x) {
 // Weights are exp2(s E - top), one fused operation, with top = max s E.  E = log2e over scores in their own units where the last bits
 // matter (f32; scores with a distance, whose slopes' gradient is f32): scale log2e and slope log2e rounded into one factor first would
 // stretch all scores by a common 2^-25, which shows in the slopes' gradient (log2e itself is 2^-26 off, top's rounding divides out).
-// bf16, with gradients rounded at 2^-9: plain scores are left as the product gives them and E = scale log2e, capped ones are multiplied
-// by log2e with the cap and E = 1.
+// bf16, with gradients rounded at 2^-9: plain scores are left as the product gives them and E = scale log2e, capped ones as their tanh and
+// E = cap log2e.
 template <class T, int X>
 struct Soft {
   static constexpr bool CAP = X & 1, NATURAL = (X >> 1) || sizeof(T) == 4;
   static constexpr int AXES = X >> 1;
-  float c, k, cap, slope;  // c: a plain score's factor
+  static constexpr bool RAW = X == 0 && !NATURAL;  // score() is not called
+  float scale, k, cap, slope, E;
   __device__ __forceinline__ Soft(const BlkAttnArgs& p, float slope_) {
-    c = p.scale * (NATURAL ? 1.f : LOG2E);
-    cap = p.cap * (NATURAL ? 1.f : LOG2E);
-    k = CAP ? p.scale / p.cap : 0.f;
+    scale = p.scale;
+    cap = p.cap;
+    k = CAP ? p.scale / p.cap * (2.f * LOG2E) : 0.f;
     slope = slope_;
+    E = LOG2E * (NATURAL ? 1.f : CAP ? p.cap : p.scale);
   }
-  // the score as it is exponentiated; fac = d(capped)/d(score), dist: what the slope multiplies
+  // the score as weight() takes it; fac = d(capped)/d(score), dist: what the slope multiplies
   __device__ __forceinline__ float score(float x, float ax, float ay, float bx, float by, float& fac, float& dist) const {
     fac = 1.f, dist = 0.f;
     if constexpr (CAP) {
-      const float t = blk_tanh<T>(x * k);
-      fac = fmaf(-t, t, 1.f);
-      x = cap * t;
+      x = blk_tanh<T>(x * k);
+      fac = fmaf(-x, x, 1.f);
+      if (NATURAL) x *= cap;
     } else {
-      x *= c;
+      x *= scale;
     }
     if constexpr (AXES == 1) dist = fabsf(ax - bx);
     if constexpr (AXES == 2) {
@@ -81,11 +84,7 @@ struct Soft {
     if constexpr (AXES) x = fmaf(-slope, dist, x);
     return x;
   }
-  static constexpr bool RAW = X == 0 && !NATURAL;  // score() is not called
-  __device__ __forceinline__ float top(float s) const { return RAW ? s * c : NATURAL ? s * LOG2E : s; }
-  __device__ __forceinline__ float weight(float s, float top) const {
-    return __builtin_amdgcn_exp2f(RAW ? fmaf(s, c, -top) : NATURAL ? fmaf(s, LOG2E, -top) : s - top);
-  }
+  __device__ __forceinline__ float weight(float s, float top) const { return __builtin_amdgcn_exp2f(fmaf(s, E, -top)); }
 };
 
 template <class T_, int DP_, int BK_ = 128 / (int)sizeof(T_)>
@@ -204,21 +203,46 @@ __device__ __forceinline__ void scores(const void* tile, const u32x4 (&own)[QF][
   }
 }
 
+// Both score-like products of a fragment's streamed rows (Q K and dO V) for one group of 16 owner rows.
+template <class G>
+__device__ __forceinline__ void scores2(const void* ta, const void* tb, const u32x4 (&a)[G::SK], const u32x4 (&b)[G::SK], int f, f32x4& x, f32x4& y,
+                                        const Lane<G>& at) {
+  x = y = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int s = 0; s < G::SK; ++s) {
+    x = Mf<typename G::T>::step(at.rows((const char*)ta, f, s), a[s], x);
+    y = Mf<typename G::T>::step(at.rows((const char*)tb, f, s), b[s], y);
+  }
+}
+
+// Four weights or score gradients of a lane as the next product takes them: bf16 rounded here, once.
+template <class T>
+struct Coef {
+  f32x4 v;
+  __device__ __forceinline__ void set(const f32x4& x) { v = x; }
+};
+template <>
+struct Coef<bf16> {
+  bf16x4 v;
+  __device__ __forceinline__ void set(const f32x4& x) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) v[r] = (bf16)x[r];
+  }
+};
+
 // acc[d][owner row] += sum over streamed rows of tile[row][d] * coef[row][owner row], the tile read transposed.  Column fragment fd's row
 // i is column 16 fd + i: a lane ends up with columns 16 fd + 4 g + {0..3} of its owner row.
 template <class G, int QF>
-__device__ __forceinline__ void accumulate(const void* tile, const f32x4 (&coef)[QF][G::F], f32x4 (&acc)[QF][G::DF], const Lane<G>& at) {
+__device__ __forceinline__ void accumulate(const void* tile, const Coef<typename G::T> (&coef)[QF][G::F], f32x4 (&acc)[QF][G::DF], const Lane<G>& at) {
   if constexpr (sizeof(typename G::T) == 2) {
-    constexpr int C = G::DF % 4 == 0 ? 4 : 2;  // column fragments read together
+    constexpr int C = 2;  // column fragments read together
 #pragma unroll
     for (int p = 0; p < G::F / 2; ++p) {
       bf16x8 a[2][C], b[QF];
 #pragma unroll
       for (int c = 0; c < C; ++c) a[0][c] = at.cols((const char*)tile, p, c);
 #pragma unroll
-      for (int j = 0; j < QF; ++j)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) b[j][r] = (bf16)coef[j][2 * p][r], b[j][4 + r] = (bf16)coef[j][2 * p + 1][r];
+      for (int j = 0; j < QF; ++j) b[j] = __builtin_shufflevector(coef[j][2 * p].v, coef[j][2 * p + 1].v, 0, 1, 2, 3, 4, 5, 6, 7);
 #pragma unroll
       for (int k = 0; k < G::DF / C; ++k) {
         if (k + 1 < G::DF / C) {
@@ -242,7 +266,7 @@ __device__ __forceinline__ void accumulate(const void* tile, const f32x4 (&coef)
         for (int fd = 0; fd < G::DF; ++fd) {
           const float a = at.col1((const char*)tile, f, r, fd);
 #pragma unroll
-          for (int j = 0; j < QF; ++j) acc[j][fd] = __builtin_amdgcn_mfma_f32_16x16x4f32(a, coef[j][f][r], acc[j][fd], 0, 0, 0);
+          for (int j = 0; j < QF; ++j) acc[j][fd] = __builtin_amdgcn_mfma_f32_16x16x4f32(a, coef[j][f].v[r], acc[j][fd], 0, 0, 0);
         }
   }
 }
@@ -268,7 +292,7 @@ __device__ __forceinline__ bool tile_not_finite(const u32x4* tile, int lane) {
 // kernels' loops (SAFE) that a workgroup runs, from the start, only if its first run came upon such a tile: beside the plain way in one
 // loop it would cost every run 40 to 100 registers.
 template <class G, int QF, class See>
-__device__ __forceinline__ void accumulate_seen(const void* tile, const f32x4 (&coef)[QF][G::F], f32x4 (&acc)[QF][G::DF], const Lane<G>& at, int lane,
+__device__ __forceinline__ void accumulate_seen(const void* tile, const Coef<typename G::T> (&coef)[QF][G::F], f32x4 (&acc)[QF][G::DF], const Lane<G>& at, int lane,
                                                 See sees) {
   constexpr bool HALF = sizeof(typename G::T) == 2;
   const int g = lane >> 4;
@@ -292,7 +316,7 @@ __device__ __forceinline__ void accumulate_seen(const void* tile, const f32x4 (&
         for (int j = 0; j < QF; ++j) {
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
-            b[e] = (bf16)coef[j][2 * p + (e >> 2)][e & 3];
+            b[e] = coef[j][2 * p + (e >> 2)].v[e & 3];
             one[e] = (bf16)(sees(j, 32 * p + 8 * g + e) ? 1.f : 0.f);
           }
           acc[j][fd] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(clean, b, acc[j][fd], 0, 0, 0);
@@ -305,7 +329,7 @@ __device__ __forceinline__ void accumulate_seen(const void* tile, const f32x4 (&
 #pragma unroll
         for (int j = 0; j < QF; ++j) {
           const float one = sees(j, 16 * (p >> 2) + 4 * g + (p & 3)) ? 1.f : 0.f;
-          acc[j][fd] = __builtin_amdgcn_mfma_f32_16x16x4f32(odd ? 0.f : x, coef[j][p >> 2][p & 3], acc[j][fd], 0, 0, 0);
+          acc[j][fd] = __builtin_amdgcn_mfma_f32_16x16x4f32(odd ? 0.f : x, coef[j][p >> 2].v[p & 3], acc[j][fd], 0, 0, 0);
           up[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(odd && !(x < 0.f) ? 1.f : 0.f, one, up[j], 0, 0, 0);
           down[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(odd && !(x > 0.f) ? 1.f : 0.f, one, down[j], 0, 0, 0);
         }

@@ -132,12 +132,13 @@ __device__ __forceinline__ void attn_fwd_rows(const BlkAttnArgs& p, int np, int 
           for (int j = 0; j < QF; ++j) s[j][f][r] = key >= lo[j] && key < hi[j] ? s[j][f][r] : -INFINITY;
         }
     }
+    Coef<T> w[QF][G::F];
 #pragma unroll
     for (int j = 0; j < QF; ++j) {
       float t = -INFINITY;
 #pragma unroll
       for (int f = 0; f < G::F; ++f) t = fmaxf(t, fmaxf(fmaxf(s[j][f][0], s[j][f][1]), fmaxf(s[j][f][2], s[j][f][3])));
-      t = soft.top(quarters_max(t));
+      t = quarters_max(t) * soft.E;
       if (__ballot(t > m[j] + 8.f)) {  // (weights up to 2^8 are as good: most tiles leave the sums as they are)
         const float mn = fmaxf(m[j], t), al = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[j] - mn);
         m[j] = mn;
@@ -148,19 +149,21 @@ __device__ __forceinline__ void attn_fwd_rows(const BlkAttnArgs& p, int np, int 
       const float mm = m[j] == -INFINITY ? 0.f : m[j];
       float sum = 0.f;
 #pragma unroll
-      for (int f = 0; f < G::F; ++f)
+      for (int f = 0; f < G::F; ++f) {
+        f32x4 e;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const float e = soft.weight(s[j][f][r], mm);
-          s[j][f][r] = e;
-          sum += e;
+          e[r] = soft.weight(s[j][f][r], mm);
+          sum += e[r];
         }
+        w[j][f].set(e);
+      }
       l[j] += sum;
     }
     if (SAFE && part && tile_not_finite<G>(tv, lane))
-      accumulate_seen<G, QF>(tv, s, acc, at, lane, [&](int j, int row) { return k0 + row >= lo[j] && k0 + row < hi[j]; });
+      accumulate_seen<G, QF>(tv, w, acc, at, lane, [&](int j, int row) { return k0 + row >= lo[j] && k0 + row < hi[j]; });
     else
-      accumulate<G, QF>(tv, s, acc, at);
+      accumulate<G, QF>(tv, w, acc, at);
   }
   if (!SAFE) {
     __syncthreads();
@@ -175,6 +178,7 @@ __device__ __forceinline__ void attn_fwd_rows(const BlkAttnArgs& p, int np, int 
     if (g == 0 && p.lse) {
       p.lse[(long)h * p.N + r] = m[j];
       p.lse[(long)(p.H + h) * p.N + r] = inv;
+      p.lse[(long)(2 * p.H + h) * p.N + r] = m[j] + __log2f(sum);
     }
     const long o = ((long)r * p.H + h) * p.D;
 #pragma unroll
@@ -187,7 +191,7 @@ __device__ __forceinline__ void attn_fwd_rows(const BlkAttnArgs& p, int np, int 
 }
 
 template <class T, int DP, int QF, int X>
-__global__ __launch_bounds__(256, 2) void blk_attn_fwd_kernel(BlkAttnArgs p, int np) {
+__global__ __launch_bounds__(256, QF == 1 && DP <= 64 ? 3 : 2) void blk_attn_fwd_kernel(BlkAttnArgs p, int np) {
   using G = Geo<T, DP>;
   __shared__ u32x4 lk[2 * G::TILE], lv[2 * G::TILE];
   __shared__ __attribute__((aligned(16))) float lx[2 * 2 * 64];
@@ -281,7 +285,7 @@ __global__ __launch_bounds__(256) void blk_attn_row_kernel(BlkAttnArgs p, int sp
         s[0][f][e] = x;
         t = fmaxf(t, x);
       }
-    t = soft.top(quarters_max(t));
+    t = quarters_max(t) * soft.E;
     if (__ballot(t > m + 8.f)) {
       const float mn = fmaxf(m, t), al = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
       m = mn;
@@ -290,14 +294,18 @@ __global__ __launch_bounds__(256) void blk_attn_row_kernel(BlkAttnArgs p, int sp
       for (int d = 0; d < G::DF; ++d) acc[0][d] *= al;
     }
     const float mm = m == -INFINITY ? 0.f : m;
+    Coef<T> w[1][G::F];
 #pragma unroll
-    for (int f = 0; f < G::F; ++f)
+    for (int f = 0; f < G::F; ++f) {
+      f32x4 x;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        s[0][f][e] = soft.weight(s[0][f][e], mm);
-        l += s[0][f][e];
+        x[e] = soft.weight(s[0][f][e], mm);
+        l += x[e];
       }
-    accumulate<G, 1>(tiles[wave][buf][1], s, acc, at);
+      w[0][f].set(x);
+    }
+    accumulate<G, 1>(tiles[wave][buf][1], w, acc, at);
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (this tile is read before the next copy goes into it)
   }
   l = quarters_sum(l);
@@ -376,8 +384,11 @@ void launch_fwd_x(const BlkAttnArgs& p, hipStream_t st) {
   }
   const int np = cdiv(p.N, 128) * 128;
   MG_LAUNCH(blk_spans_kernel, dim3(np / 64), dim3(256), 0, st, p, np);
-  if ((long)cdiv(p.N, 128) * p.H >= 256)  // enough workgroups of 128 rows to fill the chip
-    MG_LAUNCH((blk_attn_fwd_kernel<T, DP, 2, X>), dim3(cdiv(p.N, 128) * p.H), dim3(256), 0, st, p, np);
+  // 128 rows a workgroup read every key once for 32 rows of a wave instead of 16, which pays where LDS is what they wait for (width 128,
+  // 16,384 rows: 0.80 against 1.10 ms); below that three smaller waves a SIMD are better (width 64: 127 against 101 us)
+  constexpr int QF = DP > 64 ? 2 : 1;
+  if (QF > 1 && (long)cdiv(p.N, 128) * p.H >= 256)
+    MG_LAUNCH((blk_attn_fwd_kernel<T, DP, QF, X>), dim3(cdiv(p.N, 64 * QF) * p.H), dim3(256), 0, st, p, np);
   else
     MG_LAUNCH((blk_attn_fwd_kernel<T, DP, 1, X>), dim3(cdiv(p.N, 64) * p.H), dim3(256), 0, st, p, np);
 }

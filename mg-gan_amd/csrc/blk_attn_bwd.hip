@@ -53,8 +53,8 @@ __device__ __forceinline__ float attn_dq_rows(const BlkAttnArgs& p, int np, floa
       }
     }
     dsum[j] = quarters_sum(d);
-    top[j] = p.lse[(long)h * p.N + rc];
-    inv[j] = p.lse[(long)(p.H + h) * p.N + rc];
+    top[j] = p.lse[((W::NATURAL ? 0 : 2L * p.H) + h) * p.N + rc];
+    inv[j] = W::NATURAL ? p.lse[(long)(p.H + h) * p.N + rc] : 1.f;
     if (r < p.N && g == 0) delta[(long)h * p.N + r] = dsum[j];
     qx[j] = AXES ? p.xy[(long)rc * AXES] : 0.f;
     qy[j] = AXES > 1 ? p.xy[(long)rc * AXES + 1] : 0.f;
@@ -87,13 +87,14 @@ __device__ __forceinline__ float attn_dq_rows(const BlkAttnArgs& p, int np, floa
     __syncthreads();
     if (k0 + G::BK < ghi) fetch(k0 + G::BK, buf ^ 1);
     if (k0 >= whi || k0 + G::BK <= wlo) continue;
-    f32x4 s[QF][G::F], dp[QF][G::F];
-    scores<G, QF>(lk + buf * G::TILE, q, s, at);
-    scores<G, QF>(lv + buf * G::TILE, dO, dp, at);
-    const u32x4* tk = lk + buf * G::TILE;
+    const u32x4 *tk = lk + buf * G::TILE, *tv = lv + buf * G::TILE;
     const bool part = k0 < flo || k0 + G::BK > fhi;
     if (!SAFE && part && tile_not_finite<G>(tk, lane)) *odd = 1;
     float ta[QF] = {}, tb[QF] = {}, tc[QF] = {};
+    f32x4 s[QF][G::F], dp[QF][G::F];
+    Coef<T> ds[QF][G::F];
+    scores<G, QF>(tk, q, s, at);
+    scores<G, QF>(tv, dO, dp, at);
 #pragma unroll
     for (int f = 0; f < G::F; ++f) {
       const int kr = G::row4(f, g);
@@ -101,17 +102,21 @@ __device__ __forceinline__ float attn_dq_rows(const BlkAttnArgs& p, int np, floa
       if (AXES) bx = *(const f32x4*)(lx + 2 * buf * 64 + kr);
       if (AXES > 1) by = *(const f32x4*)(lx + (2 * buf + 1) * 64 + kr);
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
+      for (int j = 0; j < QF; ++j) {
+        f32x4 dl;
 #pragma unroll
-        for (int j = 0; j < QF; ++j) {
+        for (int r = 0; r < 4; ++r) {
           float x = s[j][f][r], fac = 1.f, dist = 0.f;
           if (!W::RAW) x = soft.score(x, qx[j], qy[j], bx[r], by[r], fac, dist);
-          float w = soft.weight(x, top[j]) * inv[j], wd = w * dp[j][f][r], dl = fmaf(-w, dsum[j], wd);
-          if (W::CAP) dl *= fac;
+          float w = soft.weight(x, top[j]);
+          if (W::NATURAL) w *= inv[j];
+          float wd = w * dp[j][f][r];
+          dl[r] = fmaf(-w, dsum[j], wd);
+          if (W::CAP) dl[r] *= fac;
           if (part) {
             const int key = k0 + kr + r;
             const bool seen = key >= lo[j] && key < hi[j];
-            dl = seen ? dl : 0.f;
+            dl[r] = seen ? dl[r] : 0.f;
             if (AXES) {
               w = seen ? w : 0.f;
               wd = seen ? wd : 0.f;
@@ -123,17 +128,18 @@ __device__ __forceinline__ float attn_dq_rows(const BlkAttnArgs& p, int np, floa
             tb[j] = fmaf(w, dist, tb[j]);
             tc[j] += wd;
           }
-          s[j][f][r] = dl;
         }
+        ds[j][f].set(dl);
+      }
     }
     if (AXES) {
 #pragma unroll
       for (int j = 0; j < QF; ++j) sa[j] += ta[j], sb[j] += tb[j], sc[j] += tc[j];
     }
     if (SAFE && part && tile_not_finite<G>(tk, lane))
-      accumulate_seen<G, QF>(tk, s, acc, at, lane, [&](int j, int row) { return k0 + row >= lo[j] && k0 + row < hi[j]; });
+      accumulate_seen<G, QF>(tk, ds, acc, at, lane, [&](int j, int row) { return k0 + row >= lo[j] && k0 + row < hi[j]; });
     else
-      accumulate<G, QF>(tk, s, acc, at);
+      accumulate<G, QF>(tk, ds, acc, at);
   }
   if (!SAFE) {
     __syncthreads();
@@ -159,7 +165,7 @@ __device__ __forceinline__ float attn_dq_rows(const BlkAttnArgs& p, int np, floa
 }
 
 template <class T, int DP, int QF, int X>
-__global__ __launch_bounds__(256, 2) void blk_attn_dq_kernel(BlkAttnArgs p, int np, float* delta, float* slope_part) {
+__global__ __launch_bounds__(256, QF == 1 && DP <= 64 ? 3 : 2) void blk_attn_dq_kernel(BlkAttnArgs p, int np, float* delta, float* slope_part) {
   using G = BwdGeo<T, DP>;
   __shared__ u32x4 lk[2 * G::TILE], lv[2 * G::TILE];
   __shared__ __attribute__((aligned(16))) float lx[2 * 2 * 64];
@@ -186,45 +192,29 @@ __global__ __launch_bounds__(256, 2) void blk_attn_dq_kernel(BlkAttnArgs p, int 
   }
 }
 
-// The slopes' gradient: a head's partial sums in their order.
-__global__ __launch_bounds__(64) void blk_slopes_kernel(const float* part, int n, float* out) {
-  const int lane = threadIdx.x;
-  double s = 0.;
-  for (int i = lane; i < n; i += 64) s += (double)part[(long)blockIdx.x * n + i];
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
-  if (lane == 0) out[blockIdx.x] = (float)-s;
-}
-
-// dK and dV of 64 QF keys of one key head (this wave's start at w0) from the queries [qa, qb) of `heads` heads from h0 on, in tiles of BK
+// dK and dV of 64 keys of one key head (this wave's 16 start at w0) from the queries [qa, qb) of `heads` heads from h0 on, in tiles of BK
 // rows; `part`: of one head alone, left in f32 for blk_attn_sum_kernel.
-template <class T, int DP, int QF, int X, bool SAFE>
+template <class T, int DP, int X, bool SAFE>
 __device__ __forceinline__ void attn_dkv_rows(const BlkAttnArgs& p, int np, const float* delta, float* part, int h0, int heads, int qa, int qb, int w0,
                                               u32x4* lq, u32x4* lo_, float* lm, int* odd) {
   using G = BwdGeo<T, DP>;
   using W = Soft<T, X>;
   constexpr int AXES = W::AXES;
+  constexpr bool ONE = sizeof(T) == 2;  // one statistic a row
   const int lane = mg_lane(), wave = mg_wave(), i16 = lane & 15, g = lane >> 4, hk = h0 / (p.H / p.Hkv), nd = p.D / G::CH;
-  float kx[QF], ky[QF];
-  u32x4 k[QF][G::SK], v[QF][G::SK];
+  u32x4 k[G::SK], v[G::SK];
+  const int rc = min(w0 + i16, p.M - 1);
+  const T* kr = (const T*)p.k + rc * p.k_row + hk * p.k_head;
+  const T* vr = (const T*)p.v + rc * p.v_row + hk * p.v_head;
 #pragma unroll
-  for (int j = 0; j < QF; ++j) {
-    const int rc = min(w0 + 16 * j + i16, p.M - 1);
-    const T* kr = (const T*)p.k + rc * p.k_row + hk * p.k_head;
-    const T* vr = (const T*)p.v + rc * p.v_row + hk * p.v_head;
-#pragma unroll
-    for (int s = 0; s < G::SK; ++s) {
-      k[j][s] = owner_chunk(kr, 4 * s + g, nd);
-      v[j][s] = owner_chunk(vr, 4 * s + g, nd);
-    }
-    kx[j] = AXES ? p.kv_xy[(long)rc * AXES] : 0.f;
-    ky[j] = AXES > 1 ? p.kv_xy[(long)rc * AXES + 1] : 0.f;
+  for (int s = 0; s < G::SK; ++s) {
+    k[s] = owner_chunk(kr, 4 * s + g, nd);
+    v[s] = owner_chunk(vr, 4 * s + g, nd);
   }
-  f32x4 dk[QF][G::DF], dv[QF][G::DF];
+  const float kx = AXES ? p.kv_xy[(long)rc * AXES] : 0.f, ky = AXES > 1 ? p.kv_xy[(long)rc * AXES + 1] : 0.f;
+  f32x4 dk[1][G::DF], dv[1][G::DF];
 #pragma unroll
-  for (int j = 0; j < QF; ++j)
-#pragma unroll
-    for (int d = 0; d < G::DF; ++d) dk[j][d] = dv[j][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int d = 0; d < G::DF; ++d) dk[0][d] = dv[0][d] = f32x4{0.f, 0.f, 0.f, 0.f};
   Lane<G> at;
   at.init(lane);
 
@@ -235,8 +225,8 @@ __device__ __forceinline__ void attn_dkv_rows(const BlkAttnArgs& p, int np, cons
     const int h = h0 + t / nt, q0 = qa + t % nt * G::BK;
     copy_tile<G>((const T*)p.q + h * p.q_head, p.q_row, q0, 0, p.N, nd, lq + buf * G::TILE);
     copy_tile<G>((const T*)p.dout + (long)h * p.D, (long)p.H * p.D, q0, 0, p.N, nd, lo_ + buf * G::TILE);
-    if (wave == 0) copy_meta(p.lse + (long)h * p.N, 1, 0, q0, p.N, meta(buf, 0));
-    if (wave == 3) copy_meta(p.lse + (long)(p.H + h) * p.N, 1, 0, q0, p.N, meta(buf, 6));
+    if (wave == 0) copy_meta(p.lse + ((ONE ? 2L * p.H : 0) + h) * p.N, 1, 0, q0, p.N, meta(buf, 0));
+    if (wave == 3 && !ONE) copy_meta(p.lse + (long)(p.H + h) * p.N, 1, 0, q0, p.N, meta(buf, 6));
     if (wave == 1) copy_meta(delta + (long)h * p.N, 1, 0, q0, p.N, meta(buf, 1));
     if (wave == 2) copy_meta(p.spans, 1, 0, q0, np, meta(buf, 2));
     if (wave == 3) copy_meta(p.spans + np, 1, 0, q0, np, meta(buf, 3));
@@ -253,108 +243,112 @@ __device__ __forceinline__ void attn_dkv_rows(const BlkAttnArgs& p, int np, cons
       const int4 u = *(const int4*)(p.spans + 2 * np + 4 * ((q0 >> 5) + i));
       slo = min(slo, u.x), shi = max(shi, u.y), flo = max(flo, u.z), fhi = min(fhi, u.w);
     }
-    if (slo >= w0 + 16 * QF || shi <= w0) continue;
-    const bool cut = w0 < flo || w0 + 16 * QF > fhi;
+    if (slo >= w0 + 16 || shi <= w0) continue;
+    const bool cut = w0 < flo || w0 + 16 > fhi;
     const W soft(p, AXES ? p.slopes[h] : 0.f);
-    f32x4 s[QF][G::F], dp[QF][G::F];
     const u32x4 *tq = lq + buf * G::TILE, *to = lo_ + buf * G::TILE;
-    scores<G, QF>(tq, k, s, at);
-    scores<G, QF>(to, v, dp, at);
+    const int key = w0 + i16;
+    Coef<T> w[1][G::F], ds[1][G::F];
 #pragma unroll
     for (int f = 0; f < G::F; ++f) {
+      f32x4 x, dp;
+      scores2<G>(tq, to, k, v, f, x, dp, at);
       const int qr = G::row4(f, g);
-      const f32x4 top = *(const f32x4*)(meta(buf, 0) + qr), dsum = *(const f32x4*)(meta(buf, 1) + qr), inv = *(const f32x4*)(meta(buf, 6) + qr);
-      f32x4 ax = {}, ay = {};
+      const f32x4 top = *(const f32x4*)(meta(buf, 0) + qr), dsum = *(const f32x4*)(meta(buf, 1) + qr);
+      f32x4 inv = {}, ax = {}, ay = {};
+      if (!ONE) inv = *(const f32x4*)(meta(buf, 6) + qr);
       if (AXES) ax = *(const f32x4*)(meta(buf, 4) + qr);
       if (AXES > 1) ay = *(const f32x4*)(meta(buf, 5) + qr);
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
-#pragma unroll
-        for (int j = 0; j < QF; ++j) {
-          float x = s[j][f][r], fac = 1.f, dist;
-          if (!W::RAW) x = soft.score(x, ax[r], ay[r], kx[j], ky[j], fac, dist);
-          float w = soft.weight(x, top[r]) * inv[r], dl = w * (dp[j][f][r] - dsum[r]);
-          if (W::CAP) dl *= fac;
-          s[j][f][r] = w;
-          dp[j][f][r] = dl;
-        }
-      if (cut) {
-        const f32x4 from = *(const f32x4*)(meta(buf, 2) + qr), to = *(const f32x4*)(meta(buf, 3) + qr);
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-#pragma unroll
-          for (int j = 0; j < QF; ++j) {
-            const int key = w0 + 16 * j + i16;
-            const bool seen = key >= __float_as_int(from[r]) && key < __float_as_int(to[r]);
-            s[j][f][r] = seen ? s[j][f][r] : 0.f;
-            dp[j][f][r] = seen ? dp[j][f][r] : 0.f;
-          }
+      for (int r = 0; r < 4; ++r) {
+        float z = x[r], fac = 1.f, dist;
+        if (!W::RAW) z = soft.score(z, ax[r], ay[r], kx, ky, fac, dist);
+        float p_ = soft.weight(z, top[r]);
+        if (!ONE) p_ *= inv[r];
+        float dl = p_ * (dp[r] - dsum[r]);
+        if (W::CAP) dl *= fac;
+        x[r] = p_;
+        dp[r] = dl;
       }
+      if (cut) {
+        const f32x4 from = *(const f32x4*)(meta(buf, 2) + qr), to_ = *(const f32x4*)(meta(buf, 3) + qr);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const bool seen = key >= __float_as_int(from[r]) && key < __float_as_int(to_[r]);
+          x[r] = seen ? x[r] : 0.f;
+          dp[r] = seen ? dp[r] : 0.f;
+        }
+      }
+      w[0][f].set(x);
+      ds[0][f].set(dp);
+      __builtin_amdgcn_sched_barrier(0);
     }
-    auto sees = [&](int j, int row) {
-      const int key = w0 + 16 * j + i16;
-      return key >= __float_as_int(meta(buf, 2)[row]) && key < __float_as_int(meta(buf, 3)[row]);
-    };
+    auto sees = [&](int, int row) { return key >= __float_as_int(meta(buf, 2)[row]) && key < __float_as_int(meta(buf, 3)[row]); };
     const bool bad = cut && (tile_not_finite<G>(to, lane) || tile_not_finite<G>(tq, lane));
     if (!SAFE && bad) *odd = 1;
     if (SAFE && bad) {
-      accumulate_seen<G, QF>(to, s, dv, at, lane, sees);
-      accumulate_seen<G, QF>(tq, dp, dk, at, lane, sees);
+      accumulate_seen<G, 1>(to, w, dv, at, lane, sees);
+      accumulate_seen<G, 1>(tq, ds, dk, at, lane, sees);
     } else {
-      accumulate<G, QF>(to, s, dv, at);
-      accumulate<G, QF>(tq, dp, dk, at);
+      accumulate<G, 1>(to, w, dv, at);
+      accumulate<G, 1>(tq, ds, dk, at);
     }
   }
   if (!SAFE) {
     __syncthreads();
     if (*odd) return;
   }
+  const int r = w0 + i16;
+  if (r >= p.M) return;
+  const long o = ((long)r * p.Hkv + hk) * p.D, po = ((long)h0 * p.M + r) * p.D;
 #pragma unroll
-  for (int j = 0; j < QF; ++j) {
-    const int r = w0 + 16 * j + i16;
-    if (r >= p.M) continue;
-    const long o = ((long)r * p.Hkv + hk) * p.D, po = ((long)h0 * p.M + r) * p.D;
-#pragma unroll
-    for (int d = 0; d < G::DF; ++d)
-      if (16 * d + 4 * g < p.D) {
-        if (part) {
-          store4<float>(part + po + 16 * d + 4 * g, dk[j][d], p.scale);
-          store4<float>(part + (long)p.H * p.M * p.D + po + 16 * d + 4 * g, dv[j][d], 1.f);
-          continue;
-        }
-        store4<T>((T*)p.dk + o + 16 * d + 4 * g, dk[j][d], p.scale);
-        store4<T>((T*)p.dv + o + 16 * d + 4 * g, dv[j][d], 1.f);
+  for (int d = 0; d < G::DF; ++d)
+    if (16 * d + 4 * g < p.D) {
+      if (part) {
+        store4<float>(part + po + 16 * d + 4 * g, dk[0][d], p.scale);
+        store4<float>(part + (long)p.H * p.M * p.D + po + 16 * d + 4 * g, dv[0][d], 1.f);
+      } else {
+        store4<T>((T*)p.dk + o + 16 * d + 4 * g, dk[0][d], p.scale);
+        store4<T>((T*)p.dv + o + 16 * d + 4 * g, dv[0][d], 1.f);
       }
-  }
+    }
 }
 
-template <class T, int DP, int QF, int X>
-__global__ __launch_bounds__(256, 2) void blk_attn_dkv_kernel(BlkAttnArgs p, int np, const float* delta, float* part) {
+template <class T, int DP, int X>
+__global__ __launch_bounds__(256, sizeof(T) == 2 || DP <= 64 ? 3 : 2) void blk_attn_dkv_kernel(BlkAttnArgs p, int np, const float* delta, float* part, const float* slope_part, int nqt) {
   using G = BwdGeo<T, DP>;
   __shared__ u32x4 lq[2 * G::TILE], lo_[2 * G::TILE];
   __shared__ __attribute__((aligned(16))) float lm[2 * 7 * 64];  // of each streamed row: top, sum(dO O), lo, hi, x, y, 1 / sum
   __shared__ int range[2], odd;
   const int group = p.H / p.Hkv, nh = part ? p.H : p.Hkv, h0 = part ? blockIdx.x % nh : blockIdx.x % nh * group, heads = part ? 1 : group;
-  const int b0 = blockIdx.x / nh * 64 * QF, w0 = b0 + mg_wave() * 16 * QF;
+  const int b0 = blockIdx.x / nh * 64, w0 = b0 + mg_wave() * 16;
 
+  // the slopes' gradient: a head's partial sums of the dQ kernel, in a fixed order, by the first wave of each of the first workgroups
+  if (X > 1 && p.dslopes && threadIdx.x < 64) {
+    for (int h = blockIdx.x; h < p.H; h += gridDim.x) {
+      double s = 0.;
+      for (int i = threadIdx.x; i < nqt; i += 64) s += (double)slope_part[(long)h * nqt + i];
+#pragma unroll
+      for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+      if (threadIdx.x == 0) p.dslopes[h] = (float)-s;
+    }
+  }
   // the rows that see any of the workgroup's keys lie between the first and the last 32 that do
   if (threadIdx.x == 0) range[0] = INT_MAX, range[1] = -1, odd = 0;
   __syncthreads();
   for (int u = threadIdx.x; u < np / 32; u += 256) {
     const int4 s = *(const int4*)(p.spans + 2 * np + 4 * u);
-    if (s.x < b0 + 64 * QF && s.y > b0) {
+    if (s.x < b0 + 64 && s.y > b0) {
       atomicMin(&range[0], u);
       atomicMax(&range[1], u);
     }
   }
   __syncthreads();
   const int first = range[0], last = range[1], qa = last < 0 ? 0 : first * 32 / G::BK * G::BK, qb = (last + 1) * 32;
-  attn_dkv_rows<T, DP, QF, X, false>(p, np, delta, part, h0, heads, qa, qb, w0, lq, lo_, lm, &odd);
+  attn_dkv_rows<T, DP, X, false>(p, np, delta, part, h0, heads, qa, qb, w0, lq, lo_, lm, &odd);
   if (!odd) return;
-  for (int j = 0; j < QF; ++j) {
-    __syncthreads();
-    attn_dkv_rows<T, DP, 1, X, true>(p, np, delta, part, h0, heads, qa, qb, afresh(w0 + 16 * j), lq, lo_, lm, &odd);
-  }
+  __syncthreads();
+  attn_dkv_rows<T, DP, X, true>(p, np, delta, part, h0, heads, qa, qb, afresh(w0), lq, lo_, lm, &odd);
 }
 
 // dK and dV (blockIdx.y) of a key head: the sums over the heads that share it, in their order; four columns a thread.
@@ -386,7 +380,7 @@ Parts parts_of(int N, int M, int H, int Hkv, int D) {
   return w;
 }
 
-template <class T, int DP, int QF, int QK, int X>
+template <class T, int DP, int QF, int X>
 void launch_bwd_tile(const BlkAttnArgs& p, hipStream_t st) {
   const int np = cdiv(p.N, 128) * 128, nqt = cdiv(p.N, 64 * QF);
   const Parts w = parts_of(p.N, p.M, p.H, p.Hkv, p.D);
@@ -394,19 +388,19 @@ void launch_bwd_tile(const BlkAttnArgs& p, hipStream_t st) {
   float* slopes = (float*)((char*)p.ws + w.slopes);
   float* heads = w.bytes > w.heads ? (float*)((char*)p.ws + w.heads) : nullptr;
   MG_LAUNCH((blk_attn_dq_kernel<T, DP, QF, X>), dim3(nqt * p.H), dim3(256), 0, st, p, np, delta, slopes);
-  if (X > 1 && p.dslopes) MG_LAUNCH(blk_slopes_kernel, dim3(p.H), dim3(64), 0, st, (const float*)slopes, nqt, p.dslopes);
-  MG_LAUNCH((blk_attn_dkv_kernel<T, DP, QK, X>), dim3(cdiv(p.M, 64 * QK) * (heads ? p.H : p.Hkv)), dim3(256), 0, st, p, np, (const float*)delta, heads);
+  MG_LAUNCH((blk_attn_dkv_kernel<T, DP, X>), dim3(cdiv(p.M, 64) * (heads ? p.H : p.Hkv)), dim3(256), 0, st, p, np, (const float*)delta, heads,
+            (const float*)slopes, nqt);
   if (heads) MG_LAUNCH((blk_attn_sum_kernel<T>), dim3(cdiv((long)p.M * p.Hkv * p.D, 1024), 2), dim3(256), 0, st, p, (const float*)heads);
 }
 template <class T, int DP, int X>
 void launch_bwd_x(const BlkAttnArgs& p, hipStream_t st) {
-  // 128 rows a workgroup halve the LDS reads a score; f32 fragments are twice as large and do not fit at the larger widths, nor do the
-  // two results of the keys' side
-  constexpr int QF = sizeof(T) == 2 || DP <= 64 ? 2 : 1, QK = DP <= 64 ? 2 : 1;
-  if ((long)cdiv(p.N, 128) * p.H >= 256)
-    launch_bwd_tile<T, DP, QF, QK, X>(p, st);
+  // rows a workgroup: as in the forward pass (width 128, 16,384 rows: dQ 1.08 against 1.23 ms; width 64: 142 against 125 us).  On the keys'
+  // side, with two results, 16 keys a wave and three waves a SIMD are better at every width (width 128: 1.71 ms against 1.91 with two).
+  constexpr int QF = sizeof(T) == 2 && DP > 64 ? 2 : 1;
+  if (QF > 1 && (long)cdiv(p.N, 128) * p.H >= 256)
+    launch_bwd_tile<T, DP, QF, X>(p, st);
   else
-    launch_bwd_tile<T, DP, 1, 1, X>(p, st);
+    launch_bwd_tile<T, DP, 1, X>(p, st);
 }
 template <class T, int DP>
 void launch_bwd(const BlkAttnArgs& p, hipStream_t st) {

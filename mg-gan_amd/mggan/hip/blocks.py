@@ -269,7 +269,7 @@ def _attn_fwd(q, k, v, slopes, rest, keep):
     (N, H, D), (M, Hkv, _), S, dev = q.shape, k.shape, scenes.shape[0], q.device
     ints, n, _ = _attn_sizes(N, M, H, Hkv, D, S)
     out = torch.empty((N, H, D), dtype=q.dtype, device=dev)
-    at = 2 * H * N + (-2 * H * N) % 4 if keep else 0  # the row intervals lie behind the softmax statistics
+    at = 3 * H * N + (-3 * H * N) % 4 if keep else 0  # the row intervals lie behind the softmax statistics
     stats = torch.empty(at + ints, dtype=_F32, device=dev)
     out32 = ws = None
     if keep:
@@ -299,7 +299,7 @@ def _attn_bwd(ctx, dout):
     n = _attn_sizes(N, M, H, Hkv, D, S)[2]
     ws = _bytes(n, q)
     ps = _p(ctx.stats)
-    at = 2 * H * N + (-2 * H * N) % 4
+    at = 3 * H * N + (-3 * H * N) % 4
     lib.mggan_block_attention_bwd(_ATTN.pack(
         _p(q), _p(k), _p(v), _p(dout), 0, _p(dq), _p(dk), _p(dv), _p(dslopes), _p(scenes), _p(kv_scenes), _p(prefix), _p(xy), _p(kv_xy),
         _p(slopes), ps, _p(out if ctx.out32 is None else ctx.out32), ps + 4 * at, _p(ws), n, q_row, q_head, k_row, k_head, v_row, v_head, N, M, H,
