@@ -42,9 +42,7 @@ struct GemmP {
   float* part;  // split reduction: (splits, M, N or 2 N)
 };
 
-#ifndef BLK_W256
-#define BLK_W256 4
-#endif
+
 enum { EPI_LINEAR = 0, EPI_GATED = 1 };
 
 template <class T, int W>
@@ -212,12 +210,12 @@ __global__ __launch_bounds__(WM* WN * 64) void blk_gemm_kernel(GemmP p) {
   __shared__ u32x4 lds[4 * BUF];
 
   int t = blockIdx.x;
-  {  // neighbouring tiles to the same XCD (blocks are dealt round the eight of them), in columns of eight row tiles
+  {  // neighbouring tiles to the same XCD (blocks are dealt round the eight of them), in columns of four row tiles
     const int nb = p.tiles_m * p.tiles_n, n8 = nb >> 3;
     if (t < n8 * 8) t = (t & 7) * n8 + (t >> 3);
   }
-  const int per = 8 * p.tiles_n, grp = t / per, gm = min(8, p.tiles_m - 8 * grp), rem = t - grp * per;
-  const int m0 = (8 * grp + rem % gm) * BM, n0 = (rem / gm) * NB;
+  const int per = 4 * p.tiles_n, grp = t / per, gm = min(4, p.tiles_m - 4 * grp), rem = t - grp * per;
+  const int m0 = (4 * grp + rem % gm) * BM, n0 = (rem / gm) * NB;
   const int lane = mg_lane(), wave = mg_wave(), i16 = lane & 15, g = lane >> 4;
   const int steps = (p.K + KS - 1) / KS;
   const int kt0 = SPLIT ? blockIdx.y * p.kt_split : 0, n = (SPLIT ? min(kt0 + p.kt_split, steps) : steps) - kt0;
@@ -298,8 +296,9 @@ __global__ __launch_bounds__(WM* WN * 64) void blk_gemm_kernel(GemmP p) {
     constexpr int READS = (CA ? (sizeof(T) == 2 ? 2 : 4) : 1) * FM + (CB ? (sizeof(T) == 2 ? 2 : 4) : 1) * FN;
     constexpr int MM = FM * FN * (sizeof(T) == 2 ? 1 : 4), EACH = MM / (READS + LOADS) > 0 ? MM / (READS + LOADS) : 1;
 #pragma unroll
-    for (int i = 0; i < READS; ++i) {
-      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);     // an LDS read
+    for (int i = 0; i < READS / 2; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x008, EACH, 0);  // multiplications
+      __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);     // an LDS read
       __builtin_amdgcn_sched_group_barrier(0x008, EACH, 0);  // multiplications
     }
 #pragma unroll
@@ -329,13 +328,26 @@ __global__ __launch_bounds__(WM* WN * 64) void blk_gemm_kernel(GemmP p) {
       wait_copies<0>();
     read(0, f0);
     int t = 0;
-    if (!(CB && p.seg)) {
-      const int whole = min(p.K / KS - kt0, n);  // (steps that lie inside k)
-      for (; t + 4 < whole; t += 2) {
+    const int kw = (CB ? min(p.K, p.kb) : p.K) / KS;  // steps that lie inside k (with two segments: inside either)
+    auto walk = [&](int end) {
+      for (; t + 4 < end; t += 2) {
         steady(t, f0, f1);
         steady(t + 1, f1, f0);
       }
+    };
+    int whole = min(kw - kt0, n);
+    if (CB && p.seg) {
+      const int s = p.seg - kt0;  // the second segment's first step
+      if (s > 0 && s < n) {
+        walk(min(kw - kt0, s));
+        for (; t < n && t + 3 <= s; t += 2) {
+          any(t, f0, f1);
+          if (t + 1 < n) any(t + 1, f1, f0);
+        }
+      }
+      whole = min(n, s < n ? s + kw : kw - kt0);
     }
+    walk(whole);
     for (; t < n; t += 2) {
       any(t, f0, f1);
       if (t + 1 < n) any(t + 1, f1, f0);
@@ -370,28 +382,108 @@ __global__ __launch_bounds__(WM* WN * 64) void blk_gemm_kernel(GemmP p) {
   }
 }
 
-// The partial sums of a split reduction joined in their order, then the epilogue; eight outputs a thread.
+// The partial sums of a split reduction, then the epilogue: four outputs a thread, whose partial sums four threads add up (each every
+// fourth, in their order).
 template <class T, int EPI>
 __global__ __launch_bounds__(256) void blk_join_kernel(GemmP p, int splits) {
-  const int per = (p.N + 7) >> 3;
-  const long id = (long)blockIdx.x * 256 + threadIdx.x;
-  if (id >= (long)per * p.M) return;
-  const int m = (int)(id / per), n = (int)(id % per) * 8;
+  __shared__ f32x4 part[EPI == EPI_GATED ? 2 : 1][4][64];
+  const int per = (p.N + 3) >> 2, x = threadIdx.x & 63, y = threadIdx.x >> 6;
+  const long id = (long)blockIdx.x * 64 + x;
+  const int m = (int)(id / per), n = (int)(id % per) * 4;
+  const bool mine = id < (long)per * p.M, vec = p.N % 4 == 0;
   const long cols = EPI == EPI_GATED ? 2L * p.N : p.N;
-  const bool vec4 = p.N % 4 == 0;
-  float v[8] = {}, u[8] = {}, t[8];
-  for (int s = 0; s < splits; ++s) {
-    const float* in = p.part + ((long)s * p.M + m) * cols + n;
-    load_n<float, 8>(in, vec4, p.N - n, t);
+  float v[4] = {}, u[4] = {}, t[4];
+  if (mine) {
+#pragma unroll 4
+    for (int s = y; s < splits; s += 4) {
+      const float* in = p.part + ((long)s * p.M + m) * cols + n;
+      load_n<float, 4>(in, vec, p.N - n, t);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] += t[i];
-    if (EPI == EPI_GATED) {
-      load_n<float, 8>(in + p.N, vec4, p.N - n, t);
+      for (int i = 0; i < 4; ++i) v[i] += t[i];
+      if (EPI == EPI_GATED) {
+        load_n<float, 4>(in + p.N, vec, p.N - n, t);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) u[i] += t[i];
+        for (int i = 0; i < 4; ++i) u[i] += t[i];
+      }
     }
   }
-  epilogue<T, EPI, 8>(p, m, n, v, u, p.N % Mf<T>::CH == 0);
+  part[0][y][x] = f32x4{v[0], v[1], v[2], v[3]};
+  if (EPI == EPI_GATED) part[EPI == EPI_GATED][y][x] = f32x4{u[0], u[1], u[2], u[3]};
+  __syncthreads();
+  if (y || !mine) return;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    v[i] = (part[0][0][x][i] + part[0][1][x][i]) + (part[0][2][x][i] + part[0][3][x][i]);
+    if (EPI == EPI_GATED) u[i] = (part[EPI == EPI_GATED][0][x][i] + part[EPI == EPI_GATED][1][x][i]) + (part[EPI == EPI_GATED][2][x][i] + part[EPI == EPI_GATED][3][x][i]);
+  }
+  epilogue<T, EPI, 4>(p, m, n, v, u, p.N % Mf<T>::CH == 0);
+}
+
+// 16 bytes of a row from element k on, rows of any alignment; what lies past the row's end is zero.
+template <class T>
+__device__ __forceinline__ u32x4 row_chunk(const T* row, int k, int K) {
+  u32x4 v = {0, 0, 0, 0};
+  if (k + Mf<T>::CH <= K) {
+    __builtin_memcpy(&v, row + k, 16);
+  } else {
+    T t[Mf<T>::CH];
+#pragma unroll
+    for (int i = 0; i < Mf<T>::CH; ++i) t[i] = k + i < K ? row[k + i] : (T)0.f;
+    __builtin_memcpy(&v, t, 16);
+  }
+  return v;
+}
+
+// The forward product of up to 16 rows of x: weights stream from memory straight into matrix-instruction operands, once, with nothing
+// between.  A workgroup takes 16 outputs (of both weights where gated), its waves a share of k each; x comes out of the caches.
+template <class T, int EPI, int WAVES>
+__global__ __launch_bounds__(WAVES * 64) void blk_few_rows_kernel(GemmP p) {
+  constexpr int CH = Mf<T>::CH, U = 8, two = EPI == EPI_GATED ? 2 : 1;
+  __shared__ f32x4 part[WAVES][two][64];
+  const int lane = mg_lane(), wave = mg_wave(), i16 = lane & 15, g = lane >> 4, n0 = blockIdx.x * 16;
+  const T* w = (const T*)p.B + (long)min(n0 + i16, p.N - 1) * p.ldb;
+  const T* w2 = (const T*)p.B2 + (long)min(n0 + i16, p.N - 1) * p.ldb;
+  const T* x = (const T*)p.A + (long)min(i16, p.M - 1) * p.lda;  // (rows past the last give outputs that are not stored)
+  const int steps = (p.K + 4 * CH - 1) / (4 * CH), share = (steps + WAVES - 1) / WAVES;
+  const int s0 = wave * share, s1 = min(s0 + share, steps), whole = min(s1, p.K / (4 * CH));
+  f32x4 acc[two] = {};
+  int s = s0;
+  for (; s + U <= whole; s += U) {
+    u32x4 a[U], b[U], c[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int k = (4 * (s + i) + g) * CH;
+      __builtin_memcpy(&a[i], w + k, 16);
+      if (two == 2) __builtin_memcpy(&b[i], w2 + k, 16);
+      __builtin_memcpy(&c[i], x + k, 16);
+    }
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      acc[0] = Mf<T>::step(a[i], c[i], acc[0]);
+      if (two == 2) acc[two - 1] = Mf<T>::step(b[i], c[i], acc[two - 1]);
+    }
+  }
+  for (; s < s1; ++s) {
+    const int k = (4 * s + g) * CH;
+    const u32x4 c = row_chunk(x, k, p.K);
+    acc[0] = Mf<T>::step(row_chunk(w, k, p.K), c, acc[0]);
+    if (two == 2) acc[two - 1] = Mf<T>::step(row_chunk(w2, k, p.K), c, acc[two - 1]);
+  }
+#pragma unroll
+  for (int i = 0; i < two; ++i) part[wave][i][lane] = acc[i];
+  __syncthreads();
+  if (wave || i16 >= p.M) return;
+  float v[4], u[4] = {};
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    v[e] = part[0][0][lane][e];
+    if (two == 2) u[e] = part[0][two - 1][lane][e];
+    for (int k = 1; k < WAVES; ++k) {
+      v[e] += part[k][0][lane][e];
+      if (two == 2) u[e] += part[k][two - 1][lane][e];
+    }
+  }
+  epilogue<T, EPI, 4>(p, i16, n0 + 4 * g, v, u, p.N % CH == 0);
 }
 
 // Rows of `cols` elements into rows of `ldo` (>= cols), the rest zeros.
@@ -544,7 +636,7 @@ int gemm_tile(GemmP& p, const Plan& q, hipStream_t st) {
   p.kt_split = q.kt_split;
   if (q.splits > 1) {
     MG_LAUNCH((blk_gemm_kernel<T, B, B, WM, WN, EPI, true, CA, CB>), dim3(p.tiles_m * p.tiles_n, q.splits), dim3(WM * WN * 64), 0, st, p);
-    MG_LAUNCH((blk_join_kernel<T, EPI>), dim3(cdiv((long)cdiv(p.N, 8) * p.M, 256)), dim3(256), 0, st, p, q.splits);
+    MG_LAUNCH((blk_join_kernel<T, EPI>), dim3(cdiv((long)cdiv(p.N, 4) * p.M, 64)), dim3(256), 0, st, p, q.splits);
   } else {
     MG_LAUNCH((blk_gemm_kernel<T, B, B, WM, WN, EPI, false, CA, CB>), dim3(p.tiles_m * p.tiles_n), dim3(WM * WN * 64), 0, st, p);
   }
@@ -556,7 +648,7 @@ int gemm(GemmP p, void* ws, hipStream_t st) {
   const Plan q = plan_of(p.M, p.N, p.K, Mf<T>::CH, EPI == EPI_GATED);
   p.part = (float*)ws;
   switch (q.tile) {
-    case 256: return gemm_tile<T, 256, 2, BLK_W256, EPI, CA, CB>(p, q, st);
+    case 256: return gemm_tile<T, 256, 2, 4, EPI, CA, CB>(p, q, st);
     case 128: return gemm_tile<T, 128, 2, 2, EPI, CA, CB>(p, q, st);
     default: return gemm_tile<T, 64, 4, 1, EPI, CA, CB>(p, q, st);
   }
@@ -602,16 +694,30 @@ struct Padded {
 template <class T, bool GATED>
 int layer_fwd(const BlkLayerArgs& l, Arena ws, size_t* need, hipStream_t st) {
   constexpr int EPI = GATED ? EPI_GATED : EPI_LINEAR;
+  GemmP p = {};
+  p.M = l.M, p.N = l.N;
+  p.C = l.y, p.ldc = l.N, p.Z = l.z, p.Z2 = l.z2, p.bias = l.b, p.bias2 = l.b2, p.res = l.res, p.act = l.act, p.slope = l.slope;
+  if (l.M <= 16) {  // one matrix instruction's worth of rows: bound by the weights' bytes
+    p.A = l.x, p.lda = l.ldx, p.B = l.w, p.B2 = l.w2, p.ldb = l.K, p.K = l.K;
+    if (need) {
+      *need = 0;
+      return MGGAN_OK;
+    }
+    const unsigned blocks = cdiv(l.N, 16);
+    if (blocks < 512)  // (few workgroups: more waves in each, for bytes in flight)
+      MG_LAUNCH((blk_few_rows_kernel<T, EPI, 8>), dim3(blocks), dim3(512), 0, st, p);
+    else
+      MG_LAUNCH((blk_few_rows_kernel<T, EPI, 4>), dim3(blocks), dim3(256), 0, st, p);
+    MG_LAUNCH_CHECK("block layer forward");
+    return MGGAN_OK;
+  }
   const Padded<T, GATED> o(l, ws, !need, true, true, st);
   void* part = ws.take(plan_of(l.M, l.N, o.Kp, Mf<T>::CH, GATED).bytes);
   if (need) {
     *need = ws.at;
     return MGGAN_OK;
   }
-  GemmP p = {};
-  p.A = o.x, p.lda = o.ldx, p.B = o.w, p.B2 = o.w2, p.ldb = o.Kp;
-  p.M = l.M, p.N = l.N, p.K = o.Kp;
-  p.C = l.y, p.ldc = l.N, p.Z = l.z, p.Z2 = l.z2, p.bias = l.b, p.bias2 = l.b2, p.res = l.res, p.act = l.act, p.slope = l.slope;
+  p.A = o.x, p.lda = o.ldx, p.B = o.w, p.B2 = o.w2, p.ldb = o.Kp, p.K = o.Kp;
   return gemm<T, EPI, false, false>(p, part, st);
 }
 

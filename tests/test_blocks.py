@@ -112,7 +112,7 @@ def test_c_entries_refuse_before_anything_runs():
     ok = dict(x=256, w=512, w2=0, b=0, b2=0, res=0, dy=0, z=0, z2=0, y=768, dx=0, dw=0, db=0, ws=0, ws_bytes=0, ldx=64, M=4, K=64, N=64, act=0,
               dtype=0, slope=0.0)
     for change in (dict(dtype=2), dict(M=0), dict(N=(1 << 20) + 1), dict(x=0), dict(act=3), dict(act=9), dict(ldx=63), dict(ldx=66), dict(x=260),
-                   dict(y=772), dict(y=0), dict(M=4, K=8192, N=64, ldx=8192), dict(w2=1024, z=2048)):
+                   dict(y=772), dict(y=0), dict(M=40, K=8192, N=64, ldx=8192), dict(w2=1024, z=2048)):
         with pytest.raises(HipError):
             lib.mggan_block_layer_fwd(B._LAYER.pack(*{**ok, **change}.values()), 0)
     with pytest.raises(HipError):

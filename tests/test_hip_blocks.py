@@ -50,7 +50,8 @@ def act_of(z, act, slope):
 
 LAYERS = [  # rows, inputs, outputs: one row, odd sizes, tails of tiles and steps, several tiles, a long reduction with few outputs
     (1, 8, 8), (1, 1, 1), (3, 5, 7), (16, 64, 64), (17, 72, 40), (65, 136, 130), (130, 1000, 96), (300, 200, 520), (257, 513, 259),
-    (2, 4096, 33), (5000, 24, 40), (1100, 264, 1032)]
+    (2, 4096, 33), (5000, 24, 40), (1100, 264, 1032),
+    (33, 40, 159), (70, 159, 127), (16, 333, 700), (15, 2005, 24), (40, 96, 320)]
 
 # enough tiles of 128 x 128 and of 256 x 256 outputs for the kernels that take those, with ragged edges
 BIG = [(1800, 200, 1736), (4000, 72, 3333), (4100, 328, 3400)]
