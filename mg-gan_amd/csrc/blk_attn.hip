@@ -195,9 +195,12 @@ __global__ __launch_bounds__(256, QF == 1 && DP <= 64 ? 3 : 2) void blk_attn_fwd
   using G = Geo<T, DP>;
   __shared__ u32x4 lk[2 * G::TILE], lv[2 * G::TILE];
   __shared__ __attribute__((aligned(16))) float lx[2 * 2 * 64];
-  __shared__ int odd;
+  __shared__ int odd, order[RANK_MAX + 1];
   const int h = blockIdx.x % p.H;
-  const int qt = gridDim.x / p.H - 1 - (int)(blockIdx.x / p.H);  // the rows at the end first: behind a causal mask they see the most
+  const int qt = by_work(blockIdx.x / p.H, gridDim.x / p.H, [&](int i) {
+    const int2 k = group_span<2 * QF>(p, np, i * 64 * QF);
+    return k.y - k.x;
+  }, order);
   const int r0 = qt * 64 * QF, w0 = r0 + mg_wave() * 16 * QF;
   if (threadIdx.x == 0) odd = 0;
   __syncthreads();
@@ -366,6 +369,7 @@ __global__ __launch_bounds__(128) void blk_attn_join_kernel(BlkAttnArgs p, int s
 int row_splits(const BlkAttnArgs& p) {
   if (p.lse || p.S == 0 || p.N > 2L * p.S || p.M / p.S < 64) return 0;
   const long blocks = (long)p.N * p.Hkv * cdiv(p.H / p.Hkv, 16);
+  if ((long)p.N * p.H > 1 << 22) return 0;  // (more workgroups than a launch takes)
   long n = cdiv(1024, blocks);
   if (n > p.M / p.S / 128) n = p.M / p.S / 128;
   return n < 1 ? 1 : n > 64 ? 64 : (int)n;
@@ -428,6 +432,7 @@ int blk_attn_check(const BlkAttnArgs* a, const char* name) {
   MG_CHECK_ARG(p.dtype == BLK_F32 || p.dtype == BLK_BF16, "%s: dtype %d (0 = f32, 1 = bf16)", name, p.dtype);
   MG_CHECK_ARG(p.N > 0 && p.M > 0 && p.N <= (1 << 24) && p.M <= (1 << 30), "%s: %d rows, %d keys", name, p.N, p.M);
   MG_CHECK_ARG(p.H > 0 && p.Hkv > 0 && p.H % p.Hkv == 0 && p.H <= 1024, "%s: %d heads over %d key heads", name, p.H, p.Hkv);
+  MG_CHECK_ARG((long)cdiv(p.N, 64) * p.H <= 1 << 23, "%s: %d rows of %d heads are too many workgroups", name, p.N, p.H);
   MG_CHECK_ARG(p.D > 0 && p.D <= 128 && p.D % 8 == 0, "%s: width %d (a multiple of 8 up to 128)", name, p.D);
   MG_CHECK_ARG(p.S >= 0 && p.axes >= 0 && p.axes <= 2 && p.scale > 0.f && p.cap >= 0.f, "%s: %d scenes, %d axes, scale %g, cap %g", name, p.S,
                p.axes, p.scale, p.cap);

@@ -165,12 +165,30 @@ __device__ __forceinline__ float attn_dq_rows(const BlkAttnArgs& p, int np, floa
 }
 
 template <class T, int DP, int QF, int X>
-__global__ __launch_bounds__(256, QF == 1 && DP <= 64 ? 3 : 2) void blk_attn_dq_kernel(BlkAttnArgs p, int np, float* delta, float* slope_part) {
+__global__ __launch_bounds__(256, QF == 1 && DP <= 64 ? 3 : 2) void blk_attn_dq_kernel(BlkAttnArgs p, int np, float* delta, float* slope_part, int2* ranges) {
   using G = BwdGeo<T, DP>;
   __shared__ u32x4 lk[2 * G::TILE], lv[2 * G::TILE];
   __shared__ __attribute__((aligned(16))) float lx[2 * 2 * 64];
-  __shared__ int odd;
-  const int wave = mg_wave(), h = blockIdx.x % p.H, nqt = gridDim.x / p.H, qt = nqt - 1 - (int)(blockIdx.x / p.H);
+  __shared__ int odd, order[RANK_MAX + 1], range[2];
+  // for the keys' side: the rows that see any of 64 keys lie between the first and the last 32 that do
+  for (int kt = blockIdx.x; kt < (p.M + 63) / 64; kt += gridDim.x) {
+    if (threadIdx.x == 0) range[0] = INT_MAX, range[1] = -1;
+    __syncthreads();
+    for (int u = threadIdx.x; u < np / 32; u += 256) {
+      const int4 s = *(const int4*)(p.spans + 2 * np + 4 * u);
+      if (s.x < kt * 64 + 64 && s.y > kt * 64) {
+        atomicMin(&range[0], u);
+        atomicMax(&range[1], u);
+      }
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) ranges[kt] = make_int2(range[0], range[1]);
+  }
+  const int wave = mg_wave(), h = blockIdx.x % p.H, nqt = gridDim.x / p.H;
+  const int qt = by_work(blockIdx.x / p.H, nqt, [&](int i) {
+    const int2 k = group_span<2 * QF>(p, np, i * 64 * QF);
+    return k.y - k.x;
+  }, order);
   const int r0 = qt * 64 * QF, w0 = r0 + wave * 16 * QF;
   if (threadIdx.x == 0) odd = 0;
   __syncthreads();
@@ -315,13 +333,14 @@ __device__ __forceinline__ void attn_dkv_rows(const BlkAttnArgs& p, int np, cons
 }
 
 template <class T, int DP, int X>
-__global__ __launch_bounds__(256, sizeof(T) == 2 || DP <= 64 ? 3 : 2) void blk_attn_dkv_kernel(BlkAttnArgs p, int np, const float* delta, float* part, const float* slope_part, int nqt) {
+__global__ __launch_bounds__(256, DP <= 64 || (sizeof(T) == 2 && DP == 128) ? 3 : 2) void blk_attn_dkv_kernel(BlkAttnArgs p, int np, const float* delta, float* part, const float* slope_part, int nqt, const int2* ranges) {
   using G = BwdGeo<T, DP>;
   __shared__ u32x4 lq[2 * G::TILE], lo_[2 * G::TILE];
   __shared__ __attribute__((aligned(16))) float lm[2 * 7 * 64];  // of each streamed row: top, sum(dO O), lo, hi, x, y, 1 / sum
-  __shared__ int range[2], odd;
+  __shared__ int odd, order[RANK_MAX + 1];
   const int group = p.H / p.Hkv, nh = part ? p.H : p.Hkv, h0 = part ? blockIdx.x % nh : blockIdx.x % nh * group, heads = part ? 1 : group;
-  const int b0 = blockIdx.x / nh * 64, w0 = b0 + mg_wave() * 16;
+  const int kt = by_work(blockIdx.x / nh, gridDim.x / nh, [&](int i) { return ranges[i].y - ranges[i].x; }, order);
+  const int w0 = kt * 64 + mg_wave() * 16;
 
   // the slopes' gradient: a head's partial sums of the dQ kernel, in a fixed order, by the first wave of each of the first workgroups
   if (X > 1 && p.dslopes && threadIdx.x < 64) {
@@ -333,18 +352,9 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 || DP <= 64 ? 3 : 2) void blk_a
       if (threadIdx.x == 0) p.dslopes[h] = (float)-s;
     }
   }
-  // the rows that see any of the workgroup's keys lie between the first and the last 32 that do
-  if (threadIdx.x == 0) range[0] = INT_MAX, range[1] = -1, odd = 0;
+  if (threadIdx.x == 0) odd = 0;
   __syncthreads();
-  for (int u = threadIdx.x; u < np / 32; u += 256) {
-    const int4 s = *(const int4*)(p.spans + 2 * np + 4 * u);
-    if (s.x < b0 + 64 && s.y > b0) {
-      atomicMin(&range[0], u);
-      atomicMax(&range[1], u);
-    }
-  }
-  __syncthreads();
-  const int first = range[0], last = range[1], qa = last < 0 ? 0 : first * 32 / G::BK * G::BK, qb = (last + 1) * 32;
+  const int first = ranges[kt].x, last = ranges[kt].y, qa = last < 0 ? 0 : first * 32 / G::BK * G::BK, qb = (last + 1) * 32;
   attn_dkv_rows<T, DP, X, false>(p, np, delta, part, h0, heads, qa, qb, w0, lq, lo_, lm, &odd);
   if (!odd) return;
   __syncthreads();
@@ -364,17 +374,18 @@ __global__ __launch_bounds__(256) void blk_attn_sum_kernel(BlkAttnArgs p, const 
   store4<T>((T*)(blockIdx.y ? p.dv : p.dk) + (r * p.Hkv + hk) * p.D + d, s, 1.f);
 }
 
-// The workspace: sum(dO O), the slopes' partial sums, and -- where the heads of a key head are taken apart -- dK and dV of every head.
+// The workspace: sum(dO O), the slopes' partial sums, the rows that see each 64 keys, and -- where the heads of a key head are taken apart -- dK and dV of every head.
 // They are where a key head's keys alone are too few workgroups: the first keys behind a causal mask are seen by all rows of all those
 // heads, and one workgroup's walk over them would be the whole time.
 struct Parts {
-  size_t slopes, heads, bytes;
+  size_t slopes, ranges, heads, bytes;
 };
 Parts parts_of(int N, int M, int H, int Hkv, int D) {
   Parts w;
   auto up = [](size_t n) { return (n + 255) / 256 * 256; };
   w.slopes = up((size_t)H * N * 4);
-  w.heads = w.slopes + up((size_t)H * cdiv(N, 64) * 4);
+  w.ranges = w.slopes + up((size_t)H * cdiv(N, 64) * 4);
+  w.heads = w.ranges + up((size_t)cdiv(M, 64) * 8);
   w.bytes = w.heads;
   if (H > Hkv && (long)cdiv(M, 64) * Hkv < 2048) w.bytes += (size_t)2 * H * M * D * 4;
   return w;
@@ -386,10 +397,11 @@ void launch_bwd_tile(const BlkAttnArgs& p, hipStream_t st) {
   const Parts w = parts_of(p.N, p.M, p.H, p.Hkv, p.D);
   float* delta = (float*)p.ws;
   float* slopes = (float*)((char*)p.ws + w.slopes);
+  int2* ranges = (int2*)((char*)p.ws + w.ranges);
   float* heads = w.bytes > w.heads ? (float*)((char*)p.ws + w.heads) : nullptr;
-  MG_LAUNCH((blk_attn_dq_kernel<T, DP, QF, X>), dim3(nqt * p.H), dim3(256), 0, st, p, np, delta, slopes);
+  MG_LAUNCH((blk_attn_dq_kernel<T, DP, QF, X>), dim3(nqt * p.H), dim3(256), 0, st, p, np, delta, slopes, ranges);
   MG_LAUNCH((blk_attn_dkv_kernel<T, DP, X>), dim3(cdiv(p.M, 64) * (heads ? p.H : p.Hkv)), dim3(256), 0, st, p, np, (const float*)delta, heads,
-            (const float*)slopes, nqt);
+            (const float*)slopes, nqt, (const int2*)ranges);
   if (heads) MG_LAUNCH((blk_attn_sum_kernel<T>), dim3(cdiv((long)p.M * p.Hkv * p.D, 1024), 2), dim3(256), 0, st, p, (const float*)heads);
 }
 template <class T, int DP, int X>
@@ -438,6 +450,7 @@ int mggan_block_attention_bwd(const void* args, hipStream_t stream) {
   const int rc = blk_attn_check(a, "block_attention_bwd");
   if (rc != MGGAN_OK) return rc;
   MG_CHECK_ARG(a->out32 && a->lse && a->dout && a->dq && a->dk && a->dv, "block_attention_bwd: null operand");
+  MG_CHECK_ARG((long)cdiv(a->M, 64) * a->H <= 1 << 23, "block_attention_bwd: %d keys of %d heads are too many workgroups", a->M, a->H);
   MG_CHECK_ARG(((size_t)a->out32 | (size_t)a->dout | (size_t)a->dq | (size_t)a->dk | (size_t)a->dv | (size_t)a->spans) % 16 == 0,
                "block_attention_bwd: operands have to be 16-byte aligned");
   const size_t need = parts_of(a->N, a->M, a->H, a->Hkv, a->D).bytes;

@@ -350,8 +350,8 @@ def attention(q, k, v, scenes, kv_scenes=None, *, causal=False, prefix=None, sca
         raise ValueError("attention: {} heads over {} key heads".format(H, Hkv))
     if D % 8 or not 0 < D <= 128:
         raise ValueError("attention: a width of {} (a multiple of 8 up to 128)".format(D))
-    if N > 1 << 24 or M > 1 << 30:
-        raise ValueError("attention: {} rows, {} keys (at most 2^24, 2^30)".format(N, M))
+    if N > 1 << 24 or M > 1 << 30 or N * H > 1 << 29:
+        raise ValueError("attention: {} rows of {} heads, {} keys (at most 2^24 rows, 2^29 rows times heads, 2^30 keys)".format(N, H, M))
     scale = D ** -0.5 if scale is None else float(scale)
     cap = 0.0 if cap is None else float(cap)
     if not 0 < scale < math.inf or not 0 <= cap < math.inf:
@@ -388,6 +388,8 @@ def attention(q, k, v, scenes, kv_scenes=None, *, causal=False, prefix=None, sca
         kv_xy = xy if same else kv_xy.contiguous()
     rest = (table, kv_table, prefix, xy, kv_xy, bool(causal), scale, cap)
     if _needs_grad(q, k, v, slopes):
+        if M * H > 1 << 29:
+            raise ValueError("attention: gradients of {} keys for {} heads (at most 2^29 keys times heads)".format(M, H))
         return AttentionFn.apply(q, k, v, slopes, rest)
     if N == 0 or M == 0:
         return torch.zeros(q.shape, dtype=q.dtype, device=q.device)
