@@ -16,7 +16,7 @@ import torch
 from torch.autograd import Function
 from torch.autograd.function import once_differentiable
 
-from .functions import ACT_LEAKY, ACT_NONE, ACT_SIGMOID, BoundedCache, _p, _s
+from .functions import _GET_DEVICE, ACT_LEAKY, ACT_NONE, ACT_SIGMOID, BoundedCache, _p, _s
 from .lib import lib
 
 ACT_SILU, ACT_GELU = 4, 5
@@ -46,20 +46,25 @@ def _bytes(n, like):
     return torch.empty(n, dtype=torch.uint8, device=like.device) if n else None
 
 
+_current_device = _GET_DEVICE or torch.cuda.current_device
+
+
 def _same(name, x, *others):
     """Every operand has x's type and device."""
-    if x.dtype not in _DTYPES:
-        raise ValueError("{}: f32 or bf16 tensors, got {}".format(name, x.dtype))
+    dtype, device = x.dtype, x.device
+    if dtype not in _DTYPES:
+        raise ValueError("{}: f32 or bf16 tensors, got {}".format(name, dtype))
     for t in others:
-        if t is not None and (t.dtype != x.dtype or t.device != x.device):
-            raise ValueError("{}: one operand is {} on {}, the first one {} on {}".format(name, t.dtype, t.device, x.dtype, x.device))
+        if t is not None and (t.dtype != dtype or t.device != device):
+            raise ValueError("{}: one operand is {} on {}, the first one {} on {}".format(name, t.dtype, t.device, dtype, device))
 
 
 def _on_current(name, x):
     """Whether x lives on the current device (the call is repeated under its own otherwise)."""
-    if not x.is_cuda:
+    at = x.get_device()
+    if at < 0:
         raise ValueError("{}: the operands are on {}; there is no CPU path".format(name, x.device))
-    return x.get_device() == torch.cuda.current_device()
+    return at == _current_device()
 
 
 def _aligned(t):
@@ -98,9 +103,10 @@ def _rows(x, K):
 
 
 def _check_layer(name, x, weight, bias, act):
-    if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1] or not weight.numel():
-        raise ValueError("{}: rows of {} and a weight of {}".format(name, tuple(x.shape), tuple(weight.shape)))
-    N, K = weight.shape
+    rows, shape = x.shape, weight.shape
+    if len(shape) != 2 or not rows or rows[-1] != shape[1] or not shape[0] or not shape[1]:
+        raise ValueError("{}: rows of {} and a weight of {}".format(name, tuple(rows), tuple(shape)))
+    N, K = shape
     if x.numel() > K << 21 or N > 1 << 20 or K > 1 << 20:
         raise ValueError("{}: sizes {} x {} over 2^21 rows, 2^20 columns".format(name, tuple(x.shape), tuple(weight.shape)))
     if act not in _ACTS:
@@ -190,8 +196,8 @@ def linear_residual(x, weight, bias=None, residual=None, act=ACT_NONE, slope=0.0
     if not _on_current("linear_residual", x):
         with torch.cuda.device(x.device):
             return linear_residual(x, weight, bias, residual, act, slope)
-    lead = x.shape[:-1]
     if not two:
+        lead = x.shape[:-1]
         x, residual = x.reshape(-1, x.shape[-1]), None if residual is None else residual.reshape(-1, N)
     if _needs_grad(x, weight, bias, residual):
         y = LayerFn.apply(x, weight, None, bias, None, residual, act, float(slope))
@@ -211,9 +217,9 @@ def gated_linear(x, w_gate, w_up, b_gate=None, b_up=None, act=ACT_SILU, slope=0.
     if not _on_current("gated_linear", x):
         with torch.cuda.device(x.device):
             return gated_linear(x, w_gate, w_up, b_gate, b_up, act, slope)
-    lead, two = x.shape[:-1], x.dim() == 2
+    two = x.dim() == 2
     if not two:
-        x = x.reshape(-1, x.shape[-1])
+        lead, x = x.shape[:-1], x.reshape(-1, x.shape[-1])
     if _needs_grad(x, w_gate, w_up, b_gate, b_up):
         y = LayerFn.apply(x, w_gate, w_up, b_gate, b_up, None, act, float(slope))
     else:
@@ -230,7 +236,8 @@ def _table(name, rows, device, limit, width):
     """int32 device tensor of a scene list (width 2) or of per-scene numbers (width 1): checked and kept by its contents when it is a
     host list, taken as it is when it is a device tensor."""
     if isinstance(rows, torch.Tensor) and rows.is_cuda:
-        if rows.dtype != torch.int32 or rows.device != device or rows.dim() != width or (width == 2 and rows.shape[1] != 2):
+        shape = rows.shape
+        if rows.dtype != torch.int32 or rows.device != device or len(shape) != width or (width == 2 and shape[1] != 2):
             raise ValueError("attention: {} has to be an int32 tensor of (scenes{}) on {}".format(name, ", 2" if width == 2 else "", device))
         return rows if rows.is_contiguous() else rows.contiguous()
     try:
@@ -343,9 +350,10 @@ def attention(q, k, v, scenes, kv_scenes=None, *, causal=False, prefix=None, sca
     xy (N, axes) and kv_xy (M, axes; by default xy), f32 with one or two axes, and slopes (H), f32: the bias by distance.  Gradients go to q,
     k, v and slopes, not to positions."""
     _same("attention", q, k, v)
-    if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape or q.shape[2] != k.shape[2]:
-        raise ValueError("attention: q {}, k {}, v {}".format(tuple(q.shape), tuple(k.shape), tuple(v.shape)))
-    (N, H, D), (M, Hkv, _) = q.shape, k.shape
+    rows, keys = q.shape, k.shape
+    if len(rows) != 3 or len(keys) != 3 or keys != v.shape or rows[2] != keys[2]:
+        raise ValueError("attention: q {}, k {}, v {}".format(tuple(rows), tuple(keys), tuple(v.shape)))
+    (N, H, D), (M, Hkv, _) = rows, keys
     if not 0 < H <= 1024 or not Hkv or H % Hkv:
         raise ValueError("attention: {} heads over {} key heads".format(H, Hkv))
     if D % 8 or not 0 < D <= 128:
@@ -364,9 +372,9 @@ def attention(q, k, v, scenes, kv_scenes=None, *, causal=False, prefix=None, sca
         raise ValueError("attention: {} rows over {} keys need kv_scenes".format(N, M))
     if xy is not None:
         kv_xy = xy if kv_xy is None else kv_xy
-        for t, rows in ((xy, N), (kv_xy, M)):
-            if t.dtype != _F32 or t.dim() != 2 or t.shape[0] != rows or t.shape[1] not in (1, 2) or t.shape[1] != xy.shape[1] or t.device != q.device:
-                raise ValueError("attention: positions {} {} on {} for {} rows: f32, one or two axes".format(t.dtype, tuple(t.shape), t.device, rows))
+        for t, n in ((xy, N), (kv_xy, M)):
+            if t.dtype != _F32 or t.dim() != 2 or t.shape[0] != n or t.shape[1] not in (1, 2) or t.shape[1] != xy.shape[1] or t.device != q.device:
+                raise ValueError("attention: positions {} {} on {} for {} rows: f32, one or two axes".format(t.dtype, tuple(t.shape), t.device, n))
             if t.requires_grad and torch.is_grad_enabled():
                 raise ValueError("attention: positions have no gradient: detach them")
         if slopes.dtype != _F32 or slopes.dim() != 1 or slopes.shape[0] != H or slopes.device != q.device:
@@ -374,12 +382,13 @@ def attention(q, k, v, scenes, kv_scenes=None, *, causal=False, prefix=None, sca
     if not _on_current("attention", q):
         with torch.cuda.device(q.device):
             return attention(q, k, v, scenes, kv_scenes, causal=causal, prefix=prefix, scale=scale, cap=cap, xy=xy, kv_xy=kv_xy, slopes=slopes)
-    table = _table("scenes", scenes, q.device, N, 2)
-    kv_table = table if kv_scenes is None else _table("kv_scenes", kv_scenes, q.device, M, 2)
+    dev = q.device
+    table = _table("scenes", scenes, dev, N, 2)
+    kv_table = table if kv_scenes is None else _table("kv_scenes", kv_scenes, dev, M, 2)
     if table.shape[0] != kv_table.shape[0]:
         raise ValueError("attention: {} scenes of rows, {} of keys".format(table.shape[0], kv_table.shape[0]))
     if prefix is not None:
-        prefix = _table("prefix", prefix, q.device, 0, 1)
+        prefix = _table("prefix", prefix, dev, 0, 1)
         if prefix.shape[0] != table.shape[0]:
             raise ValueError("attention: {} prefixes for {} scenes".format(prefix.shape[0], table.shape[0]))
     if xy is not None:

@@ -600,8 +600,12 @@ def test_caches_beyond_32_bit_offsets():
         a = B_.attention(q, k, k, [(0, 200)], [(M - 700, M)], causal=True)
         assert torch.equal(a, B_.attention(q, tail, tail, [(0, 200)], [(0, 700)], causal=True))
         a = B_.attention(q[:1], k, k, [(0, 1)], [(M - 700, M)])
-        b = B_.attention(q[:1], tail, tail, [(0, 1)], [(0, 700)])
-        torch.testing.assert_close(a.double(), b.double(), rtol=4 * U[torch.bfloat16], atol=1e-4)
+        # the keys are split by the cache's size, and every share rounds its weights (u each) against a maximum of its own, so this one is not
+        # the same bits as over the short cache: both are held to the definition, within (u + f32 sums) sum P |v| + u |out|
+        see = torch.ones(1, 700, dtype=torch.bool, device="cuda")
+        want = reference(q[:1], tail, tail, see, q[:1], D ** -0.5, 0.0, None, None, None)["out"]
+        close(a, *want, "long cache")
+        close(B_.attention(q[:1], tail, tail, [(0, 1)], [(0, 700)]), *want, "short cache")
 
 
 def test_a_second_derivative_is_refused():
