@@ -48,6 +48,14 @@ __device__ __forceinline__ void lds_copy16(const void* g, void* lds) {
   __builtin_amdgcn_global_load_lds((MG_GLB const void*)g, (MG_LDS void*)lds, 16, 0, 0);
 }
 
+// Copies into LDS are waited for by hand: copies_done() for all of them, a counted wait where some may stay under way.  Left to itself the
+// compiler waits for every copy before any read that might meet one, the next tile's included, which undoes the double buffer.  It does not
+// where a kernel has one __shared__ object and where the pointer of a transposing read is its own (__restrict: nothing is written while
+// the function runs).  Training pass of the gated layer, 8,192 rows of 4,096: 2.95 -> 2.79 ms; attention's forward pass at width 128: 854 -> 830 us.
+__device__ __forceinline__ void copies_done() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+// The transposing read: four 16-bit values of each of the lane's group's rows.
+__device__ __forceinline__ s16x4 lds_transposed(const char* __restrict p) { return __builtin_amdgcn_ds_read_tr16_b64_v4i16((MG_LDS s16x4*)p); }
+
 template <class T>
 __device__ __forceinline__ float to_f(T v) {
   return (float)v;

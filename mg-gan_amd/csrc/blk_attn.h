@@ -143,8 +143,8 @@ struct Lane {
   // bf16: columns 16 fd + i of rows 32 p + 8 g + {0..7}, transposed: first operand of a product over the tile's rows
   __device__ __forceinline__ bf16x8 cols(const char* tile, int p, int fd) const {
     const char* a = tile + col[WIDE ? fd & 3 : fd & 1] + 32 * p * ROW + (WIDE ? (fd >> 2) * 128 : (fd >> 1) * 64);
-    const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((MG_LDS s16x4*)a);
-    const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((MG_LDS s16x4*)(a + 4 * ROW));
+    const s16x4 x = lds_transposed(a);
+    const s16x4 y = lds_transposed(a + 4 * ROW);
     return __builtin_bit_cast(bf16x8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
   }
   // f32: column 16 fd + i of row 16 f + 4 g + r
@@ -210,8 +210,9 @@ __device__ __forceinline__ void scores2(const void* ta, const void* tb, const u3
   x = y = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int s = 0; s < G::SK; ++s) {
-    x = Mf<typename G::T>::step(at.rows((const char*)ta, f, s), a[s], x);
-    y = Mf<typename G::T>::step(at.rows((const char*)tb, f, s), b[s], y);
+    const u32x4 ra = at.rows((const char*)ta, f, s), rb = at.rows((const char*)tb, f, s);
+    x = Mf<typename G::T>::step(ra, a[s], x);
+    y = Mf<typename G::T>::step(rb, b[s], y);
   }
 }
 

@@ -98,7 +98,7 @@ __device__ __forceinline__ void attn_fwd_rows(const BlkAttnArgs& p, int np, int 
   if (glo < ghi) fetch(glo, 0);
   int buf = 0;
   for (int k0 = glo; k0 < ghi; k0 += G::BK, buf ^= 1) {
-    __syncthreads();
+    copies_done();
     if (k0 + G::BK < ghi) fetch(k0 + G::BK, buf ^ 1);
     if (k0 >= whi || k0 + G::BK <= wlo) continue;  // (the wave's: nothing of this tile is seen)
     const u32x4* tv = lv + buf * G::TILE;
@@ -193,23 +193,25 @@ __device__ __forceinline__ void attn_fwd_rows(const BlkAttnArgs& p, int np, int 
 template <class T, int DP, int QF, int X>
 __global__ __launch_bounds__(256, QF == 1 && DP <= 64 ? 3 : 2) void blk_attn_fwd_kernel(BlkAttnArgs p, int np) {
   using G = Geo<T, DP>;
-  __shared__ u32x4 lk[2 * G::TILE], lv[2 * G::TILE];
-  __shared__ __attribute__((aligned(16))) float lx[2 * 2 * 64];
-  __shared__ int odd, order[RANK_MAX + 1];
+  __shared__ struct {
+    u32x4 k[2 * G::TILE], v[2 * G::TILE];
+    float x[2 * 2 * 64];
+    int odd, order[RANK_MAX + 1];
+  } lds;
   const int h = blockIdx.x % p.H;
   const int qt = by_work(blockIdx.x / p.H, gridDim.x / p.H, [&](int i) {
     const int2 k = group_span<2 * QF>(p, np, i * 64 * QF);
     return k.y - k.x;
-  }, order);
+  }, lds.order);
   const int r0 = qt * 64 * QF, w0 = r0 + mg_wave() * 16 * QF;
-  if (threadIdx.x == 0) odd = 0;
+  if (threadIdx.x == 0) lds.odd = 0;
   __syncthreads();
   const int2 keys = group_span<2 * QF>(p, np, r0);  // (what the workgroup's rows see)
-  attn_fwd_rows<T, DP, QF, X, false>(p, np, h, keys.x, keys.y, w0, lk, lv, lx, &odd);
-  if (!odd) return;
+  attn_fwd_rows<T, DP, QF, X, false>(p, np, h, keys.x, keys.y, w0, lds.k, lds.v, lds.x, &lds.odd);
+  if (!lds.odd) return;
   for (int j = 0; j < QF; ++j) {
     __syncthreads();
-    attn_fwd_rows<T, DP, 1, X, true>(p, np, h, keys.x, keys.y, afresh(w0 + 16 * j), lk, lv, lx, &odd);
+    attn_fwd_rows<T, DP, 1, X, true>(p, np, h, keys.x, keys.y, afresh(w0 + 16 * j), lds.k, lds.v, lds.x, &lds.odd);
   }
 }
 
@@ -223,8 +225,11 @@ __global__ __launch_bounds__(256) void blk_attn_row_kernel(BlkAttnArgs p, int sp
   using W = Soft<T, X>;
   constexpr int AXES = W::AXES;
   constexpr int LOADS = 2 * G::TILE / 64;  // copies of a tile of keys and one of values
-  __shared__ u32x4 tiles[4][2][2][G::TILE];
-  __shared__ int scene;
+  __shared__ struct {
+    u32x4 tiles[4][2][2][G::TILE];
+    int scene;
+  } lds;
+  auto& tiles = lds.tiles;
   const int lane = mg_lane(), wave = mg_wave(), i16 = lane & 15, g = lane >> 4, nd = p.D / G::CH;
   int id = blockIdx.x;
   const int sp = id % splits;
@@ -235,12 +240,12 @@ __global__ __launch_bounds__(256) void blk_attn_row_kernel(BlkAttnArgs p, int sp
   const int head = hk * group + hg * 16 + i16;
   const bool mine = hg * 16 + i16 < group;
 
-  if (threadIdx.x == 0) scene = -1;
+  if (threadIdx.x == 0) lds.scene = -1;
   __syncthreads();
   for (int s = threadIdx.x; s < p.S; s += 256)
-    if (p.scenes[2 * s] <= r && r < p.scenes[2 * s + 1]) atomicMax(&scene, s);
+    if (p.scenes[2 * s] <= r && r < p.scenes[2 * s + 1]) atomicMax(&lds.scene, s);
   __syncthreads();
-  const int2 span = blk_span(p, scene, r);
+  const int2 span = blk_span(p, lds.scene, r);
   const int n = span.y - span.x, per = ((n + splits - 1) / splits + G::BK - 1) / G::BK * G::BK;
   const int lo = min(span.x + sp * per, span.y), hi = min(lo + per, span.y);
 

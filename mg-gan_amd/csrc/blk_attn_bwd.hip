@@ -84,7 +84,7 @@ __device__ __forceinline__ float attn_dq_rows(const BlkAttnArgs& p, int np, floa
   if (glo < ghi) fetch(glo, 0);
   int buf = 0;
   for (int k0 = glo; k0 < ghi; k0 += G::BK, buf ^= 1) {
-    __syncthreads();
+    copies_done();
     if (k0 + G::BK < ghi) fetch(k0 + G::BK, buf ^ 1);
     if (k0 >= whi || k0 + G::BK <= wlo) continue;
     const u32x4 *tk = lk + buf * G::TILE, *tv = lv + buf * G::TILE;
@@ -167,46 +167,48 @@ __device__ __forceinline__ float attn_dq_rows(const BlkAttnArgs& p, int np, floa
 template <class T, int DP, int QF, int X>
 __global__ __launch_bounds__(256, QF == 1 && DP <= 64 ? 3 : 2) void blk_attn_dq_kernel(BlkAttnArgs p, int np, float* delta, float* slope_part, int2* ranges) {
   using G = BwdGeo<T, DP>;
-  __shared__ u32x4 lk[2 * G::TILE], lv[2 * G::TILE];
-  __shared__ __attribute__((aligned(16))) float lx[2 * 2 * 64];
-  __shared__ int odd, order[RANK_MAX + 1], range[2];
+  __shared__ struct {
+    u32x4 k[2 * G::TILE], v[2 * G::TILE];
+    float x[2 * 2 * 64];
+    int odd, order[RANK_MAX + 1], range[2];
+  } lds;
   // for the keys' side: the rows that see any of 64 keys lie between the first and the last 32 that do
   for (int kt = blockIdx.x; kt < (p.M + 63) / 64; kt += gridDim.x) {
-    if (threadIdx.x == 0) range[0] = INT_MAX, range[1] = -1;
+    if (threadIdx.x == 0) lds.range[0] = INT_MAX, lds.range[1] = -1;
     __syncthreads();
     for (int u = threadIdx.x; u < np / 32; u += 256) {
       const int4 s = *(const int4*)(p.spans + 2 * np + 4 * u);
       if (s.x < kt * 64 + 64 && s.y > kt * 64) {
-        atomicMin(&range[0], u);
-        atomicMax(&range[1], u);
+        atomicMin(&lds.range[0], u);
+        atomicMax(&lds.range[1], u);
       }
     }
     __syncthreads();
-    if (threadIdx.x == 0) ranges[kt] = make_int2(range[0], range[1]);
+    if (threadIdx.x == 0) ranges[kt] = make_int2(lds.range[0], lds.range[1]);
   }
   const int wave = mg_wave(), h = blockIdx.x % p.H, nqt = gridDim.x / p.H;
   const int qt = by_work(blockIdx.x / p.H, nqt, [&](int i) {
     const int2 k = group_span<2 * QF>(p, np, i * 64 * QF);
     return k.y - k.x;
-  }, order);
+  }, lds.order);
   const int r0 = qt * 64 * QF, w0 = r0 + wave * 16 * QF;
-  if (threadIdx.x == 0) odd = 0;
+  if (threadIdx.x == 0) lds.odd = 0;
   __syncthreads();
   const int2 keys = group_span<2 * QF>(p, np, r0);
-  float sum = attn_dq_rows<T, DP, QF, X, false>(p, np, delta, h, keys.x, keys.y, w0, lk, lv, lx, &odd);
-  if (odd) {
+  float sum = attn_dq_rows<T, DP, QF, X, false>(p, np, delta, h, keys.x, keys.y, w0, lds.k, lds.v, lds.x, &lds.odd);
+  if (lds.odd) {
     sum = 0.f;
     for (int j = 0; j < QF; ++j) {
       __syncthreads();
-      sum += attn_dq_rows<T, DP, 1, X, true>(p, np, delta, h, keys.x, keys.y, afresh(w0 + 16 * j), lk, lv, lx, &odd);
+      sum += attn_dq_rows<T, DP, 1, X, true>(p, np, delta, h, keys.x, keys.y, afresh(w0 + 16 * j), lds.k, lds.v, lds.x, &lds.odd);
     }
   }
   if (X > 1 && p.dslopes) {
     __syncthreads();
     sum = wave_sum(sum);
-    if (mg_lane() == 0) lx[wave] = sum;
+    if (mg_lane() == 0) lds.x[wave] = sum;
     __syncthreads();
-    if (threadIdx.x == 0) slope_part[(long)h * nqt + qt] = (lx[0] + lx[1]) + (lx[2] + lx[3]);
+    if (threadIdx.x == 0) slope_part[(long)h * nqt + qt] = (lds.x[0] + lds.x[1]) + (lds.x[2] + lds.x[3]);
   }
 }
 
@@ -221,6 +223,7 @@ __device__ __forceinline__ void attn_dkv_rows(const BlkAttnArgs& p, int np, cons
   constexpr bool ONE = sizeof(T) == 2;  // one statistic a row
   const int lane = mg_lane(), wave = mg_wave(), i16 = lane & 15, g = lane >> 4, hk = h0 / (p.H / p.Hkv), nd = p.D / G::CH;
   u32x4 k[G::SK], v[G::SK];
+  f32x4 dk[1][G::DF], dv[1][G::DF];
   const int rc = min(w0 + i16, p.M - 1);
   const T* kr = (const T*)p.k + rc * p.k_row + hk * p.k_head;
   const T* vr = (const T*)p.v + rc * p.v_row + hk * p.v_head;
@@ -230,13 +233,12 @@ __device__ __forceinline__ void attn_dkv_rows(const BlkAttnArgs& p, int np, cons
     v[s] = owner_chunk(vr, 4 * s + g, nd);
   }
   const float kx = AXES ? p.kv_xy[(long)rc * AXES] : 0.f, ky = AXES > 1 ? p.kv_xy[(long)rc * AXES + 1] : 0.f;
-  f32x4 dk[1][G::DF], dv[1][G::DF];
 #pragma unroll
   for (int d = 0; d < G::DF; ++d) dk[0][d] = dv[0][d] = f32x4{0.f, 0.f, 0.f, 0.f};
   Lane<G> at;
   at.init(lane);
 
-  auto meta = [&](int buf, int i) { return lm + (7 * buf + i) * 64; };
+  auto meta = [&](int buf, int i) { return lm + (8 * buf + i) * 64; };
   // (head, tile) pairs in one sequence, so that the copies of the next head's first tile are under way too
   const int nt = qb > qa ? (qb - qa + G::BK - 1) / G::BK : 0, total = nt * heads;
   auto fetch = [&](int t, int buf) {
@@ -248,22 +250,26 @@ __device__ __forceinline__ void attn_dkv_rows(const BlkAttnArgs& p, int np, cons
     if (wave == 1) copy_meta(delta + (long)h * p.N, 1, 0, q0, p.N, meta(buf, 1));
     if (wave == 2) copy_meta(p.spans, 1, 0, q0, np, meta(buf, 2));
     if (wave == 3) copy_meta(p.spans + np, 1, 0, q0, np, meta(buf, 3));
+    if (wave == 2) copy_meta(p.spans + 2 * np, 1, 0, q0 >> 3, np >> 3, meta(buf, 7));
     if (wave < AXES) copy_meta(p.xy, AXES, wave, q0, p.N, meta(buf, 4 + wave));
   };
   if (total > 0) fetch(0, 0);
+  float slope = 0.f;
   for (int t = 0; t < total; ++t) {
     const int buf = t & 1, q0 = qa + t % nt * G::BK, h = h0 + t / nt;
-    __syncthreads();
+    copies_done();
+    if (AXES && t % nt == 0) slope = __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(p.slopes[h])));
     if (t + 1 < total) fetch(t + 1, buf ^ 1);
     int slo = INT_MAX, shi = 0, flo = 0, fhi = INT_MAX;
 #pragma unroll
     for (int i = 0; i < G::BK / 32; ++i) {
-      const int4 u = *(const int4*)(p.spans + 2 * np + 4 * ((q0 >> 5) + i));
+      const int4 u = *(const int4*)(meta(buf, 7) + 4 * i);  // (a load from memory would be waited for behind the copies)
       slo = min(slo, u.x), shi = max(shi, u.y), flo = max(flo, u.z), fhi = min(fhi, u.w);
     }
+    slo = __builtin_amdgcn_readfirstlane(slo), shi = __builtin_amdgcn_readfirstlane(shi);
     if (slo >= w0 + 16 || shi <= w0) continue;
-    const bool cut = w0 < flo || w0 + 16 > fhi;
-    const W soft(p, AXES ? p.slopes[h] : 0.f);
+    const bool cut = __builtin_amdgcn_readfirstlane(w0 < flo || w0 + 16 > fhi);
+    const W soft(p, slope);
     const u32x4 *tq = lq + buf * G::TILE, *to = lo_ + buf * G::TILE;
     const int key = w0 + i16;
     Coef<T> w[1][G::F], ds[1][G::F];
@@ -335,11 +341,13 @@ __device__ __forceinline__ void attn_dkv_rows(const BlkAttnArgs& p, int np, cons
 template <class T, int DP, int X>
 __global__ __launch_bounds__(256, DP <= 64 || (sizeof(T) == 2 && DP == 128) ? 3 : 2) void blk_attn_dkv_kernel(BlkAttnArgs p, int np, const float* delta, float* part, const float* slope_part, int nqt, const int2* ranges) {
   using G = BwdGeo<T, DP>;
-  __shared__ u32x4 lq[2 * G::TILE], lo_[2 * G::TILE];
-  __shared__ __attribute__((aligned(16))) float lm[2 * 7 * 64];  // of each streamed row: top, sum(dO O), lo, hi, x, y, 1 / sum
-  __shared__ int odd, order[RANK_MAX + 1];
+  __shared__ struct {
+    u32x4 q[2 * G::TILE], o[2 * G::TILE];
+    float m[2 * 8 * 64];  // of each streamed row: top, sum(dO O), lo, hi, x, y, 1 / sum; then what 32 rows see
+    int odd, order[RANK_MAX + 1];
+  } lds;
   const int group = p.H / p.Hkv, nh = part ? p.H : p.Hkv, h0 = part ? blockIdx.x % nh : blockIdx.x % nh * group, heads = part ? 1 : group;
-  const int kt = by_work(blockIdx.x / nh, gridDim.x / nh, [&](int i) { return ranges[i].y - ranges[i].x; }, order);
+  const int kt = by_work(blockIdx.x / nh, gridDim.x / nh, [&](int i) { return ranges[i].y - ranges[i].x; }, lds.order);
   const int w0 = kt * 64 + mg_wave() * 16;
 
   // the slopes' gradient: a head's partial sums of the dQ kernel, in a fixed order, by the first wave of each of the first workgroups
@@ -352,13 +360,13 @@ __global__ __launch_bounds__(256, DP <= 64 || (sizeof(T) == 2 && DP == 128) ? 3 
       if (threadIdx.x == 0) p.dslopes[h] = (float)-s;
     }
   }
-  if (threadIdx.x == 0) odd = 0;
+  if (threadIdx.x == 0) lds.odd = 0;
   __syncthreads();
   const int first = ranges[kt].x, last = ranges[kt].y, qa = last < 0 ? 0 : first * 32 / G::BK * G::BK, qb = (last + 1) * 32;
-  attn_dkv_rows<T, DP, X, false>(p, np, delta, part, h0, heads, qa, qb, w0, lq, lo_, lm, &odd);
-  if (!odd) return;
+  attn_dkv_rows<T, DP, X, false>(p, np, delta, part, h0, heads, qa, qb, w0, lds.q, lds.o, lds.m, &lds.odd);
+  if (!lds.odd) return;
   __syncthreads();
-  attn_dkv_rows<T, DP, X, true>(p, np, delta, part, h0, heads, qa, qb, afresh(w0), lq, lo_, lm, &odd);
+  attn_dkv_rows<T, DP, X, true>(p, np, delta, part, h0, heads, qa, qb, afresh(w0), lds.q, lds.o, lds.m, &lds.odd);
 }
 
 // dK and dV (blockIdx.y) of a key head: the sums over the heads that share it, in their order; four columns a thread.
@@ -400,8 +408,9 @@ void launch_bwd_tile(const BlkAttnArgs& p, hipStream_t st) {
   int2* ranges = (int2*)((char*)p.ws + w.ranges);
   float* heads = w.bytes > w.heads ? (float*)((char*)p.ws + w.heads) : nullptr;
   MG_LAUNCH((blk_attn_dq_kernel<T, DP, QF, X>), dim3(nqt * p.H), dim3(256), 0, st, p, np, delta, slopes, ranges);
-  MG_LAUNCH((blk_attn_dkv_kernel<T, DP, X>), dim3(cdiv(p.M, 64) * (heads ? p.H : p.Hkv)), dim3(256), 0, st, p, np, (const float*)delta, heads,
-            (const float*)slopes, nqt, (const int2*)ranges);
+  const int nh = heads ? p.H : p.Hkv;
+  MG_LAUNCH((blk_attn_dkv_kernel<T, DP, X>), dim3(cdiv(p.M, 64) * nh), dim3(256), 0, st, p, np, (const float*)delta, heads, (const float*)slopes, nqt,
+            (const int2*)ranges);
   if (heads) MG_LAUNCH((blk_attn_sum_kernel<T>), dim3(cdiv((long)p.M * p.Hkv * p.D, 1024), 2), dim3(256), 0, st, p, (const float*)heads);
 }
 template <class T, int DP, int X>

@@ -175,8 +175,8 @@ struct Side {
     } else if constexpr (sizeof(T) == 2) {
       const int k = 8 * g + (i16 >> 2), sw = swz(k), ch = (first >> 3) + ((i16 & 3) >> 1);
       const char* a = (const char*)(t + k * NC + (ch ^ sw)) + 8 * (i16 & 1);
-      const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((MG_LDS s16x4*)a);
-      const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((MG_LDS s16x4*)(a + 4 * NC * 16));  // (k + 4: the same swizzle)
+      const s16x4 x = lds_transposed(a);
+      const s16x4 y = lds_transposed(a + 4 * NC * 16);  // (k + 4: the same swizzle)
       return __builtin_bit_cast(u32x4, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
     } else {
       u32x4 v;
@@ -190,10 +190,11 @@ struct Side {
   }
 };
 
-// Waits until at most n of this wave's copies are under way (they end in their order), then for the other waves.
+// Waits until at most n of this wave's copies are under way (they end in their order) and its LDS reads are done (the next copies go into
+// what they read), then for the other waves.
 template <int n>
 __device__ __forceinline__ void wait_copies() {
-  asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(n) : "memory");
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(n) : "memory");
 }
 
 // A tile of BM x BN outputs, WM x WN waves; k in steps of 64 bytes through a ring of four LDS buffers.  In step t the copies of step
