@@ -439,8 +439,9 @@ int blk_attn_check(const BlkAttnArgs* a, const char* name) {
   MG_CHECK_ARG(p.H > 0 && p.Hkv > 0 && p.H % p.Hkv == 0 && p.H <= 1024, "%s: %d heads over %d key heads", name, p.H, p.Hkv);
   MG_CHECK_ARG((long)cdiv(p.N, 64) * p.H <= 1 << 23, "%s: %d rows of %d heads are too many workgroups", name, p.N, p.H);
   MG_CHECK_ARG(p.D > 0 && p.D <= 128 && p.D % 8 == 0, "%s: width %d (a multiple of 8 up to 128)", name, p.D);
-  MG_CHECK_ARG(p.S >= 0 && p.axes >= 0 && p.axes <= 2 && p.scale > 0.f && p.cap >= 0.f, "%s: %d scenes, %d axes, scale %g, cap %g", name, p.S,
-               p.axes, p.scale, p.cap);
+  auto in_range = [](float x) { return x >= 0x1p-60f && x <= 0x1p60f; };  // (quotient and products stay normal numbers)
+  MG_CHECK_ARG(p.S >= 0 && p.axes >= 0 && p.axes <= 2 && in_range(p.scale) && (p.cap == 0.f || in_range(p.cap)),
+               "%s: %d scenes, %d axes, scale %g, cap %g", name, p.S, p.axes, p.scale, p.cap);
   MG_CHECK_ARG(p.q && p.k && p.v && p.spans && (p.S == 0 || (p.scenes && p.kv_scenes)), "%s: null operand", name);
   MG_CHECK_ARG(!p.axes || (p.xy && p.kv_xy && p.slopes), "%s: positions without coordinates or slopes", name);
   const long ch = p.dtype == BLK_BF16 ? 8 : 4;

@@ -9,8 +9,8 @@ rounded once.  Work goes to torch's current stream, outputs and workspaces come 
 into a HIP graph), gradients are returned through autograd and are the same bits in every run.  Arguments that do not fit raise
 ValueError, a failing launch raises HipError; there is no CPU path."""
 import functools
-import math
 import struct
+from itertools import chain
 
 import torch
 from torch.autograd import Function
@@ -144,7 +144,7 @@ def _layer_fwd(x, w, w2, b, b2, res, act, slope, keep):
 
 
 def _layer_bwd(ctx, dy):
-    x, w, w2 = ctx.saved_tensors
+    x, w, w2, z = ctx.saved_tensors
     gated, need = w2 is not None, ctx.needs_input_grad
     (x, ldx), (N, K) = _rows(x, w.shape[1]), w.shape
     M, dev, dt = x.shape[0], x.device, x.dtype
@@ -155,7 +155,7 @@ def _layer_bwd(ctx, dy):
     dw = make(off + N, K, dtype=dt, device=dev) if need[1] or need[2] else None
     db = make((1 + gated) * N, dtype=dt, device=dev) if need[3] or need[4] else None
     if M and (dx is not None or dw is not None or db is not None):
-        g, z = _aligned(dy), ctx.z
+        g = _aligned(dy)
         n = _layer_workspace(M, K, N, gated, 1, ctx.act, code)
         ws = _bytes(n, x)
         lib.mggan_block_layer_bwd(_LAYER.pack(_p(x), _p(w), _p(w2), 0, 0, 0, _p(g), _p(z), _p(z) + 4 * z.stride(0) if gated else 0, 0, _p(dx),
@@ -174,9 +174,9 @@ class LayerFn(Function):
 
     @staticmethod
     def forward(ctx, x, w, w2, b, b2, res, act, slope):
-        y, ctx.z, x, w, w2 = _layer_fwd(x, w, w2, b, b2, res, act, slope, True)
+        y, z, x, w, w2 = _layer_fwd(x, w, w2, b, b2, res, act, slope, True)
         ctx.act, ctx.slope = act, slope
-        ctx.save_for_backward(x, w, w2)
+        ctx.save_for_backward(x, w, w2, z)
         return y
 
     @staticmethod
@@ -230,6 +230,7 @@ def gated_linear(x, w_gate, w_up, b_gate=None, b_up=None, act=ACT_SILU, slope=0.
 # ---- attention ---------------------------------------------------------------------------------------------------------------
 
 _TABLES = BoundedCache(64)
+_LEAST = 2.0 ** -60  # of scale and cap: their quotient and their products with log2 e stay normal f32 numbers
 
 
 def _table(name, rows, device, limit, width):
@@ -241,19 +242,29 @@ def _table(name, rows, device, limit, width):
             raise ValueError("attention: {} has to be an int32 tensor of (scenes{}) on {}".format(name, ", 2" if width == 2 else "", device))
         return rows if rows.is_contiguous() else rows.contiguous()
     try:
-        key = tuple((int(a), int(b)) for a, b in rows) if width == 2 else tuple(int(a) for a in rows)
+        key = tuple(map(tuple, rows)) if width == 2 else tuple(rows)
+        if not {int}.issuperset(map(type, chain.from_iterable(key) if width == 2 else key)) or width == 2 and not {2}.issuperset(map(len, key)):
+            key = tuple((int(a), int(b)) for a, b in key) if width == 2 else tuple(int(a) for a in key)
     except (TypeError, ValueError):
         raise ValueError("attention: {} has to be a list or an int32 device tensor".format(name)) from None
-    for k in key:
-        if width == 2 and not 0 <= k[0] <= k[1] <= limit:
-            raise ValueError("attention: {} names rows [{}, {}) of {}".format(name, k[0], k[1], limit))
-        if width == 1 and abs(k) >= 1 << 31:
-            raise ValueError("attention: {} out of range".format(name))
-    hit = _TABLES.get((key, device))
+    key = (key, limit, device)
+    hit = _TABLES.get(key)
     if hit is None:
-        hit = torch.tensor(key, dtype=torch.int32).reshape((-1, 2) if width == 2 else (-1,)).to(device)
-        _TABLES.put((key, device), hit)
-    return hit
+        for k in key[0]:
+            if width == 2 and not 0 <= k[0] <= k[1] <= limit:
+                raise ValueError("attention: {} names rows [{}, {}) of {}".format(name, k[0], k[1], limit))
+            if width == 1 and abs(k) >= 1 << 31:
+                raise ValueError("attention: {} out of range".format(name))
+        if torch.cuda.is_current_stream_capturing():
+            raise ValueError("attention: {} is a list that no call before the capture had: a capture cannot copy it to the device".format(name))
+        table = torch.tensor(key[0], dtype=torch.int32).reshape((-1, 2) if width == 2 else (-1,)).to(device)  # (a copy that is waited for)
+        _TABLES.put(key, (table, _s()))
+        return table
+    if torch.cuda.is_current_stream_capturing():
+        _TABLES.pinned.add(key)  # (the graph reads it at every replay: it is never dropped)
+    elif hit[1] != _s():
+        hit[0].record_stream(torch.cuda.current_stream())  # (dropped from the table, its memory waits for this stream too)
+    return hit[0]
 
 
 def _heads(t):
@@ -292,10 +303,10 @@ def _attn_fwd(q, k, v, slopes, rest, keep):
 
 
 def _attn_bwd(ctx, dout):
-    q, k, v, slopes, out = ctx.saved_tensors
-    if ctx.stats is None:
+    q, k, v, slopes, out32, stats, xy, kv_xy = ctx.saved_tensors
+    if stats is None:
         return tuple(None if t is None else torch.zeros_like(t) for t in (q, k, v, slopes)) + (None,)
-    scenes, kv_scenes, prefix, xy, kv_xy, causal, scale, cap = ctx.rest
+    scenes, kv_scenes, prefix, _, _, causal, scale, cap = ctx.rest
     (q, q_row, q_head), (k, k_row, k_head), (v, v_row, v_head) = _heads(q), _heads(k), _heads(v)
     (N, H, D), (M, Hkv, _), S, dev, dt = q.shape, k.shape, scenes.shape[0], q.device, q.dtype
     dout = _aligned(dout)
@@ -305,11 +316,11 @@ def _attn_bwd(ctx, dout):
     dslopes = torch.empty(H, dtype=_F32, device=dev) if slopes is not None and ctx.needs_input_grad[3] else None
     n = _attn_sizes(N, M, H, Hkv, D, S)[2]
     ws = _bytes(n, q)
-    ps = _p(ctx.stats)
+    ps = _p(stats)
     at = 3 * H * N + (-3 * H * N) % 4
     lib.mggan_block_attention_bwd(_ATTN.pack(
         _p(q), _p(k), _p(v), _p(dout), 0, _p(dq), _p(dk), _p(dv), _p(dslopes), _p(scenes), _p(kv_scenes), _p(prefix), _p(xy), _p(kv_xy),
-        _p(slopes), ps, _p(out if ctx.out32 is None else ctx.out32), ps + 4 * at, _p(ws), n, q_row, q_head, k_row, k_head, v_row, v_head, N, M, H,
+        _p(slopes), ps, _p(out32), ps + 4 * at, _p(ws), n, q_row, q_head, k_row, k_head, v_row, v_head, N, M, H,
         Hkv, D, S, causal, 0 if xy is None else xy.shape[1], _DTYPES[dt], scale, cap), _s())
     return dq, dk, dv, dslopes, None
 
@@ -320,14 +331,14 @@ _attn_bwd_once = once_differentiable(_attn_bwd)
 class AttentionFn(Function):
     @staticmethod
     def forward(ctx, q, k, v, slopes, rest):
-        ctx.rest, ctx.stats, ctx.out32, out = rest, None, None, None
+        # (what the backward pass reads is saved, the positions too: an operand that is written in between raises there.  The scene tables
+        # are not read again: the intervals lie behind the statistics)
+        ctx.rest = rest[:3] + (None, None) + rest[5:]
         if q.shape[0] == 0 or k.shape[0] == 0:
-            ctx.save_for_backward(q, k, v, slopes, None)
+            ctx.save_for_backward(q, k, v, slopes, None, None, None, None)
             return torch.zeros(q.shape, dtype=q.dtype, device=q.device)
-        out, out32, ctx.stats, q, k, v = _attn_fwd(q, k, v, slopes, rest, True)
-        if out32 is not out:
-            ctx.out32 = out32
-        ctx.save_for_backward(q, k, v, slopes, out if out32 is out else None)
+        out, out32, stats, q, k, v = _attn_fwd(q, k, v, slopes, rest, True)
+        ctx.save_for_backward(q, k, v, slopes, out32, stats, rest[3], rest[4])
         return out
 
     @staticmethod
@@ -343,10 +354,12 @@ def attention(q, k, v, scenes, kv_scenes=None, *, causal=False, prefix=None, sca
 
     scenes, kv_scenes: rows [start, end) of q and of k / v that belong to each scene, as a list of pairs (the framework's
     seq_start_end) or as an int32 device tensor (scenes, 2), which is read when the kernel runs (and clamped to the operands' rows);
-    kv_scenes defaults to scenes.  In any order; scenes may share keys; of a row that several scenes name the last one counts.  Rows of
+    kv_scenes defaults to scenes.  A list is copied to the device once for its contents, so inside a capture it has to be one that a call
+    before the capture had; a device tensor is read at every replay.  In any order; scenes may share keys; of a row that several scenes name the last one counts.  Rows of
     no scene and rows that see no key give zeros.  What lies outside a row's visible keys is never mixed in, infinities and NaN included.
     causal: row i of a scene of Lq rows and Lk keys sees keys j <= i + Lk - Lq, and in any case those before prefix[scene] (list or int32
-    device tensor).  One new row over a long cache is Lq = 1.  scale: > 0, D ** -0.5 by default; cap: 0 for none.
+    device tensor).  One new row over a long cache is Lq = 1.  scale: > 0, D ** -0.5 by default; cap: 0 for none;
+    both between 2^-60 and 2^60.
     xy (N, axes) and kv_xy (M, axes; by default xy), f32 with one or two axes, and slopes (H), f32: the bias by distance.  Gradients go to q,
     k, v and slopes, not to positions."""
     _same("attention", q, k, v)
@@ -362,8 +375,8 @@ def attention(q, k, v, scenes, kv_scenes=None, *, causal=False, prefix=None, sca
         raise ValueError("attention: {} rows of {} heads, {} keys (at most 2^24 rows, 2^29 rows times heads, 2^30 keys)".format(N, H, M))
     scale = D ** -0.5 if scale is None else float(scale)
     cap = 0.0 if cap is None else float(cap)
-    if not 0 < scale < math.inf or not 0 <= cap < math.inf:
-        raise ValueError("attention: scale {} (has to be positive), cap {} (0 or positive)".format(scale, cap))
+    if not _LEAST <= scale <= 1 / _LEAST or not (cap == 0 or _LEAST <= cap <= 1 / _LEAST):
+        raise ValueError("attention: scale {} (has to be positive), cap {} (0 or positive), both within 2^-60 and 2^60".format(scale, cap))
     if prefix is not None and not causal:
         raise ValueError("attention: a prefix without causal")
     if (xy is None) != (slopes is None) or (xy is None and kv_xy is not None):

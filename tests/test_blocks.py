@@ -129,3 +129,33 @@ def test_c_entries_refuse_before_anything_runs():
         lib.mggan_block_attention_bwd(B._ATTN.pack(*attn.values()), 0)
     with pytest.raises(HipError):
         lib.mggan_block_attention_fwd(0, 0)
+
+
+@pytest.mark.parametrize("kw", [{"scale": 1e-30}, {"scale": 1e39}, {"cap": 1e-30}, {"cap": 1e30}])
+def test_scale_and_cap_stay_in_f32s_range(kw):
+    """Their quotient and products are f32 factors: outside 2^-60 .. 2^60 the call is refused instead of giving NaN."""
+    with pytest.raises(ValueError, match="2\\^60"):
+        B.attention(*QKV, S, **kw)
+
+
+def test_tables_are_told_apart_by_contents(monkeypatch):
+    """Kept by value: the same list with other numbers, another limit or other element types is never taken for the one before."""
+    monkeypatch.setattr(B, "_s", lambda: 0)
+    monkeypatch.setattr(B, "_TABLES", B.BoundedCache(64))
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    cpu, rows = torch.device("cpu"), [[0, 2], [2, 5]]
+    first = B._table("scenes", rows, cpu, 6, 2)
+    assert first.tolist() == rows and B._table("scenes", [(0, 2), (2, 5)], cpu, 6, 2) is first
+    rows[1][1] = 6
+    assert B._table("scenes", rows, cpu, 6, 2).tolist() == [[0, 2], [2, 6]]
+    with pytest.raises(ValueError, match="of 5"):
+        B._table("scenes", rows, cpu, 5, 2)
+    t = torch.tensor(rows)
+    assert B._table("scenes", t, cpu, 6, 2).tolist() == [[0, 2], [2, 6]]
+    t[0, 1] = 1
+    assert B._table("scenes", t, cpu, 6, 2).tolist() == [[0, 1], [2, 6]]
+    assert B._table("prefix", [3, 4], cpu, 0, 1).tolist() == [3, 4]
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    assert B._table("prefix", [3, 4], cpu, 0, 1).tolist() == [3, 4] and len(B._TABLES.pinned) == 1
+    with pytest.raises(ValueError, match="capture"):
+        B._table("prefix", [3, 5], cpu, 0, 1)

@@ -615,3 +615,56 @@ def test_a_second_derivative_is_refused():
         g, = torch.autograd.grad(y.sum(), x, create_graph=True)
         with pytest.raises(RuntimeError):
             torch.autograd.grad(g.sum(), x)
+
+
+def test_positions_written_before_the_backward_pass_are_noticed():
+    """The distances are formed again in the backward pass: positions that changed in between raise, as every saved operand does."""
+    gen = torch.Generator().manual_seed(2)
+    q, xy = rnd(gen, 6, 2, 8, dtype=torch.float32).requires_grad_(), rnd(gen, 6, 2, dtype=torch.float32)
+    slopes = torch.ones(2, device="cuda")
+    out = B().attention(q, q, q, [(0, 6)], xy=xy, slopes=slopes)
+    xy.add_(1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.sum().backward()
+
+
+def test_kept_values_go_through_saved_tensors():
+    """Activation inputs and softmax statistics can be offloaded by hooks and are freed with the graph."""
+    gen = torch.Generator().manual_seed(3)
+    x, w = rnd(gen, 20, 32, dtype=torch.bfloat16).requires_grad_(), rnd(gen, 24, 32, dtype=torch.bfloat16)
+    seen = []
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: (seen.append(tuple(t.shape)), t.cpu())[1], lambda t: t.cuda()):
+        y = B().gated_linear(x, w, w)
+        out = B().attention(y.view(20, 3, 8), y.view(20, 3, 8), y.view(20, 3, 8), [(0, 20)])
+    offloaded, = torch.autograd.grad(out.float().square().sum(), x)
+    assert (2, 20, 24) in seen and (20, 3, 8) in seen and any(len(s) == 1 and s[0] >= 3 * 3 * 20 for s in seen)
+    y = B().gated_linear(x, w, w)
+    out = B().attention(y.view(20, 3, 8), y.view(20, 3, 8), y.view(20, 3, 8), [(0, 20)])
+    assert torch.equal(offloaded, torch.autograd.grad(out.float().square().sum(), x)[0])
+
+
+def test_a_list_of_scenes_in_a_captured_graph():
+    """The graph keeps the table that it reads, however many other lists come later; a list that is new in a capture is refused."""
+    gen = torch.Generator().manual_seed(4)
+    q = rnd(gen, 40, 2, 16, dtype=torch.float32)
+    scenes = [(0, 7), (7, 40)]
+    B_ = B()
+    with torch.no_grad():
+        want = B_.attention(q, q, q, scenes)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = B_.attention(q, q, q, scenes)
+            with pytest.raises(ValueError, match="capture"):
+                B_.attention(q, q, q, [(0, 9), (9, 40)])
+        side = torch.cuda.Stream()
+        for i in range(200):  # (the cache is emptied several times over, its memory used again)
+            B_.attention(q, q, q, [(0, 1 + i % 39), (1 + i % 39, 40), (0, i // 39)])
+            with torch.cuda.stream(side):
+                B_.attention(q, q, q, [(0, 1 + i % 39), (1 + i % 39, 40), (0, i // 39)])
+        for _ in range(3):
+            out.zero_()
+            g.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, want)
+            assert torch.equal(B_.attention(q, q, q, scenes), want)
