@@ -219,7 +219,7 @@ __global__ __launch_bounds__(256, QF == 1 && DP <= 64 ? 3 : 2) void blk_attn_fwd
   }
 }
 
-// Single rows over long caches.  A workgroup takes one row, the heads of one key head (up to 16: the columns of the matrix
+// Few rows over long caches.  A workgroup takes one row, the heads of one key head (up to 16: the columns of the matrix
 // instruction) and one of `splits` shares of the row's keys; its four waves take the share's tiles in turn, each with LDS of its own and
 // no barrier between them: what counts is bytes in flight (two tiles of keys and values a wave, 64 KB a CU at width 128).  Bound by the cache's
 // bytes: 32 rows over 16,384 keys each, width 128, 1.62 GB in 287 us, 5.6 TB/s.  Shares leave
@@ -375,10 +375,18 @@ __global__ __launch_bounds__(128) void blk_attn_join_kernel(BlkAttnArgs p, int s
   if (d < p.D) ((T*)p.out)[(long)blockIdx.x * p.D + d] = (T)(o * inv);
 }
 
-// Single rows over long caches (no gradient kept): how many shares of the keys; 0 where the tile kernel runs instead.
+// Few rows a scene over long caches (no gradient kept): how many shares of the keys; 0 where the tile kernel runs instead.
+// A row's keys are read for it alone here; the tile kernel reads them once for 64 rows, but by few workgroups where rows are few, and through
+// the keys of every scene that its 64 rows span.  So this one is taken while its workgroups are at most 400 for each round of the tile kernel's
+// (512 of them run at once) and each scene spanned.  Measured, this kernel / the tiles, us: one row over 1,000 keys 9.4 / 35; 32 x 1 over 16,384,
+// 223 / 23,580; 16 x 16 over 1,000 (102) 13 / 55; 64 x 16 over 500 (410) 29 / 36; 64 rows of one scene over 4,000, 8 key heads (512) 89 / 80; 64 x 32
+// over 200 (5,461) 119 / 19.  Below 64 keys a scene both are
+// launches (4.6 / 8.0).
 int row_splits(const BlkAttnArgs& p) {
-  if (p.lse || p.S == 0 || p.N > 2L * p.S || p.M / p.S < 64) return 0;
-  const long blocks = (long)p.N * p.Hkv * cdiv(p.H / p.Hkv, 16);
+  if (p.lse || p.S == 0 || p.N > 64L * p.S || p.M / p.S < 64) return 0;
+  const long blocks = (long)p.N * p.Hkv * cdiv(p.H / p.Hkv, 16), rounds = cdiv((long)cdiv(p.N, 64) * p.H, 512);
+  const long spanned = 64L * p.S / p.N + 1;
+  if (blocks > 400 * rounds * (spanned < p.S ? spanned : p.S)) return 0;
   if ((long)p.N * p.H > 1 << 22) return 0;  // (more workgroups than a launch takes)
   long n = cdiv(1024, blocks);
   if (n > p.M / p.S / 512) n = p.M / p.S / 512;  // (a share of fewer keys is not worth the launch that joins: 1,000 keys 20 -> 17 us)

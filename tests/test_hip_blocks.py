@@ -668,3 +668,32 @@ def test_a_list_of_scenes_in_a_captured_graph():
             torch.cuda.synchronize()
             assert torch.equal(out, want)
             assert torch.equal(B_.attention(q, q, q, scenes), want)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("Hkv,D,cap,axes,splits", [(2, 64, 0.0, 0, False), (8, 128, 5.0, 0, False), (1, 40, 0.0, 2, True), (4, 32, 3.0, 1, True)])
+def test_a_few_rows_for_each_of_several_caches(dtype, Hkv, D, cap, axes, splits):
+    """Chunks of 1 to 11 rows behind a mask, without a gradient: every row reads its own keys (split over shares where the caches are long),
+    and the rows of a scene without keys and of no scene are zeros."""
+    gen = torch.Generator().manual_seed(D)
+    chunks, room, H = [1, 3, 11, 0, 8, 2], 2100 if splits else 150, 8
+    lens = [room, 64, 77, 5, 0, room - 1]
+    starts = [sum(chunks[:i]) for i in range(len(chunks))]
+    scenes = [(a, a + n) for a, n in zip(starts, chunks)]
+    kv = [(i * room, i * room + n) for i, n in enumerate(lens)]
+    N, M = sum(chunks) + 1, room * len(chunks)
+    prefix = [0, 70, 0, 0, 3, 4]
+    q, k, v = rnd(gen, N, H, D, dtype=dtype), rnd(gen, M, Hkv, D, dtype=dtype), rnd(gen, M, Hkv, D, dtype=dtype)
+    for a, b in zip([e for _, e in kv], [s for s, _ in kv[1:]] + [M]):
+        k[a:b], v[a:b] = float("nan"), float("inf")  # (what no row sees)
+    xy = kv_xy = slopes = None
+    if axes:
+        xy, kv_xy = rnd(gen, N, axes, dtype=torch.float32), rnd(gen, M, axes, dtype=torch.float32)
+        slopes = torch.linspace(0.2, 1.0, H, device="cuda")
+    see = visible(N, M, scenes, kv, True, prefix)
+    clean = [t.where(torch.isfinite(t), torch.zeros_like(t)) for t in (k, v)]
+    want = reference(q, *clean, see, q, D ** -0.5, cap, xy, kv_xy, slopes)["out"]
+    with torch.no_grad():
+        out = B().attention(q, k, v, scenes, kv, causal=True, prefix=prefix, cap=cap, xy=xy, kv_xy=kv_xy, slopes=slopes)
+    close(out, *want, "out")
+    assert not out[-1].any() and not out[starts[4]:starts[4] + 8].any()
