@@ -344,7 +344,9 @@ __device__ __forceinline__ void attn_dkv_rows(const BlkAttnArgs& p, int np, cons
 }
 
 template <class T, int DP, int X>
-__global__ __launch_bounds__(256, DP <= 64 || (sizeof(T) == 2 && DP == 128) ? 3 : 2) void blk_attn_dkv_kernel(BlkAttnArgs p, int np, const float* delta, float* part, const float* slope_part, int nqt, const int2* ranges) {
+__global__ __launch_bounds__(256, DP <= 64 || (sizeof(T) == 2 && DP == 128) ? 3 : 2) void blk_attn_dkv_kernel(BlkAttnArgs p, int np, const float* delta,
+                                                                                                                         float* part, const float* slope_part, int nqt,
+                                                                                                                         const int2* ranges) {
   using G = BwdGeo<T, DP>;
   __shared__ struct {
     u32x4 q[2 * G::TILE], o[2 * G::TILE];

@@ -202,9 +202,9 @@ __device__ __forceinline__ void wait_copies() {
 // memory (two steps of slack) nor for LDS (one step).
 // Bound by the matrix cores from about 256 tiles on.  A tile of 256 x 256 takes 32 KB of copies for 4.2 MFLOP, so that its bytes come out of the
 // L2; its eight waves of 128 x 64 read 12 fragments for 32 multiplications (four waves of 128 x 128 would read less, but 256 accumulators
-// leave no room for a second set of fragments: 634 TFLOP/s).  8,192 x 4,096 x 4,096 bf16: 1.12-1.18 PFLOP/s (the library: 1.24-1.6), the
-// gated training pass' products of twice that size 1.07 (forward), 1.21 (dX) and 1.29 (dW); f32, 4,096 each way: 145 TFLOP/s (136).  Its matrix
-// cores are busy 62-73 % of the time; copies of two steps behind one barrier made it 964 instead of 1,150 TFLOP/s.
+// leave no room for a second set of fragments: 634 TFLOP/s).  8,192 x 4,096 x 4,096 bf16: 204 us, 1.35 PFLOP/s (the library: 1.24-1.6), the
+// gated training pass' products of four times that work 1.07 (forward), 1.21 (dX) and 1.29 (dW); f32, 4,096 each way: 145 TFLOP/s (136).  Its matrix
+// cores are busy 62-75 % of the time in these; copies of two steps behind one barrier made it 964 instead of 1,150 TFLOP/s.
 template <class T, int BM, int BN, int WM, int WN, int EPI, bool SPLIT, bool CA, bool CB>
 __global__ __launch_bounds__(WM* WN * 64) void blk_gemm_kernel(GemmP p) {
   constexpr int NT = WM * WN * 64, CH = Mf<T>::CH, KS = 4 * CH;
@@ -421,7 +421,7 @@ __global__ __launch_bounds__(256) void blk_join_kernel(GemmP p, int splits) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     v[i] = (part[0][0][x][i] + part[0][1][x][i]) + (part[0][2][x][i] + part[0][3][x][i]);
-    if (EPI == EPI_GATED) u[i] = (part[EPI == EPI_GATED][0][x][i] + part[EPI == EPI_GATED][1][x][i]) + (part[EPI == EPI_GATED][2][x][i] + part[EPI == EPI_GATED][3][x][i]);
+    if constexpr (EPI == EPI_GATED) u[i] = (part[1][0][x][i] + part[1][1][x][i]) + (part[1][2][x][i] + part[1][3][x][i]);
   }
   epilogue<T, EPI, 4>(p, m, n, v, u, p.N % Mf<T>::CH == 0);
 }
