@@ -7,13 +7,13 @@
 All operands of a call have one type and live on one device; sums, activations and softmax statistics are held in f32 and
 rounded once.  Work goes to torch's current stream, outputs and workspaces come from torch's allocator (so a call can be captured
 into a HIP graph), gradients are returned through autograd and are the same bits in every run.  Arguments that do not fit raise
-ValueError, a failing launch raises HipError; there is no CPU path."""
+ValueError, a failing launch raises HipError, forward-mode tangents raise NotImplementedError; there is no CPU path."""
 import functools
 import struct
 from itertools import chain
 
 import torch
-from torch.autograd import Function
+from torch.autograd import Function, forward_ad
 from torch.autograd.function import once_differentiable
 
 from .functions import _GET_DEVICE, ACT_LEAKY, ACT_NONE, ACT_SIGMOID, BoundedCache, _p, _s
@@ -76,12 +76,21 @@ def _aligned(t):
     return t.clone() if t.data_ptr() % 16 else t
 
 
+def _any_dual(*tensors):
+    """Whether one of them carries a forward-mode tangent (torch.autograd.forward_ad); without an open level none does."""
+    if getattr(forward_ad, "_current_level", 0) < 0:
+        return False
+    return any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
 def _needs_grad(*tensors):
+    """Whether the call goes through its autograd function: for a gradient, or for an operand with a forward-mode tangent, which the
+    function refuses (NotImplementedError) where the kernel alone would drop it."""
     if torch.is_grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:
                 return True
-    return False
+    return _any_dual(*tensors)
 
 
 # ---- layers ------------------------------------------------------------------------------------------------------------------
@@ -388,7 +397,7 @@ def attention(q, k, v, scenes, kv_scenes=None, *, causal=False, prefix=None, sca
         for t, n in ((xy, N), (kv_xy, M)):
             if t.dtype != _F32 or t.dim() != 2 or t.shape[0] != n or t.shape[1] not in (1, 2) or t.shape[1] != xy.shape[1] or t.device != q.device:
                 raise ValueError("attention: positions {} {} on {} for {} rows: f32, one or two axes".format(t.dtype, tuple(t.shape), t.device, n))
-            if t.requires_grad and torch.is_grad_enabled():
+            if t.requires_grad and torch.is_grad_enabled() or _any_dual(t):
                 raise ValueError("attention: positions have no gradient: detach them")
         if slopes.dtype != _F32 or slopes.dim() != 1 or slopes.shape[0] != H or slopes.device != q.device:
             raise ValueError("attention: slopes {} {} on {} for {} heads".format(slopes.dtype, tuple(slopes.shape), slopes.device, H))

@@ -159,3 +159,44 @@ def test_tables_are_told_apart_by_contents(monkeypatch):
     assert B._table("prefix", [3, 4], cpu, 0, 1).tolist() == [3, 4] and len(B._TABLES.pinned) == 1
     with pytest.raises(ValueError, match="capture"):
         B._table("prefix", [3, 5], cpu, 0, 1)
+
+
+def stubbed(monkeypatch):
+    """The layers and attention without their launches, on the CPU: outputs of the right shapes that carry no derivative."""
+    monkeypatch.setattr(B, "_on_current", lambda name, t: True)
+    monkeypatch.setattr(B, "_layer_fwd", lambda t, w, w2, b, b2, res, act, slope, keep: (torch.zeros(len(t), len(w)), None, t, w, w2))
+    monkeypatch.setattr(B, "_attn_fwd", lambda q, k, v, slopes, rest, keep: (torch.zeros(q.shape), None, None, q, k, v))
+    monkeypatch.setattr(B, "_table", lambda name, rows, device, limit, width: torch.tensor(rows, dtype=torch.int32))
+
+
+FORWARD_MODE = [  # the call of one operand, its shape
+    (lambda t: B.linear_residual(t, x(5, 4)), (3, 4)), (lambda t: B.linear_residual(x(3, 4), t), (5, 4)),
+    (lambda t: B.linear_residual(x(3, 4), x(5, 4), t), (5,)), (lambda t: B.linear_residual(x(3, 4), x(5, 4), None, t), (3, 5)),
+    (lambda t: B.gated_linear(t, x(5, 4), x(5, 4)), (2, 3, 4)), (lambda t: B.gated_linear(x(3, 4), x(5, 4), t), (5, 4)),
+    (lambda t: B.gated_linear(x(3, 4), x(5, 4), x(5, 4), x(5), t), (5,)),
+    (lambda t: B.attention(t, x(6, 2, 16), x(6, 2, 16), S), (6, 4, 16)), (lambda t: B.attention(x(6, 4, 16), t, x(6, 2, 16), S), (6, 2, 16)),
+    (lambda t: B.attention(x(6, 4, 16), x(6, 2, 16), t, S), (6, 2, 16)), (lambda t: B.attention(*QKV, S, xy=x(6, 2), slopes=t), (4,))]
+
+
+@pytest.mark.parametrize("grad", [True, False])
+@pytest.mark.parametrize("call,shape", FORWARD_MODE)
+def test_forward_mode_is_refused(call, shape, grad, monkeypatch):
+    """A tangent on any operand raises, whether or not a gradient is recorded: the output would silently have none."""
+    stubbed(monkeypatch)
+    fw = torch.autograd.forward_ad
+    with torch.set_grad_enabled(grad):
+        call(x(*shape))
+        with fw.dual_level():
+            call(x(*shape))  # (an open level alone is nothing to refuse)
+            with pytest.raises(NotImplementedError):
+                call(fw.make_dual(x(*shape), x(*shape)))
+        with pytest.raises(Exception):
+            torch.func.jvp(call, (x(*shape),), (x(*shape),))
+
+
+@pytest.mark.parametrize("name", ["xy", "kv_xy"])
+def test_positions_with_a_tangent_are_refused(name, monkeypatch):
+    stubbed(monkeypatch)
+    fw = torch.autograd.forward_ad
+    with fw.dual_level(), pytest.raises(ValueError, match="positions have no gradient"):
+        B.attention(*QKV, S, slopes=x(4), **{"xy": x(6, 2), "kv_xy": x(6, 2), name: fw.make_dual(x(6, 2), x(6, 2))})

@@ -697,3 +697,15 @@ def test_a_few_rows_for_each_of_several_caches(dtype, Hkv, D, cap, axes, splits)
         out = B().attention(q, k, v, scenes, kv, causal=True, prefix=prefix, cap=cap, xy=xy, kv_xy=kv_xy, slopes=slopes)
     close(out, *want, "out")
     assert not out[-1].any() and not out[starts[4]:starts[4] + 8].any()
+
+
+def test_forward_mode_raises_instead_of_losing_the_tangent():
+    B_, gen, fw = B(), torch.Generator().manual_seed(1), torch.autograd.forward_ad
+    t, w = rnd(gen, 8, 16, dtype=torch.float32), rnd(gen, 16, 16, dtype=torch.float32)
+    rows = lambda u: u.view(8, 2, 8)
+    for call in (lambda u: B_.linear_residual(u, w), lambda u: B_.gated_linear(u, w, w), lambda u: B_.attention(rows(u), rows(u), rows(u), [(0, 8)])):
+        want = call(t)
+        with fw.dual_level():
+            assert torch.equal(call(t), want)
+            with pytest.raises(NotImplementedError):
+                call(fw.make_dual(t, t))
