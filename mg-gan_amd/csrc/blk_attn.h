@@ -36,18 +36,20 @@ __device__ __attribute__((aligned(16))) const unsigned blk_attn_zeros[4] = {0, 0
 
 constexpr float LOG2E = 1.44269504f;
 
-// tanh(x) from z = 2 log2e x.  f32 operands: near zero by its series (to x^11: 2^-26 of the value at 0.35), so that a score keeps its
-// relative precision through the cap; bf16 operands carry 2^-9 themselves, there the quotient does everywhere.
-template <class T>
+// tanh(x) from z = 2 log2e x.  The quotient is off by up to 12 steps of 2^-24 however small x is, and the cap multiplies that.  SERIES: near
+// zero by the series instead (to x^11: 2^-26 of the value at 0.35), so that a score keeps its relative precision through any cap.
+template <bool SERIES>
 __device__ __forceinline__ float blk_tanh(float z) {
   const float big = fmaf(-2.0f, mg_rcp(__builtin_amdgcn_exp2f(z) + 1.0f), 1.0f);
-  if constexpr (sizeof(T) == 2) return big;
+  if constexpr (!SERIES) return big;
   const float x = z * (0.5f / LOG2E), y = x * x;
   const float s = fmaf(y, fmaf(y, fmaf(y, fmaf(y, fmaf(y, -0.0088632355f, 0.0218694885f), -0.0539682540f), 0.1333333333f), -0.3333333333f), 1.f) * x;
   return fabsf(x) < 0.35f ? s : big;
 }
 
-// What is done to a score q.k, by the kernels' template argument X: bit 0 a cap, bits 1-2 the axes of the distance.
+// What is done to a score q.k, by the kernels' template argument X: bit 0 a cap, bits 1-2 the axes of the distance, bit 3 (bf16 with a cap
+// above SERIES_FROM; f32 does so always) the cap's tanh by its series near zero.  bf16 up to there takes the quotient alone: 64 times its 12 F
+// are 2^-14.4 of a weight, which is rounded to 2^-8 of itself anyway, and the series would be seven instructions more a score.
 // Weights are exp2(s E - top), one fused operation, with top = max s E.  E = log2e over scores in their own units where the last bits
 // matter (f32; scores with a distance, whose slopes' gradient is f32): scale log2e and slope log2e rounded into one factor first would
 // stretch all scores by a common 2^-25, which shows in the slopes' gradient (log2e itself is 2^-26 off, top's rounding divides out).
@@ -55,8 +57,8 @@ __device__ __forceinline__ float blk_tanh(float z) {
 // E = cap log2e.
 template <class T, int X>
 struct Soft {
-  static constexpr bool CAP = X & 1, NATURAL = (X >> 1) || sizeof(T) == 4;
-  static constexpr int AXES = X >> 1;
+  static constexpr int AXES = (X >> 1) & 3;
+  static constexpr bool CAP = X & 1, SERIES = (X & 8) || sizeof(T) == 4, NATURAL = AXES || sizeof(T) == 4;
   static constexpr bool RAW = X == 0 && !NATURAL;  // score() is not called
   float scale, k, cap, slope, E;
   __device__ __forceinline__ Soft(const BlkAttnArgs& p, float slope_) {
@@ -70,7 +72,7 @@ struct Soft {
   __device__ __forceinline__ float score(float x, float ax, float ay, float bx, float by, float& fac, float& dist) const {
     fac = 1.f, dist = 0.f;
     if constexpr (CAP) {
-      x = blk_tanh<T>(x * k);
+      x = blk_tanh<SERIES>(x * k);
       fac = fmaf(-x, x, 1.f);
       if (NATURAL) x *= cap;
     } else {
@@ -86,6 +88,12 @@ struct Soft {
   }
   __device__ __forceinline__ float weight(float s, float top) const { return __builtin_amdgcn_exp2f(fmaf(s, E, -top)); }
 };
+
+constexpr float SERIES_FROM = 64.f;
+template <class T>
+int blk_attn_x(const BlkAttnArgs& p) {
+  return (p.cap > 0.f ? 1 : 0) + 2 * p.axes + (sizeof(T) == 2 && p.cap > SERIES_FROM ? 8 : 0);
+}
 
 template <class T_, int DP_, int BK_ = 128 / (int)sizeof(T_)>
 struct Geo {

@@ -416,7 +416,15 @@ void launch_fwd_x(const BlkAttnArgs& p, hipStream_t st) {
 }
 template <class T, int DP>
 void launch_fwd(const BlkAttnArgs& p, hipStream_t st) {
-  switch ((p.cap > 0.f ? 1 : 0) + 2 * p.axes) {
+  const int x = blk_attn_x<T>(p);
+  if constexpr (sizeof(T) == 2) {
+    switch (x) {
+      case 9: return launch_fwd_x<T, DP, 9>(p, st);
+      case 11: return launch_fwd_x<T, DP, 11>(p, st);
+      case 13: return launch_fwd_x<T, DP, 13>(p, st);
+    }
+  }
+  switch (x) {
     case 0: return launch_fwd_x<T, DP, 0>(p, st);
     case 1: return launch_fwd_x<T, DP, 1>(p, st);
     case 2: return launch_fwd_x<T, DP, 2>(p, st);

@@ -205,7 +205,7 @@ __global__ __launch_bounds__(256, QF == 1 && DP <= 64 ? 3 : 2) void blk_attn_dq_
       sum += attn_dq_rows<T, DP, 1, X, true>(p, np, delta, h, keys.x, keys.y, afresh(w0 + 16 * j), lds.k, lds.v, lds.x, &lds.odd);
     }
   }
-  if (X > 1 && p.dslopes) {
+  if (Soft<T, X>::AXES && p.dslopes) {
     __syncthreads();
     sum = wave_sum(sum);
     if (mg_lane() == 0) lds.x[wave] = sum;
@@ -358,7 +358,7 @@ __global__ __launch_bounds__(256, DP <= 64 || (sizeof(T) == 2 && DP == 128) ? 3 
   const int w0 = kt * 64 + mg_wave() * 16;
 
   // the slopes' gradient: a head's partial sums of the dQ kernel, in a fixed order, by the first wave of each of the first workgroups
-  if (X > 1 && p.dslopes && threadIdx.x < 64) {
+  if (Soft<T, X>::AXES && p.dslopes && threadIdx.x < 64) {
     for (int h = blockIdx.x; h < p.H; h += gridDim.x) {
       double s = 0.;
       for (int i = threadIdx.x; i < nqt; i += 64) s += (double)slope_part[(long)h * nqt + i];
@@ -434,7 +434,15 @@ void launch_bwd_x(const BlkAttnArgs& p, hipStream_t st) {
 }
 template <class T, int DP>
 void launch_bwd(const BlkAttnArgs& p, hipStream_t st) {
-  switch ((p.cap > 0.f ? 1 : 0) + 2 * p.axes) {
+  const int x = blk_attn_x<T>(p);
+  if constexpr (sizeof(T) == 2) {
+    switch (x) {
+      case 9: return launch_bwd_x<T, DP, 9>(p, st);
+      case 11: return launch_bwd_x<T, DP, 11>(p, st);
+      case 13: return launch_bwd_x<T, DP, 13>(p, st);
+    }
+  }
+  switch (x) {
     case 0: return launch_bwd_x<T, DP, 0>(p, st);
     case 1: return launch_bwd_x<T, DP, 1>(p, st);
     case 2: return launch_bwd_x<T, DP, 2>(p, st);

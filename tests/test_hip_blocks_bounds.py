@@ -1,0 +1,145 @@
+"""GPU: the transformer-block operators (mggan/hip/blocks.py) against their definitions in 64 bits with the roundings that the kernels
+make on purpose carried out, so that the bounds hold what is f32 in between to f32.
+
+u = half a step of the operands' type (2^-8 bf16, 2^-24 f32), F = 2^-24.  With bf16 operands the softmax's weights P, the scores' gradient dS
+and a layer's dZ are rounded to bf16 where they enter a matrix instruction.  Where the value before that rounding is known to within e (P and
+dS of the backward pass, dZ) the rounded value lies between the roundings of its two ends, and `entered` says how far that is from the
+rounding of the exact value: zero but where a border between two steps lies in between.  Everything else is f32: a sum of n products is off by
+n F of the sum of their absolute values, exp2 and rcp by a step (2 F) of their value.  Outputs are rounded once, by u."""
+import pytest
+import torch
+
+from test_hip_blocks import B, F, TYPES, U, close, lengths_to_scenes, rnd, visible
+
+pytestmark = pytest.mark.gpu
+
+SERIES_FROM = 64.0  # caps above it, and all in f32: tanh by its series near zero
+
+
+def entered(x, e, dtype):
+    """x, known to within e, as it enters a product: (its rounding, how far that of the kernel's value can be from it).  Rounding never
+    changes an order, so the kernel's value lies between the roundings of both ends."""
+    if dtype == torch.float32:
+        return x, e
+    at = lambda t: t.to(torch.float32).to(dtype).double()
+    c = at(x)
+    return c, torch.maximum((at(x + e) - c).abs(), (at(x - e) - c).abs())
+
+
+def attention64(q, k, v, see, dout, scale, cap=0.0, xy=None, kv_xy=None, slopes=None):
+    """{name: (value, bound)}.  Scores: a product of D terms, its factor and a few roundings, (D + 8) F of the absolute terms.  The cap's
+    tanh: its series is off by 8 F of itself, the quotient 1 - 2 / (e + 1) by at most 2 / (e + 1) times 5 F and a rounding, 12 F, whatever
+    the value (it is taken where |x| >= 0.35, or everywhere in bf16 with a cap of at most 64: 64 x 12 F = 2^-14.4 against u = 2^-8 of the
+    weights).  A weight is exp2 of a score less its row's maximum: 8 F of the largest score, and the sum's (n + 16) F; in bf16 the backward
+    pass takes both statistics in one number of up to 32 + |score|, a rounding of F of it more."""
+    (N, H, D), (M, Hkv, _), dtype = q.shape, k.shape, q.dtype
+    u, half, G = U[dtype], dtype == torch.bfloat16, H // Hkv
+    ub = u if half else 0.0
+    Q, K, V, dO = (t.detach().double().transpose(0, 1) for t in (q, k, v, dout))
+    Kh, Vh = K.repeat_interleave(G, 0), V.repeat_interleave(G, 0)
+    z = scale * (Q @ Kh.transpose(1, 2))
+    es = (D + 8) * F * scale * (Q.abs() @ Kh.abs().transpose(1, 2))
+    s, fac, efac = z, 1.0, 0.0
+    if cap:
+        t = torch.tanh(z / cap)
+        et = torch.full_like(t, 12 * F)
+        if not half or cap > SERIES_FROM:
+            et = torch.where((z / cap).abs() < 0.34, 8 * F * t.abs(), et)
+        et = es / cap + 4 * F * (z / cap).abs() * (1 - t * t) + et
+        s, es, fac = cap * t, cap * et + 2 * F * cap * t.abs(), 1 - t * t
+        efac = 2 * t.abs() * et + 3 * F
+    dist = None
+    if xy is not None:
+        dist = (xy.double()[:, None] - kv_xy.double()[None]).norm(dim=-1)
+        bias = slopes.detach().double()[:, None, None] * dist
+        s, es = s - bias, es + 8 * F * bias.abs()
+    es = es + 8 * F * s.abs()
+    s = s.masked_fill(~see, -torch.inf)
+    P = torch.softmax(s, -1).nan_to_num(0.0)
+    n = see.sum(-1).double()[None, :, None]
+    rel = 2 * (es * see).amax(-1, keepdim=True) + (n + 16 + (32 if half else 0)) * F
+    O, A = P @ Vh, P @ Vh.abs()
+    eO = (rel + ub) * A + (n + 4) * F * A
+    dP = dO @ Vh.transpose(1, 2)
+    edP = (D + 4) * F * (dO.abs() @ Vh.abs().transpose(1, 2))
+    delta = (dO * O).sum(-1, keepdim=True)
+    edelta = (dO.abs() * (eO + (D + 4) * F * O.abs())).sum(-1, keepdim=True)  # (of the output before it is rounded)
+    dL = P * (dP - delta)
+    edL = rel * dL.abs() + P * (edP + edelta) * (1 + rel) + 4 * F * P * (dP.abs() + delta.abs())
+    dS, eS = entered(dL * fac, edL * fac + (dL.abs() + edL) * efac, dtype)
+    Pe, eP = entered(P, rel * P, dtype)
+    m = see.sum(0).double()[None, :, None] * G
+    dQ, eQ = scale * (dS @ Kh), scale * ((eS + (n + 4) * F * (dS.abs() + eS)) @ Kh.abs())
+    dSt, eSt, Pt = dS.transpose(1, 2), eS.transpose(1, 2), Pe.transpose(1, 2)
+    dK, eK = scale * (dSt @ Q), scale * (eSt @ Q.abs() + (m + 4) * F * ((dSt.abs() + eSt) @ Q.abs()))
+    dV, eV = Pt @ dO, eP.transpose(1, 2) @ dO.abs() + (m + 4) * F * (Pt @ dO.abs())
+    fold = lambda x: x.reshape(Hkv, G, M, D).sum(1)
+    out = {"out": (O, eO), "dq": (dQ, eQ), "dk": (fold(dK), fold(eK)), "dv": (fold(dV), fold(eV))}
+    out = {name: (x.transpose(0, 1), (e + u * (x.abs() + e)).transpose(0, 1)) for name, (x, e) in out.items()}
+    if xy is not None:
+        # row by row a - c b with a = sum P dP dist, b = sum P dist, c = sum P dP: nothing in it is rounded to bf16
+        w, f = P * dP.abs(), (n + 8) * F
+        a, b, c = (P * dP * dist).sum(-1, keepdim=True), (P * dist).sum(-1, keepdim=True), (P * dP).sum(-1, keepdim=True)
+        ea = ((rel + f) * w * dist + P * edP * dist).sum(-1, keepdim=True)
+        eb, ec = (rel + f) * b, ((rel + f) * w + P * edP).sum(-1, keepdim=True)
+        row = a - c * b
+        e = ea + c.abs() * eb + b * ec + eb * ec + 3 * F * (a.abs() + (c * b).abs())
+        # (then sums of up to 12 in f32 -- two rows a lane, 64 lanes, four waves -- and the rest in 64 bits)
+        out["dslopes"] = (-row.sum((1, 2)), (e + 14 * F * row.abs()).sum((1, 2)))
+    return out
+
+
+def run(q, k, v, dout, scenes, kv_scenes=None, **opt):
+    """Output, output without a gradient kept, and all gradients."""
+    leaves = {"dq": q, "dk": k, "dv": v}
+    if opt.get("slopes") is not None:
+        leaves["dslopes"] = opt["slopes"]
+    leaves = {n: t.detach().requires_grad_() for n, t in leaves.items()}
+    if "dslopes" in leaves:
+        opt["slopes"] = leaves["dslopes"]
+    out = B().attention(leaves["dq"], leaves["dk"], leaves["dv"], scenes, kv_scenes, **opt)
+    got = {"out": out.detach(), **dict(zip(leaves, torch.autograd.grad(out, list(leaves.values()), dout)))}
+    with torch.no_grad():
+        return got, B().attention(q, k, v, scenes, kv_scenes, **opt)
+
+
+def check(got, alone, want):
+    assert set(got) == set(want)
+    for name, (x, e) in want.items():
+        close(got[name], x, e, name)
+    close(alone, *want["out"], "out without gradients")
+
+
+CAPS = [2.0, 50.0, 64.0, 100.0, 1e4, 1e6, 1e7, 2.0 ** 25, 2.0 ** 60]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("axes,D", [(0, 64), (1, 32), (2, 128)])
+@pytest.mark.parametrize("cap", CAPS)
+def test_caps_of_any_size(cap, axes, D, dtype):
+    """A large cap leaves the scores as they are: the score's error is bounded by its own size, not by the cap's."""
+    gen = torch.Generator().manual_seed(D)
+    scenes, N, H, Hkv = [(0, 70), (70, 71), (71, 150)], 150, 4, 2
+    q, k, v, dout = (rnd(gen, N, h, D, dtype=dtype, std=s) for h, s in ((H, 2.0), (Hkv, 1.0), (Hkv, 1.0), (H, 1.0)))
+    xy = slopes = None
+    if axes:
+        xy, slopes = (torch.rand(N, axes, generator=gen) * 9).cuda(), (torch.rand(H, generator=gen) * 0.3).cuda()
+    got, alone = run(q, k, v, dout, scenes, causal=True, cap=cap, xy=xy, slopes=slopes)
+    see = visible(N, N, scenes, scenes, True, None)
+    want = attention64(q, k, v, see, dout, D ** -0.5, cap, xy, xy, slopes)
+    check(got, alone, want)
+    if cap >= 2.0 ** 25:  # (tanh(x) = x - x^3 / 3 + ..: below 2^-40 of the scores here, so the same definition without a cap holds too)
+        check(got, alone, attention64(q, k, v, see, dout, D ** -0.5, 0.0, xy, xy, slopes))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("cap", CAPS)
+def test_caps_of_any_size_for_single_rows(cap, dtype):
+    gen = torch.Generator().manual_seed(7)
+    H, D, lens = 8, 64, [300, 1200, 1]
+    kv, M = lengths_to_scenes(lens), sum(lens)
+    q, k, v = rnd(gen, 3, H, D, dtype=dtype, std=2.0), rnd(gen, M, 2, D, dtype=dtype), rnd(gen, M, 2, D, dtype=dtype)
+    scenes = [(i, i + 1) for i in range(3)]
+    with torch.no_grad():
+        out = B().attention(q, k, v, scenes, kv, cap=cap)
+    close(out, *attention64(q, k, v, visible(3, M, scenes, kv, False, None), q, D ** -0.5, cap)["out"], "out")
