@@ -677,7 +677,8 @@ size_t mggan_block_attention_span_ints(int rows);
 size_t mggan_block_attention_fwd_workspace(int rows, int keys, int heads, int kv_heads, int width, int scenes);
 int mggan_block_attention_fwd(const void* args, mggan_stream_t stream);
 /* dq, dk, dv, and dslopes (H) if not NULL, written in a fixed order of summation; out32, lse, spans as the forward call left them.
- * ws: mggan_block_attention_bwd_workspace bytes, 256-byte aligned. */
+ * ws: mggan_block_attention_bwd_workspace bytes, 256-byte aligned: about 5 bytes a row and head, 8 a 64 keys, and up to 1 GiB of partial dK and
+ * dV where heads share key heads that few workgroups walk (0 for sizes that no call takes). */
 size_t mggan_block_attention_bwd_workspace(int rows, int keys, int heads, int kv_heads, int width);
 int mggan_block_attention_bwd(const void* args, mggan_stream_t stream);
 

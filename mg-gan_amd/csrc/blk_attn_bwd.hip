@@ -215,12 +215,12 @@ __global__ __launch_bounds__(256, QF == 1 && DP <= 64 ? 3 : 2) void blk_attn_dq_
 }
 
 // dK and dV of 64 keys of one key head (this wave's 16 start at w0) from the queries [qa, qb) of `heads` heads from h0 on, in tiles of BK
-// rows; `part`: of one head alone, left in f32 for blk_attn_sum_kernel.  Four products a tile, both streamed operands read twice.  Bound by LDS: 16
+// rows; `part`: of some of the key head's heads, left in f32 for blk_attn_sum_kernel as the slot-th of `slots` such results.  Four products a tile, both streamed operands read twice.  Bound by LDS: 16
 // keys a wave take a kilobyte of reads for every multiplication, and LDS is busy 77 % of the time at width 128 (1.51 ms at 16,384 causal rows; width
 // 64, packed 8,192 rows: 165 us).  32 keys a wave would halve the reads, but two results, keys and values of 32 rows leave too few registers (1.8 to 9
 // ms, spilled or with two waves a SIMD).
 template <class T, int DP, int X, bool SAFE>
-__device__ __forceinline__ void attn_dkv_rows(const BlkAttnArgs& p, int np, const float* delta, float* part, int h0, int heads, int qa, int qb, int w0,
+__device__ __forceinline__ void attn_dkv_rows(const BlkAttnArgs& p, int np, const float* delta, float* part, int slot, int slots, int h0, int heads, int qa, int qb, int w0,
                                               u32x4* lq, u32x4* lo_, float* lm, int* odd) {
   using G = BwdGeo<T, DP>;
   using W = Soft<T, X>;
@@ -329,13 +329,13 @@ __device__ __forceinline__ void attn_dkv_rows(const BlkAttnArgs& p, int np, cons
   }
   const int r = w0 + i16;
   if (r >= p.M) return;
-  const long o = ((long)r * p.Hkv + hk) * p.D, po = ((long)h0 * p.M + r) * p.D;
+  const long o = ((long)r * p.Hkv + hk) * p.D, po = ((long)slot * p.M + r) * p.D;
 #pragma unroll
   for (int d = 0; d < G::DF; ++d)
     if (16 * d + 4 * g < p.D) {
       if (part) {
         store4<float>(part + po + 16 * d + 4 * g, dk[0][d], p.scale);
-        store4<float>(part + (long)p.H * p.M * p.D + po + 16 * d + 4 * g, dv[0][d], 1.f);
+        store4<float>(part + (long)slots * p.M * p.D + po + 16 * d + 4 * g, dv[0][d], 1.f);
       } else {
         store4<T>((T*)p.dk + o + 16 * d + 4 * g, dk[0][d], p.scale);
         store4<T>((T*)p.dv + o + 16 * d + 4 * g, dv[0][d], 1.f);
@@ -345,15 +345,16 @@ __device__ __forceinline__ void attn_dkv_rows(const BlkAttnArgs& p, int np, cons
 
 template <class T, int DP, int X>
 __global__ __launch_bounds__(256, DP <= 64 || (sizeof(T) == 2 && DP == 128) ? 3 : 2) void blk_attn_dkv_kernel(BlkAttnArgs p, int np, const float* delta,
-                                                                                                                         float* part, const float* slope_part, int nqt,
-                                                                                                                         const int2* ranges) {
+                                                                                                                         float* part, int parts, int per, const float* slope_part,
+                                                                                                                         int nqt, const int2* ranges) {
   using G = BwdGeo<T, DP>;
   __shared__ struct {
     u32x4 q[2 * G::TILE], o[2 * G::TILE];
     float m[2 * 8 * 64];  // of each streamed row: top, sum(dO O), lo, hi, x, y, 1 / sum; then what 32 rows see
     int odd, order[RANK_MAX + 1];
   } lds;
-  const int group = p.H / p.Hkv, nh = part ? p.H : p.Hkv, h0 = part ? blockIdx.x % nh : blockIdx.x % nh * group, heads = part ? 1 : group;
+  const int group = p.H / p.Hkv, nh = p.Hkv * parts, slot = blockIdx.x % nh, sub = slot % parts;
+  const int h0 = slot / parts * group + sub * per, heads = min(per, group - sub * per);
   const int kt = by_work(blockIdx.x / nh, gridDim.x / nh, [&](int i) { return ranges[i].y - ranges[i].x; }, lds.order);
   const int w0 = kt * 64 + mg_wave() * 16;
 
@@ -370,32 +371,36 @@ __global__ __launch_bounds__(256, DP <= 64 || (sizeof(T) == 2 && DP == 128) ? 3 
   if (threadIdx.x == 0) lds.odd = 0;
   __syncthreads();
   const int first = ranges[kt].x, last = ranges[kt].y, qa = last < 0 ? 0 : first * 32 / G::BK * G::BK, qb = (last + 1) * 32;
-  attn_dkv_rows<T, DP, X, false>(p, np, delta, part, h0, heads, qa, qb, w0, lds.q, lds.o, lds.m, &lds.odd);
+  attn_dkv_rows<T, DP, X, false>(p, np, delta, part, slot, nh, h0, heads, qa, qb, w0, lds.q, lds.o, lds.m, &lds.odd);
   if (!lds.odd) return;
   __syncthreads();
-  attn_dkv_rows<T, DP, X, true>(p, np, delta, part, h0, heads, qa, qb, afresh(w0), lds.q, lds.o, lds.m, &lds.odd);
+  attn_dkv_rows<T, DP, X, true>(p, np, delta, part, slot, nh, h0, heads, qa, qb, afresh(w0), lds.q, lds.o, lds.m, &lds.odd);
 }
 
-// dK and dV (blockIdx.y) of a key head: the sums over the heads that share it, in their order; four columns a thread.  Bound by bytes (12 us for the
+// dK and dV (blockIdx.y) of a key head: the sum of its `parts` partial results, in their order; four columns a thread.  Bound by bytes (12 us for the
 // packed 8,192 rows at width 64).
 template <class T>
-__global__ __launch_bounds__(256) void blk_attn_sum_kernel(BlkAttnArgs p, const float* part) {
+__global__ __launch_bounds__(256) void blk_attn_sum_kernel(BlkAttnArgs p, const float* part, int parts) {
   const long per = (long)p.M * p.D, id = ((long)blockIdx.x * 256 + threadIdx.x) * 4;
   if (id >= per * p.Hkv) return;
-  const int group = p.H / p.Hkv;
   const long hk = id / per, at = id - hk * per, r = at / p.D, d = at - r * p.D;
-  const float* in = part + (blockIdx.y * (long)p.H + hk * group) * per + at;
+  const float* in = part + (blockIdx.y * (long)p.Hkv + hk) * parts * per + at;
   f32x4 s = {};
-  for (int g = 0; g < group; ++g) s += *(const f32x4*)(in + g * per);
+  for (int g = 0; g < parts; ++g) s += *(const f32x4*)(in + g * per);
   store4<T>((T*)(blockIdx.y ? p.dv : p.dk) + (r * p.Hkv + hk) * p.D + d, s, 1.f);
 }
 
-// The workspace: sum(dO O), the slopes' partial sums, the rows that see each 64 keys, and -- where the heads of a key head are taken apart -- dK and dV of every head.
+// The workspace: sum(dO O), the slopes' partial sums, the rows that see each 64 keys, and -- where the heads of a key head are taken apart -- dK and dV
+// of each `per` of them, `parts` a key head.
 // They are where a key head's keys alone are too few workgroups: the first keys behind a causal mask are seen by all rows of all those
 // heads, and one workgroup's walk over them would be the whole time (backward pass, together / apart, causal: 256 workgroups 1.16 / 0.51 ms,
-// 1,024: 5.21 / 4.34; 2,048: 5.76 / 5.73, not worth the memory).
+// 1,024: 5.21 / 4.34; 2,048: 5.76 / 5.73, not worth the memory).  One head each while their f32 results stay within PART_BYTES, else as many
+// together as it takes: below 2,048 workgroups a key head's dK and dV are 134 MB at most, so eight parts always fit, and the memory does not grow
+// with the heads.
+constexpr size_t PART_BYTES = (size_t)1 << 30;
 struct Parts {
   size_t slopes, ranges, heads, bytes;
+  int parts, per;
 };
 Parts parts_of(int N, int M, int H, int Hkv, int D) {
   Parts w;
@@ -403,8 +408,12 @@ Parts parts_of(int N, int M, int H, int Hkv, int D) {
   w.slopes = up((size_t)H * N * 4);
   w.ranges = w.slopes + up((size_t)H * cdiv(N, 64) * 4);
   w.heads = w.ranges + up((size_t)cdiv(M, 64) * 8);
-  w.bytes = w.heads;
-  if (H > Hkv && (long)cdiv(M, 64) * Hkv < 2048) w.bytes += (size_t)2 * H * M * D * 4;
+  const int group = H / Hkv;
+  const size_t one = (size_t)2 * Hkv * M * D * 4;  // dK and dV of one part of each key head
+  w.per = group;
+  if (group > 1 && (long)cdiv(M, 64) * Hkv < 2048) w.per = cdiv(group, (long)(PART_BYTES / one));
+  w.parts = cdiv(group, w.per);
+  w.bytes = w.heads + (w.parts > 1 ? w.parts * one : 0);
   return w;
 }
 
@@ -417,10 +426,9 @@ void launch_bwd_tile(const BlkAttnArgs& p, hipStream_t st) {
   int2* ranges = (int2*)((char*)p.ws + w.ranges);
   float* heads = w.bytes > w.heads ? (float*)((char*)p.ws + w.heads) : nullptr;
   MG_LAUNCH((blk_attn_dq_kernel<T, DP, QF, X>), dim3(nqt * p.H), dim3(256), 0, st, p, np, delta, slopes, ranges);
-  const int nh = heads ? p.H : p.Hkv;
-  MG_LAUNCH((blk_attn_dkv_kernel<T, DP, X>), dim3(cdiv(p.M, 64) * nh), dim3(256), 0, st, p, np, (const float*)delta, heads, (const float*)slopes, nqt,
-            (const int2*)ranges);
-  if (heads) MG_LAUNCH((blk_attn_sum_kernel<T>), dim3(cdiv((long)p.M * p.Hkv * p.D, 1024), 2), dim3(256), 0, st, p, (const float*)heads);
+  MG_LAUNCH((blk_attn_dkv_kernel<T, DP, X>), dim3(cdiv(p.M, 64) * p.Hkv * w.parts), dim3(256), 0, st, p, np, (const float*)delta, heads, w.parts, w.per,
+            (const float*)slopes, nqt, (const int2*)ranges);
+  if (heads) MG_LAUNCH((blk_attn_sum_kernel<T>), dim3(cdiv((long)p.M * p.Hkv * p.D, 1024), 2), dim3(256), 0, st, p, (const float*)heads, w.parts);
 }
 template <class T, int DP, int X>
 void launch_bwd_x(const BlkAttnArgs& p, hipStream_t st) {
@@ -468,7 +476,7 @@ void launch_bwd_width(const BlkAttnArgs& p, hipStream_t st) {
 extern "C" {
 
 size_t mggan_block_attention_bwd_workspace(int rows, int keys, int heads, int kv_heads, int width) {
-  return rows > 0 && keys > 0 && heads > 0 && kv_heads > 0 && width > 0 ? parts_of(rows, keys, heads, kv_heads, width).bytes : 0;
+  return rows > 0 && keys > 0 && heads > 0 && kv_heads > 0 && heads % kv_heads == 0 && width > 0 && width <= 128 ? parts_of(rows, keys, heads, kv_heads, width).bytes : 0;
 }
 
 int mggan_block_attention_bwd(const void* args, hipStream_t stream) {

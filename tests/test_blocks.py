@@ -200,3 +200,15 @@ def test_positions_with_a_tangent_are_refused(name, monkeypatch):
     fw = torch.autograd.forward_ad
     with fw.dual_level(), pytest.raises(ValueError, match="positions have no gradient"):
         B.attention(*QKV, S, slopes=x(4), **{"xy": x(6, 2), "kv_xy": x(6, 2), name: fw.make_dual(x(6, 2), x(6, 2))})
+
+
+@pytest.mark.parametrize("keys", [64, 5000, 16384, 131008, 131072, 1 << 20])
+@pytest.mark.parametrize("H,Hkv,D", [(8, 1, 128), (64, 1, 128), (1024, 1, 128), (1024, 2, 64), (13, 1, 8), (48, 16, 96), (32, 32, 128)])
+def test_the_backward_passs_workspace_does_not_grow_with_the_heads(H, Hkv, D, keys):
+    """Partial dK and dV stay within 1 GiB (8 bytes a key, head and column they were, 137 GB at 131,008 keys of 1,024 heads)."""
+    rows = 1000
+    got = L.mggan_block_attention_bwd_workspace(rows, keys, H, Hkv, D)
+    rest = 4 * H * rows + 4 * H * -(-rows // 64) + 8 * -(-keys // 64)  # sum(dO O), the slopes' partial sums, the ranges of rows
+    assert rest <= got <= rest + 3 * 256 + (1 << 30)
+    if H > Hkv and keys * Hkv <= 64 * 2000 and 8 * H * keys * D <= 1 << 30:
+        assert got >= rest + 8 * H * keys * D  # (one part a head where they fit)

@@ -143,3 +143,32 @@ def test_caps_of_any_size_for_single_rows(cap, dtype):
     with torch.no_grad():
         out = B().attention(q, k, v, scenes, kv, cap=cap)
     close(out, *attention64(q, k, v, visible(3, M, scenes, kv, False, None), q, D ** -0.5, cap)["out"], "out")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("H,Hkv,per", [(40, 1, 2), (112, 2, 3)])
+def test_several_heads_a_partial_result(H, Hkv, per, dtype):
+    """Keys and heads of which a part each would pass 1 GiB: `per` heads of a key head are walked by one workgroup (the last part of 56
+    fewer), and the parts are joined.  Scenes are independent, so three of them are held to the definition."""
+    gen = torch.Generator().manual_seed(H)
+    N, D, n = 40_000, 128, 40
+    keys = N if Hkv == 1 else N // 2
+    if Hkv == 2:
+        N = keys
+    parts = (1 << 30) // (8 * Hkv * keys * D)
+    assert -(-(H // Hkv) // parts) == per
+    scenes = [(i, i + n) for i in range(0, N, n)]
+    q, dout = (torch.empty(N, H, D, dtype=dtype, device="cuda") for _ in range(2))
+    k, v = (torch.empty(N, Hkv, D, dtype=dtype, device="cuda") for _ in range(2))
+    cgen = torch.Generator(device="cuda").manual_seed(H)
+    for t in (q, k, v, dout):
+        t.normal_(generator=cgen)
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    out = B().attention(*leaves, scenes, causal=True)
+    grads = torch.autograd.grad(out, leaves, dout)
+    with torch.no_grad():
+        for a, b in (scenes[0], scenes[len(scenes) // 2], scenes[-1]):
+            see = visible(n, n, [(0, n)], [(0, n)], True, None)
+            want = attention64(q[a:b], k[a:b], v[a:b], see, dout[a:b], D ** -0.5)
+            for name, got in zip(("out", "dq", "dk", "dv"), (out,) + grads):
+                close(got[a:b], *want[name], name)
