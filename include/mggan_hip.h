@@ -654,7 +654,7 @@ int mggan_crop_patches(const unsigned char* atlas, const long long* img_off, con
  * NULL).  Backward: dx (M, K), dw (N, K), db (N), each NULL if not wanted; with w2 dw is (off + N, K), off = N rounded up to 64 bytes of
  * elements: the gate weight's gradient in rows [0, N), the up weight's from off on; db (2 N).  Written, not accumulated; fixed order of
  * summation.  ws: mggan_block_layer_workspace bytes, 256-byte aligned, free again when the call's work on `stream` is done.  Limits:
- * M <= 2^21, K, N <= 2^20. */
+ * M <= 2^21, K, N <= 2^20 (beyond them the workspace is 0 and the calls refuse). */
 size_t mggan_block_layer_workspace(int rows, int K, int N, int gated, int backward, int act, int dtype);
 int mggan_block_layer_fwd(const void* args, mggan_stream_t stream);
 int mggan_block_layer_bwd(const void* args, mggan_stream_t stream);
@@ -673,7 +673,7 @@ int mggan_block_layer_bwd(const void* args, mggan_stream_t stream);
  * aligned, written by the forward call and read by the backward call.  Rows without keys: zeros. */
 size_t mggan_block_attention_span_ints(int rows);
 /* Without lse (nothing kept for a backward pass) single rows over long caches are split over their keys: ws as large as this says
- * (0: none needed). */
+ * (0: none needed, or sizes that no call takes). */
 size_t mggan_block_attention_fwd_workspace(int rows, int keys, int heads, int kv_heads, int width, int scenes);
 int mggan_block_attention_fwd(const void* args, mggan_stream_t stream);
 /* dq, dk, dv, and dslopes (H) if not NULL, written in a fixed order of summation; out32, lse, spans as the forward call left them.

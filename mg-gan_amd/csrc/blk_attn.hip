@@ -481,7 +481,7 @@ size_t mggan_block_attention_span_ints(int rows) {
 size_t mggan_block_attention_fwd_workspace(int rows, int keys, int heads, int kv_heads, int width, int scenes) {
   BlkAttnArgs p = {};
   p.N = rows, p.M = keys, p.H = heads, p.Hkv = kv_heads, p.D = width, p.S = scenes;
-  return rows > 0 && heads > 0 && kv_heads > 0 && width > 0 && scenes > 0 ? fwd_workspace(p) : 0;
+  return rows > 0 && keys > 0 && heads > 0 && kv_heads > 0 && heads % kv_heads == 0 && width > 0 && scenes > 0 ? fwd_workspace(p) : 0;
 }
 
 int mggan_block_attention_fwd(const void* args, hipStream_t stream) {

@@ -792,13 +792,14 @@ int layer(const BlkLayerArgs& l, bool gated, bool bwd, void* ws, size_t* need, h
   return gated ? layer_fwd<float, true>(l, a, need, st) : layer_fwd<float, false>(l, a, need, st);
 }
 
+bool sizes_fit(int M, int K, int N) { return M > 0 && K > 0 && N > 0 && M <= (1 << 21) && K <= (1 << 20) && N <= (1 << 20); }
+
 int check(const char* name, const BlkLayerArgs* a, bool bwd) {
   MG_CHECK_ARG(a, "%s: no arguments", name);
   const BlkLayerArgs& l = *a;
   const bool gated = l.w2 != nullptr;
   MG_CHECK_ARG(l.dtype == BLK_F32 || l.dtype == BLK_BF16, "%s: dtype %d (0 = f32, 1 = bf16)", name, l.dtype);
-  MG_CHECK_ARG(l.M > 0 && l.K > 0 && l.N > 0 && l.M <= (1 << 21) && l.K <= (1 << 20) && l.N <= (1 << 20),
-               "%s: sizes %d x %d x %d (limits 2^21 x 2^20 x 2^20)", name, l.M, l.K, l.N);
+  MG_CHECK_ARG(sizes_fit(l.M, l.K, l.N), "%s: sizes %d x %d x %d (limits 2^21 x 2^20 x 2^20)", name, l.M, l.K, l.N);
   MG_CHECK_ARG(l.x && l.w, "%s: null operand", name);
   MG_CHECK_ARG((l.act >= ACT_NONE && l.act <= ACT_SIGMOID) || l.act == ACT_SILU || l.act == ACT_GELU, "%s: activation %d", name, l.act);
   const int ch = l.dtype == BLK_BF16 ? 8 : 4;
@@ -818,7 +819,7 @@ int check(const char* name, const BlkLayerArgs* a, bool bwd) {
 extern "C" {
 
 size_t mggan_block_layer_workspace(int rows, int K, int N, int gated, int backward, int act, int dtype) {
-  if (rows <= 0 || K <= 0 || N <= 0) return 0;
+  if (!sizes_fit(rows, K, N)) return 0;
   BlkLayerArgs l = {};
   l.M = rows, l.K = K, l.N = N, l.ldx = K, l.act = act, l.dtype = dtype;
   size_t need = 0;

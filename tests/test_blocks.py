@@ -1,6 +1,8 @@
 """CPU: what the transformer-block operators (mggan/hip/blocks.py) refuse, and that their C structures match."""
 import os
 import re
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -212,3 +214,14 @@ def test_the_backward_passs_workspace_does_not_grow_with_the_heads(H, Hkv, D, ke
     assert rest <= got <= rest + 3 * 256 + (1 << 30)
     if H > Hkv and keys * Hkv <= 64 * 2000 and 8 * H * keys * D <= 1 << 30:
         assert got >= rest + 8 * H * keys * D  # (one part a head where they fit)
+
+
+def test_workspace_queries_of_sizes_that_no_call_takes():
+    """They say 0 -- in a process of its own: heads that key heads do not divide ended it by a division by zero."""
+    big = (1 << 31) - 1
+    calls = ["mggan_block_attention_fwd_workspace(1, 1000, 1, 2, 64, 1)", "mggan_block_attention_fwd_workspace(1, 0, 1, 1, 64, 1)",
+             "mggan_block_attention_bwd_workspace(1, 1000, 1, 2, 64)", "mggan_block_attention_bwd_workspace(1, 1000, 8, 2, %d)" % big,
+             "mggan_block_layer_workspace(100, %d, %d, 0, 0, 0, 0)" % (big, big), "mggan_block_layer_workspace(%d, 8, 8, 1, 1, 4, 1)" % big]
+    code = "from mggan.hip import lib\nfor n in (%s,):\n    assert n == 0, n\nprint('all 0')" % ", ".join("lib." + c for c in calls)
+    run = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, cwd=os.path.join(ROOT, "mg-gan_amd"))
+    assert run.returncode == 0 and run.stdout.strip() == "all 0", (run.returncode, run.stderr[-500:])
