@@ -296,10 +296,13 @@ __device__ __forceinline__ bool tile_not_finite(const u32x4* tile, int lane) {
   }
   return __ballot(bad) != 0;
 }
-// accumulate() for a tile that is partly masked AND holds such values: they are taken as zeros, and where a row sees one (a second product,
-// of where they are with what `sees`) the sum becomes the infinity or the NaN that it would have been.  It is in a second copy of the
-// kernels' loops (SAFE) that a workgroup runs, from the start, only if its first run came upon such a tile: beside the plain way in one
-// loop it would cost every run 40 to 100 registers.
+// accumulate() for a tile that is partly masked AND holds such values: they are taken as zeros, and where a row sees some the sum becomes the
+// infinity or the NaN that it would have been, by two more products: of ones where they are with ones where the row sees (how many terms are not
+// finite) and of their signs with the coefficients' signs (how many are +inf less how many -inf; a NaN and a coefficient of zero count nothing, so
+// a term that is a NaN, as zero times infinity is, leaves the two apart; an infinite coefficient that meets one gives a NaN).  It is in a second copy of the kernels' loops (SAFE) that a workgroup
+// runs, from the start, only if its first run came upon such a tile: beside the plain way in one loop it would cost every run 40 to 100 registers.
+// (One product after the other: their operands together would cost the plain run's waves theirs, width 64 with a cap 342 -> 350 us.)
+__device__ __forceinline__ float sign_of(float x) { return x > 0.f ? 1.f : x < 0.f ? -1.f : 0.f; }
 template <class G, int QF, class See>
 __device__ __forceinline__ void accumulate_seen(const void* tile, const Coef<typename G::T> (&coef)[QF][G::F], f32x4 (&acc)[QF][G::DF], const Lane<G>& at, int lane,
                                                 See sees) {
@@ -307,50 +310,49 @@ __device__ __forceinline__ void accumulate_seen(const void* tile, const Coef<typ
   const int g = lane >> 4;
 #pragma unroll
   for (int fd = 0; fd < G::DF; ++fd) {
-    f32x4 up[QF] = {}, down[QF] = {};
+    f32x4 many[QF] = {}, sign[QF] = {};
 #pragma unroll
     for (int p = 0; p < (HALF ? G::F / 2 : G::F * 4); ++p) {
       if constexpr (HALF) {
         const bf16x8 a = at.cols((const char*)tile, p, fd);
-        bf16x8 clean, hi, lo, b, one;
+        auto product = [&](f32x4(&to)[QF], auto left, auto right) {
+          bf16x8 x, y;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float x = (float)a[e];
-          const bool odd = !(fabsf(x) < INFINITY);
-          clean[e] = odd ? (bf16)0.f : a[e];
-          hi[e] = (bf16)(odd && !(x < 0.f) ? 1.f : 0.f);
-          lo[e] = (bf16)(odd && !(x > 0.f) ? 1.f : 0.f);
-        }
+          for (int e = 0; e < 8; ++e) x[e] = (bf16)left((float)a[e], !(fabsf((float)a[e]) < INFINITY));
 #pragma unroll
-        for (int j = 0; j < QF; ++j) {
+          for (int j = 0; j < QF; ++j) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            b[e] = coef[j][2 * p + (e >> 2)].v[e & 3];
-            one[e] = (bf16)(sees(j, 32 * p + 8 * g + e) ? 1.f : 0.f);
+            for (int e = 0; e < 8; ++e) y[e] = (bf16)right(j, (float)coef[j][2 * p + (e >> 2)].v[e & 3], 32 * p + 8 * g + e);
+            to[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, y, to[j], 0, 0, 0);
           }
-          acc[j][fd] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(clean, b, acc[j][fd], 0, 0, 0);
-          up[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hi, one, up[j], 0, 0, 0);
-          down[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(lo, one, down[j], 0, 0, 0);
-        }
+          __builtin_amdgcn_sched_barrier(0);
+        };
+        f32x4 t[QF];
+#pragma unroll
+        for (int j = 0; j < QF; ++j) t[j] = acc[j][fd];
+        product(t, [](float x, bool odd) { return odd ? 0.f : x; }, [](int, float c, int) { return c; });
+#pragma unroll
+        for (int j = 0; j < QF; ++j) acc[j][fd] = t[j];
+        product(many, [](float, bool odd) { return odd ? 1.f : 0.f; }, [&](int j, float, int row) { return sees(j, row) ? 1.f : 0.f; });
+        product(sign, [](float x, bool odd) { return odd ? sign_of(x) : 0.f; }, [&](int j, float c, int row) { return sees(j, row) ? sign_of(c) : 0.f; });
       } else {
         const float x = at.col1((const char*)tile, p >> 2, p & 3, fd);
         const bool odd = !(fabsf(x) < INFINITY);
 #pragma unroll
         for (int j = 0; j < QF; ++j) {
-          const float one = sees(j, 16 * (p >> 2) + 4 * g + (p & 3)) ? 1.f : 0.f;
-          acc[j][fd] = __builtin_amdgcn_mfma_f32_16x16x4f32(odd ? 0.f : x, coef[j][p >> 2].v[p & 3], acc[j][fd], 0, 0, 0);
-          up[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(odd && !(x < 0.f) ? 1.f : 0.f, one, up[j], 0, 0, 0);
-          down[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(odd && !(x > 0.f) ? 1.f : 0.f, one, down[j], 0, 0, 0);
+          const float c = coef[j][p >> 2].v[p & 3];
+          const bool seen = sees(j, 16 * (p >> 2) + 4 * g + (p & 3));
+          acc[j][fd] = __builtin_amdgcn_mfma_f32_16x16x4f32(odd ? 0.f : x, c, acc[j][fd], 0, 0, 0);
+          many[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(odd ? 1.f : 0.f, seen ? 1.f : 0.f, many[j], 0, 0, 0);
+          sign[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(odd ? sign_of(x) : 0.f, seen ? sign_of(c) : 0.f, sign[j], 0, 0, 0);
         }
       }
     }
 #pragma unroll
     for (int j = 0; j < QF; ++j)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        if (up[j][e] > 0.f) acc[j][fd][e] += INFINITY;
-        if (down[j][e] > 0.f) acc[j][fd][e] -= INFINITY;
-      }
+      for (int e = 0; e < 4; ++e)
+        if (many[j][e] > 0.f) acc[j][fd][e] += many[j][e] == sign[j][e] ? INFINITY : many[j][e] == -sign[j][e] ? -INFINITY : NAN;
     __builtin_amdgcn_sched_barrier(0);
   }
 }

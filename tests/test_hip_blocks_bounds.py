@@ -172,3 +172,47 @@ def test_several_heads_a_partial_result(H, Hkv, per, dtype):
             want = attention64(q[a:b], k[a:b], v[a:b], see, dout[a:b], D ** -0.5)
             for name, got in zip(("out", "dq", "dk", "dv"), (out,) + grads):
                 close(got[a:b], *want[name], name)
+
+
+def visible_only(q, k, v, dout, see, scale, cap):
+    """The definition in 64 bits, each row over the keys that it sees and nothing else: what infinities and NaN become."""
+    (N, H, D), G = q.shape, q.shape[1] // k.shape[1]
+    q, k, v, dout = (t.detach().double().cpu() for t in (q, k, v, dout))
+    out = {"out": torch.zeros_like(q), "dq": torch.zeros_like(q), "dk": torch.zeros_like(k), "dv": torch.zeros_like(v)}
+    dot = lambda a, b: (a * b).sum(-1)
+    for i in range(N):
+        j = see[i].nonzero()[:, 0].cpu()
+        for h in range(H):
+            K, V, do = k[j, h // G], v[j, h // G], dout[i, h]
+            z = scale * dot(K, q[i, h])
+            t = torch.tanh(z / cap) if cap else None
+            P = torch.softmax(cap * t if cap else z, 0)
+            O = (P[:, None] * V).sum(0)
+            dS = P * (dot(V, do) - dot(do, O)) * (1 - t * t if cap else 1.0)
+            out["out"][i, h], out["dq"][i, h] = O, scale * (dS[:, None] * K).sum(0)
+            out["dk"][j, h // G] += scale * dS[:, None] * q[i, h]
+            out["dv"][j, h // G] += P[:, None] * do
+    return out
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("cap", [0.0, 20.0])
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), float("-inf")])
+@pytest.mark.parametrize("which", ["q", "k", "v", "dout"])
+def test_what_a_value_that_is_not_finite_becomes(which, value, cap, dtype):
+    """In every output and gradient the same places are +inf, -inf, NaN or finite as in the definition -- whether the tile that holds the
+    value is partly masked (rows near it) or seen as a whole (rows far behind it).  Under a cap an infinite score is a finite one of slope zero,
+    and zero times infinity is NaN."""
+    gen = torch.Generator().manual_seed(11)
+    N, H, D, at = 200, 2, 32, 10
+    t = {n: rnd(gen, N, H, D, dtype=dtype) for n in ("q", "k", "v", "dout")}
+    t["q"][:, 0, 3].abs_()  # (a key of -inf there leaves some rows finite scores and others none)
+    t["q"][::3, 0, 3].neg_()
+    t[which][at, 0, 3], t[which][at + 5, 1, 7] = value, value
+    got, _ = run(t["q"], t["k"], t["v"], t["dout"], [(0, N)], causal=True, cap=cap)
+    see = visible(N, N, [(0, N)], [(0, N)], True, None)
+    want = visible_only(*t.values(), see, D ** -0.5, cap)
+    kind = lambda x: torch.where(x.isnan(), 2, torch.where(x.isinf(), x.sign(), 0.0))
+    for name, x in want.items():
+        a, b = kind(got[name].double().cpu()), kind(x)
+        assert torch.equal(a, b), (name, [(i, float(a[tuple(i)]), float(b[tuple(i)])) for i in (a != b).nonzero().tolist()[:6]], int((a != b).sum()))
