@@ -22,7 +22,7 @@ from .lib import lib
 ACT_SILU, ACT_GELU = 4, 5
 _ACTS = (ACT_NONE, ACT_LEAKY, ACT_SIGMOID, ACT_SILU, ACT_GELU)
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1}
-_F32 = torch.float32
+_F32, _F32_MAX = torch.float32, torch.finfo(torch.float32).max
 
 # The calls' arguments as the C structures of csrc/blk_gemm.hip and csrc/blk_attn.h lay them out, packed in one go (a small call is
 # bound by the host: filling a ctypes structure field by field took 6 us of a 36 us forward call).
@@ -93,6 +93,16 @@ def _needs_grad(*tensors):
     return _any_dual(*tensors)
 
 
+def _number(name, what, value):
+    """A factor of the call as a float (an f32 one in the kernels): no tensor that a gradient is wanted of."""
+    if isinstance(value, torch.Tensor) and (value.requires_grad and torch.is_grad_enabled() or _any_dual(value)):
+        raise ValueError("{}: {} has no gradient: detach it".format(name, what))
+    try:
+        return float(value)
+    except (TypeError, ValueError, RuntimeError, OverflowError):
+        raise ValueError("{}: {} is not a number: {!r}".format(name, what, value)) from None
+
+
 # ---- layers ------------------------------------------------------------------------------------------------------------------
 
 def _rows(x, K):
@@ -111,17 +121,23 @@ def _rows(x, K):
     return x, ld
 
 
-def _check_layer(name, x, weight, bias, act):
+def _check_layer(name, x, weight, bias, act, slope):
+    """-> the slope as a float"""
     rows, shape = x.shape, weight.shape
     if len(shape) != 2 or not rows or rows[-1] != shape[1] or not shape[0] or not shape[1]:
         raise ValueError("{}: rows of {} and a weight of {}".format(name, tuple(rows), tuple(shape)))
     N, K = shape
     if x.numel() > K << 21 or N > 1 << 20 or K > 1 << 20:
         raise ValueError("{}: sizes {} x {} over 2^21 rows, 2^20 columns".format(name, tuple(x.shape), tuple(weight.shape)))
-    if act not in _ACTS:
+    if not isinstance(act, int) or act not in _ACTS:
         raise ValueError("{}: unknown activation {}".format(name, act))
     if bias is not None and (bias.dim() != 1 or bias.shape[0] != N):
         raise ValueError("{}: a bias of {} for {} outputs".format(name, tuple(bias.shape), N))
+    if type(slope) is not float:
+        slope = _number(name, "slope", slope)
+    if not -_F32_MAX <= slope <= _F32_MAX:
+        raise ValueError("{}: slope {} is not a finite f32 number".format(name, slope))
+    return slope
 
 
 def _layer_fwd(x, w, w2, b, b2, res, act, slope, keep):
@@ -195,9 +211,10 @@ class LayerFn(Function):
 
 def linear_residual(x, weight, bias=None, residual=None, act=ACT_NONE, slope=0.0):
     """act(x W^T + b) + residual: x (..., K), weight (N, K), bias (N) or None, residual (..., N) or None -> (..., N).
-    act: ACT_NONE, ACT_LEAKY (with `slope`; 0 is ReLU), ACT_SIGMOID, ACT_SILU or ACT_GELU.  x may be a view with any row stride."""
+    act: ACT_NONE, ACT_LEAKY (with `slope`; 0 is ReLU), ACT_SIGMOID, ACT_SILU or ACT_GELU; the slope is a
+    number, without a gradient.  x may be a view with any row stride."""
     _same("linear_residual", x, weight, bias, residual)
-    _check_layer("linear_residual", x, weight, bias, act)
+    slope = _check_layer("linear_residual", x, weight, bias, act, slope)
     N, two = weight.shape[0], x.dim() == 2
     if residual is not None and residual.shape != x.shape[:-1] + (N,):
         raise ValueError("linear_residual: a residual of {} for outputs of {} (it is not broadcast)".format(
@@ -209,7 +226,7 @@ def linear_residual(x, weight, bias=None, residual=None, act=ACT_NONE, slope=0.0
         lead = x.shape[:-1]
         x, residual = x.reshape(-1, x.shape[-1]), None if residual is None else residual.reshape(-1, N)
     if _needs_grad(x, weight, bias, residual):
-        y = LayerFn.apply(x, weight, None, bias, None, residual, act, float(slope))
+        y = LayerFn.apply(x, weight, None, bias, None, residual, act, slope)
     else:
         y = _layer_fwd(x, weight, None, bias, None, residual, act, slope, False)[0]
     return y if two else y.reshape(*lead, N)
@@ -219,8 +236,8 @@ def gated_linear(x, w_gate, w_up, b_gate=None, b_up=None, act=ACT_SILU, slope=0.
     """act(x Wg^T + bg) * (x Wu^T + bu): x (..., K), w_gate and w_up (N, K), biases (N) or None -> (..., N); activations as in
     linear_residual."""
     _same("gated_linear", x, w_gate, w_up, b_gate, b_up)
-    _check_layer("gated_linear", x, w_gate, b_gate, act)
-    _check_layer("gated_linear", x, w_up, b_up, act)
+    slope = _check_layer("gated_linear", x, w_gate, b_gate, act, slope)
+    _check_layer("gated_linear", x, w_up, b_up, act, slope)
     if w_gate.shape != w_up.shape:
         raise ValueError("gated_linear: weights of {} and {}".format(tuple(w_gate.shape), tuple(w_up.shape)))
     if not _on_current("gated_linear", x):
@@ -230,7 +247,7 @@ def gated_linear(x, w_gate, w_up, b_gate=None, b_up=None, act=ACT_SILU, slope=0.
     if not two:
         lead, x = x.shape[:-1], x.reshape(-1, x.shape[-1])
     if _needs_grad(x, w_gate, w_up, b_gate, b_up):
-        y = LayerFn.apply(x, w_gate, w_up, b_gate, b_up, None, act, float(slope))
+        y = LayerFn.apply(x, w_gate, w_up, b_gate, b_up, None, act, slope)
     else:
         y = _layer_fwd(x, w_gate, w_up, b_gate, b_up, None, act, slope, False)[0]
     return y if two else y.reshape(*lead, w_gate.shape[0])
@@ -368,7 +385,7 @@ def attention(q, k, v, scenes, kv_scenes=None, *, causal=False, prefix=None, sca
     no scene and rows that see no key give zeros.  What lies outside a row's visible keys is never mixed in, infinities and NaN included.
     causal: row i of a scene of Lq rows and Lk keys sees keys j <= i + Lk - Lq, and in any case those before prefix[scene] (list or int32
     device tensor).  One new row over a long cache is Lq = 1.  scale: > 0, D ** -0.5 by default; cap: 0 for none;
-    both between 2^-60 and 2^60.
+    both numbers between 2^-60 and 2^60, without a gradient.
     xy (N, axes) and kv_xy (M, axes; by default xy), f32 with one or two axes, and slopes (H), f32: the bias by distance.  Gradients go to q,
     k, v and slopes, not to positions."""
     _same("attention", q, k, v)
@@ -382,8 +399,8 @@ def attention(q, k, v, scenes, kv_scenes=None, *, causal=False, prefix=None, sca
         raise ValueError("attention: a width of {} (a multiple of 8 up to 128)".format(D))
     if N > 1 << 24 or M > 1 << 30 or N * H > 1 << 29:
         raise ValueError("attention: {} rows of {} heads, {} keys (at most 2^24 rows, 2^29 rows times heads, 2^30 keys)".format(N, H, M))
-    scale = D ** -0.5 if scale is None else float(scale)
-    cap = 0.0 if cap is None else float(cap)
+    scale = D ** -0.5 if scale is None else _number("attention", "scale", scale)
+    cap = 0.0 if cap is None else _number("attention", "cap", cap)
     if not _LEAST <= scale <= 1 / _LEAST or not (cap == 0 or _LEAST <= cap <= 1 / _LEAST):
         raise ValueError("attention: scale {} (has to be positive), cap {} (0 or positive), both within 2^-60 and 2^60".format(scale, cap))
     if prefix is not None and not causal:

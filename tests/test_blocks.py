@@ -4,6 +4,7 @@ import re
 import subprocess
 import sys
 
+import numpy as np
 import pytest
 import torch
 
@@ -225,3 +226,36 @@ def test_workspace_queries_of_sizes_that_no_call_takes():
     code = "from mggan.hip import lib\nfor n in (%s,):\n    assert n == 0, n\nprint('all 0')" % ", ".join("lib." + c for c in calls)
     run = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, cwd=os.path.join(ROOT, "mg-gan_amd"))
     assert run.returncode == 0 and run.stdout.strip() == "all 0", (run.returncode, run.stderr[-500:])
+
+
+@pytest.mark.parametrize("slope", [1e39, -1e39, float("nan"), float("inf"), "a", None, torch.tensor(0.2, requires_grad=True), torch.zeros(2)])
+def test_slopes_that_are_no_f32_number(slope, monkeypatch):
+    """Refused as every argument is (ValueError), and a tensor that a gradient is wanted of, which none would go to."""
+    stubbed(monkeypatch)
+    with pytest.raises(ValueError, match="linear_residual: slope"):
+        B.linear_residual(x(3, 4), x(5, 4), act=B.ACT_LEAKY, slope=slope)
+    with pytest.raises(ValueError, match="gated_linear: slope"):
+        B.gated_linear(x(3, 4), x(5, 4), x(5, 4), act=B.ACT_LEAKY, slope=slope)
+
+
+def test_numbers_of_any_kind_are_taken(monkeypatch):
+    got = []
+    stubbed(monkeypatch)
+    monkeypatch.setattr(B, "_layer_fwd", lambda t, w, w2, b, b2, res, act, slope, keep: (got.append(slope), (x(3, 5), None, t, w, w2))[1])
+    with torch.no_grad():
+        for slope in (0, 1, -0.25, True, np.float32(0.5), torch.tensor(2.0, requires_grad=True), 1e38):
+            B.linear_residual(x(3, 4), x(5, 4), act=B.ACT_LEAKY, slope=slope)
+    assert got == [0.0, 1.0, -0.25, 1.0, 0.5, 2.0, 1e38] and {type(s) for s in got} == {float}
+
+
+@pytest.mark.parametrize("act", [1.0, "silu", None, 4.5])
+def test_activations_are_codes(act):
+    with pytest.raises(ValueError, match="activation"):
+        B.linear_residual(x(3, 4), x(5, 4), act=act)
+
+
+@pytest.mark.parametrize("kw", [{"scale": torch.tensor(0.5, requires_grad=True)}, {"cap": torch.tensor(5.0, requires_grad=True)}, {"scale": "a"},
+                                {"cap": [1.0]}])
+def test_scale_and_cap_are_numbers(kw):
+    with pytest.raises(ValueError, match="attention: (scale|cap)"):
+        B.attention(*QKV, S, **kw)
