@@ -9,6 +9,7 @@ rounded once.  Work goes to torch's current stream, outputs and workspaces come 
 into a HIP graph), gradients are returned through autograd and are the same bits in every run.  Arguments that do not fit raise
 ValueError, a failing launch raises HipError, forward-mode tangents raise NotImplementedError; there is no CPU path."""
 import functools
+import operator
 import struct
 from itertools import chain
 
@@ -270,9 +271,9 @@ def _table(name, rows, device, limit, width):
     try:
         key = tuple(map(tuple, rows)) if width == 2 else tuple(rows)
         if not {int}.issuperset(map(type, chain.from_iterable(key) if width == 2 else key)) or width == 2 and not {2}.issuperset(map(len, key)):
-            key = tuple((int(a), int(b)) for a, b in key) if width == 2 else tuple(int(a) for a in key)
+            key = tuple((operator.index(a), operator.index(b)) for a, b in key) if width == 2 else tuple(map(operator.index, key))
     except (TypeError, ValueError):
-        raise ValueError("attention: {} has to be a list or an int32 device tensor".format(name)) from None
+        raise ValueError("attention: {} has to be a list of whole numbers or an int32 device tensor".format(name)) from None
     key = (key, limit, device)
     hit = _TABLES.get(key)
     if hit is None:

@@ -259,3 +259,18 @@ def test_activations_are_codes(act):
 def test_scale_and_cap_are_numbers(kw):
     with pytest.raises(ValueError, match="attention: (scale|cap)"):
         B.attention(*QKV, S, **kw)
+
+
+@pytest.mark.parametrize("rows,width", [([(0, 2.7)], 2), (torch.tensor([[0.0, 2.5]]), 2), ([("0", "3")], 2), (np.array([[0.0, 3.0]]), 2), ([1.5], 1)])
+def test_tables_of_numbers_that_are_not_whole(rows, width):
+    """They were cut off: rows [0, 2.7) became [0, 2)."""
+    with pytest.raises(ValueError, match="whole numbers"):
+        B._table("scenes", rows, torch.device("cpu"), 6, width)
+
+
+@pytest.mark.parametrize("rows", [np.array([[0, 2], [2, 6]]), torch.tensor([[0, 2], [2, 6]]), [np.array([0, 2]), (np.int32(2), 6)]])
+def test_tables_of_whole_numbers_of_any_kind(rows, monkeypatch):
+    monkeypatch.setattr(B, "_s", lambda: 0)
+    monkeypatch.setattr(B, "_TABLES", B.BoundedCache(64))
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    assert B._table("scenes", rows, torch.device("cpu"), 6, 2).tolist() == [[0, 2], [2, 6]]
