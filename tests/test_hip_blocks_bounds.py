@@ -216,3 +216,255 @@ def test_what_a_value_that_is_not_finite_becomes(which, value, cap, dtype):
     for name, x in want.items():
         a, b = kind(got[name].double().cpu()), kind(x)
         assert torch.equal(a, b), (name, [(i, float(a[tuple(i)]), float(b[tuple(i)])) for i in (a != b).nonzero().tolist()[:6]], int((a != b).sum()))
+
+
+# ---- every kernel that a call can reach ----------------------------------------------------------------------------------------
+
+NAMES = {torch.float32: "f", torch.bfloat16: "DF16b"}
+
+
+def launched(call):
+    """(what call gives, the kernels that it and its backward pass launched, by their mangled names)"""
+    from mggan.hip.lib import load
+
+    load().launch_log(True)
+    try:
+        out = call()
+        return out, [name for name, _ in load().read_launches()]
+    finally:
+        load().launch_log(False)
+
+
+def ran(names, kernel, dtype, *args):
+    """Whether the instantiation with these template arguments (numbers and truth values) is among the launches."""
+    want = "{}I{}{}E".format(kernel, NAMES[dtype], "".join("L{}{}E".format("b" if isinstance(a, bool) else "i", int(a)) for a in args))
+    return any(want in n for n in names)
+
+
+def ways(dtype):
+    """What is done to a score (the kernels' argument X), with a cap and axes that lead there."""
+    small = [(0, 0.0, 0), (1, 9.0, 0), (2, 0.0, 1), (3, 30.0, 1), (4, 0.0, 2), (5, 64.0, 2)]
+    return small if dtype == torch.float32 else small + [(9, 65.0, 0), (11, 500.0, 1), (13, 1e5, 2)]
+
+
+WIDTHS = {32: 24, 64: 64, 96: 88, 128: 128}  # the kernels' widths, one of an operand's each
+
+
+@pytest.mark.parametrize("dtype,X,cap,axes", [(t,) + w for t in TYPES for w in ways(t)])
+@pytest.mark.parametrize("DP,QF", [(32, 1), (64, 1), (96, 1), (128, 1), (96, 2), (128, 2)])
+def test_every_attention_kernel(DP, QF, dtype, X, cap, axes):
+    """64 and 128 rows a workgroup, all widths, caps and distances: forward, dQ and dK / dV against the definition."""
+    gen = torch.Generator().manual_seed(100 * DP + 10 * QF + X)
+    D, (H, Hkv) = WIDTHS[DP], (86, 43) if QF == 2 else (4, 2)
+    lengths, prefix = [150, 1, 40, 0, 107], [17, 0, 40, 2, 90]
+    scenes, N = lengths_to_scenes(lengths), sum(lengths) + 2  # (three tiles of 128 rows: 258 workgroups with 86 heads; two rows of no scene)
+    q, k, v, dout = (rnd(gen, N, h, D, dtype=dtype) for h in (H, Hkv, Hkv, H))
+    xy = slopes = None
+    if axes:
+        xy, slopes = (torch.rand(N, axes, generator=gen) * 12).cuda(), (torch.rand(H, generator=gen) * 0.4).cuda()
+    causal = X % 2 == 0
+    opt = dict(causal=causal, prefix=prefix if causal else None, cap=cap, xy=xy, slopes=slopes)
+    (got, alone), names = launched(lambda: run(q, k, v, dout, scenes, **opt))
+    assert ran(names, "blk_attn_fwd_kernel", dtype, DP, QF, X) and ran(names, "blk_attn_dkv_kernel", dtype, DP, X)
+    assert ran(names, "blk_attn_dq_kernel", dtype, DP, QF if dtype == torch.bfloat16 else 1, X)
+    see = visible(N, N, scenes, scenes, causal, opt["prefix"])
+    check(got, alone, attention64(q, k, v, see, dout, D ** -0.5, cap, xy, xy, slopes))
+
+
+@pytest.mark.parametrize("dtype,X,cap,axes", [(t,) + w for t in TYPES for w in ways(t)])
+@pytest.mark.parametrize("DP", list(WIDTHS))
+def test_every_kernel_for_single_rows(DP, dtype, X, cap, axes):
+    gen = torch.Generator().manual_seed(10 * DP + X)
+    D, H, Hkv, lens = WIDTHS[DP], 6, 2, [1100, 1, 0, 133, 700]
+    kv, M, S = lengths_to_scenes(lens, 2), sum(lens) + 5, len(lens)
+    q, k, v = rnd(gen, S, H, D, dtype=dtype), rnd(gen, M, Hkv, D, dtype=dtype), rnd(gen, M, Hkv, D, dtype=dtype)
+    xy = kv_xy = slopes = None
+    if axes:
+        xy, kv_xy = ((torch.rand(n, axes, generator=gen) * 12).cuda() for n in (S, M))
+        slopes = (torch.rand(H, generator=gen) * 0.4).cuda()
+    rows = [(i, i + 1) for i in range(S)]
+    with torch.no_grad():
+        out, names = launched(lambda: B().attention(q, k, v, rows, kv, causal=True, cap=cap, xy=xy, kv_xy=kv_xy, slopes=slopes))
+    assert ran(names, "blk_attn_row_kernel", dtype, DP, X)
+    close(out, *attention64(q, k, v, visible(S, M, rows, kv, True, None), q, D ** -0.5, cap, xy, kv_xy, slopes)["out"], "out")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_values_that_are_not_finite_with_128_rows_a_workgroup(dtype):
+    """The second run of such a workgroup goes over its rows 16 at a time: what no row sees changes nothing, what rows see is the definition's."""
+    gen = torch.Generator().manual_seed(3)
+    H, D, scenes, N = 86, 128, [(0, 100), (100, 290), (290, 300)], 300
+    t = {n: rnd(gen, N, H, D, dtype=dtype) for n in ("q", "k", "v", "dout")}
+    see = visible(N, N, scenes, scenes, True, None)
+    want, _ = run(*t.values(), scenes, causal=True)
+    for name, x in t.items():
+        x[200 if name in "kv" else 150, 1, 5], x[130, 2, 9] = float("inf"), float("nan")
+    (got, alone), names = launched(lambda: run(*t.values(), scenes, causal=True))
+    assert ran(names, "blk_attn_fwd_kernel", dtype, 128, 2, 0) and ran(names, "blk_attn_dq_kernel", dtype, 128, 2 if dtype == torch.bfloat16 else 1, 0)
+    kinds = visible_only(*(x[:, :3] for x in t.values()), see, D ** -0.5, 0.0)
+    kind = lambda x: torch.where(x.isnan(), 2, torch.where(x.isinf(), x.sign(), 0.0))
+    for name, x in kinds.items():
+        assert torch.equal(kind(got[name][:, :3].double().cpu()), kind(x)), name
+        assert torch.isfinite(got[name][:, 3:]).all(), name
+        clean = torch.isfinite(x).all(-1)  # (rows without such a value: the sums are the same ones, through another product)
+        clean[100:290, 1:] = False
+        a, b = got[name][:, :3][clean.cuda()].double(), want[name][:, :3][clean.cuda()].double()
+        torch.testing.assert_close(a, b, rtol=4 * U[dtype], atol=64 * F * float(b.abs().max()))
+    assert torch.equal(kind(alone[:, :3].double().cpu()), kind(kinds["out"]))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("D", [32, 128])
+def test_more_tiles_than_are_ranked_and_heads_walked_together(D, dtype):
+    """131,100 rows: their tiles are taken from the last on, and with 2,048 workgroups of keys one walks both heads of a key head.  Output
+    gradients are zero but in three scenes, which the slopes' gradient then is a sum over."""
+    gen = torch.Generator(device="cuda").manual_seed(D)
+    n, S, H = 60, 2185, 2
+    N = n * S
+    q, k, v, dout = (torch.randn(N, h, D, generator=gen, device="cuda").to(dtype) for h in (H, 1, 1, H))
+    xy, slopes = torch.rand(N, 1, generator=gen, device="cuda") * 9, torch.tensor([0.05, 0.7], device="cuda")
+    some = [0, 1100, S - 1]
+    keep = torch.zeros(S, 1, dtype=torch.bool, device="cuda")
+    keep[some] = True
+    dout.mul_(keep.expand(S, n).reshape(N, 1, 1))
+    scenes = [(i * n, i * n + n) for i in range(S)]
+    (got, alone), names = launched(lambda: run(q, k, v, dout, scenes, causal=True, xy=xy, slopes=slopes))
+    assert ran(names, "blk_attn_dkv_kernel", dtype, D, 2) and not any("blk_attn_sum_kernel" in name for name in names)
+    see = visible(n, n, [(0, n)], [(0, n)], True, None)
+    slope, err = 0.0, 0.0
+    for s in some:
+        at = slice(s * n, s * n + n)
+        want = attention64(q[at], k[at], v[at], see, dout[at], D ** -0.5, 0.0, xy[at], xy[at], slopes)
+        close(alone[at], *want["out"], "out without gradients")
+        for name in ("out", "dq", "dk", "dv"):
+            close(got[name][at], *want[name], name)
+        slope, err = slope + want["dslopes"][0], err + want["dslopes"][1]
+    close(got["dslopes"], slope, err, "dslopes")
+    others = ~keep.expand(S, n).reshape(N)
+    assert not any(got[name][others].any() for name in ("dq", "dk", "dv"))
+
+
+def act64(z, ez, act, slope):
+    """(value, derivative, what the value is off by, what the derivative is off by) of z known to within ez.  The slopes of value and
+    derivative are at most 1.13 and 0.1 / 0.5 / 0.8; sigmoid and SiLU are evaluated to (8 + |z|) 2 F of themselves, their derivatives to twice
+    that; GELU is z (0.5 + 0.5 erf): half a unit's few F times |z|, and of itself."""
+    if act == 0:
+        return z, torch.ones_like(z), ez, torch.zeros_like(z)
+    if act == 1:
+        a, d = torch.where(z > 0, z, z * slope), torch.where(z > 0, 1.0, slope).double()
+        return a, d, ez * max(1.0, abs(slope)) + F * a.abs(), (z.abs() <= ez) * abs(1 - slope)
+    grow = (8 + z.abs()) * 2 * F
+    s = torch.sigmoid(z)
+    if act == 2:
+        return s, s * (1 - s), 0.25 * ez + grow * s, 0.1 * ez + 2 * grow
+    if act == 4:
+        a = z * s
+        return a, s * (1 + z * (1 - s)), 1.13 * ez + grow * a.abs(), 0.5 * ez + 2 * grow
+    cdf = 0.5 * torch.erfc(-z * 0.5 ** 0.5)
+    a = z * cdf
+    return a, cdf + z * torch.exp(-0.5 * z * z) * 0.3989422804014327, 1.13 * ez + 4 * F * (z.abs() + a.abs()), 0.8 * ez + 2 * grow
+
+
+def product64(x, w, b):
+    size = x.abs() @ w.abs().t()
+    z = x @ w.t()
+    if b is not None:
+        z, size = z + b, size + b.abs()
+    return z, (x.shape[1] + 4) * F * size
+
+
+def check_layer(dtype, x, w, v, b, c, r, dy, act, slope, y, grads):
+    """Output and gradients of either layer (v: the up weight, or None).  dZ / dG / dU are rounded to the type once, from what f32 makes of
+    activation inputs kept in f32; the bias gradients are sums from before that."""
+    u, gated = U[dtype], v is not None
+    up = lambda t: None if t is None else t.detach().double()
+    x, w, v, b, c, r, dy = map(up, (x, w, v, b, c, r, dy))
+    z, ez = product64(x, w, b)
+    a, d, ea, ed = act64(z, ez, act, slope)
+    if gated:
+        g, eg = product64(x, v, c)
+        ref = a * g
+        e = ea * (g.abs() + eg) + a.abs() * eg + F * ref.abs()
+        dz, du = dy * g * d, dy * a
+        es = dy.abs() * (ed * (g.abs() + eg) + d.abs() * eg) + 3 * F * dz.abs()
+        esu = dy.abs() * ea + 2 * F * du.abs()
+    else:
+        ref, e = (a, ea) if r is None else (a + r, ea + F * (a + r).abs())
+        dz = dy * d
+        es = dy.abs() * ed + (F * dz.abs() if act else 0)
+    final = lambda want, err: (want, err + u * (want.abs() + err))
+    close(y, *final(ref, e), "y")
+    (M, K), N = x.shape, w.shape[0]
+    zr, ezr = entered(dz, es, dtype)
+    want, err = zr @ w, ezr @ w.abs() + (N + 4) * F * ((zr.abs() + ezr) @ w.abs())
+    parts = [("w", zr, ezr), ("b", dz, es)]
+    if gated:
+        ur, eur = entered(du, esu, dtype)
+        more = ur.abs() + eur
+        want = want + ur @ v
+        err = err + eur @ v.abs() + (2 * N + 68) * F * ((zr.abs() + ezr) @ w.abs() + more @ v.abs())
+        parts += [("v", ur, eur), ("c", du, esu)]
+    close(grads["x"], *final(want, err), "dx")
+    for name, t, et in parts:
+        if name in "wv":
+            close(grads[name], *final(t.t() @ x, et.t() @ x.abs() + (M + 4) * F * ((t.abs() + et).t() @ x.abs())), "d" + name)
+        elif name in grads:
+            close(grads[name], *final(t.sum(0), et.sum(0) + (M + 4) * F * (t.abs() + et).sum(0)), "d" + name)
+
+
+def run_layer(gen, dtype, M, K, N, gated, act, bias=True, residual=True, slope=0.2):
+    """-> a call that runs the layer with its backward pass and gives check_layer's arguments"""
+    x = rnd(gen, M, K, dtype=dtype)
+    w, v = (rnd(gen, N, K, dtype=dtype, std=K ** -0.5) for _ in range(2))
+    b, c = (rnd(gen, N, dtype=dtype) if bias else None for _ in range(2))
+    r, dy = rnd(gen, M, N, dtype=dtype) if residual and not gated else None, rnd(gen, M, N, dtype=dtype)
+    leaves = {"x": x, "w": w, "b": b, **({"v": v, "c": c} if gated else {"r": r})}
+    leaves = {n: t.requires_grad_() for n, t in leaves.items() if t is not None}
+
+    def call():
+        y = B().gated_linear(x, w, v, b, c, act=act, slope=slope) if gated else B().linear_residual(x, w, b, r, act=act, slope=slope)
+        grads = dict(zip(leaves, torch.autograd.grad(y, list(leaves.values()), dy)))
+        return dtype, x, w, v if gated else None, b, c if gated else None, r, dy, act, slope, y.detach(), grads
+
+    return call
+
+
+F32, BF16 = TYPES
+TILES = [  # type, gated, rows x inputs x outputs, (tile, split) of the forward product, of dX and of dW: every one that the plan chooses
+    (F32, 0, (3209, 2246, 7039), (128, False), (256, True), (256, False)), (F32, 0, (3381, 6752, 2136), (256, True), (128, False), (256, False)),
+    (F32, 0, (6584, 3333, 2143), (256, False), (128, False), (256, True)), (F32, 0, (3343, 3993, 251), (64, False), (256, False), (64, False)),
+    (F32, 0, (3331, 1396, 336), (64, True), (64, False), (128, True)), (F32, 0, (1391, 3118, 326), (128, True), (64, False), (64, True)),
+    (F32, 0, (324, 1356, 2826), (64, True), (128, True), (128, False)), (F32, 0, (253, 257, 333), (64, False), (64, True), (64, False)),
+    (F32, 1, (2155, 6876, 1665), (256, True), (256, False), (128, False)), (F32, 1, (6587, 2450, 1481), (128, False), (64, False), (256, True)),
+    (F32, 1, (917, 1867, 8504), (64, False), (256, True), (128, False)), (F32, 1, (261, 3157, 2116), (64, True), (64, False), (256, False)),
+    (F32, 1, (2251, 251, 2952), (256, False), (64, True), (64, True)), (F32, 1, (6353, 408, 417), (64, False), (64, False), (128, True)),
+    (F32, 1, (424, 6121, 419), (128, True), (64, False), (64, False)), (F32, 1, (1291, 2311, 259), (64, False), (128, False), (64, True)),
+    (F32, 1, (337, 1384, 1667), (64, True), (128, True), (64, False)), (BF16, 0, (5669, 1861, 2214), (256, False), (256, False), (256, True)),
+    (BF16, 0, (1989, 2057, 5616), (256, False), (256, True), (256, False)), (BF16, 0, (2329, 5565, 1742), (256, True), (256, False), (256, False)),
+    (BF16, 0, (3771, 647, 343), (64, False), (128, False), (128, True)), (BF16, 0, (646, 330, 3827), (128, False), (128, True), (64, False)),
+    (BF16, 0, (273, 3580, 769), (128, True), (64, False), (128, False)), (BF16, 0, (252, 1585, 300), (64, True), (64, False), (64, False)),
+    (BF16, 0, (1679, 258, 266), (64, False), (64, False), (64, True)), (BF16, 0, (259, 253, 1513), (64, False), (64, True), (64, False)),
+    (BF16, 1, (5557, 1801, 1146), (256, False), (256, False), (256, True)), (BF16, 1, (1166, 5569, 1718), (256, True), (128, False), (128, False)),
+    (BF16, 1, (775, 1222, 6958), (256, False), (256, True), (128, False)), (BF16, 1, (272, 1288, 2977), (64, False), (64, True), (256, False)),
+    (BF16, 1, (267, 3824, 390), (128, True), (64, False), (128, False)), (BF16, 1, (3689, 264, 393), (128, False), (64, False), (128, True)),
+    (BF16, 1, (801, 261, 1830), (128, False), (128, True), (64, False)), (BF16, 1, (270, 1857, 251), (64, True), (64, False), (64, False)),
+    (BF16, 1, (1844, 251, 255), (64, False), (64, False), (64, True))]
+
+
+@pytest.mark.parametrize("dtype,gated,sizes,fwd,dx,dw", TILES)
+def test_every_product_kernel(dtype, gated, sizes, fwd, dx, dw):
+    """All tiles, whole and split over k, of the forward product and of both products of the backward pass, with ragged edges."""
+    waves = {256: (2, 4), 128: (2, 2), 64: (4, 1)}
+    gen = torch.Generator().manual_seed(sum(sizes))
+    result, names = launched(run_layer(gen, dtype, *sizes, gated, (4 if gated else 5) if sum(sizes) % 2 else 1))
+    for epi, (tile, split), columns in ((gated, fwd, (False, False)), (0, dx, (False, True)), (0, dw, (True, True))):
+        assert ran(names, "blk_gemm_kernel", dtype, tile, tile, *waves[tile], epi, split, *columns), (tile, split, columns, names)
+    check_layer(*result)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("gated,M,K,N", [(0, 16, 40, 16400), (1, 7, 65, 9000), (0, 1, 24, 33), (1, 16, 129, 100)])
+def test_every_kernel_for_a_few_rows(gated, M, K, N, dtype):
+    result, names = launched(run_layer(torch.Generator().manual_seed(N), dtype, M, K, N, gated, 4))
+    assert ran(names, "blk_few_rows_kernel", dtype, gated, 4 if -(-N // 16) * (1 + gated) >= 1024 else 8)
+    check_layer(*result)
