@@ -274,3 +274,55 @@ def test_tables_of_whole_numbers_of_any_kind(rows, monkeypatch):
     monkeypatch.setattr(B, "_TABLES", B.BoundedCache(64))
     monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
     assert B._table("scenes", rows, torch.device("cpu"), 6, 2).tolist() == [[0, 2], [2, 6]]
+
+
+@pytest.mark.parametrize("gated,M,K,N", [(0, 300, 96, 520), (1, 200, 72, 264), (0, 70, 159, 127), (1, 33, 40, 159)])
+@pytest.mark.parametrize("act", [2, 4, 5])
+@pytest.mark.parametrize("mistake,where", [(None, None), ("activation inputs", "dx|dw"), ("bias gradients", "db")])
+def test_the_layers_bounds_tell_a_rounding_of_what_is_kept_in_f32(mistake, where, act, gated, M, K, N):
+    """The GPU tests' bounds on a layer that is computed here, in 64 bits: it passes, and with activation inputs rounded to bf16 or bias
+    gradients summed from the rounded dZ it does not."""
+    import test_hip_blocks_bounds as T
+
+    gen, bf16 = torch.Generator().manual_seed(M + act), torch.bfloat16
+    rand = lambda *shape, std=1.0: (torch.randn(*shape, generator=gen) * std).to(bf16)
+    round_ = lambda t: t.float().to(bf16)
+    t, w, v, b, c, dy = rand(M, K), rand(N, K, std=K ** -0.5), rand(N, K, std=K ** -0.5), rand(N), rand(N), rand(M, N)
+    X, W, V, DY = (u.double() for u in (t, w, v, dy))
+    z, u = X @ W.t() + b.double(), X @ V.t() + c.double() if gated else 1.0
+    y = round_(T.act64(z, 0 * z, act, 0.2)[0] * u)
+    if mistake == "activation inputs":
+        z, u = round_(z).double(), round_(u).double() if gated else 1.0
+    a, d = T.act64(z, 0 * z, act, 0.2)[:2]
+    dz, du = DY * d * u, DY * a
+    zr, ur = round_(dz).double(), round_(du).double()
+    if mistake == "bias gradients":
+        dz, du = zr, ur
+    grads = {"x": zr @ W + (ur @ V if gated else 0), "w": zr.t() @ X, "b": dz.sum(0)}
+    if gated:
+        grads.update(v=ur.t() @ X, c=du.sum(0))
+    check = lambda: T.check_layer(bf16, t, w, v if gated else None, b, c if gated else None, None, dy, act, 0.2, y,
+                                  {n: round_(g) for n, g in grads.items()})
+    if mistake is None:
+        return check()
+    with pytest.raises(AssertionError, match=where):
+        check()
+
+
+def test_the_slopes_bound_tells_a_rounding_of_the_scores_gradients():
+    import test_hip_blocks_bounds as T
+
+    gen, (N, H, D) = torch.Generator().manual_seed(2), (8, 3, 32)  # (few rows: the bound adds up what roundings do not)
+    q, k, v, dout = (torch.randn(N, H, D, generator=gen).to(torch.bfloat16) for _ in range(4))
+    xy, slopes = torch.rand(N, 1, generator=gen) * 9, torch.tensor([0.1, 0.3, 0.5])
+    see = torch.ones(N, N).tril().bool()
+    want, bound = T.attention64(q, k, v, see, dout, D ** -0.5, 0.0, xy, xy, slopes)["dslopes"]
+    Q, K, V, dO = (t.double().transpose(0, 1) for t in (q, k, v, dout))
+    dist = (xy - xy.t()).abs().double()
+    P = torch.softmax((D ** -0.5 * Q @ K.transpose(1, 2) - slopes.double()[:, None, None] * dist).masked_fill(~see, -torch.inf), -1)
+    dP = dO @ V.transpose(1, 2)
+    dL = P * (dP - (P * dP).sum(-1, keepdim=True))
+    assert ((-(dL * dist).sum((1, 2)) - want).abs() <= bound).all()
+    rounded = P * (dP - (dO * (P @ V).to(torch.float32).to(torch.bfloat16).double()).sum(-1, keepdim=True))  # (sum(dO O) of a rounded output)
+    for wrong in (dL.to(torch.float32).to(torch.bfloat16).double(), rounded):
+        assert ((-(wrong * dist).sum((1, 2)) - want).abs() > 2 * bound).all()

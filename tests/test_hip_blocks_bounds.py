@@ -468,3 +468,53 @@ def test_every_kernel_for_a_few_rows(gated, M, K, N, dtype):
     result, names = launched(run_layer(torch.Generator().manual_seed(N), dtype, M, K, N, gated, 4))
     assert ran(names, "blk_few_rows_kernel", dtype, gated, 4 if -(-N // 16) * (1 + gated) >= 1024 else 8)
     check_layer(*result)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("act", [0, 1, 2, 4, 5])
+@pytest.mark.parametrize("gated,M,K,N", [(0, 300, 96, 520), (1, 200, 72, 264), (0, 70, 159, 127), (1, 33, 40, 159)])
+def test_layers_keep_in_f32_what_is_not_an_operand(gated, M, K, N, act, dtype):
+    """Activation inputs are kept in f32 and bias gradients summed before dZ's rounding: bounds without a rounding of either."""
+    check_layer(*run_layer(torch.Generator().manual_seed(M + act), dtype, M, K, N, gated, act, residual=act != 2)())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("D", [32, 64, 128])
+def test_attention_keeps_the_output_in_f32_for_the_backward_pass(D, dtype):
+    """Rows that weigh 64 keys equally (q = 0) have weights that bf16 holds exactly, and values of 1 or 1 + 2^-7 have means that it does not:
+    sum(dO O) of a rounded output would be off by up to 2^-8 of itself, many times the scores' gradients, which are differences of 2^-7 at most.
+    Without a rounding of P the output before its own is good to f32, so the bounds have none in sum(dO O)."""
+    gen = torch.Generator().manual_seed(D)
+    n, H, S = 64, 2, 3
+    N, scenes = n * S, [(i * n, i * n + n) for i in range(S)]
+    q, k = torch.zeros(N, H, D, dtype=dtype, device="cuda"), 1 + rnd(gen, N, H, D, dtype=dtype, std=0.1)
+    v = (1 + (torch.rand(N, H, D, generator=gen) < 0.3).float() * 2.0 ** -7).to(dtype).cuda()
+    dout = rnd(gen, N, H, D, dtype=dtype).abs()
+    got, _ = run(q, k, v, dout, scenes)
+    u, up = U[dtype], lambda t: t.double().view(S, n, H, D).transpose(1, 2)
+    K, V, dO = up(k), up(v), up(dout)
+    O = V.mean(2, keepdim=True)
+    dP, delta = dO @ V.transpose(2, 3), (dO * O).sum(-1, keepdim=True)
+    e = ((D + 4) * F * (dO.abs() @ V.transpose(2, 3).abs()) + (D + n + 24) * F * (dO.abs() * O.abs()).sum(-1, keepdim=True)) / n
+    dS, eS = entered((dP - delta) / n, e + 40 * F * (dP - delta).abs() / n, dtype)
+    want, err = dS @ K, eS @ K.abs() + (n + 4) * F * (dS.abs() @ K.abs())
+    want, err = (t.transpose(1, 2).reshape(N, H, D) * D ** -0.5 for t in (want, err))
+    close(got["dq"], want, err + u * (want.abs() + err), "dq")
+    rounded = O.to(torch.float32).to(dtype).double()  # (that the inputs tell the two apart)
+    if dtype == torch.bfloat16:
+        off = ((dO * (rounded - O)).sum(-1, keepdim=True) / n * K.sum(2, keepdim=True)).transpose(1, 2).reshape(N, H, D) * D ** -0.5
+        assert ((off.abs() > 4 * (err + u * (want.abs() + err))).float().mean()) > 0.5
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("cap", [0.0, 20.0])
+@pytest.mark.parametrize("D,axes", [(32, 2), (128, 1)])
+def test_slopes_gradient_of_a_small_scene(D, axes, cap, dtype):
+    """Of so few pairs that the bound is many times below a rounding of the scores' gradients or of the output to bf16."""
+    for seed in range(6):
+        gen = torch.Generator().manual_seed(seed)
+        N, H = 8, 4
+        q, k, v, dout = (rnd(gen, N, H, D, dtype=dtype) for _ in range(4))
+        xy, slopes = (torch.rand(N, axes, generator=gen) * 9).cuda(), (torch.rand(H, generator=gen) * 0.4).cuda()
+        got, alone = run(q, k, v, dout, [(0, N)], causal=True, cap=cap, xy=xy, slopes=slopes)
+        check(got, alone, attention64(q, k, v, visible(N, N, [(0, N)], [(0, N)], True, None), dout, D ** -0.5, cap, xy, xy, slopes))
