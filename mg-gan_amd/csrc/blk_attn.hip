@@ -488,7 +488,7 @@ int mggan_block_attention_fwd(const void* args, hipStream_t stream) {
   const BlkAttnArgs* a = (const BlkAttnArgs*)args;
   const int rc = blk_attn_check(a, "block_attention_fwd");
   if (rc != MGGAN_OK) return rc;
-  MG_CHECK_ARG(a->out && (size_t)a->out % 16 == 0 && (size_t)a->spans % 16 == 0, "block_attention_fwd: output or spans null or unaligned");
+  MG_CHECK_ARG(a->out && ((size_t)a->out | (size_t)a->out32 | (size_t)a->spans) % 16 == 0, "block_attention_fwd: output or spans null or unaligned");
   const size_t need = fwd_workspace(*a);
   MG_CHECK_ARG(!need || (a->ws && (size_t)a->ws_bytes >= need), "block_attention_fwd: workspace of %zu bytes (got %ld)", need, a->ws_bytes);
   if (a->dtype == BLK_BF16)

@@ -326,3 +326,12 @@ def test_the_slopes_bound_tells_a_rounding_of_the_scores_gradients():
     rounded = P * (dP - (dO * (P @ V).to(torch.float32).to(torch.bfloat16).double()).sum(-1, keepdim=True))  # (sum(dO O) of a rounded output)
     for wrong in (dL.to(torch.float32).to(torch.bfloat16).double(), rounded):
         assert ((-(wrong * dist).sum((1, 2)) - want).abs() > 2 * bound).all()
+
+
+def test_the_c_entry_refuses_an_unaligned_f32_output():
+    """It is written 16 bytes at a time, as the output is."""
+    attn = dict(q=256, k=256, v=256, dout=0, out=256, dq=0, dk=0, dv=0, dslopes=0, scenes=256, kv_scenes=256, prefix=0, xy=0, kv_xy=0, slopes=0, lse=256,
+                out32=260, spans=256, ws=0, ws_bytes=0, q_row=64, q_head=16, k_row=32, k_head=16, v_row=32, v_head=16, N=8, M=8, H=4, Hkv=2, D=16, S=1,
+                causal=0, axes=0, dtype=1, scale=1.0, cap=0.0)
+    with pytest.raises(HipError, match="unaligned"):
+        L.mggan_block_attention_fwd(B._ATTN.pack(*attn.values()), 0)
