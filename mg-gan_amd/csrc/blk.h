@@ -56,11 +56,6 @@ __device__ __forceinline__ void copies_done() { asm volatile("s_waitcnt vmcnt(0)
 // The transposing read: four 16-bit values of each of the lane's group's rows.
 __device__ __forceinline__ s16x4 lds_transposed(const char* __restrict p) { return __builtin_amdgcn_ds_read_tr16_b64_v4i16((MG_LDS s16x4*)p); }
 
-template <class T>
-__device__ __forceinline__ float to_f(T v) {
-  return (float)v;
-}
-
 // Activation and derivative by its INPUT z.  exp through __expf (2 ulp); gelu is the exact form z Phi(z).
 __device__ __forceinline__ float blk_act(float z, int act, float slope) {
   switch (act) {
