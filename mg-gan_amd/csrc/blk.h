@@ -56,7 +56,8 @@ __device__ __forceinline__ void copies_done() { asm volatile("s_waitcnt vmcnt(0)
 // The transposing read: four 16-bit values of each of the lane's group's rows.
 __device__ __forceinline__ s16x4 lds_transposed(const char* __restrict p) { return __builtin_amdgcn_ds_read_tr16_b64_v4i16((MG_LDS s16x4*)p); }
 
-// Activation and derivative by its INPUT z.  exp through __expf (2 ulp); gelu is the exact form z Phi(z).
+// Activation and derivative by its INPUT z.  exp through __expf, whose error grows with its argument: (8 + |z|) 2^-23 of the value at most.
+// gelu is the exact form z Phi(z), Phi by erf: a few 2^-24 of |z|.
 __device__ __forceinline__ float blk_act(float z, int act, float slope) {
   switch (act) {
     case ACT_LEAKY: return z > 0.f ? z : z * slope;

@@ -111,8 +111,9 @@ struct Geo {
   }
   static __device__ __forceinline__ int row4(int f, int g) { return sizeof(T) == 2 ? 32 * (f >> 1) + 8 * g + 4 * (f & 1) : 16 * f + 4 * g; }
   // Place of a chunk in its row.  Row reads take one chunk of 16 rows ({0-3, 8-11, ..} (+4) with bf16, 0-15 with f32): any eight lanes meet
-  // eight bank groups.  The transposing reads of bf16 take two chunks of rows 8 g + {0..3}: eight bank groups again.  Neither depends on which
-  // fragment it is, so a lane's addresses are a few bases plus constants (Lane).
+  // eight groups of four banks.  The transposing reads of bf16 take two chunks of rows 8 g + {0..3}: eight groups again.  Neither depends on which
+  // fragment it is, so a lane's addresses are a few bases plus constants (Lane).  Eight groups are 128 of the 256 bytes that LDS serves in a
+  // cycle, so the reads are not free of conflicts: 1.9 to 2.5 cycles of them an LDS instruction (counters, widths 64 and 128).
   static __device__ __forceinline__ int swz(int r) {
     if (sizeof(T) == 4) return (r & 7) ^ ((r >> 1) & 4);
     return NCH % 8 == 0 ? (r & 3) << 1 | ((r >> 3) & 1) : (r & 2) | ((r >> 3) & 1);
@@ -224,7 +225,10 @@ __device__ __forceinline__ void scores2(const void* ta, const void* tb, const u3
   }
 }
 
-// Four weights or score gradients of a lane as the next product takes them: bf16 rounded here, once.
+// Four weights or score gradients of a lane as the next product takes them.  bf16 operands: rounded to bf16 here, once -- the matrix
+// instructions take both operands in one type, so P V, P^T dO, dS K and dS^T Q carry half a step of P or dS (2^-8) beside that of their other operand.
+// Against 64 bits that makes 0.0023 to 0.0024 of outputs and gradients that are 0.0017 off with P and dS in f32 (the final rounding alone); P as the
+// sum of two bf16 numbers would take each of these products twice.
 template <class T>
 struct Coef {
   f32x4 v;

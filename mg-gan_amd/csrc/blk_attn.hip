@@ -50,9 +50,9 @@ __global__ __launch_bounds__(256) void blk_spans_kernel(BlkAttnArgs p, int np) {
 
 // 64 QF query rows of one head: four waves of 16 QF rows each (this one's start at w0); keys and values in tiles of BK rows, two buffers.
 //   m' = max(m, max_j s_j)    l' = l 2^(m-m') + sum_j 2^(s_j-m')    acc' = acc 2^(m-m') + sum_j 2^(s_j-m') v_j    out = acc / l
-// Bound by the vector instructions of the softmax: with a cap at width 64 they fill 90 % of the cycles (four an instruction, sixteen an exp2 or rcp),
-// the matrix cores 12 %; at width 128 with a distance 70 to 80 and 35 %.  16,384 causal rows of 8 heads at width 128 take 0.84 ms, packed 8,192
-// rows of 16 heads at width 64 with a cap 92 us.
+// Bound by the vector instructions around the softmax: they fill 71 % of the time (an exp2 or rcp counts as two), both at width 64 with a cap, where
+// the matrix cores are busy 12 %, and at width 128 with a distance, 35 %.  16,384 causal rows of 8 heads at width 128 take 0.85 ms, packed 8,192
+// rows of 16 heads at width 64 with a cap 95 us.
 template <class T, int DP, int QF, int X, bool SAFE>
 __device__ __forceinline__ void attn_fwd_rows(const BlkAttnArgs& p, int np, int h, int glo, int ghi, int w0, u32x4* lk, u32x4* lv, float* lx, int* odd) {
   using G = Geo<T, DP>;

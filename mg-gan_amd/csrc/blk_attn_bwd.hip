@@ -2,7 +2,8 @@
 // gradient), one owns keys (dK, dV, summed over the heads that share them); both form the scores again from the operands and the kept
 // softmax statistics.  With P and D = sum(dO O):
 //   dV = P^T dO      dL = P (dO V^T - D)      dslope = -sum dL |xy - kv_xy|      dS = dL (1 - tanh^2)      dQ = scale dS K      dK = scale dS^T Q
-// P and dS are rounded to the operands' type where they enter a product, as every operand is.
+// P and dS are rounded to the operands' type where they enter a product, as every operand is (Coef in blk_attn.h); what is summed without a
+// product -- sum(dO O), the slopes' gradient -- takes them in f32.
 #include <limits.h>
 #include "blk_attn.h"
 #include "../../include/mggan_hip.h"
@@ -16,8 +17,9 @@ template <class T, int DP>
 using BwdGeo = Geo<T, DP, sizeof(T) == 2 && DP % 64 ? 64 : 32>;
 
 // dQ of 64 QF rows of one head (this wave's start at w0), and the sum that the rows' slopes' gradient is.  Three products a tile: keys are read
-// twice (rows, then transposed), values once.  Bound by the waves' instructions around the products (matrix cores busy 36 % at width 128, vector
-// instructions about 60 %): 16,384 causal rows of 8 heads at width 128, 1.11 ms; packed 8,192 rows of 16 heads at width 64, 104 us.
+// twice (rows, then transposed), values once.  Bound by the waves' instructions around the products (width 128 with a distance: vector instructions
+// 62 % of the time, matrix cores 36 %; width 64 with a cap: 82 and 17 %): 16,384 causal rows of 8 heads at width 128, 1.14 ms; packed 8,192 rows of
+// 16 heads at width 64, 107 us.
 template <class T, int DP, int QF, int X, bool SAFE>
 __device__ __forceinline__ float attn_dq_rows(const BlkAttnArgs& p, int np, float* delta, int h, int glo, int ghi, int w0, u32x4* lk, u32x4* lv,
                                               float* lx, int* odd) {
@@ -215,9 +217,9 @@ __global__ __launch_bounds__(256, QF == 1 && DP <= 64 ? 3 : 2) void blk_attn_dq_
 }
 
 // dK and dV of 64 keys of one key head (this wave's 16 start at w0) from the queries [qa, qb) of `heads` heads from h0 on, in tiles of BK
-// rows; `part`: of some of the key head's heads, left in f32 for blk_attn_sum_kernel as the slot-th of `slots` such results.  Four products a tile, both streamed operands read twice.  Bound by LDS: 16
-// keys a wave take a kilobyte of reads for every multiplication, and LDS is busy 77 % of the time at width 128 (1.51 ms at 16,384 causal rows; width
-// 64, packed 8,192 rows: 165 us).  32 keys a wave would halve the reads, but two results, keys and values of 32 rows leave too few registers (1.8 to 9
+// rows; `part`: of some of the key head's heads, left in f32 for blk_attn_sum_kernel as the slot-th of `slots` such results.  Four products a tile, both streamed operands read twice.  Bound by LDS at width 128:
+// 16 keys a wave take a kilobyte of reads for every multiplication, and LDS is busy 75 % of the time, 45 % of that with bank conflicts (1.58 ms at 16,384
+// causal rows).  At width 64 with a cap vector instructions fill 57 % and LDS 38 % (packed 8,192 rows: 170 us).  32 keys a wave would halve the reads, but two results, keys and values of 32 rows leave too few registers (1.8 to 9
 // ms, spilled or with two waves a SIMD).
 template <class T, int DP, int X, bool SAFE>
 __device__ __forceinline__ void attn_dkv_rows(const BlkAttnArgs& p, int np, const float* delta, float* part, int slot, int slots, int h0, int heads, int qa, int qb, int w0,

@@ -127,6 +127,8 @@ __device__ __forceinline__ void epilogue(const GemmP& p, int m, int n, float (&v
 //            any eight lanes of either set fall on eight bank groups.
 //   columns: [64 / sizeof(T) values of k][R / CH chunks]: bf16 is read by the transposing LDS read (16 lanes take 4 k x 16 columns: four
 //            rows of two chunks each, on eight bank groups), f32 element by element (4 k x 16 columns: two passes, the least for 256 bytes).
+// Eight groups of four banks are half of what LDS serves in a cycle, so conflicts remain: 2.7 cycles beside the 4 of a 16-byte read, 2.0 beside
+// the 2 of a transposing one (counters).
 template <class T, int R, int NT, bool COLS>
 struct Side {
   static constexpr int CH = Mf<T>::CH, KS = 4 * CH, L = R * 4 / NT, NC = COLS ? R / CH : 4, SIZE = R * 4;
@@ -203,8 +205,8 @@ __device__ __forceinline__ void wait_copies() {
 // Bound by the matrix cores from about 256 tiles on.  A tile of 256 x 256 takes 32 KB of copies for 4.2 MFLOP, so that its bytes come out of the
 // L2; its eight waves of 128 x 64 read 12 fragments for 32 multiplications (four waves of 128 x 128 would read less, but 256 accumulators
 // leave no room for a second set of fragments: 634 TFLOP/s).  8,192 x 4,096 x 4,096 bf16: 204 us, 1.35 PFLOP/s (the library: 1.24-1.6), the
-// gated training pass' products of four times that work 1.07 (forward), 1.21 (dX) and 1.29 (dW); f32, 4,096 each way: 145 TFLOP/s (136).  Its matrix
-// cores are busy 62-75 % of the time in these; copies of two steps behind one barrier made it 964 instead of 1,150 TFLOP/s.
+// gated training pass' products of four times that work 1.05 (forward), 1.15 (dX) and 1.24 (dW); f32, 4,096 each way: 145 TFLOP/s (136).  Its matrix
+// cores are busy 65, 70 and 76 % of the time in these; copies of two steps behind one barrier made it 964 instead of 1,150 TFLOP/s.
 template <class T, int BM, int BN, int WM, int WN, int EPI, bool SPLIT, bool CA, bool CB>
 __global__ __launch_bounds__(WM* WN * 64) void blk_gemm_kernel(GemmP p) {
   constexpr int NT = WM * WN * 64, CH = Mf<T>::CH, KS = 4 * CH;
@@ -506,7 +508,7 @@ __global__ __launch_bounds__(256) void blk_pad_kernel(const T* in, long ldi, T* 
 
 // dY -> dZ = dY act'(z) (linear) or dG = dY u act'(g), dU = dY act(g) (gated), as rows of ld ldz (dU `off` behind dG, zeros up to the
 // end of each), and the columns' sums of DZ_ROWS rows in f32 for the bias gradients.  dZ is rounded to the operands' type once: it is an
-// operand of both products, and half a step is what every operand has.  A thread takes eight columns of every eighth row.
+// operand of both products, and half a step is what every operand has (bf16 gradients 0.0023 to 0.0024 off against 64 bits, 0.0017 with dZ in f32).  A thread takes eight columns of every eighth row.
 // Bound by bytes (gated bf16: 10 read and 4 written an output): 8,192 x 8,192 gated 200 us, 4.7 TB/s.
 constexpr int DZ_ROWS = 64;
 struct DzP {
