@@ -518,3 +518,52 @@ def test_slopes_gradient_of_a_small_scene(D, axes, cap, dtype):
         xy, slopes = (torch.rand(N, axes, generator=gen) * 9).cuda(), (torch.rand(H, generator=gen) * 0.4).cuda()
         got, alone = run(q, k, v, dout, [(0, N)], causal=True, cap=cap, xy=xy, slopes=slopes)
         check(got, alone, attention64(q, k, v, visible(N, N, [(0, N)], [(0, N)], True, None), dout, D ** -0.5, cap, xy, xy, slopes))
+
+
+@pytest.mark.parametrize("gated", [0, 1])
+def test_layers_beyond_32_bit_offsets(gated):
+    """2^21 rows of 1,032 inputs and 1,040 outputs: inputs, outputs, kept values and gradients of more than 2^31 elements each.  The output's
+    gradient is zero but in rows at both ends, which the weights' gradients then are sums over."""
+    gen = torch.Generator(device="cuda").manual_seed(gated)
+    M, K, N, dtype, act = 1 << 21, 1032, 1040, torch.bfloat16, 4
+    x = torch.empty(M, K, dtype=dtype, device="cuda").normal_(generator=gen)
+    w, v = (torch.empty(N, K, dtype=dtype, device="cuda").normal_(std=K ** -0.5, generator=gen) for _ in range(2))
+    b = torch.empty(N, dtype=dtype, device="cuda").normal_(generator=gen)
+    some = torch.cat([torch.arange(50), torch.arange(M - 70, M)]).cuda()
+    dy = torch.zeros(M, N, dtype=dtype, device="cuda")
+    dy[some] = torch.randn(len(some), N, generator=gen, device="cuda").to(dtype)
+    leaves = {"x": x, "w": w, "b": b, **({"v": v} if gated else {})}
+    for t in leaves.values():
+        t.requires_grad_()
+    y = B().gated_linear(x, w, v, b, None, act=act) if gated else B().linear_residual(x, w, b, act=act)
+    grads = dict(zip(leaves, torch.autograd.grad(y, list(leaves.values()), dy)))
+    assert not grads["x"][50:M - 70].any()
+    grads["x"] = grads["x"][some]
+    check_layer(dtype, x[some], w, v if gated else None, b, None, None, dy[some], act, 0.0, y.detach()[some], grads)
+    with torch.no_grad():
+        y0 = B().gated_linear(x, w, v, b, None, act=act) if gated else B().linear_residual(x, w, b, act=act)
+        assert torch.equal(y0, y)
+
+
+def test_attention_beyond_32_bit_offsets():
+    """1,100,000 rows of 16 heads of 128: more than 2^31 elements of every operand, output and gradient (and of the f32 output)."""
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    n, S, H, D, dtype = 50, 22_000, 16, 128, torch.bfloat16
+    N = n * S
+    q, k, v, dout = (torch.empty(N, H, D, dtype=dtype, device="cuda").normal_(generator=gen) for _ in range(4))
+    xy, slopes = torch.rand(N, 1, generator=gen, device="cuda") * 9, torch.rand(H, generator=gen, device="cuda") * 0.3
+    scenes = (torch.arange(S + 1, dtype=torch.int32, device="cuda") * n).unfold(0, 2, 1).contiguous()
+    some = [0, S // 2, S - 1]
+    keep = torch.zeros(S, 1, dtype=torch.bool, device="cuda")
+    keep[some] = True
+    dout.mul_(keep.expand(S, n).reshape(N, 1, 1))
+    got, alone = run(q, k, v, dout, scenes, causal=True, xy=xy, slopes=slopes)
+    see, slope, err = visible(n, n, [(0, n)], [(0, n)], True, None), 0.0, 0.0
+    for s in some:
+        at = slice(s * n, s * n + n)
+        want = attention64(q[at], k[at], v[at], see, dout[at], D ** -0.5, 0.0, xy[at], xy[at], slopes)
+        close(alone[at], *want["out"], "out without gradients")
+        for name in ("out", "dq", "dk", "dv"):
+            close(got[name][at], *want[name], name)
+        slope, err = slope + want["dslopes"][0], err + want["dslopes"][1]
+    close(got["dslopes"], slope, err, "dslopes")
